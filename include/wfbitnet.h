@@ -400,6 +400,64 @@ int wfb_rmsnorm_grad(const void* x, int x_dtype, const void* gamma, int gamma_dt
                      int64_t m, int64_t h, void* grad_x, void* grad_gamma, int ggamma_dtype, float* work,
                      void* stream);
 
+/* ---- int8 key/value cache -------------------------------------------------------------------- */
+
+/* A key/value cache held as int8 codes with one fp32 scale per (token, kv head): half the bytes of a bf16 cache.  Of a
+ * row's D = head_dim elements x (a key after the rotary embedding, or a value): m = max|x|, scale = m / 127, code =
+ * round_half_even(x * (127 / m)), every operation rounded to fp32; m < 2^-100 gives scale 0 and codes 0, a NaN or an
+ * infinity in the row scale NaN.  The row stands for code * scale.
+ *   k        int8 [batch, num_kv_heads, cap, head_dim]
+ *   v        int8 [batch, num_kv_heads, cap / 64, head_dim, 64]   (blocks of 64 keys, transposed)
+ *   k_scale, v_scale  fp32 [batch, num_kv_heads, cap]
+ * cap: keys per sequence, a multiple of WFB_KV_I8_BLOCK with cap * head_dim < 2^31; k and v 16-byte aligned, the
+ * scales too.  No counterpart in the reference, whose engine keeps an fp32 cache
+ * (SGB/sgl-kernel/csrc/inference/kv_cache.h:81-101). */
+#define WFB_KV_I8_BLOCK 64
+typedef struct wfb_kv_i8 {
+  int8_t* k;
+  float* k_scale;
+  int8_t* v;
+  float* v_scale;
+  int64_t cap;
+} wfb_kv_i8;
+
+/* Rotary embedding of new keys and quantising write of new keys and values: token i of sequence b, i < lengths[b], goes
+ * to position start[b] + i.  k_new / v_new [batch*T, ldk / ldv] of dtype (WFB_F32 or WFB_BF16), row b*T + i, 16-byte
+ * aligned rows.  start_dev int64 [batch] on the device, or NULL for `start` in every sequence; lengths_dev likewise, or
+ * NULL for T.  rope_cos / rope_sin fp32 [rope_len, head_dim/2], 16-byte aligned: position p takes row p + turn (turn:
+ * the length of a prefix that precedes every sequence's own positions); both NULL for no rotary embedding.
+ * Positions on the device are checked there: a sequence whose length is outside 0..T, or whose positions are outside
+ * [0, cap) or (with turn) the rotary tables, is not written at all. */
+int wfb_kv_write_i8(const void* k_new, int64_t ldk, const void* v_new, int64_t ldv, int dtype,
+                    const float* rope_cos, const float* rope_sin, int64_t rope_len, int64_t turn,
+                    const wfb_kv_i8* cache, const int64_t* start_dev, int64_t start, const int64_t* lengths_dev,
+                    int64_t batch, int64_t t, int64_t num_kv_heads, int64_t head_dim, void* stream);
+
+/* Positions start[b] .. start[b] + count - 1 of every sequence back as k_out / v_out [batch, num_kv_heads, count,
+ * head_dim] of dtype (16-byte aligned); positions outside the cache read as zeros. */
+int wfb_kv_read_i8(const wfb_kv_i8* cache, const int64_t* start_dev, int64_t start, int64_t batch, int64_t count,
+                   int64_t num_kv_heads, int64_t head_dim, void* k_out, void* v_out, int dtype, void* stream);
+
+/* wfb_kv_write_i8 of T tokens per sequence, and their attention: token i of sequence b at position p = start[b] + i,
+ * query head h: softmax_j(rope(q)_h . k_j * scale) v_j over the prefix_len keys of `prefix` (a cache of one sequence
+ * that the whole batch shares, or NULL) and the sequence's own keys 0 .. p, all as the caches hold them, the new
+ * tokens' own among them: a result does not depend on how a prompt was cut into calls.  The rotary embedding takes row
+ * prefix_len + p.  Scores, softmax and sums are fp32, the products exact integers of the codes with q and the
+ * probabilities as fixed-point numbers of 16 bits (dtype WFB_BF16) or 24 (WFB_F32) of their row's largest; the output is
+ * rounded once to dtype.  T = 1 with start_dev is a decode step.
+ * q, out [batch*T, ldq / ldo] and k_new, v_new as in wfb_kv_write_i8 (rows 16-byte aligned); num_heads / num_kv_heads
+ * in 1..16, head_dim 64 or 128.  Rows at and behind lengths[b] are zeros; a sequence that does not fit (see above) gives
+ * NaN rows and is not written.  workspace: the floats that wfb_gqa_attention_i8_workspace (host only) reports, 16-byte
+ * aligned, or NULL if that is 0. */
+int wfb_gqa_attention_i8_workspace(int64_t batch, int64_t t, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                   int64_t cap, int64_t prefix_len, int64_t* floats);
+int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t ldk, const void* v_new, int64_t ldv,
+                         int dtype, const float* rope_cos, const float* rope_sin, int64_t rope_len,
+                         const wfb_kv_i8* cache, const int64_t* start_dev, int64_t start, const int64_t* lengths_dev,
+                         const wfb_kv_i8* prefix, int64_t prefix_len, int64_t batch, int64_t t, int64_t num_heads,
+                         int64_t num_kv_heads, int64_t head_dim, float scale, void* out, int64_t ldo, float* workspace,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,7 @@ WFB_NORM_MAX_H = 16384
 WFB_MAX_SEGMENTS = 8
 WFB_SCALE_REFERENCE = 0
 WFB_SCALE_CHECKPOINT = 1
+WFB_KV_I8_BLOCK = 64
 WFB_ACT_SILU = 1
 WFB_ACT_RELU2 = 2
 
@@ -31,6 +32,14 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+
+
+
+class KvI8Struct(ctypes.Structure):
+    """wfb_kv_i8: the four tensors of an int8 key/value cache and its keys per sequence."""
+
+    _fields_ = [("k", _vp), ("k_scale", _vp), ("v", _vp), ("v_scale", _vp), ("cap", _i64)]
+
 
 # name -> argtypes (restype is int for all but the two queries)
 SIGNATURES = {
@@ -63,6 +72,12 @@ SIGNATURES = {
                                          _i64, _i64, _i64, _f32, _vp, _i64, _vp],
     "wfb_gqa_prefill_attention": [_vp, _i64, _vp, _i64, _vp, _i64, _int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                   _i64, _i64, _i64, _f32, _vp, _i64, _vp],
+    "wfb_kv_write_i8": [_vp, _i64, _vp, _i64, _int, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+                        _vp],
+    "wfb_kv_read_i8": [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _int, _vp],
+    "wfb_gqa_attention_i8_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
+    "wfb_gqa_attention_i8": [_vp, _i64, _vp, _i64, _vp, _i64, _int, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64,
+                             _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i64, _vp, _vp],
     "wfb_linear_i2s_glu": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _int, _int, _vp, _i64, _vp],
     "wfb_rmsnorm_linear_i2s": [_vp, _int, _i64, _vp, _int, _f32, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _vp,
                                _int, _i64, _vp, _int, _i64, _vp],

@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <string>
 
+#include "kv_i8.h"
 #include "wfb_common.h"
 
 namespace {
@@ -163,6 +164,50 @@ int check_decode_attention(const char* name, const void* q, int64_t ldq, const v
   if (batch == 0) return ok();
   if (!q || !k_new || !v_new || !k_cache || !v_cache || !pos || !out) return fail(WFB_EINVAL, "%s: null pointer", name);
   if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return fail(WFB_EINVAL, "%s: caches must be 16-byte aligned", name);
+  return WFB_OK;
+}
+
+// Host checks of the int8 cache's entry points.
+int check_kv_i8(const char* name, const wfb_kv_i8* c, int64_t batch, int64_t num_kv_heads, int64_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return fail(WFB_EINVAL, "%s: head_dim (%lld) must be 64 or 128", name, (long long)head_dim);
+  if (batch < 0 || batch > 65535 || num_kv_heads <= 0 || num_kv_heads > 65535)
+    return fail(WFB_EINVAL, "%s: batch (%lld) must be in 0..65535 and num_kv_heads (%lld) in 1..65535", name,
+                (long long)batch, (long long)num_kv_heads);
+  if (!c) return fail(WFB_EINVAL, "%s: null cache", name);
+  if (c->cap <= 0 || c->cap % WFB_KV_I8_BLOCK != 0 || c->cap > INT32_MAX / head_dim)
+    return fail(WFB_EINVAL, "%s: cache capacity (%lld) must be a positive multiple of %d with capacity*head_dim < 2^31",
+                name, (long long)c->cap, WFB_KV_I8_BLOCK);
+  if (batch == 0) return WFB_OK;
+  if (!c->k || !c->k_scale || !c->v || !c->v_scale) return fail(WFB_EINVAL, "%s: null cache pointer", name);
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))
+    return fail(WFB_EINVAL, "%s: cache pointers must be 16-byte aligned", name);
+  return WFB_OK;
+}
+
+// The new rows of a call and where they go; fills the span.
+int check_kv_new(const char* name, const void* k_new, int64_t ldk, const void* v_new, int64_t ldv, int dtype,
+                 const float* rope_cos, const float* rope_sin, int64_t rope_len, int64_t turn, const wfb_kv_i8* c,
+                 const int64_t* start_dev, int64_t start, const int64_t* lengths_dev, int64_t batch, int64_t t,
+                 int64_t num_kv_heads, int64_t head_dim, wfb::KvSpan& span) {
+  if (dtype != WFB_F32 && dtype != WFB_BF16) return fail(WFB_EINVAL, "%s: dtype must be WFB_F32 or WFB_BF16", name);
+  const int64_t per16 = dtype == WFB_F32 ? 4 : 8;
+  if (t < 0 || t > (1 << 24)) return fail(WFB_EINVAL, "%s: T (%lld) must be in 0..2^24", name, (long long)t);
+  if (ldk < num_kv_heads * head_dim || ldv < num_kv_heads * head_dim || ldk % per16 || ldv % per16)
+    return fail(WFB_EINVAL, "%s: key and value row strides must cover num_kv_heads*head_dim and be multiples of 16 bytes",
+                name);
+  if ((rope_cos == nullptr) != (rope_sin == nullptr))
+    return fail(WFB_EINVAL, "%s: rope_cos and rope_sin must both be given or both be NULL", name);
+  if (turn < 0 || turn > INT32_MAX) return fail(WFB_EINVAL, "%s: the prefix length (%lld) must be in 0..2^31-1", name, (long long)turn);
+  int64_t limit = c->cap;
+  if (rope_cos) limit = std::min(limit, rope_len - turn);
+  if (!start_dev && (start < 0 || start > limit - t))
+    return fail(WFB_EINVAL, "%s: start (%lld) + T (%lld) must be within the cache (%lld) and, behind the prefix, the "
+                "rotary tables (%lld)", name, (long long)start, (long long)t, (long long)c->cap, (long long)rope_len);
+  span = wfb::KvSpan{start_dev, start, lengths_dev, t, limit};
+  if (batch == 0 || t == 0) return WFB_OK;
+  if (!k_new || !v_new) return fail(WFB_EINVAL, "%s: null pointer", name);
+  if (!aligned(k_new, 16) || !aligned(v_new, 16) || !aligned(rope_cos, 16) || !aligned(rope_sin, 16))
+    return fail(WFB_EINVAL, "%s: keys, values and the rotary tables must be 16-byte aligned", name);
   return WFB_OK;
 }
 }  // namespace
@@ -693,6 +738,107 @@ int wfb_rope_tables(double theta, int64_t head_dim, int64_t max_len, float* cos_
     }
   }
   return ok();
+}
+
+int wfb_kv_write_i8(const void* k_new, int64_t ldk, const void* v_new, int64_t ldv, int dtype, const float* rope_cos,
+                    const float* rope_sin, int64_t rope_len, int64_t turn, const wfb_kv_i8* cache,
+                    const int64_t* start_dev, int64_t start, const int64_t* lengths_dev, int64_t batch, int64_t t,
+                    int64_t num_kv_heads, int64_t head_dim, void* stream) {
+  const char* name = "wfb_kv_write_i8";
+  int st = check_kv_i8(name, cache, batch, num_kv_heads, head_dim);
+  if (st != WFB_OK) return st;
+  wfb::KvSpan span;
+  st = check_kv_new(name, k_new, ldk, v_new, ldv, dtype, rope_cos, rope_sin, rope_len, turn, cache, start_dev, start,
+                    lengths_dev, batch, t, num_kv_heads, head_dim, span);
+  if (st != WFB_OK) return st;
+  if (batch == 0 || t == 0) return ok();
+  return hip_status(wfb::launch_kv_write_i8(dtype, (int)head_dim, k_new, ldk, v_new, ldv, rope_cos, rope_sin, turn,
+                                            *cache, span, (int)batch, (int)num_kv_heads, as_stream(stream)),
+                    name);
+}
+
+int wfb_kv_read_i8(const wfb_kv_i8* cache, const int64_t* start_dev, int64_t start, int64_t batch, int64_t count,
+                   int64_t num_kv_heads, int64_t head_dim, void* k_out, void* v_out, int dtype, void* stream) {
+  const char* name = "wfb_kv_read_i8";
+  const int st = check_kv_i8(name, cache, batch, num_kv_heads, head_dim);
+  if (st != WFB_OK) return st;
+  if (dtype != WFB_F32 && dtype != WFB_BF16) return fail(WFB_EINVAL, "%s: dtype must be WFB_F32 or WFB_BF16", name);
+  if (count < 0 || count > (1 << 24)) return fail(WFB_EINVAL, "%s: count (%lld) must be in 0..2^24", name, (long long)count);
+  if (batch == 0 || count == 0) return ok();
+  if (!k_out || !v_out) return fail(WFB_EINVAL, "%s: null pointer", name);
+  if (!aligned(k_out, 16) || !aligned(v_out, 16)) return fail(WFB_EINVAL, "%s: outputs must be 16-byte aligned", name);
+  return hip_status(wfb::launch_kv_read_i8(dtype, (int)head_dim, *cache, start_dev, start, (int)batch, count,
+                                           (int)num_kv_heads, k_out, v_out, as_stream(stream)),
+                    name);
+}
+
+static int check_heads_i8(const char* name, int64_t num_heads, int64_t num_kv_heads) {
+  if (num_heads <= 0 || num_heads % num_kv_heads != 0 || num_heads / num_kv_heads > 16)
+    return fail(WFB_EINVAL, "%s: num_heads (%lld) must be 1..16 times num_kv_heads (%lld)", name, (long long)num_heads,
+                (long long)num_kv_heads);
+  return WFB_OK;
+}
+
+int wfb_gqa_attention_i8_workspace(int64_t batch, int64_t t, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                   int64_t cap, int64_t prefix_len, int64_t* floats) {
+  const char* name = "wfb_gqa_attention_i8_workspace";
+  const wfb_kv_i8 c{nullptr, nullptr, nullptr, nullptr, cap};
+  int st = check_kv_i8(name, &c, 0, num_kv_heads, head_dim);
+  if (st == WFB_OK) st = check_heads_i8(name, num_heads, num_kv_heads);
+  if (st != WFB_OK) return st;
+  if (batch < 0 || batch > 65535 || t < 0 || t > (1 << 24) || prefix_len < 0 || prefix_len > INT32_MAX)
+    return fail(WFB_EINVAL, "%s: batch (%lld), T (%lld) or prefix length (%lld) out of range", name, (long long)batch,
+                (long long)t, (long long)prefix_len);
+  if (!floats) return fail(WFB_EINVAL, "%s: null pointer", name);
+  *floats = batch == 0 || t == 0
+                ? 0
+                : wfb::kv_attn_workspace_floats(batch, t, num_heads, num_kv_heads, head_dim, cap, prefix_len);
+  return ok();
+}
+
+int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t ldk, const void* v_new, int64_t ldv,
+                         int dtype, const float* rope_cos, const float* rope_sin, int64_t rope_len,
+                         const wfb_kv_i8* cache, const int64_t* start_dev, int64_t start, const int64_t* lengths_dev,
+                         const wfb_kv_i8* prefix, int64_t prefix_len, int64_t batch, int64_t t, int64_t num_heads,
+                         int64_t num_kv_heads, int64_t head_dim, float scale, void* out, int64_t ldo, float* workspace,
+                         void* stream) {
+  const char* name = "wfb_gqa_attention_i8";
+  int st = check_kv_i8(name, cache, batch, num_kv_heads, head_dim);
+  if (st == WFB_OK) st = check_heads_i8(name, num_heads, num_kv_heads);
+  if (st != WFB_OK) return st;
+  if (prefix_len < 0 || (prefix_len > 0 && !prefix))
+    return fail(WFB_EINVAL, "%s: prefix length (%lld) without a prefix", name, (long long)prefix_len);
+  if (prefix && prefix_len > 0) {
+    st = check_kv_i8(name, prefix, batch > 0 ? 1 : 0, num_kv_heads, head_dim);
+    if (st != WFB_OK) return st;
+    if (prefix_len > prefix->cap)
+      return fail(WFB_EINVAL, "%s: prefix length (%lld) exceeds the prefix's capacity (%lld)", name,
+                  (long long)prefix_len, (long long)prefix->cap);
+  }
+  wfb::KvAttn a{};
+  st = check_kv_new(name, k_new, ldk, v_new, ldv, dtype, rope_cos, rope_sin, rope_len, prefix_len, cache, start_dev,
+                    start, lengths_dev, batch, t, num_kv_heads, head_dim, a.span);
+  if (st != WFB_OK) return st;
+  const int64_t per16 = dtype == WFB_F32 ? 4 : 8;
+  if (ldq < num_heads * head_dim || ldo < num_heads * head_dim || ldq % per16 || ldo % per16)
+    return fail(WFB_EINVAL, "%s: q and out row strides must cover num_heads*head_dim and be multiples of 16 bytes", name);
+  if (!std::isfinite(scale)) return fail(WFB_EINVAL, "%s: scale must be finite", name);
+  if (batch * t * num_heads > INT32_MAX)
+    return fail(WFB_EINVAL, "%s: batch*T*num_heads (%lld) must be < 2^31", name, (long long)(batch * t * num_heads));
+  if (batch == 0 || t == 0) return ok();
+  if (!q || !out) return fail(WFB_EINVAL, "%s: null pointer", name);
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16))
+    return fail(WFB_EINVAL, "%s: q, out and workspace must be 16-byte aligned", name);
+  if (!workspace &&
+      wfb::kv_attn_workspace_floats(batch, t, num_heads, num_kv_heads, head_dim, cache->cap, prefix_len) > 0)
+    return fail(WFB_EINVAL, "%s: these sizes need a workspace", name);
+  a.q = q, a.ldq = ldq, a.kn = k_new, a.ldk = ldk, a.vn = v_new, a.ldv = ldv, a.rc = rope_cos, a.rs = rope_sin;
+  a.own = *cache;
+  if (prefix_len > 0) a.pre = *prefix;
+  a.npre = prefix_len;
+  a.b = (int)batch, a.t = (int)t, a.hq = (int)num_heads, a.hkv = (int)num_kv_heads, a.d = (int)head_dim, a.dt = dtype;
+  a.scale = scale, a.out = out, a.ldo = ldo, a.ws = workspace;
+  return hip_status(wfb::launch_kv_attention(a, as_stream(stream)), name);
 }
 
 }  // extern "C"

@@ -18,13 +18,13 @@ import collections
 import contextlib
 import ctypes
 import weakref
-from typing import Optional, Sequence, Tuple, Union
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
 from ._lib import (WFB_ABSMEAN_WS_DOUBLES, WFB_ACT_RELU2, WFB_ACT_SILU, WFB_BF16, WFB_F16, WFB_F32,
-                   WFB_MAX_SEGMENTS, WFB_QK_I2S, WFB_SCALE_CHECKPOINT, WFB_SCALE_REFERENCE)
+                   WFB_KV_I8_BLOCK, WFB_MAX_SEGMENTS, WFB_QK_I2S, WFB_SCALE_CHECKPOINT, WFB_SCALE_REFERENCE)
 
 QK_I2_S = WFB_QK_I2S
 
@@ -984,6 +984,210 @@ def gqa_prefill_attention(
             _stream(dev),
         )
     return out
+
+
+# ---- int8 key/value cache -----------------------------------------------------------------------
+
+
+class KVCacheI8(NamedTuple):
+    """A key/value cache of int8 codes with an fp32 scale per (token, kv head), half the bytes of a bf16 cache: ``k``
+    int8 [batch, kv_heads, cap, head_dim], ``v`` int8 [batch, kv_heads, cap / 64, head_dim, 64] (blocks of 64 keys,
+    transposed), ``k_scale`` and ``v_scale`` fp32 [batch, kv_heads, cap].  The ops take any four such tensors in this
+    order."""
+
+    k: torch.Tensor
+    k_scale: torch.Tensor
+    v: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def kv_cache_i8(batch: int, kv_heads: int, max_len: int, head_dim: int, device="cuda") -> KVCacheI8:
+    """A zeroed int8 cache for ``max_len`` keys per sequence, rounded up to a multiple of 64."""
+    cap = -(-int(max_len) // WFB_KV_I8_BLOCK) * WFB_KV_I8_BLOCK
+    if head_dim not in (64, 128) or batch < 1 or kv_heads < 1 or max_len < 1:
+        raise ValueError("kv_cache_i8: sizes must be positive and head_dim 64 or 128")
+    z = lambda dt, *shape: torch.zeros(shape, dtype=dt, device=device)  # noqa: E731
+    return KVCacheI8(z(torch.int8, batch, kv_heads, cap, head_dim), z(torch.float32, batch, kv_heads, cap),
+                     z(torch.int8, batch, kv_heads, cap // WFB_KV_I8_BLOCK, head_dim, WFB_KV_I8_BLOCK),
+                     z(torch.float32, batch, kv_heads, cap))
+
+
+def _cache_i8(name: str, what: str, cache) -> Tuple["_lib.KvI8Struct", int, int, int, int]:
+    """(C struct, batch, kv_heads, cap, head_dim) of the four tensors of an int8 cache."""
+    if len(cache) != 4:
+        raise RuntimeError(f"{name}: {what} must be the four tensors k, k_scale, v, v_scale")
+    k, ks, v, vs = cache
+    if k.dim() != 4 or k.dtype != torch.int8 or v.dtype != torch.int8 or ks.dtype != torch.float32 \
+            or vs.dtype != torch.float32:
+        raise RuntimeError(f"{name}: {what} must hold int8 codes [batch, kv_heads, cap, head_dim] and fp32 scales")
+    b, h, cap, d = k.shape
+    if cap % WFB_KV_I8_BLOCK or v.shape != (b, h, cap // WFB_KV_I8_BLOCK, d, WFB_KV_I8_BLOCK) \
+            or ks.shape != (b, h, cap) or vs.shape != (b, h, cap):
+        raise RuntimeError(f"{name}: {what}'s tensors do not belong together: {[tuple(t.shape) for t in cache]}")
+    return _lib.KvI8Struct(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), cap), b, h, cap, d
+
+
+def _per_sequence(name: str, what: str, x, b: int, dev: torch.device) -> Tuple[Optional[int], int]:
+    """(device pointer or None, host value) of an int or an int64 device tensor [batch]."""
+    if not isinstance(x, torch.Tensor):
+        return None, int(x)
+    if x.dtype != torch.int64 or x.numel() != b or x.device != dev or not x.is_contiguous():
+        raise RuntimeError(f"{name}: {what} must be an int or contiguous int64 [{b}] on {dev}")
+    return x.data_ptr(), 0
+
+
+def _rows16(name: str, x: torch.Tensor, rows: int, width: int, dtype: torch.dtype, dev: torch.device):
+    """(view or copy of x as [rows, width], row stride) with rows that start on 16 bytes."""
+    if x.dtype != dtype or x.device != dev or x.numel() != rows * width:
+        raise RuntimeError(f"{name}: expected {rows} x {width} elements of {dtype} on {dev}, got {tuple(x.shape)} "
+                           f"{x.dtype} on {x.device}")
+    x2 = x if x.dim() == 2 and x.shape[0] == rows else x.reshape(rows, width)
+    per16 = 16 // x2.element_size()
+    ld = x2.stride(0) if rows > 1 else width
+    if x2.stride(1) != 1 or ld % per16 or x2.data_ptr() % 16 or ld < width:
+        x2 = torch.empty((rows, width), dtype=dtype, device=dev).copy_(x2)
+        ld = width
+    return x2, ld
+
+
+def _rope_i8(name: str, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], d: int, dev: torch.device):
+    """(cos, sin, rows) of the rotary tables, which may be longer than the cache."""
+    if cos is None and sin is None:
+        return None, None, 0
+    if cos is None or sin is None:
+        raise RuntimeError(f"{name}: give both rope tables or neither")
+    for x in (cos, sin):
+        if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != d // 2 or x.device != dev \
+                or not x.is_contiguous() or x.shape != cos.shape:
+            raise RuntimeError(f"{name}: rope tables must be contiguous fp32 [positions, {d // 2}] on {dev}")
+    if cos.data_ptr() % 16 or sin.data_ptr() % 16:
+        cos, sin = cos.clone(), sin.clone()
+    return cos, sin, cos.shape[0]
+
+
+def kv_cache_write_i8(
+    k_new: torch.Tensor, v_new: torch.Tensor, cache: Sequence[torch.Tensor], start: Union[int, torch.Tensor], t: int,
+    rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None, rope_offset: int = 0,
+) -> None:
+    """Quantising write of a chunk of t tokens per sequence into an int8 cache at positions start .. start + t - 1, the
+    keys after the rotary embedding.
+
+    k_new / v_new [batch*t, kv_heads*head_dim] float32 or bfloat16, token-major (column slices of one q|k|v output do).
+    ``start``: an int, or int64 [batch] on the device; ``lengths``: int64 [batch] on the device, the tokens of each
+    sequence that are real (t by default); a sequence whose positions do not fit is not written (a start given as an int
+    is checked here).  Position p takes row p + rope_offset of the tables."""
+    name = "kv_cache_write_i8"
+    st, b, h, _, d = _cache_i8(name, "cache", cache)
+    dev = _require_gpu(name, *cache)
+    t = int(t)
+    k2, ldk = _rows16(name, k_new, b * t, h * d, k_new.dtype, dev)
+    v2, ldv = _rows16(name, v_new, b * t, h * d, k_new.dtype, dev)
+    cos, sin, n_rope = _rope_i8(name, rope_cos, rope_sin, d, dev)
+    s_dev, s_host = _per_sequence(name, "start", start, b, dev)
+    l_dev = None if lengths is None else _per_sequence(name, "lengths", lengths, b, dev)[0]
+    with _on(dev):
+        _lib.call("wfb_kv_write_i8", _p(k2), ldk, _p(v2), ldv, _float_dtype(name, k2), _p(cos), _p(sin), n_rope,
+                  int(rope_offset), ctypes.addressof(st), s_dev, s_host, l_dev, b, t, h, d, _stream(dev))
+
+
+def kv_cache_read_i8(
+    cache: Sequence[torch.Tensor], start: Union[int, torch.Tensor], count: int, dtype: torch.dtype = torch.bfloat16,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [batch, kv_heads, count, head_dim] of ``dtype`` (float32 or bfloat16): what an int8 cache holds at positions
+    start .. start + count - 1 (``start`` an int or int64 [batch] on the device); zeros outside the cache."""
+    name = "kv_cache_read_i8"
+    st, b, h, _, d = _cache_i8(name, "cache", cache)
+    dev = _require_gpu(name, *cache)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{name}: dtype must be float32 or bfloat16, got {dtype}")
+    s_dev, s_host = _per_sequence(name, "start", start, b, dev)
+    k = torch.empty((b, h, int(count), d), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with _on(dev):
+        _lib.call("wfb_kv_read_i8", ctypes.addressof(st), s_dev, s_host, b, int(count), h, d, _p(k), _p(v), _DT[dtype],
+                  _stream(dev))
+    return k, v
+
+
+def _attention_i8(name, q, k_new, v_new, cache, start, t, rope_cos, rope_sin, scale, out, lengths, prefix, prefix_len):
+    st, b, h, cap, d = _cache_i8(name, "cache", cache)
+    dev = _require_gpu(name, *cache)
+    rows = b * t
+    prefix_len = int(prefix_len)
+    pst = None
+    if prefix is not None:
+        pst, pb, ph, _, pd = _cache_i8(name, "prefix", prefix)
+        if pb != 1 or ph != h or pd != d or _require_gpu(name, *prefix) != dev:
+            raise RuntimeError(f"{name}: prefix must be an int8 cache of one sequence with {h} kv heads of {d} on {dev}")
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{name}: dtype must be float32 or bfloat16, got {q.dtype}")
+    if rows == 0:
+        return q.new_empty((0, q.shape[-1])) if out is None else out
+    if q.numel() % (rows * d) != 0:
+        raise RuntimeError(f"{name}: q has {q.numel()} elements, not a multiple of {rows} rows of head_dim")
+    hq = q.numel() // (rows * d)
+    q2, ldq = _rows16(name, q, rows, hq * d, q.dtype, dev)
+    k2, ldk = _rows16(name, k_new, rows, h * d, q.dtype, dev)
+    v2, ldv = _rows16(name, v_new, rows, h * d, q.dtype, dev)
+    cos, sin, n_rope = _rope_i8(name, rope_cos, rope_sin, d, dev)
+    s_dev, s_host = _per_sequence(name, "start", start, b, dev)
+    l_dev = None if lengths is None else _per_sequence(name, "lengths", lengths, b, dev)[0]
+    if out is not None and (out.dtype != q.dtype or out.shape != (rows, hq * d) or out.device != dev):
+        raise RuntimeError(f"{name}: out must be [{rows}, {hq * d}] {q.dtype} on {dev}")
+    o2 = out
+    if out is None or out.stride(1) != 1 or out.data_ptr() % 16 \
+            or (rows > 1 and (out.stride(0) * out.element_size() % 16 or out.stride(0) < hq * d)):
+        o2 = torch.empty((rows, hq * d), dtype=q.dtype, device=dev)
+    ldo = o2.stride(0) if rows > 1 else hq * d
+    size = ctypes.c_int64(0)
+    _lib.call("wfb_gqa_attention_i8_workspace", b, t, hq, h, d, cap, prefix_len, ctypes.addressof(size))
+    work = torch.empty(size.value, dtype=torch.float32, device=dev) if size.value else None
+    sc = 1.0 / float(d) ** 0.5 if scale is None else float(scale)
+    with _on(dev):
+        _lib.call("wfb_gqa_attention_i8", _p(q2), ldq, _p(k2), ldk, _p(v2), ldv, _DT[q.dtype], _p(cos), _p(sin), n_rope,
+                  ctypes.addressof(st), s_dev, s_host, l_dev, None if pst is None else ctypes.addressof(pst),
+                  prefix_len, b, t, hq, h, d, sc, _p(o2), ldo, _p(work), _stream(dev))
+    if out is None:
+        return o2
+    return out if o2 is out else out.copy_(o2)
+
+
+def gqa_decode_attention_i8(
+    q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: Sequence[torch.Tensor], pos: torch.Tensor,
+    rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None, prefix: Optional[Sequence[torch.Tensor]] = None, prefix_len: int = 0,
+) -> torch.Tensor:
+    """``gqa_decode_attention`` over an int8 cache (``kv_cache_i8``): rotary embedding of q / k_new, quantising append at
+    pos[b], attention over positions 0..pos[b] as the cache holds them.  Returns out [batch, num_heads * head_dim].
+
+    q, k_new, v_new float32 or bfloat16, rows as for ``gqa_decode_attention``; up to 16 query heads per kv head; rope
+    tables fp32 [positions, head_dim/2], as long as the positions need.  ``prefix``: an int8 cache of one sequence whose
+    first ``prefix_len`` keys precede every sequence's own (a shared prompt, read once for the whole batch); ``pos`` stays
+    the position in the sequence's own cache, the rotary embedding takes row prefix_len + pos.  A position outside the
+    cache or the tables gives a NaN row and leaves the cache as it is."""
+    name = "gqa_decode_attention_i8"
+    if not isinstance(pos, torch.Tensor):
+        raise RuntimeError(f"{name}: pos must be int64 [batch] on the device")
+    return _attention_i8(name, q, k_new, v_new, cache, pos, 1, rope_cos, rope_sin, scale, out, None, prefix, prefix_len)
+
+
+def gqa_prefill_attention_i8(
+    q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: Sequence[torch.Tensor],
+    start: Union[int, torch.Tensor], t: int, rope_cos: Optional[torch.Tensor] = None,
+    rope_sin: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None, prefix: Optional[Sequence[torch.Tensor]] = None, prefix_len: int = 0,
+) -> torch.Tensor:
+    """``gqa_prefill_attention`` over an int8 cache: a chunk of t tokens per sequence, appended at positions start ..
+    start + t - 1 and causal over what the cache then holds, so a prompt gives the same cut into any chunks.  Returns
+    out [batch*t, num_heads*head_dim] (row b*t + i).
+
+    ``start``: an int, or int64 [batch] on the device; ``lengths``: int64 [batch] on the device for a batch padded to t
+    tokens: sequence b has lengths[b] of them, the rows behind are zeros and nothing is written for them.  A sequence
+    that does not fit the cache or the rope tables gives NaN rows and is not written (a ``start`` given as an int is
+    checked here instead).  ``prefix`` / ``prefix_len`` and the types as for ``gqa_decode_attention_i8``."""
+    return _attention_i8("gqa_prefill_attention_i8", q, k_new, v_new, cache, start, int(t), rope_cos, rope_sin, scale,
+                         out, lengths, prefix, prefix_len)
 
 
 def bitnet_gemv(packed_weights: torch.Tensor, activations: torch.Tensor, scale: Scale) -> torch.Tensor:
