@@ -6,101 +6,940 @@ namespace wfb {
 
 namespace {
 
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr int kThreads = 256;
+constexpr float kNoMax = -1e30f;  // running maximum of a row that has met no key: finite, so that no difference is NaN
+constexpr float kLog2e = 1.4426950408889634f;
+
 template <int DT>
 __device__ __forceinline__ void store_elem(void* p, int64_t i, float v) {
   if constexpr (DT == WFB_F32) reinterpret_cast<float*>(p)[i] = v;
   else reinterpret_cast<uint16_t*>(p)[i] = f32_to_bf16_rne(v);
 }
 
-// One workgroup per (query head, token): scores of 256 keys at a time, a running softmax, the weighted sum of values
-// with the threads over (element, key residue).
-template <int DT, int D>
-__global__ __launch_bounds__(256) void kv_attention_kernel(KvAttn a) {
-  constexpr int HD = D / 2, NG = 256 / D;
-  __shared__ float qs[D], ps[256], red[4], acc_s[NG][D];
-  const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
-  const int64_t row = (int64_t)b * a.t + i;
-  int64_t first;
-  int n;
-  const bool fits = kv_span(a.span, b, first, n);
-  if (!fits || i >= n) {
-    if (t < D) store_elem<DT>(a.out, row * a.ldo + (int64_t)h * D + t, fits ? 0.0f : __builtin_nanf(""));
-    return;
+template <int DT>
+__device__ __forceinline__ void store4(void* p, int64_t i, const float (&v)[4]) {
+  if constexpr (DT == WFB_F32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    const bf16x2_t lo = __builtin_convertvector((f32x2_t){v[0], v[1]}, bf16x2_t);
+    const bf16x2_t hi = __builtin_convertvector((f32x2_t){v[2], v[3]}, bf16x2_t);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) =
+        make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
   }
-  const int64_t pos = first + i;
-  const int kvh = h / (a.hq / a.hkv);
-  if (t < HD) {
-    float x1 = load_elem<DT>(a.q, row * a.ldq + (int64_t)h * D + t);
-    float x2 = load_elem<DT>(a.q, row * a.ldq + (int64_t)h * D + t + HD);
-    if (a.rc) {
-      const float cs = a.rc[(pos + a.npre) * HD + t], sn = a.rs[(pos + a.npre) * HD + t];
-      const float y1 = __fsub_rn(__fmul_rn(x1, cs), __fmul_rn(x2, sn));
-      x2 = __fadd_rn(__fmul_rn(x2, cs), __fmul_rn(x1, sn));
-      x1 = y1;
+}
+
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  v = umax(v, (uint32_t)xor_lanes<32>((int)v));
+  v = umax(v, (uint32_t)xor_lanes<16>((int)v));
+  v = umax(v, (uint32_t)xor_lanes<8>((int)v));
+  v = umax(v, (uint32_t)xor_lanes<4>((int)v));
+  v = umax(v, (uint32_t)xor_lanes<2>((int)v));
+  return umax(v, (uint32_t)xor_lanes<1>((int)v));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += xor_lanes_f32<32>(v);
+  v += xor_lanes_f32<16>(v);
+  v += xor_lanes_f32<8>(v);
+  v += xor_lanes_f32<4>(v);
+  v += xor_lanes_f32<2>(v);
+  return v + xor_lanes_f32<1>(v);
+}
+
+// ---- plan ---------------------------------------------------------------------------------------
+
+// How a call is cut: `own` workgroups along the sequences' own keys and `pre` along the prefix's, whose partial results
+// (unnormalised output, running maximum, sum of weights) a last kernel joins; own = 1 without prefix needs none.
+struct Plan {
+  int own, pre;
+  bool decode;    // one token per sequence: decode kernel, else the rows kernel
+  bool pre_rows;  // the prefix by the rows kernel
+};
+
+constexpr int kLive = 768;          // workgroups that a cut call aims at: three per CU
+constexpr int kRowsPerGroup = 128;  // rows (token, query head) of one workgroup of the rows kernel
+constexpr int kColumns = 16;        // rows of one workgroup of the decode kernel
+
+int cut(int64_t groups, int64_t target, int64_t most) {
+  const int64_t n = (target + groups - 1) / groups;
+  return (int)(n < 1 ? 1 : n > most ? most : n);
+}
+
+Plan make_plan(int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t cap, int64_t npre, bool lengths) {
+  const int64_t g = hq / hkv, pb = (npre + kKvBlock - 1) / kKvBlock, cb = cap / kKvBlock;
+  Plan p{};
+  p.decode = t == 1 && !lengths;
+  if (p.decode) {
+    p.own = cut(b * hkv, kLive, (cb + 3) / 4);
+    if (npre > 0) {
+      const int64_t rows = b * g;
+      p.pre_rows = rows > 64;
+      if (p.pre_rows) p.pre = cut(hkv * ((rows + kRowsPerGroup - 1) / kRowsPerGroup), 512, (pb + 3) / 4);
+      else p.pre = cut(hkv * ((rows + kColumns - 1) / kColumns), kLive, (pb + 3) / 4);
     }
-    qs[t] = x1 * a.scale;
-    qs[t + HD] = x2 * a.scale;
+  } else {
+    const int64_t groups = b * hkv * ((t * g + kRowsPerGroup - 1) / kRowsPerGroup);
+    p.own = groups >= 192 ? 1 : cut(groups, 512, (pb + cb + 3) / 4);
+  }
+  return p;
+}
+
+bool has_parts(const Plan& p) { return p.own > 1 || p.pre > 0; }
+
+// Partials: unnormalised outputs [slots][rows][D], then maximum and sum [slots][rows]; row = (b * t + i) * hq + h.
+struct Parts {
+  float* o;
+  float2* ml;
+  int64_t rows;
+};
+
+Parts parts_of(const KvAttn& a, const Plan& p) {
+  Parts r{nullptr, nullptr, (int64_t)a.b * a.t * a.hq};
+  if (has_parts(p)) {
+    r.o = a.ws;
+    r.ml = reinterpret_cast<float2*>(a.ws + (int64_t)(p.own + p.pre) * r.rows * a.d);
+  }
+  return r;
+}
+
+// Blocks of 64 keys per split, in whole rounds of the four waves, when nb blocks are cut into at most n.
+__device__ __forceinline__ int64_t split_blocks(int64_t nb, int n) { return ((nb + n - 1) / n + 3) / 4 * 4; }
+
+// ---- decode: few rows -----------------------------------------------------------------------------
+
+// Up to 16 rows (query heads of one kv head; behind a prefix also of several sequences) against the keys of a split, a
+// 64-key block per wave at a time, straight from the cache into the matrix cores as they are stored:
+//   S^T[key, row] = K Q^T        v_mfma_i32_16x16x64_i8, the query as NP signed base-256 digits of a fixed-point row
+//   w = exp2(s - m) * v_scale    fp32, running maximum per row
+//   O^T[d, row] = V^T W^T        the same instruction, w as NP digits of its block's largest in the row
+// The products are exact; a block's sums of V^T W^T come to less than 2^31 (127 * 2^15 * 64 < 2^28) and are added up in fp32.
+// The key that row R of score tile n stands for is chosen as 16 (R / 4) + 4 n + R % 4: a lane then holds 16 consecutive
+// keys, the ones that it feeds into the second product.
+template <int NP>
+struct Digits;
+template <>
+struct Digits<2> {
+  static constexpr float kMax = 127.0f * 256.0f;
+};
+template <>
+struct Digits<3> {
+  static constexpr float kMax = 127.0f * 65536.0f;
+};
+
+// Signed digits of four fixed-point numbers |x| <= Digits<NP>::kMax, packed, the most significant first: adding 0x80 to
+// every lower byte carries a digit over 127 into the next one, and the byte less 128 is the digit.
+template <int NP>
+__device__ __forceinline__ void digits4(const int (&x)[4], uint32_t (&d)[NP]) {
+  constexpr uint32_t bias = NP == 2 ? 0x80u : 0x8080u;
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = (uint32_t)x[i] + bias;
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    const uint32_t byte = NP - 1 - n;
+    const uint32_t sel = byte | (byte + 4) << 8 | 0x0c0c0000u;  // byte of both sources, two zeros
+    const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], sel), hi = __builtin_amdgcn_perm(u[3], u[2], sel);
+    d[n] = (lo | hi << 16) ^ (n == 0 ? 0u : 0x80808080u);
+  }
+}
+
+template <int DT, int D, bool PREFIX>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void kv_decode_kernel(KvAttn a, Parts parts, int slot0, int nsplit) {
+  constexpr int NP = DT == WFB_F32 ? 3 : 2;
+  constexpr int HD = D / 2, KS = D / 64, DTL = D / 16;
+  constexpr float QM = Digits<NP>::kMax;
+  __shared__ float qs[kColumns][D];
+  __shared__ __attribute__((aligned(16))) uint8_t qd[NP][kColumns][D];
+  __shared__ float qscale[kColumns];
+  __shared__ float kvn[2][D];        // the new key and value, then what the cache holds for them
+  __shared__ float snew[kColumns];
+  __shared__ float red[4][kColumns][D];
+  __shared__ float mw[4][kColumns], lw[4][kColumns];
+
+  const int kvh = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int g = a.hq / a.hkv;
+  const int split = blockIdx.z;
+  const int grp = lane >> 4, col = lane & 15;
+  // rows of this workgroup: the heads of one sequence, or the next 16 of all sequences' (sequence, head) pairs
+  const int b0 = PREFIX ? 0 : blockIdx.y, r0 = PREFIX ? (int)blockIdx.y * kColumns : 0;
+  const int nrows = PREFIX ? (a.b * g - r0 < kColumns ? a.b * g - r0 : kColumns) : g;
+  int64_t pos = 0;
+  int n1 = 1;
+  if constexpr (!PREFIX) {
+    if (!kv_span(a.span, b0, pos, n1)) {  // uniform: the rows are flagged, here or by the joining kernel
+      if (!parts.o)
+        for (int i = t; i < g * D; i += kThreads)
+          store_elem<DT>(a.out, (int64_t)b0 * a.ldo + (int64_t)kvh * g * D + i, __builtin_nanf(""));
+      return;
+    }
+  }
+  const int64_t keys = PREFIX ? a.npre : pos;  // read from the cache
+  const int64_t nb = (keys + kKvBlock - 1) / kKvBlock, per = split_blocks(nb, nsplit);
+  const int64_t kb0 = split * per, kb1 = kb0 + per < nb ? kb0 + per : nb;
+  if (split > 0 && kb0 >= nb) return;  // (split 0 of a sequence without older keys takes the new one)
+  const bool owns_new = !PREFIX && kb1 == nb;
+
+  const wfb_kv_i8& c = PREFIX ? a.pre : a.own;
+  const int64_t base = PREFIX ? kvh : (int64_t)b0 * a.hkv + kvh;
+  const int8_t* kp = c.k + base * c.cap * D;
+  const int8_t* vp = c.v + base * c.cap * D;
+  // codes behind the last key are met with weights of zero; scales there read as zeros
+  const buf_t ksb = make_buf(c.k_scale + base * c.cap, (uint32_t)(keys * 4));
+  const buf_t vsb = make_buf(c.v_scale + base * c.cap, (uint32_t)(keys * 4));
+
+  v4i kf[4][KS], vf[DTL], sk[4], sv[4];
+  auto load_k = [&](int64_t kb) {
+    const buf_t p = make_buf(kp + kb * kKvBlock * D, kKvBlock * D);
+    const int off = (16 * (col >> 2) + (col & 3)) * D + 16 * grp;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[n][s] = buf_load16(p, off + 4 * n * D + 64 * s);
+  };
+  auto load_v = [&](int64_t kb) {
+    const buf_t p = make_buf(vp + kb * kKvBlock * D, kKvBlock * D);
+    const int off = col * kKvBlock + 16 * grp;
+#pragma unroll
+    for (int d = 0; d < DTL; ++d) vf[d] = buf_load16(p, off + 16 * d * kKvBlock);
+  };
+  auto load_s = [&](int64_t kb) {
+    const uint32_t off = (uint32_t)(kb * kKvBlock + 16 * grp) * 4;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sk[n] = buf_load16(ksb, off + 16 * n);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sv[n] = buf_load16(vsb, off + 16 * n);
+  };
+  int64_t kb = kb0 + w;
+  if (kb < kb1) {
+    load_k(kb);
+    load_s(kb);
+    load_v(kb);
+  }
+
+  // ---- the rows' queries, the new key and value
+  auto turn_pair = [&](float& x1, float& x2, int64_t p, int j) {
+    if (!a.rc) return;
+    const float cs = a.rc[p * HD + j], sn = a.rs[p * HD + j];
+    const float y1 = __fsub_rn(__fmul_rn(x1, cs), __fmul_rn(x2, sn));
+    x2 = __fadd_rn(__fmul_rn(x2, cs), __fmul_rn(x1, sn));
+    x1 = y1;
+  };
+  for (int i = t; i < nrows * HD; i += kThreads) {
+    const int r = i / HD, j = i % HD;
+    const int sb = PREFIX ? (r0 + r) / g : b0, h = kvh * g + (PREFIX ? (r0 + r) % g : r);
+    int64_t p = pos;
+    bool fits = true;
+    if constexpr (PREFIX) fits = kv_span(a.span, sb, p, n1);
+    float x1 = 0.0f, x2 = 0.0f;
+    if (fits) {
+      const int64_t off = (int64_t)sb * a.ldq + (int64_t)h * D + j;
+      x1 = load_elem<DT>(a.q, off);
+      x2 = load_elem<DT>(a.q, off + HD);
+      turn_pair(x1, x2, p + a.npre, j);
+    }
+    qs[r][j] = x1;
+    qs[r][j + HD] = x2;
+  }
+  if (owns_new) {
+    if (t < HD) {
+      const int64_t off = (int64_t)b0 * a.ldk + (int64_t)kvh * D + t;
+      float x1 = load_elem<DT>(a.kn, off), x2 = load_elem<DT>(a.kn, off + HD);
+      turn_pair(x1, x2, pos + a.npre, t);
+      kvn[0][t] = x1;
+      kvn[0][t + HD] = x2;
+    } else if (t >= 128 && t - 128 < D) {
+      kvn[1][t - 128] = load_elem<DT>(a.vn, (int64_t)b0 * a.ldv + (int64_t)kvh * D + t - 128);
+    }
   }
   __syncthreads();
-  float m = -1e30f, l = 0.0f, acc = 0.0f;
-  for (int part = 0; part < 2; ++part) {
-    const wfb_kv_i8& c = part ? a.own : a.pre;
-    const int64_t keys = part ? pos + 1 : a.npre, base = part ? (int64_t)b * a.hkv + kvh : kvh;
-    for (int64_t k0 = 0; k0 < keys; k0 += 256) {
-      const int64_t key = k0 + t;
-      float s = -__builtin_inff();
-      if (key < keys) {
-        const int8_t* kr = c.k + (base * c.cap + key) * D;
-        float dot = 0.0f;
-        for (int e = 0; e < D; ++e) dot += qs[e] * (float)kr[e];
-        s = dot * c.k_scale[base * c.cap + key];
+  for (int r = w; r < kColumns; r += 4) {  // uniform: a wave takes a row
+    float x[D / 64];
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      x[e] = r < nrows ? qs[r][lane + 64 * e] : 0.0f;
+      m = umax(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+    m = wave_umax(m);
+    const float mf = __uint_as_float(m);
+    const bool some = m < 0x7f800000u && mf >= kKvTiny;
+    const float inv = some ? (a.scale < 0.0f ? -QM : QM) / mf : 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      const int q = some ? (int)__builtin_rintf(x[e] * inv) : 0;
+      const uint32_t u = (uint32_t)q + (NP == 2 ? 0x80u : 0x8080u);
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+        qd[n][r][lane + 64 * e] = (uint8_t)((u >> 8 * (NP - 1 - n)) ^ (n == 0 ? 0u : 0x80u));
+    }
+    if (lane == 0)  // one step of the digits in units of the exponent of two; NaN for a row with one
+      qscale[r] = m >= 0x7f800000u ? __builtin_nanf("") : some ? mf * (1.0f / QM) * (fabsf(a.scale) * kLog2e) : 0.0f;
+  }
+  if (owns_new && w < 2) {  // wave 0 the key, wave 1 the value: into the cache, and back as the values it stands for
+    float x[D / 64];
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      x[e] = kvn[w][lane + 64 * e];
+      m = umax(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+    float scale, inv;
+    kv_scale(wave_umax(m), scale, inv);
+    if (lane == 0) (w == 0 ? a.own.k_scale : a.own.v_scale)[base * c.cap + pos] = scale;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      const int j = lane + 64 * e, q = kv_code(x[e], inv);
+      if (w == 0) a.own.k[(base * c.cap + pos) * D + j] = (int8_t)q;
+      else a.own.v[(base * c.cap + pos / kKvBlock * kKvBlock) * D + (int64_t)j * kKvBlock + pos % kKvBlock] = (int8_t)q;
+      kvn[w][j] = (float)q * scale;
+    }
+  }
+  __syncthreads();
+  if (owns_new) {
+    for (int r = w; r < nrows; r += 4) {
+      float p = 0.0f;
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) p += qs[r][lane + 64 * e] * kvn[0][lane + 64 * e];
+      p = wave_sum(p);
+      if (lane == 0) snew[r] = p * (a.scale * kLog2e);
+    }
+  }
+  v4i qf[NP][KS];
+#pragma unroll
+  for (int n = 0; n < NP; ++n)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[n][s] = *reinterpret_cast<const v4i*>(&qd[n][col][64 * s + 16 * grp]);
+  const float cq = qscale[col];
+
+  float o[DTL][4];
+#pragma unroll
+  for (int d = 0; d < DTL; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[d][i] = 0.0f;
+  float m_run = kNoMax, l_run = 0.0f;
+
+  for (; kb < kb1; kb += 4) {
+    const bool more = kb + 4 < kb1;
+    float s[4][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      v4i acc = {0, 0, 0, 0}, low = {0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[n][k], qf[0][k], acc, 0, 0, 0);
+      acc <<= 8;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[n][k], qf[1][k], acc, 0, 0, 0);
+      if constexpr (NP == 3) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) low = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[n][k], qf[2][k], low, 0, 0, 0);
       }
-      float mx = s;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        s[n][i] = (NP == 3 ? __builtin_fmaf((float)acc[i], 256.0f, (float)low[i]) : (float)acc[i]) *
+                  (cq * __int_as_float(sk[n][i]));
+    }
+    if (more) load_k(kb + 4);
+    const int left = (int)(keys - kb * kKvBlock);  // keys of this block that there are
+    if (left < kKvBlock) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * grp + 4 * n + i >= left) s[n][i] = -__builtin_inff();
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[n][i]);
+    mx = fmaxf(mx, xor_lanes_f32<16>(mx));
+    mx = fmaxf(mx, xor_lanes_f32<32>(mx));
+    const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    m_run = m_new;
+    float ps = 0.0f;
+    uint32_t wm = 0;  // the largest weight, as bits: a NaN is larger than any number
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[n][i] - m_new);
+        ps += p;
+        s[n][i] = p * __int_as_float(sv[n][i]);
+        wm = umax(wm, __float_as_uint(s[n][i]));
+      }
+    if (more) load_s(kb + 4);
+    l_run = l_run * alpha + ps;
+    wm = umax(wm, (uint32_t)xor_lanes<16>((int)wm));
+    wm = umax(wm, (uint32_t)xor_lanes<32>((int)wm));
+    // step of the weights' digits; not below 2^-120, so that its inverse is finite (and left NaN)
+    float step = __uint_as_float(wm) * (1.0f / QM);
+    step = step < 0x1p-120f ? 0x1p-120f : step;
+    const float inv = __builtin_amdgcn_rcpf(step);
+    v4i pf[NP];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      int x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (int)__builtin_rintf(s[n][i] * inv);
+      uint32_t dg[NP];
+      digits4<NP>(x, dg);
+#pragma unroll
+      for (int k = 0; k < NP; ++k) pf[k][n] = (int)dg[k];
+    }
+#pragma unroll
+    for (int d = 0; d < DTL; ++d) {
+      v4i acc = {0, 0, 0, 0}, low = {0, 0, 0, 0};
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[d], pf[0], acc, 0, 0, 0);
+      acc <<= 8;
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[d], pf[1], acc, 0, 0, 0);
+      if constexpr (NP == 3) low = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[d], pf[2], low, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = NP == 3 ? __builtin_fmaf((float)acc[i], 256.0f, (float)low[i]) : (float)acc[i];
+        o[d][i] = __builtin_fmaf(o[d][i], alpha, x * step);
+      }
+    }
+    if (more) load_v(kb + 4);
+  }
+
+  l_run += xor_lanes_f32<16>(l_run);
+  l_run += xor_lanes_f32<32>(l_run);
+  if (grp == 0) {
+    mw[w][col] = m_run;
+    lw[w][col] = l_run;
+  }
+  if (col < nrows) {
+#pragma unroll
+    for (int d = 0; d < DTL; ++d)
+      *reinterpret_cast<float4*>(&red[w][col][16 * d + 4 * grp]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+  }
+  __syncthreads();
+  // the four waves and the new key, four elements of a row per thread
+  for (int i = t; i < nrows * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), j = 4 * (i % (D / 4));
+    float m = fmaxf(fmaxf(mw[0][r], mw[1][r]), fmaxf(mw[2][r], mw[3][r]));
+    if (owns_new) m = fmaxf(m, snew[r]);
+    float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float e = __builtin_amdgcn_exp2f(mw[x][r] - m);
+      const float4 f = *reinterpret_cast<const float4*>(&red[x][r][j]);
+      l += lw[x][r] * e;
+      v[0] += f.x * e;
+      v[1] += f.y * e;
+      v[2] += f.z * e;
+      v[3] += f.w * e;
+    }
+    if (owns_new) {
+      const float e = __builtin_amdgcn_exp2f(snew[r] - m);
+      l += e;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[x] += e * kvn[1][j + x];
+    }
+    const int sb = PREFIX ? (r0 + r) / g : b0, h = kvh * g + (PREFIX ? (r0 + r) % g : r);
+    if (parts.o) {
+      const int64_t row = (int64_t)(slot0 + split) * parts.rows + (int64_t)sb * a.hq + h;
+      *reinterpret_cast<float4*>(parts.o + row * D + j) = make_float4(v[0], v[1], v[2], v[3]);
+      if (j == 0) parts.ml[row] = make_float2(m, l);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[x] /= l;
+      store4<DT>(a.out, (int64_t)sb * a.ldo + (int64_t)h * D + j, v);
+    }
+  }
+}
+
+// ---- prompt chunks, and a prefix that many rows share ------------------------------------------------
+
+// 16 codes of a row as fp16, exactly: a code plus 128 in the low byte of 0x64xx is 1024 + 128 + code.
+__device__ __forceinline__ void codes_to_f16(const v4i& c, v4i (&f)[2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = (uint32_t)c[i] ^ 0x80808080u;
+    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);  // bytes u0, 64, u1, 64
+    const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    const f16x2_t k = {(_Float16)1152.0f, (_Float16)1152.0f};
+    f[i / 2][2 * (i % 2)] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, lo) - k);
+    f[i / 2][2 * (i % 2) + 1] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, hi) - k);
+  }
+}
+
+// Two numbers as packed fp16: one part, or two (x = hi + lo to 22 bits).  The packed pair is pinned before lo is formed: the
+// compiler may fold the product behind x into one of two conversions only, and the two round differently.
+template <int NP>
+__device__ __forceinline__ void f16_parts(float x0, float x1, uint32_t (&part)[NP]) {
+  const f16x2_t hi = {(_Float16)x0, (_Float16)x1};
+  uint32_t h = __builtin_bit_cast(uint32_t, hi);
+  if constexpr (NP == 2) {
+    asm("" : "+v"(h));
+    const f16x2_t b = __builtin_bit_cast(f16x2_t, h);
+    const f16x2_t lo = {(_Float16)(x0 - (float)b[0]), (_Float16)(x1 - (float)b[1])};
+    part[NP - 1] = __builtin_bit_cast(uint32_t, lo);
+  }
+  part[0] = h;
+}
+
+// Rows r of one kv head (row r: token r / G, query head r % G), 32 per wave, 128 per workgroup, against blocks of 64 keys
+// that the workgroup converts to fp16 (exactly) into LDS.  PREFIX: the rows of all sequences of a decode step against the
+// shared prefix; else the prefix first, if there is one, then the sequence's own keys, causal.
+//   S^T[key, row] = K Q^T         v_mfma_f32_32x32x16_f16; q in fp16 of its row's largest (fp32 rows: two parts)
+//   p = exp2(s k_scale c - m)     fp32, a reference m that follows the row's maximum in steps of 2^8 or more
+//   O^T[d, row] += V^T W^T        w = p v_scale / (reference of the scales) in fp16 (fp32 rows: two parts)
+// As in the decode kernel the key of a score tile's row is chosen so that a lane holds the keys that it feeds into the
+// second product, 8 consecutive ones per step.
+template <int DT, int D, bool PREFIX>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void kv_rows_kernel(KvAttn a, Parts parts,
+                                                                                                   int slot0,
+                                                                                                   int nsplit) {
+  constexpr int NP = DT == WFB_F32 ? 2 : 1;
+  constexpr int HD = D / 2, KS = D / 16, DTL = D / 32;
+  // weights reach 2^(kSlack - 1) kUp <= 2^15 (a scale is at most half its reference): one part leaves a reference that
+  // rarely moves, two parts keep the lower part of weights down to 2^-16 of the row's largest out of the subnormal numbers
+  constexpr float kSlack = NP == 1 ? 8.0f : 1.0f, kUp = NP == 1 ? 0x1p8f : 0x1p15f;
+  constexpr int kRing = 4;                           // fragments read ahead of their products
+  constexpr int CK = D / 16;                         // pieces of 16 codes of a key
+  constexpr int PK = kKvBlock * CK / kThreads;       // of K (and of V) per thread
+  __shared__ __attribute__((aligned(16))) uint16_t kt[2][kKvBlock * D], vt[2][kKvBlock * D];
+  __shared__ __attribute__((aligned(16))) float sks[2][kKvBlock], svs[2][kKvBlock];
+  __shared__ float vref_s[2];
+
+  const int g = a.hq / a.hkv;
+  const int nhb = PREFIX ? a.hkv : a.hkv * a.b;
+  const int64_t R = PREFIX ? (int64_t)a.b * g : (int64_t)a.t * g;
+  const int nrb = (int)((R + kRowsPerGroup - 1) / kRowsPerGroup);
+  // the heads' workgroups are nhb apart, so an XCD's L2 holds few heads; the longest rows (the last) come first
+  const int hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
+  const int split = rest % nsplit, rb = nrb - 1 - rest / nsplit;
+  const int kvh = hb % a.hkv, b = hb / a.hkv;
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int col = lane & 31, grp = lane >> 5;
+  const int64_t r = (int64_t)rb * kRowsPerGroup + 32 * w + col;
+  const int tok = (int)(r / g), h = kvh * g + (int)(r % g);
+
+  int64_t first = 0;
+  int n = 0;
+  bool fits = true;
+  bool valid = r < R;
+  if constexpr (PREFIX) {
+    valid = valid && kv_span(a.span, tok, first, n);
+  } else {
+    fits = kv_span(a.span, b, first, n);
+    valid = valid && fits && tok < n;
+  }
+  const int64_t pos = PREFIX ? first : first + tok;
+  const int64_t qrow = PREFIX ? tok : (int64_t)b * a.t + tok;
+  int64_t own = 0;  // own keys that the workgroup's last row sees
+  if constexpr (!PREFIX) {
+    const int64_t tok0 = (int64_t)rb * kRowsPerGroup / g;
+    if (!fits || tok0 >= n) {  // uniform: no row here
+      if (!parts.o && r < R) {
+        const float v = fits ? 0.0f : __builtin_nanf("");
+        for (int j = grp; j < D; j += 2) store_elem<DT>(a.out, qrow * a.ldo + (int64_t)h * D + j, v);
+      }
+      return;
+    }
+    const int64_t tok1 = ((int64_t)(rb + 1) * kRowsPerGroup + g - 1) / g;  // past the last row's token
+    own = first + (tok1 < n ? tok1 : n);
+  }
+  const int64_t pb = (a.npre + kKvBlock - 1) / kKvBlock, nb = pb + (own + kKvBlock - 1) / kKvBlock;
+  const int64_t per = (nb + nsplit - 1) / nsplit;
+  const int64_t kb0 = split * per, kb1 = kb0 + per < nb ? kb0 + per : nb;
+
+  // ---- the row's query in fp16 of its largest: lane holds elements 16 s + 8 grp .. + 7
+  v4i qf[NP][KS];
+  float cq;
+  {
+    float x[KS][8];
+    uint32_t m = 0;
+    if (valid) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) load8<DT>(a.q, qrow * a.ldq + (int64_t)h * D + 16 * s + 8 * grp, x[s]);
+      if (a.rc) {
+#pragma unroll
+        for (int s = 0; s < KS / 2; ++s) {
+          float cs[8], sn[8];
+          load8<WFB_F32>(a.rc, (pos + a.npre) * HD + 16 * s + 8 * grp, cs);
+          load8<WFB_F32>(a.rs, (pos + a.npre) * HD + 16 * s + 8 * grp, sn);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float x1 = x[s][j], x2 = x[s + KS / 2][j];
+            x[s][j] = __fsub_rn(__fmul_rn(x1, cs[j]), __fmul_rn(x2, sn[j]));
+            x[s + KS / 2][j] = __fadd_rn(__fmul_rn(x2, cs[j]), __fmul_rn(x1, sn[j]));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] = 0.0f;
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = umax(m, __float_as_uint(x[s][j]) & 0x7fffffffu);
+    m = umax(m, (uint32_t)xor_lanes<32>((int)m));
+    // by a power of two to [2^14, 2^15): exact, the small elements far from fp16's subnormal numbers
+    const bool some = m < 0x7f800000u && __uint_as_float(m) >= kKvTiny;
+    const int e = (int)(m >> 23) - 127;
+    const float up = some ? __uint_as_float((uint32_t)(127 + 14 - e) << 23) : 0.0f;
+    const float down = some ? __uint_as_float((uint32_t)(127 - 14 + e) << 23) : 0.0f;
+    const float sign = a.scale < 0.0f ? -up : up;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float y0 = some ? x[s][j] * sign : 0.0f, y1 = some ? x[s][j + 1] * sign : 0.0f;
+        uint32_t part[NP];
+        f16_parts<NP>(y0, y1, part);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) qf[p][s][j / 2] = (int)part[p];
+      }
+    // not below the smallest normal number: a masked score's -inf must not meet a zero
+    cq = fmaxf(down * (fabsf(a.scale) * kLog2e), 0x1p-126f);
+    if (m >= 0x7f800000u) cq = __builtin_nanf("");
+  }
+
+  f32x16_t o[DTL];
+#pragma unroll
+  for (int d = 0; d < DTL; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  float m_ref = kNoMax, l_run = 0.0f, vref = 0x1p-100f;
+
+  // ---- staging: K row-major [key][D], V as it is [element][64 keys], 16-byte chunks at chunk ^ (row's swizzle) so that
+  // 16 lanes reading one chunk of 16 rows meet 16 different bank groups
+  auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
+  auto vswz = [](int d) { return (d >> 1) & 7; };
+  v4i kr[PK], vr[PK];
+  float sk = 0.0f, sv = 0.0f;  // (waves 0 and 1) the scales of key `lane`
+  auto fetch = [&](int64_t kb) {
+    const bool in_pre = kb < pb;
+    const wfb_kv_i8& c = in_pre ? a.pre : a.own;
+    const int64_t base = in_pre ? kvh : (int64_t)b * a.hkv + kvh, blk = in_pre ? kb : kb - pb;
+    const int64_t off = (base * c.cap + blk * kKvBlock) * D;
+    const buf_t kb_ = make_buf(c.k + off, kKvBlock * D), vb_ = make_buf(c.v + off, kKvBlock * D);
+#pragma unroll
+    for (int i = 0; i < PK; ++i) {
+      kr[i] = buf_load16(kb_, 16 * (t + i * kThreads));
+      vr[i] = buf_load16(vb_, 16 * (t + i * kThreads));
+    }
+    if (w < 2) {  // (zeros behind the last key)
+      const int64_t left = (in_pre ? a.npre : own) - blk * kKvBlock, at = base * c.cap + blk * kKvBlock;
+      const uint32_t bytes = 4 * (uint32_t)(left < kKvBlock ? left : kKvBlock);
+      sk = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c.k_scale + at, bytes), 4 * lane, 0, 0));
+      sv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c.v_scale + at, bytes), 4 * lane, 0, 0));
+    }
+  };
+  float ref = 0x1p-100f;  // (wave 1) reference of the value scales
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < PK; ++i) {
+      const int p = t + i * kThreads;
+      v4i f[2];
+      codes_to_f16(kr[i], f);
+      const int key = p / CK, kc = 2 * (p % CK), kx = kswz(key);
+      *reinterpret_cast<v4i*>(&kt[buf][key * D + 8 * (kc ^ kx)]) = f[0];
+      *reinterpret_cast<v4i*>(&kt[buf][key * D + 8 * ((kc + 1) ^ kx)]) = f[1];
+      codes_to_f16(vr[i], f);
+      const int d = p / 4, vc = 2 * (p % 4), vx = vswz(d);
+      *reinterpret_cast<v4i*>(&vt[buf][d * kKvBlock + 8 * (vc ^ vx)]) = f[0];
+      *reinterpret_cast<v4i*>(&vt[buf][d * kKvBlock + 8 * ((vc + 1) ^ vx)]) = f[1];
+    }
+    // a value row that is not finite makes NaN of its key's scores, which a mask can take away, and counts as zeros
+    if (w == 0) {
+      sks[buf][lane] = sv != sv ? sv : sk;
+    } else if (w == 1) {
+      sv = fmaxf(sv, 0.0f);
+      float mx = sv;
       mx = fmaxf(mx, xor_lanes_f32<32>(mx));
       mx = fmaxf(mx, xor_lanes_f32<16>(mx));
       mx = fmaxf(mx, xor_lanes_f32<8>(mx));
       mx = fmaxf(mx, xor_lanes_f32<4>(mx));
       mx = fmaxf(mx, xor_lanes_f32<2>(mx));
       mx = fmaxf(mx, xor_lanes_f32<1>(mx));
-      __syncthreads();
-      if (t % 64 == 0) red[t / 64] = mx;
-      __syncthreads();
-      const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-      const float al = __expf(m - mn), p = __expf(s - mn);
-      m = mn;
-      l = l * al + p;  // this thread's keys
-      ps[t] = key < keys ? p * c.v_scale[base * c.cap + key] : 0.0f;
-      __syncthreads();
-      acc *= al;
-      const int8_t* vb = c.v + (base * c.cap + k0) * D + (t % D) * kKvBlock;
-      for (int j = t / D; j < 256 && k0 + j < keys; j += NG)
-        acc += ps[j] * (float)vb[(j / kKvBlock) * kKvBlock * D + j % kKvBlock];
+      if (mx > ref)  // the next power of two, and twice that: growth below it costs nothing
+        ref = fmaxf(__uint_as_float(((__float_as_uint(mx) + 0x7fffffu) & 0x7f800000u) + 0x800000u), 0x1p-100f);
+      svs[buf][lane] = sv * (kUp / ref);
+      if (lane == 0) vref_s[buf] = ref;
+    }
+  };
+
+  const int key = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+  const int ka = key * D, kx = kswz(key), va = col * kKvBlock, vx = vswz(col);  // (a tile's 32 rows repeat the swizzle)
+  auto block = [&](int64_t kb, int buf) {
+    const uint16_t* ks = kt[buf];
+    const uint16_t* vs = vt[buf];
+    if (vref_s[buf] != vref) {  // uniform
+      const float f = vref / vref_s[buf];
+      vref = vref_s[buf];
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) o[d] *= f;
+    }
+    // S^T, fragments kRing steps ahead of their products; row R = 8 a + 4 e + i of a tile stands for key 16 (a / 2) + 8 e +
+    // 4 (a % 2) + i
+    f32x16_t s[2];
+#pragma unroll
+    for (int nb2 = 0; nb2 < 2; ++nb2)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[nb2][i] = 0.0f;
+    {
+      v4i f[kRing];
+      auto read_k = [&](int i) {
+        f[i % kRing] = *reinterpret_cast<const v4i*>(&ks[32 * D * (i & 1) + ka + 8 * ((2 * (i >> 1) + grp) ^ kx)]);
+      };
+#pragma unroll
+      for (int i = 0; i < kRing; ++i) read_k(i);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, f[i % kRing]),
+                                                            __builtin_bit_cast(f16x8_t, qf[p][i >> 1]), s[i & 1], 0, 0, 0);
+        if (i + kRing < 2 * KS) read_k(i + kRing);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, kRing, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NP, 0);
+        if (i + kRing < 2 * KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // register 8 c + j of tile nb2 holds key 32 nb2 + 16 c + 8 grp + j
+    float bmax = -__builtin_inff();
+    const int64_t k0 = (kb < pb ? kb : kb - pb) * kKvBlock;
+#pragma unroll
+    for (int nb2 = 0; nb2 < 2; ++nb2)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(&sks[buf][32 * nb2 + 16 * (i / 8) + 8 * grp + i % 8]);
+        s[nb2][i] *= f.x;
+        s[nb2][i + 1] *= f.y;
+        s[nb2][i + 2] *= f.z;
+        s[nb2][i + 3] *= f.w;
+      }
+    const int64_t seen64 = kb < pb ? a.npre - k0 : PREFIX ? 0 : pos + 1 - k0;
+    const int seen = seen64 > kKvBlock ? kKvBlock : (int)seen64;  // keys of this block that the row sees (or less)
+    if (__any(seen < kKvBlock)) {
+#pragma unroll
+      for (int nb2 = 0; nb2 < 2; ++nb2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * nb2 + 16 * (i / 8) + 8 * grp + i % 8 >= seen) s[nb2][i] = -__builtin_inff();
+    }
+#pragma unroll
+    for (int nb2 = 0; nb2 < 2; ++nb2)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bmax = fmaxf(bmax, s[nb2][i]);
+    bmax = fmaxf(bmax, xor_lanes_f32<32>(bmax)) * cq;
+    if (__any(bmax > m_ref + kSlack)) {
+      const float m_new = fmaxf(m_ref, bmax), alpha = __builtin_amdgcn_exp2f(m_ref - m_new);
+      m_ref = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) o[d] *= alpha;
+    }
+    // O^T over 4 steps of 16 keys, 8 of them this lane's; a step's weights are formed under the products of the one before
+    float psum = 0.0f;
+    v4i pf[2][NP];
+    auto weights = [&](int c) {
+      const float4 f0 = *reinterpret_cast<const float4*>(&svs[buf][16 * c + 8 * grp]);
+      const float4 f1 = *reinterpret_cast<const float4*>(&svs[buf][16 * c + 8 * grp + 4]);
+      const float v[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j], cq, -m_ref));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j + 1], cq, -m_ref));
+        psum += p0;
+        psum += p1;
+        uint32_t part[NP];
+        f16_parts<NP>(p0 * v[j], p1 * v[j + 1], part);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) pf[c & 1][p][j / 2] = (int)part[p];
+      }
+    };
+    v4i vf[kRing];
+    auto read_v = [&](int i) {
+      vf[i % kRing] = *reinterpret_cast<const v4i*>(
+          &vs[32 * kKvBlock * (i % DTL) + va + 8 * ((2 * (i / DTL) + grp) ^ vx)]);
+    };
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) read_v(i);
+    weights(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (c + 1 < 4) weights(c + 1);
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) {
+        const int i = c * DTL + d;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[i % kRing]),
+                                                        __builtin_bit_cast(f16x8_t, pf[c & 1][p]), o[d], 0, 0, 0);
+        if (i + kRing < 4 * DTL) read_v(i + kRing);
+      }
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NP, 0);
+        if (c + 1 < 4) __builtin_amdgcn_sched_group_barrier(0x002, 40 / DTL, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l_run += psum;
+  };
+
+  if (kb0 < kb1) {
+    fetch(kb0);
+    stage(0);
+    for (int64_t kb = kb0; kb < kb1; ++kb) {
+      const int buf = (int)(kb - kb0) & 1;
+      if (kb + 1 < kb1) fetch(kb + 1);
+      __syncthreads();  // block kb is staged, and everyone is done with block kb - 1
+      block(kb, buf);
+      if (kb + 1 < kb1) stage(buf ^ 1);
     }
   }
-  acc_s[t / D][t % D] = acc;
-  l = group_sum_f32<64>(l);
-  __syncthreads();
-  if (t % 64 == 0) red[t / 64] = l;
-  __syncthreads();
-  if (t < D) {
-    float o = 0.0f;
-    for (int g = 0; g < NG; ++g) o += acc_s[g][t];
-    store_elem<DT>(a.out, row * a.ldo + (int64_t)h * D + t, o / ((red[0] + red[1]) + (red[2] + red[3])));
+
+  l_run += xor_lanes_f32<32>(l_run);
+  if (r >= R) return;
+  // lane holds O^T[32 d + 8 (i / 4) + 4 grp + i % 4]
+  const float unit = vref * (1.0f / kUp);
+  if (parts.o) {
+    if (!valid) return;
+    const int64_t row = (int64_t)(slot0 + split) * parts.rows + qrow * a.hq + h;
+#pragma unroll
+    for (int d = 0; d < DTL; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(parts.o + row * D + 32 * d + 2 * i + 4 * grp) =
+            make_float4(o[d][i] * unit, o[d][i + 1] * unit, o[d][i + 2] * unit, o[d][i + 3] * unit);
+    if (grp == 0) parts.ml[row] = make_float2(m_ref, l_run);
+    return;
   }
+  const float f = valid ? unit / l_run : 0.0f;
+#pragma unroll
+  for (int d = 0; d < DTL; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      float v[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[x] = valid ? o[d][i + x] * f : 0.0f;
+      store4<DT>(a.out, qrow * a.ldo + (int64_t)h * D + 32 * d + 2 * i + 4 * grp, v);
+    }
+}
+
+// ---- joining ----------------------------------------------------------------------------------------
+
+// One wave per row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the slots that were written.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void kv_join_kernel(KvAttn a, Parts parts, Plan plan) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= parts.rows) return;
+  const int h = (int)(row % a.hq), i = (int)(row / a.hq % a.t), b = (int)(row / a.hq / a.t);
+  const int64_t out = ((int64_t)b * a.t + i) * a.ldo + (int64_t)h * D + lane * E;
+  int64_t first;
+  int n;
+  const bool fits = kv_span(a.span, b, first, n);
+  if (!fits || i >= n) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) store_elem<DT>(a.out, out + e, fits ? 0.0f : __builtin_nanf(""));
+    return;
+  }
+  int own = plan.own;
+  if (plan.decode) {
+    const int64_t nb = (first + kKvBlock - 1) / kKvBlock, per = split_blocks(nb, plan.own);
+    own = nb == 0 ? 1 : (int)((nb + per - 1) / per);
+  }
+  int pre = plan.pre;
+  if (plan.decode && !plan.pre_rows && pre > 0) {
+    const int64_t nb = (a.npre + kKvBlock - 1) / kKvBlock, per = split_blocks(nb, pre);
+    pre = (int)((nb + per - 1) / per);
+  }
+  const int total = own + pre;
+  auto slot = [&](int s) { return (int64_t)(s < own ? s : plan.own + s - own) * parts.rows + row; };
+  float m = kNoMax;
+  for (int s = lane; s < total; s += 64) m = fmaxf(m, parts.ml[slot(s)].x);
+  m = fmaxf(m, xor_lanes_f32<32>(m));
+  m = fmaxf(m, xor_lanes_f32<16>(m));
+  m = fmaxf(m, xor_lanes_f32<8>(m));
+  m = fmaxf(m, xor_lanes_f32<4>(m));
+  m = fmaxf(m, xor_lanes_f32<2>(m));
+  m = fmaxf(m, xor_lanes_f32<1>(m));
+  float l = 0.0f, v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < total; ++s) {
+    const int64_t at = slot(s);
+    const float2 ml = parts.ml[at];
+    const float f = __builtin_amdgcn_exp2f(ml.x - m);
+    l += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] += parts.o[at * D + lane * E + e] * f;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) store_elem<DT>(a.out, out + e, v[e] / l);
+}
+
+template <int DT, int D>
+hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
+  const Plan p = make_plan(a.b, a.t, a.hq, a.hkv, a.own.cap, a.npre, a.span.len_dev != nullptr);
+  const Parts parts = parts_of(a, p);
+  const int g = a.hq / a.hkv;
+  hipError_t e;
+  if (p.decode) {
+    hipLaunchKernelGGL((kv_decode_kernel<DT, D, false>), dim3(a.hkv, a.b, p.own), dim3(kThreads), 0, s, a, parts, 0, p.own);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (p.pre > 0) {
+      const int rows = a.b * g;
+      if (p.pre_rows)
+        hipLaunchKernelGGL((kv_rows_kernel<DT, D, true>),
+                           dim3((unsigned)((rows + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * p.pre)), dim3(kThreads), 0,
+                           s, a, parts, p.own, p.pre);
+      else
+        hipLaunchKernelGGL((kv_decode_kernel<DT, D, true>), dim3(a.hkv, (rows + kColumns - 1) / kColumns, p.pre),
+                           dim3(kThreads), 0, s, a, parts, p.own, p.pre);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+  } else {
+    e = launch_kv_write_i8(a.dt, a.d, a.kn, a.ldk, a.vn, a.ldv, a.rc, a.rs, a.npre, a.own, a.span, a.b, a.hkv, s);
+    if (e != hipSuccess) return e;
+    const int64_t groups = ((int64_t)a.t * g + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * a.b * p.own;
+    if (groups > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((kv_rows_kernel<DT, D, false>), dim3((unsigned)groups), dim3(kThreads), 0, s, a, parts, 0, p.own);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  if (!has_parts(p)) return hipSuccess;
+  hipLaunchKernelGGL((kv_join_kernel<DT, D>), dim3((unsigned)((parts.rows + 3) / 4)), dim3(kThreads), 0, s, a, parts, p);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t kv_attn_workspace_floats(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+int64_t kv_attn_workspace_floats(int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t d, int64_t cap, int64_t npre) {
+  // (with lengths a call of one token per sequence takes the rows kernel: room for either)
+  int64_t most = 0;
+  for (int lengths = 0; lengths < 2; ++lengths) {
+    const Plan p = make_plan(b, t, hq, hkv, cap, npre, lengths != 0);
+    if (has_parts(p)) most = most > p.own + p.pre ? most : p.own + p.pre;
+  }
+  return most * b * t * hq * (d + 2);
+}
 
 hipError_t launch_kv_attention(const KvAttn& a, hipStream_t s) {
-  hipError_t e = launch_kv_write_i8(a.dt, a.d, a.kn, a.ldk, a.vn, a.ldv, a.rc, a.rs, a.npre, a.own, a.span, a.b, a.hkv, s);
-  if (e != hipSuccess) return e;
-  const dim3 grid(a.hq, a.t, a.b);
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
-  if (a.dt == WFB_F32) a.d == 64 ? go(kv_attention_kernel<WFB_F32, 64>) : go(kv_attention_kernel<WFB_F32, 128>);
-  else a.d == 64 ? go(kv_attention_kernel<WFB_BF16, 64>) : go(kv_attention_kernel<WFB_BF16, 128>);
-  return hipGetLastError();
+  if (a.dt == WFB_F32) return a.d == 64 ? launch_dd<WFB_F32, 64>(a, s) : launch_dd<WFB_F32, 128>(a, s);
+  return a.d == 64 ? launch_dd<WFB_BF16, 64>(a, s) : launch_dd<WFB_BF16, 128>(a, s);
 }
 
 }  // namespace wfb
