@@ -61,11 +61,12 @@ struct Plan {
 };
 
 constexpr int kLive = 768;          // workgroups that a cut call aims at: three per CU
-constexpr int kRowsPerGroup = 128;  // rows (token, query head) of one workgroup of the rows kernel
+constexpr int kRowsWaves = 8;
+constexpr int kRowsPerGroup = 32 * kRowsWaves;  // rows (token, query head) of one workgroup of the rows kernel
 constexpr int kColumns = 16;        // rows of one workgroup of the decode kernel
 
 int cut(int64_t groups, int64_t target, int64_t most) {
-  const int64_t n = (target + groups - 1) / groups;
+  const int64_t n = target / groups;
   return (int)(n < 1 ? 1 : n > most ? most : n);
 }
 
@@ -78,12 +79,12 @@ Plan make_plan(int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t cap, int64
     if (npre > 0) {
       const int64_t rows = b * g;
       p.pre_rows = rows > 64;
-      if (p.pre_rows) p.pre = cut(hkv * ((rows + kRowsPerGroup - 1) / kRowsPerGroup), 512, (pb + 3) / 4);
+      if (p.pre_rows) p.pre = cut(hkv * ((rows + kRowsPerGroup - 1) / kRowsPerGroup), 256, (pb + 3) / 4);
       else p.pre = cut(hkv * ((rows + kColumns - 1) / kColumns), kLive, (pb + 3) / 4);
     }
   } else {
     const int64_t groups = b * hkv * ((t * g + kRowsPerGroup - 1) / kRowsPerGroup);
-    p.own = groups >= 192 ? 1 : cut(groups, 512, (pb + cb + 3) / 4);
+    p.own = groups >= 96 ? 1 : cut(groups, 256, (pb + cb + 3) / 4);
   }
   return p;
 }
@@ -456,17 +457,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 
 // ---- prompt chunks, and a prefix that many rows share ------------------------------------------------
 
-// 16 codes of a row as fp16, exactly: a code plus 128 in the low byte of 0x64xx is 1024 + 128 + code.
-__device__ __forceinline__ void codes_to_f16(const v4i& c, v4i (&f)[2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = (uint32_t)c[i] ^ 0x80808080u;
-    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);  // bytes u0, 64, u1, 64
-    const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    const f16x2_t k = {(_Float16)1152.0f, (_Float16)1152.0f};
-    f[i / 2][2 * (i % 2)] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, lo) - k);
-    f[i / 2][2 * (i % 2) + 1] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, hi) - k);
-  }
+// Four codes as fp16, exactly: a code plus 128 in the low byte of 0x64xx is 1024 + 128 + code.
+__device__ __forceinline__ void codes_to_f16(int codes, int& f0, int& f1) {
+  const uint32_t u = (uint32_t)codes ^ 0x80808080u;
+  const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);  // bytes u0, 64, u1, 64
+  const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+  const f16x2_t k = {(_Float16)1152.0f, (_Float16)1152.0f};
+  f0 = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, lo) - k);
+  f1 = __builtin_bit_cast(int, __builtin_bit_cast(f16x2_t, hi) - k);
 }
 
 // Two numbers as packed fp16: one part, or two (x = hi + lo to 22 bits).  The packed pair is pinned before lo is formed: the
@@ -492,26 +490,35 @@ __device__ __forceinline__ void f16_parts(float x0, float x1, uint32_t (&part)[N
 //   O^T[d, row] += V^T W^T        w = p v_scale / (reference of the scales) in fp16 (fp32 rows: two parts)
 // As in the decode kernel the key of a score tile's row is chosen so that a lane holds the keys that it feeds into the
 // second product, 8 consecutive ones per step.
-template <int DT, int D, bool PREFIX>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void kv_rows_kernel(KvAttn a, Parts parts,
-                                                                                                   int slot0,
-                                                                                                   int nsplit) {
+template <int DT, int D, int W, bool PREFIX>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void kv_rows_kernel(KvAttn a, Parts parts,
+                                                                                                int slot0, int nsplit) {
   constexpr int NP = DT == WFB_F32 ? 2 : 1;
+  constexpr int kRows = 32 * W;
+  // With one part the values' scales are multiplied into their codes as these become fp16 (two roundings to 11 bits of a
+  // value, like that of p, an eighth of the output's); with two they stay factors of the weights.  The keys' scales are
+  // factors of the scores in both: a score may be large, and 11 bits of it too few.
+  constexpr bool kScaled = NP == 1;
   constexpr int HD = D / 2, KS = D / 16, DTL = D / 32;
-  // weights reach 2^(kSlack - 1) kUp <= 2^15 (a scale is at most half its reference): one part leaves a reference that
-  // rarely moves, two parts keep the lower part of weights down to 2^-16 of the row's largest out of the subnormal numbers
+  // (a scale is at most half its reference.)  One part: weights reach 2^kSlack, so their reference rarely moves, and values
+  // 127 kUp / 2 < 2^14.  Two parts: weights reach 2^(kSlack - 1) kUp = 2^15, which keeps the lower part of weights down to
+  // 2^-16 of the row's largest out of the subnormal numbers.
   constexpr float kSlack = NP == 1 ? 8.0f : 1.0f, kUp = NP == 1 ? 0x1p8f : 0x1p15f;
-  constexpr int kRing = 4;                           // fragments read ahead of their products
-  constexpr int CK = D / 16;                         // pieces of 16 codes of a key
-  constexpr int PK = kKvBlock * CK / kThreads;       // of K (and of V) per thread
-  __shared__ __attribute__((aligned(16))) uint16_t kt[2][kKvBlock * D], vt[2][kKvBlock * D];
-  __shared__ __attribute__((aligned(16))) float sks[2][kKvBlock], svs[2][kKvBlock];
-  __shared__ float vref_s[2];
+  constexpr int kRingK = 4, kRingV = 4;                           // fragments read ahead of their products
+  constexpr int CK = D / 16;               // pieces of 16 codes of a key
+  constexpr int KP = kKvBlock * CK;        // of a block's keys; as many of its values
+  constexpr int PT = 2 * KP / (64 * W);    // per thread
+  static_assert(PT * 64 * W == 2 * KP && KP % 64 == 0, "whole waves take keys or values");
+  static_assert(KP % (64 * W) == 0 || D == kKvBlock, "a round of keys and values needs rows of one length");
+  __shared__ __attribute__((aligned(16))) uint16_t tile[2][2][kKvBlock * D];  // [buffer][keys, values]
+  // scales of a block's keys and values and of the two behind it; svs: as fp16 if kScaled
+  __shared__ __attribute__((aligned(16))) float sks[3][kKvBlock], svs[3][kKvBlock];
+  __shared__ float vref_s[3];
 
   const int g = a.hq / a.hkv;
   const int nhb = PREFIX ? a.hkv : a.hkv * a.b;
   const int64_t R = PREFIX ? (int64_t)a.b * g : (int64_t)a.t * g;
-  const int nrb = (int)((R + kRowsPerGroup - 1) / kRowsPerGroup);
+  const int nrb = (int)((R + kRows - 1) / kRows);
   // the heads' workgroups are nhb apart, so an XCD's L2 holds few heads; the longest rows (the last) come first
   const int hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
   const int split = rest % nsplit, rb = nrb - 1 - rest / nsplit;
@@ -519,7 +526,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int col = lane & 31, grp = lane >> 5;
-  const int64_t r = (int64_t)rb * kRowsPerGroup + 32 * w + col;
+  const int64_t r = (int64_t)rb * kRows + 32 * w + col;
   const int tok = (int)(r / g), h = kvh * g + (int)(r % g);
 
   int64_t first = 0;
@@ -533,10 +540,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     valid = valid && fits && tok < n;
   }
   const int64_t pos = PREFIX ? first : first + tok;
+  const int64_t rw = (int64_t)rb * kRows + 32 * w;  // the wave's first row and (not PREFIX) its position
+  const int64_t pos_low = first + rw / g;
   const int64_t qrow = PREFIX ? tok : (int64_t)b * a.t + tok;
   int64_t own = 0;  // own keys that the workgroup's last row sees
   if constexpr (!PREFIX) {
-    const int64_t tok0 = (int64_t)rb * kRowsPerGroup / g;
+    const int64_t tok0 = (int64_t)rb * kRows / g;
     if (!fits || tok0 >= n) {  // uniform: no row here
       if (!parts.o && r < R) {
         const float v = fits ? 0.0f : __builtin_nanf("");
@@ -544,7 +553,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       }
       return;
     }
-    const int64_t tok1 = ((int64_t)(rb + 1) * kRowsPerGroup + g - 1) / g;  // past the last row's token
+    const int64_t tok1 = ((int64_t)(rb + 1) * kRows + g - 1) / g;  // past the last row's token
     own = first + (tok1 < n ? tok1 : n);
   }
   const int64_t pb = (a.npre + kKvBlock - 1) / kKvBlock, nb = pb + (own + kKvBlock - 1) / kKvBlock;
@@ -617,72 +626,121 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   // 16 lanes reading one chunk of 16 rows meet 16 different bank groups
   auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
   auto vswz = [](int d) { return (d >> 1) & 7; };
-  v4i kr[PK], vr[PK];
-  float sk = 0.0f, sv = 0.0f;  // (waves 0 and 1) the scales of key `lane`
-  auto fetch = [&](int64_t kb) {
+  v4i raw[2][PT] = {};  // codes of the next block and of the one behind it
+  auto place = [&](int64_t kb, const wfb_kv_i8*& c, int64_t& at, int64_t& left) {  // uniform
     const bool in_pre = kb < pb;
-    const wfb_kv_i8& c = in_pre ? a.pre : a.own;
-    const int64_t base = in_pre ? kvh : (int64_t)b * a.hkv + kvh, blk = in_pre ? kb : kb - pb;
-    const int64_t off = (base * c.cap + blk * kKvBlock) * D;
-    const buf_t kb_ = make_buf(c.k + off, kKvBlock * D), vb_ = make_buf(c.v + off, kKvBlock * D);
+    const int64_t k0 = (in_pre ? kb : kb - pb) * kKvBlock;
+    c = in_pre ? &a.pre : &a.own;
+    at = (in_pre ? kvh : (int64_t)b * a.hkv + kvh) * c->cap + k0;
+    left = (in_pre ? a.npre : own) - k0;
+  };
+  auto fetch_codes = [&](int64_t kb, int set) {
+    const wfb_kv_i8* c;
+    int64_t at, left;
+    place(kb, c, at, left);
+    const buf_t kb_ = make_buf(c->k + at * D, kKvBlock * D), vb_ = make_buf(c->v + at * D, kKvBlock * D);
 #pragma unroll
-    for (int i = 0; i < PK; ++i) {
-      kr[i] = buf_load16(kb_, 16 * (t + i * kThreads));
-      vr[i] = buf_load16(vb_, 16 * (t + i * kThreads));
-    }
-    if (w < 2) {  // (zeros behind the last key)
-      const int64_t left = (in_pre ? a.npre : own) - blk * kKvBlock, at = base * c.cap + blk * kKvBlock;
-      const uint32_t bytes = 4 * (uint32_t)(left < kKvBlock ? left : kKvBlock);
-      sk = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c.k_scale + at, bytes), 4 * lane, 0, 0));
-      sv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c.v_scale + at, bytes), 4 * lane, 0, 0));
+    for (int i = 0; i < PT; ++i) {
+      const int p0 = 64 * (w + i * W);  // uniform
+      raw[set][i] = p0 < KP ? buf_load16(kb_, 16 * (p0 + lane)) : buf_load16(vb_, 16 * (p0 - KP + lane));
     }
   };
-  float ref = 0x1p-100f;  // (wave 1) reference of the value scales
-  auto stage = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < PK; ++i) {
-      const int p = t + i * kThreads;
-      v4i f[2];
-      codes_to_f16(kr[i], f);
-      const int key = p / CK, kc = 2 * (p % CK), kx = kswz(key);
-      *reinterpret_cast<v4i*>(&kt[buf][key * D + 8 * (kc ^ kx)]) = f[0];
-      *reinterpret_cast<v4i*>(&kt[buf][key * D + 8 * ((kc + 1) ^ kx)]) = f[1];
-      codes_to_f16(vr[i], f);
-      const int d = p / 4, vc = 2 * (p % 4), vx = vswz(d);
-      *reinterpret_cast<v4i*>(&vt[buf][d * kKvBlock + 8 * (vc ^ vx)]) = f[0];
-      *reinterpret_cast<v4i*>(&vt[buf][d * kKvBlock + 8 * ((vc + 1) ^ vx)]) = f[1];
-    }
+  float sk = 0.0f, sv = 0.0f;  // (waves 0 and 1) the scales of key `lane`, zeros behind the last key
+  auto fetch_scales = [&](int64_t kb) {
+    if (w >= 2) return;
+    const wfb_kv_i8* c;
+    int64_t at, left;
+    place(kb, c, at, left);
+    const uint32_t bytes = 4 * (uint32_t)(left < kKvBlock ? left : kKvBlock);
+    sk = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->k_scale + at, bytes), 4 * lane, 0, 0));
+    sv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->v_scale + at, bytes), 4 * lane, 0, 0));
+  };
+  float ref = 0x1p-100f;  // (wave 1) reference of the value scales so far
+  auto stage_scales = [&](int slot) {
     // a value row that is not finite makes NaN of its key's scores, which a mask can take away, and counts as zeros
     if (w == 0) {
-      sks[buf][lane] = sv != sv ? sv : sk;
+      sks[slot][lane] = sv != sv ? sv : sk;
     } else if (w == 1) {
-      sv = fmaxf(sv, 0.0f);
-      float mx = sv;
+      const float x = fmaxf(sv, 0.0f);
+      float mx = x;
       mx = fmaxf(mx, xor_lanes_f32<32>(mx));
       mx = fmaxf(mx, xor_lanes_f32<16>(mx));
       mx = fmaxf(mx, xor_lanes_f32<8>(mx));
       mx = fmaxf(mx, xor_lanes_f32<4>(mx));
       mx = fmaxf(mx, xor_lanes_f32<2>(mx));
       mx = fmaxf(mx, xor_lanes_f32<1>(mx));
-      if (mx > ref)  // the next power of two, and twice that: growth below it costs nothing
-        ref = fmaxf(__uint_as_float(((__float_as_uint(mx) + 0x7fffffu) & 0x7f800000u) + 0x800000u), 0x1p-100f);
-      svs[buf][lane] = sv * (kUp / ref);
-      if (lane == 0) vref_s[buf] = ref;
+      if (mx > ref)  // twice the next power of two: growth below it costs nothing
+        ref = __uint_as_float(((__float_as_uint(mx) + 0x7fffffu) & 0x7f800000u) + 0x800000u);
+      const float y = x * (kUp * __uint_as_float(0x7f000000u - __float_as_uint(ref)));
+      if constexpr (kScaled) reinterpret_cast<_Float16*>(svs[slot])[lane] = (_Float16)y;
+      else svs[slot][lane] = y;
+      if (lane == 0) vref_s[slot] = ref;
     }
+  };
+  // pieces of 16 codes: whole waves, and but for D = 64 with 8 waves whole rounds, take keys or values; there the row
+  // formulas of the two agree
+  auto piece = [&](int i, bool& isk, int& row, int& c) {
+    const int p0 = 64 * (w + i * W);
+    isk = 64 * W * (i + 1) <= KP || (64 * W * i < KP && p0 < KP);
+    const int p = (isk ? p0 : p0 - KP) + lane, per = 64 * W * (i + 1) <= KP ? CK : 4;
+    row = p / per;
+    c = p % per;
+  };
+  v4i half[2];
+  uint32_t factor[8];
+  auto read_factors = [&](int i, int slot) {  // of piece i
+    if constexpr (kScaled) {
+      if (64 * W * (i + 1) <= KP) return;
+      bool isk;
+      int row, c;
+      piece(i, isk, row, c);
+      const v4i f0 = *reinterpret_cast<const v4i*>(&svs[slot][8 * c]);
+      const v4i f1 = *reinterpret_cast<const v4i*>(&svs[slot][8 * c + 4]);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) factor[x] = isk ? 0x3c003c00u : (uint32_t)(x < 4 ? f0[x] : f1[x - 4]);  // (ones)
+    }
+  };
+  auto convert = [&](int i, int set) {  // word i of the thread's codes
+    int f[2];
+    codes_to_f16(raw[set][i / 4][i % 4], f[0], f[1]);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (kScaled && 64 * W * (i / 4 + 1) > KP)
+        f[x] = __builtin_bit_cast(
+            int, __builtin_bit_cast(f16x2_t, f[x]) * __builtin_bit_cast(f16x2_t, factor[2 * (i % 4) + x]));
+      half[i % 4 / 2][2 * (i % 2) + x] = f[x];
+    }
+  };
+  auto stage_codes = [&](int i, int buf) {  // piece i
+    bool isk;
+    int row, c;
+    piece(i, isk, row, c);
+    const bool krow = 64 * W * (i + 1) <= KP;
+    const int x = krow ? kswz(row) : vswz(row);
+    uint16_t* dst = &tile[buf][isk ? 0 : 1][row * (krow ? D : kKvBlock)];
+    *reinterpret_cast<v4i*>(dst + 8 * ((2 * c) ^ x)) = half[0];
+    *reinterpret_cast<v4i*>(dst + 8 * ((2 * c + 1) ^ x)) = half[1];
   };
 
   const int key = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
   const int ka = key * D, kx = kswz(key), va = col * kKvBlock, vx = vswz(col);  // (a tile's 32 rows repeat the swizzle)
-  auto block = [&](int64_t kb, int buf) {
-    const uint16_t* ks = kt[buf];
-    const uint16_t* vs = vt[buf];
-    if (vref_s[buf] != vref) {  // uniform
-      const float f = vref / vref_s[buf];
-      vref = vref_s[buf];
+  // Block kb, in buffer buf and scale slot `slot`.  Under the first products the next block's codes, fetched during the
+  // block before, become fp16 and then go to the other buffer; the scales of the one behind it go to the next slot but one.
+  auto block = [&](int64_t kb, int buf, int slot) {
+    const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
+    const uint16_t* ks = tile[buf][0];
+    const uint16_t* vs = tile[buf][1];
+    if (kb + 2 < kb1) fetch_codes(kb + 2, buf);
+    const int64_t k0 = (kb < pb ? kb : kb - pb) * kKvBlock;
+    read_factors(0, slot1);
+    const float vnew = vref_s[slot];
+    if (vnew != vref) {  // uniform
+      const float f = vref / vnew;
+      vref = vnew;
 #pragma unroll
       for (int d = 0; d < DTL; ++d) o[d] *= f;
     }
-    // S^T, fragments kRing steps ahead of their products; row R = 8 a + 4 e + i of a tile stands for key 16 (a / 2) + 8 e +
+    // S^T, fragments kRingK steps ahead of their products; row R = 8 a + 4 e + i of a tile stands for key 16 (a / 2) + 8 e +
     // 4 (a % 2) + i
     f32x16_t s[2];
 #pragma unroll
@@ -690,44 +748,51 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[nb2][i] = 0.0f;
     {
-      v4i f[kRing];
+      v4i f[kRingK];
       auto read_k = [&](int i) {
-        f[i % kRing] = *reinterpret_cast<const v4i*>(&ks[32 * D * (i & 1) + ka + 8 * ((2 * (i >> 1) + grp) ^ kx)]);
+        f[i % kRingK] = *reinterpret_cast<const v4i*>(&ks[32 * D * (i & 1) + ka + 8 * ((2 * (i >> 1) + grp) ^ kx)]);
       };
 #pragma unroll
-      for (int i = 0; i < kRing; ++i) read_k(i);
+      for (int i = 0; i < kRingK; ++i) read_k(i);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 2 * KS; ++i) {
+      for (int i = 0; i < 2 * KS; ++i) {  // in this order: a product, a read ahead, a part of the conversion
 #pragma unroll
         for (int p = 0; p < NP; ++p)
-          s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, f[i % kRing]),
+          s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, f[i % kRingK]),
                                                             __builtin_bit_cast(f16x8_t, qf[p][i >> 1]), s[i & 1], 0, 0, 0);
-        if (i + kRing < 2 * KS) read_k(i + kRing);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x100, kRing, 0);
+        if (i + kRingK < 2 * KS) read_k(i + kRingK);
+        // word x of the codes behind step (x + 1) 2 KS / (4 PT) - 1, the last of a piece with the piece's way to the tile
+        // (behind the last block: of no meaning, and never read)
 #pragma unroll
-      for (int i = 0; i < 2 * KS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, NP, 0);
-        if (i + kRing < 2 * KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        for (int x = 0; x < 4 * PT; ++x)
+          if (i == (x + 1) * 2 * KS / (4 * PT) - 1) {
+            convert(x, buf ^ 1);
+            if (x % 4 == 3) {
+              stage_codes(x / 4, buf ^ 1);
+              if (x / 4 + 1 < PT) read_factors(x / 4 + 1, slot1);
+            }
+          }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
+    if (kb + 2 < kb1) stage_scales(slot2);
+    if (kb + 3 < kb1) fetch_scales(kb + 3);
     // register 8 c + j of tile nb2 holds key 32 nb2 + 16 c + 8 grp + j
     float bmax = -__builtin_inff();
-    const int64_t k0 = (kb < pb ? kb : kb - pb) * kKvBlock;
 #pragma unroll
     for (int nb2 = 0; nb2 < 2; ++nb2)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(&sks[buf][32 * nb2 + 16 * (i / 8) + 8 * grp + i % 8]);
+        const float4 f = *reinterpret_cast<const float4*>(&sks[slot][32 * nb2 + 16 * (i / 8) + 8 * grp + i % 8]);
         s[nb2][i] *= f.x;
         s[nb2][i + 1] *= f.y;
         s[nb2][i + 2] *= f.z;
         s[nb2][i + 3] *= f.w;
       }
-    const int64_t seen64 = kb < pb ? a.npre - k0 : PREFIX ? 0 : pos + 1 - k0;
-    const int seen = seen64 > kKvBlock ? kKvBlock : (int)seen64;  // keys of this block that the row sees (or less)
-    if (__any(seen < kKvBlock)) {
+    const int64_t seen64 = kb < pb ? a.npre - k0 : pos + 1 - k0, low64 = kb < pb ? a.npre - k0 : pos_low + 1 - k0;
+    if (low64 < kKvBlock) {  // uniform: some row of the wave does not see all keys of the block
+      const int seen = seen64 > kKvBlock ? kKvBlock : (int)seen64;
 #pragma unroll
       for (int nb2 = 0; nb2 < 2; ++nb2)
 #pragma unroll
@@ -749,63 +814,90 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     // O^T over 4 steps of 16 keys, 8 of them this lane's; a step's weights are formed under the products of the one before
     float psum = 0.0f;
     v4i pf[2][NP];
-    auto weights = [&](int c) {
-      const float4 f0 = *reinterpret_cast<const float4*>(&svs[buf][16 * c + 8 * grp]);
-      const float4 f1 = *reinterpret_cast<const float4*>(&svs[buf][16 * c + 8 * grp + 4]);
-      const float v[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j], cq, -m_ref));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j + 1], cq, -m_ref));
-        psum += p0;
-        psum += p1;
-        uint32_t part[NP];
-        f16_parts<NP>(p0 * v[j], p1 * v[j + 1], part);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) pf[c & 1][p][j / 2] = (int)part[p];
+    float v[8];
+    auto read_scales = [&](int c) {
+      if constexpr (!kScaled) {
+        const float4 f0 = *reinterpret_cast<const float4*>(&svs[slot][16 * c + 8 * grp]);
+        const float4 f1 = *reinterpret_cast<const float4*>(&svs[slot][16 * c + 8 * grp + 4]);
+        v[0] = f0.x, v[1] = f0.y, v[2] = f0.z, v[3] = f0.w, v[4] = f1.x, v[5] = f1.y, v[6] = f1.z, v[7] = f1.w;
       }
     };
-    v4i vf[kRing];
+    auto weights = [&](int c, int j) {  // keys j and j + 1 of step c
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j], cq, -m_ref));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j + 1], cq, -m_ref));
+      uint32_t part[NP];
+      if constexpr (kScaled) {
+        f16_parts<NP>(p0, p1, part);
+        const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};  // the sum of the weights as they are used
+        psum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, part[0]), one, psum, false);
+      } else {
+        psum += p0;
+        psum += p1;
+        f16_parts<NP>(p0 * v[j], p1 * v[j + 1], part);
+      }
+#pragma unroll
+      for (int p = 0; p < NP; ++p) pf[c & 1][p][j / 2] = (int)part[p];
+      asm volatile("" : "+v"(psum));  // here, under the products, not where the sum is used
+    };
+    v4i vf[kRingV];
     auto read_v = [&](int i) {
-      vf[i % kRing] = *reinterpret_cast<const v4i*>(
+      vf[i % kRingV] = *reinterpret_cast<const v4i*>(
           &vs[32 * kKvBlock * (i % DTL) + va + 8 * ((2 * (i / DTL) + grp) ^ vx)]);
     };
+    read_scales(0);
 #pragma unroll
-    for (int i = 0; i < kRing; ++i) read_v(i);
-    weights(0);
+    for (int i = 0; i < kRingV; ++i) read_v(i);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) weights(0, j);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      if (c + 1 < 4) weights(c + 1);
+      if (c + 1 < 4) read_scales(c + 1);
 #pragma unroll
       for (int d = 0; d < DTL; ++d) {
         const int i = c * DTL + d;
 #pragma unroll
         for (int p = 0; p < NP; ++p)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[i % kRing]),
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[i % kRingV]),
                                                         __builtin_bit_cast(f16x8_t, pf[c & 1][p]), o[d], 0, 0, 0);
-        if (i + kRing < 4 * DTL) read_v(i + kRing);
-      }
+        if (i + kRingV < 4 * DTL) read_v(i + kRingV);
+        if (c + 1 < 4) {
 #pragma unroll
-      for (int d = 0; d < DTL; ++d) {
-        __builtin_amdgcn_sched_group_barrier(0x008, NP, 0);
-        if (c + 1 < 4) __builtin_amdgcn_sched_group_barrier(0x002, 40 / DTL, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          for (int j = 8 * d / DTL; j < 8 * (d + 1) / DTL; j += 2) weights(c + 1, j);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
     l_run += psum;
   };
 
   if (kb0 < kb1) {
-    fetch(kb0);
-    stage(0);
-    for (int64_t kb = kb0; kb < kb1; ++kb) {
-      const int buf = (int)(kb - kb0) & 1;
-      if (kb + 1 < kb1) fetch(kb + 1);
-      __syncthreads();  // block kb is staged, and everyone is done with block kb - 1
-      block(kb, buf);
-      if (kb + 1 < kb1) stage(buf ^ 1);
+    fetch_codes(kb0, 0);
+    fetch_scales(kb0);
+    stage_scales(0);
+    if (kb0 + 1 < kb1) {
+      fetch_scales(kb0 + 1);
+      stage_scales(1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      read_factors(i, 0);
+#pragma unroll
+      for (int x = 4 * i; x < 4 * i + 4; ++x) convert(x, 0);
+      stage_codes(i, 0);
+    }
+    if (kb0 + 1 < kb1) fetch_codes(kb0 + 1, 1);
+    if (kb0 + 2 < kb1) fetch_scales(kb0 + 2);
+    int slot = 0;
+    for (int64_t kb = kb0; kb < kb1; kb += 2) {
+      __syncthreads();  // block kb and its scales are staged, and everyone is done with block kb - 1
+      block(kb, 0, slot);
+      slot = slot == 2 ? 0 : slot + 1;
+      if (kb + 1 >= kb1) break;
+      __syncthreads();
+      block(kb + 1, 1, slot);
+      slot = slot == 2 ? 0 : slot + 1;
     }
   }
 
@@ -904,8 +996,8 @@ hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
     if (p.pre > 0) {
       const int rows = a.b * g;
       if (p.pre_rows)
-        hipLaunchKernelGGL((kv_rows_kernel<DT, D, true>),
-                           dim3((unsigned)((rows + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * p.pre)), dim3(kThreads), 0,
+        hipLaunchKernelGGL((kv_rows_kernel<DT, D, kRowsWaves, true>),
+                           dim3((unsigned)((rows + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * p.pre)), dim3(64 * kRowsWaves), 0,
                            s, a, parts, p.own, p.pre);
       else
         hipLaunchKernelGGL((kv_decode_kernel<DT, D, true>), dim3(a.hkv, (rows + kColumns - 1) / kColumns, p.pre),
@@ -917,7 +1009,7 @@ hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
     if (e != hipSuccess) return e;
     const int64_t groups = ((int64_t)a.t * g + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * a.b * p.own;
     if (groups > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((kv_rows_kernel<DT, D, false>), dim3((unsigned)groups), dim3(kThreads), 0, s, a, parts, 0, p.own);
+    hipLaunchKernelGGL((kv_rows_kernel<DT, D, kRowsWaves, false>), dim3((unsigned)groups), dim3(64 * kRowsWaves), 0, s, a, parts, 0, p.own);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!has_parts(p)) return hipSuccess;
