@@ -931,21 +931,24 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
 
 // ---- joining ----------------------------------------------------------------------------------------
 
-// One wave per row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the slots that were written.
-template <int DT, int D>
+// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the slots that were written, W waves per row: D / 4 lanes take
+// four elements each, the groups of lanes the slots in turn.
+template <int DT, int D, int W>
 __global__ __launch_bounds__(kThreads) void kv_join_kernel(KvAttn a, Parts parts, Plan plan) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= parts.rows) return;
+  constexpr int L = D / 4, G = 64 * W / L;  // lanes of a group, groups of a row
+  __shared__ float4 os[W > 1 ? G : 1][L];
+  __shared__ float ls[W > 1 ? G : 1];
+  const int t = threadIdx.x % (64 * W), lane = t & 63, j = t % L, g = t / L;
+  const int64_t row = (int64_t)blockIdx.x * (4 / W) + __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * W));
+  if (row >= parts.rows) return;  // (uniform over the waves of a row)
   const int h = (int)(row % a.hq), i = (int)(row / a.hq % a.t), b = (int)(row / a.hq / a.t);
-  const int64_t out = ((int64_t)b * a.t + i) * a.ldo + (int64_t)h * D + lane * E;
+  const int64_t out = ((int64_t)b * a.t + i) * a.ldo + (int64_t)h * D + 4 * j;
   int64_t first;
   int n;
   const bool fits = kv_span(a.span, b, first, n);
   if (!fits || i >= n) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) store_elem<DT>(a.out, out + e, fits ? 0.0f : __builtin_nanf(""));
+    const float x = fits ? 0.0f : __builtin_nanf(""), v[4] = {x, x, x, x};
+    if (g == 0) store4<DT>(a.out, out, v);
     return;
   }
   int own = plan.own;
@@ -968,20 +971,46 @@ __global__ __launch_bounds__(kThreads) void kv_join_kernel(KvAttn a, Parts parts
   m = fmaxf(m, xor_lanes_f32<4>(m));
   m = fmaxf(m, xor_lanes_f32<2>(m));
   m = fmaxf(m, xor_lanes_f32<1>(m));
-  float l = 0.0f, v[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = 0.0f;
+  float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int s = 0; s < total; ++s) {
+  for (int s = g; s < total; s += G) {
     const int64_t at = slot(s);
     const float2 ml = parts.ml[at];
+    const float4 x = *reinterpret_cast<const float4*>(parts.o + at * D + 4 * j);
     const float f = __builtin_amdgcn_exp2f(ml.x - m);
     l += ml.y * f;
+    v[0] += x.x * f;
+    v[1] += x.y * f;
+    v[2] += x.z * f;
+    v[3] += x.w * f;
+  }
+  if constexpr (W == 1) {
+    // the groups of the wave: 2 of 32 lanes, or 4 of 16
+    auto add = [&](float& x) {
+      if constexpr (L == 16) x += xor_lanes_f32<16>(x);
+      x += xor_lanes_f32<32>(x);
+    };
+    add(l);
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] += parts.o[at * D + lane * E + e] * f;
+    for (int e = 0; e < 4; ++e) add(v[e]);
+  } else {
+    os[g][j] = make_float4(v[0], v[1], v[2], v[3]);
+    if (j == 0) ls[g] = l;
+    __syncthreads();
+    if (g > 0) return;
+    l = 0.0f, v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < G; ++x) {
+      l += ls[x];
+      v[0] += os[x][j].x;
+      v[1] += os[x][j].y;
+      v[2] += os[x][j].z;
+      v[3] += os[x][j].w;
+    }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) store_elem<DT>(a.out, out + e, v[e] / l);
+  for (int e = 0; e < 4; ++e) v[e] /= l;
+  if (g == 0) store4<DT>(a.out, out, v);
 }
 
 template <int DT, int D>
@@ -1013,7 +1042,11 @@ hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!has_parts(p)) return hipSuccess;
-  hipLaunchKernelGGL((kv_join_kernel<DT, D>), dim3((unsigned)((parts.rows + 3) / 4)), dim3(kThreads), 0, s, a, parts, p);
+  // a row's slots by one wave, or by four where they are many
+  if (p.own + p.pre <= 16)
+    hipLaunchKernelGGL((kv_join_kernel<DT, D, 1>), dim3((unsigned)((parts.rows + 3) / 4)), dim3(kThreads), 0, s, a, parts, p);
+  else
+    hipLaunchKernelGGL((kv_join_kernel<DT, D, 4>), dim3((unsigned)parts.rows), dim3(kThreads), 0, s, a, parts, p);
   return hipGetLastError();
 }
 

@@ -39,9 +39,9 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& scale) {
   return make_uint2(q[0], q[1]);
 }
 
-// One workgroup per (64-key block of the cache, kv head, sequence): the new tokens that fall into the block.  A row is
-// read by D / 8 lanes, 8 elements each (the rotary partner D / 2 away sits in the lane half a group away); the value
-// codes pass through LDS, row by row in and 4 x 4 bytes transposed out, 8 keys of 4 elements per thread.
+// One workgroup per (64-key block of the cache, kv head, sequence, keys or values): the new tokens that fall into the block.
+// A row is read by D / 8 lanes, 8 elements each (the rotary partner D / 2 away sits in the lane half a group away); the
+// value codes pass through LDS, row by row in and 4 x 4 bytes transposed out, 8 keys of 4 elements per thread.
 // What bounds it: HBM.  8 x 2048 tokens of 8 heads of 128, bf16: 67 MB in and 35 MB out.
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const void* __restrict__ kn, int64_t ldk,
@@ -49,9 +49,11 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const void* __restri
                                                             const float* __restrict__ rc, const float* __restrict__ rs,
                                                             int64_t turn, wfb_kv_i8 c, KvSpan sp, int hkv) {
   constexpr int HD = D / 2, L = D / 8, RPP = kThreads / L;  // lanes per row, rows per pass
+  constexpr int NP = kKvBlock / RPP;                        // passes
   constexpr int kPitch = D + 8;                             // of an LDS row: the transposed reads spread over the banks
   __shared__ __attribute__((aligned(16))) uint8_t vt[kKvBlock * kPitch];
-  const int t = threadIdx.x, l = t % L, h = blockIdx.y, b = blockIdx.z;
+  const int t = threadIdx.x, l = t % L, h = blockIdx.y >> 1, b = blockIdx.z;
+  const bool keys = (blockIdx.y & 1) == 0;
   int64_t first;
   int n;
   if (!kv_span(sp, b, first, n)) return;
@@ -63,35 +65,39 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const void* __restri
   if (lo >= hi) return;
   const int64_t slice = ((int64_t)b * hkv + h) * c.cap;
   const int64_t row0 = (int64_t)b * sp.t + (k0 - first);  // input row of slot 0
-  for (int p0 = lo / RPP * RPP; p0 < hi; p0 += RPP) {  // uniform
-    const int slot = p0 + t / L;
-    const bool in = slot >= lo && slot < hi;
-    const int64_t row = row0 + (in ? slot : lo), pos = k0 + (in ? slot : lo);
-    float x[8], v[8];
-    load8<DT>(kn, row * ldk + (int64_t)h * D + 8 * l, x);
-    load8<DT>(vn, row * ldv + (int64_t)h * D + 8 * l, v);
-    if (rc) {
+  auto at = [&](int p) {  // slot of pass p; one that is not written is read as the first that is
+    const int slot = p * RPP + t / L;
+    return slot >= lo && slot < hi ? slot : lo;
+  };
+  float x[NP][8];
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+    if (p * RPP < hi && (p + 1) * RPP > lo)  // uniform
+      load8<DT>(keys ? kn : vn, (row0 + at(p)) * (keys ? ldk : ldv) + (int64_t)h * D + 8 * l, x[p]);
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    if (p * RPP >= hi || (p + 1) * RPP <= lo) continue;
+    const int slot = at(p);
+    const int64_t pos = k0 + slot;
+    if (keys && rc) {
       float cs[8], sn[8];
       load8<WFB_F32>(rc, (pos + turn) * HD + 8 * (l % (L / 2)), cs);
       load8<WFB_F32>(rs, (pos + turn) * HD + 8 * (l % (L / 2)), sn);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float other = xor_lanes_f32<L / 2>(x[j]);
-        const float y = __fmul_rn(x[j], cs[j]), z = __fmul_rn(other, sn[j]);
-        x[j] = l < L / 2 ? __fsub_rn(y, z) : __fadd_rn(y, z);
+        const float other = xor_lanes_f32<L / 2>(x[p][j]);
+        const float y = __fmul_rn(x[p][j], cs[j]), z = __fmul_rn(other, sn[j]);
+        x[p][j] = l < L / 2 ? __fsub_rn(y, z) : __fadd_rn(y, z);
       }
     }
-    float ks, vs;
-    const uint2 kq = quantise8<L>(x, ks), vq = quantise8<L>(v, vs);
-    if (in) {
-      *reinterpret_cast<uint2*>(c.k + (slice + pos) * D + 8 * l) = kq;
-      *reinterpret_cast<uint2*>(&vt[slot * kPitch + 8 * l]) = vq;
-      if (l == 0) {
-        c.k_scale[slice + pos] = ks;
-        c.v_scale[slice + pos] = vs;
-      }
-    }
+    float scale;
+    const uint2 q = quantise8<L>(x[p], scale);
+    if (slot != p * RPP + t / L) continue;
+    if (keys) *reinterpret_cast<uint2*>(c.k + (slice + pos) * D + 8 * l) = q;
+    else *reinterpret_cast<uint2*>(&vt[slot * kPitch + 8 * l]) = q;
+    if (l == 0) (keys ? c.k_scale : c.v_scale)[slice + pos] = scale;
   }
+  if (keys) return;
   __syncthreads();
   int8_t* vb = c.v + (slice + k0) * D;
   for (int i = t; i < D / 4 * 8; i += kThreads) {
@@ -139,17 +145,19 @@ __device__ __forceinline__ void store4(void* p, int64_t i, const float (&v)[4]) 
   }
 }
 
-// k / v [batch, kv_heads, count, D].  One workgroup per (64-key block, kv head, sequence), the blocks counted from the one
-// that holds the first position; positions outside the cache read as zeros.  A value block passes through LDS as it is
-// stored and is read 4 keys x 4 elements at a time.
+// k / v [batch, kv_heads, count, D].  One workgroup per (64-key block, kv head, sequence, keys or values), the blocks counted
+// from the one that holds the first position; positions outside the cache read as zeros.  A value block passes through
+// LDS as it is stored and is read 4 keys x 4 elements at a time.
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(wfb_kv_i8 c, const int64_t* __restrict__ start_dev, int64_t start,
                                                            int64_t count, int hkv, void* __restrict__ k,
                                                            void* __restrict__ v) {
   constexpr int kPitch = kKvBlock + 4;
   __shared__ __attribute__((aligned(16))) uint8_t vt[D * kPitch];
+  __shared__ float vs[kKvBlock];
   const int t = threadIdx.x;
-  const int64_t base = (int64_t)blockIdx.z * hkv + blockIdx.y;
+  const bool keys = (blockIdx.y & 1) == 0;
+  const int64_t base = (int64_t)blockIdx.z * hkv + (blockIdx.y >> 1);
   int64_t first = start_dev ? start_dev[blockIdx.z] : start;
   first = first < -count ? -count : first > c.cap ? c.cap : first;  // (nothing inside on either side of these)
   constexpr int64_t kUp = int64_t(1) << 30;  // (first is above -2^24: rounded down to a block, not towards zero)
@@ -159,30 +167,41 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(wfb_kv_i8 c, const in
   if (lo >= hi) return;
   const bool in = k0 >= 0 && k0 < c.cap;  // uniform (the capacity is a multiple of a block)
   const int64_t at = base * c.cap + (in ? k0 : 0), out0 = base * count + (k0 - first);  // output row of slot 0
+  if (keys) {  // 16 elements per thread
+    constexpr int L = D / 16;
+#pragma unroll
+    for (int p = 0; p < kKvBlock * L / kThreads; ++p) {
+      const int i = t + p * kThreads, slot = i / L, d0 = 16 * (i % L);
+      if (slot < lo || slot >= hi) continue;
+      v4i q = {0, 0, 0, 0};
+      float sc = 0.0f;
+      if (in) {
+        q = *reinterpret_cast<const v4i*>(c.k + (at + slot) * D + d0);
+        sc = c.k_scale[at + slot];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x[4];
+        values4((uint32_t)q[e], sc, x);
+        store4<DT>(k, (out0 + slot) * D + d0 + 4 * e, x);
+      }
+    }
+    return;
+  }
   if (in) {
-    for (int i = t; i < D * 4; i += kThreads) {
+#pragma unroll
+    for (int p = 0; p < D * 4 / kThreads; ++p) {
+      const int i = t + p * kThreads;
       const v4i q = *reinterpret_cast<const v4i*>(c.v + at * D + 16 * i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) *reinterpret_cast<int*>(&vt[i / 4 * kPitch + 16 * (i % 4) + 4 * e]) = q[e];
     }
-  }
-  // keys: 8 elements per thread
-  const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = lo * (D / 8) + t; i < hi * (D / 8); i += kThreads) {
-    const int slot = i / (D / 8), d0 = 8 * (i % (D / 8));
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (in) {
-      const float sc = c.k_scale[at + slot];
-      const uint2 q = *reinterpret_cast<const uint2*>(c.k + (at + slot) * D + d0);
-      values4(q.x, sc, x);
-      values4(q.y, sc, y);
-    }
-    store4<DT>(k, (out0 + slot) * D + d0, x);
-    store4<DT>(k, (out0 + slot) * D + d0 + 4, y);
+    if (t < kKvBlock) vs[t] = c.v_scale[at + t];
   }
   __syncthreads();
-  for (int i = t; i < (D / 4) * (kKvBlock / 4); i += kThreads) {
-    const int d0 = 4 * (i % (D / 4)), s0 = 4 * (i / (D / 4));
+#pragma unroll
+  for (int p = 0; p < (D / 4) * (kKvBlock / 4) / kThreads; ++p) {
+    const int i = t + p * kThreads, d0 = 4 * (i % (D / 4)), s0 = 4 * (i / (D / 4));
     if (s0 + 4 <= lo || s0 >= hi) continue;
     uint32_t q[4], r[4];
 #pragma unroll
@@ -192,8 +211,8 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(wfb_kv_i8 c, const in
     for (int e = 0; e < 4; ++e)
       if (s0 + e >= lo && s0 + e < hi) {
         float x[4];
-        values4(r[e], in ? c.v_scale[at + s0 + e] : 0.0f, x);
-        store4<DT>(v, (out0 + s0 + e) * D + d0, in ? x : none);
+        values4(r[e], in ? vs[s0 + e] : 0.0f, x);
+        store4<DT>(v, (out0 + s0 + e) * D + d0, x);
       }
   }
 }
@@ -203,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(wfb_kv_i8 c, const in
 hipError_t launch_kv_write_i8(int dt, int d, const void* kn, int64_t ldk, const void* vn, int64_t ldv, const float* rc,
                               const float* rs, int64_t turn, const wfb_kv_i8& c, const KvSpan& sp, int b, int hkv,
                               hipStream_t s) {
-  const dim3 grid((unsigned)((sp.t + kKvBlock - 2) / kKvBlock + 1), hkv, b);  // blocks that t positions can touch
+  const dim3 grid((unsigned)((sp.t + kKvBlock - 2) / kKvBlock + 1), 2 * hkv, b);  // blocks that t positions can touch
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, kn, ldk, vn, ldv, rc, rs, turn, c, sp, hkv); };
   if (dt == WFB_F32) d == 64 ? go(kv_write_kernel<WFB_F32, 64>) : go(kv_write_kernel<WFB_F32, 128>);
   else d == 64 ? go(kv_write_kernel<WFB_BF16, 64>) : go(kv_write_kernel<WFB_BF16, 128>);
@@ -212,7 +231,7 @@ hipError_t launch_kv_write_i8(int dt, int d, const void* kn, int64_t ldk, const 
 
 hipError_t launch_kv_read_i8(int dt, int d, const wfb_kv_i8& c, const int64_t* start_dev, int64_t start, int b,
                              int64_t count, int hkv, void* k, void* v, hipStream_t s) {
-  const dim3 grid((unsigned)((count + kKvBlock - 2) / kKvBlock + 1), hkv, b);
+  const dim3 grid((unsigned)((count + kKvBlock - 2) / kKvBlock + 1), 2 * hkv, b);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, c, start_dev, start, count, hkv, k, v); };
   if (dt == WFB_F32) d == 64 ? go(kv_read_kernel<WFB_F32, 64>) : go(kv_read_kernel<WFB_F32, 128>);
   else d == 64 ? go(kv_read_kernel<WFB_BF16, 64>) : go(kv_read_kernel<WFB_BF16, 128>);
