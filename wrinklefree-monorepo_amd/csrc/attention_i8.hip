@@ -60,14 +60,15 @@ struct Plan {
   bool pre_rows;  // the prefix by the rows kernel
 };
 
-constexpr int kLive = 768;          // workgroups that a cut call aims at: three per CU
-constexpr int kRowsWaves = 8;
-constexpr int kRowsPerGroup = 32 * kRowsWaves;  // rows (token, query head) of one workgroup of the rows kernel
-constexpr int kColumns = 16;        // rows of one workgroup of the decode kernel
+constexpr int kLive = 512;         // workgroups of four waves that fill the GPU: two per CU by their registers
+constexpr int kColumns = 16;       // rows (token, query head) of a workgroup of decode_part
+constexpr int kRowsWaves = 8;      // of a workgroup of prompt rows, 32 rows each
+constexpr int kPrefixWaves = 4;    // of a workgroup of a decode step's rows against the prefix
+constexpr int kRowsPerGroup = 32 * kRowsWaves;
 
 int cut(int64_t groups, int64_t target, int64_t most) {
   const int64_t n = target / groups;
-  return (int)(n < 1 ? 1 : n > most ? most : n);
+  return (int)(n > most ? (most < 1 ? 1 : most) : n < 1 ? 1 : n);
 }
 
 Plan make_plan(int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t cap, int64_t npre, bool lengths) {
@@ -75,11 +76,15 @@ Plan make_plan(int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t cap, int64
   Plan p{};
   p.decode = t == 1 && !lengths;
   if (p.decode) {
-    p.own = cut(b * hkv, kLive, (cb + 3) / 4);
+    // Splits of four blocks (one a wave) or more.  A cache of up to 1024 keys that needs no joining otherwise stays whole:
+    // 3 heads of 64, 32-bit, us in a graph, whole against split at a quarter and at all of 512 keys 5.3, 7.0 against 7.9,
+    // 8.5; of 1024 5.7, 9.3 against 8.5, 8.7; of 2048 8.5, 12.0 (splits of 16 blocks) against 8.6, 9.0.
+    p.own = npre == 0 && cb <= 16 ? 1 : cut(b * hkv, kLive, (cb + 3) / 4);
+    if (cb / p.own > 64) p.own = cut(b * hkv, 2 * kLive, cb);  // long splits: sequences of different lengths even out
     if (npre > 0) {
       const int64_t rows = b * g;
       p.pre_rows = rows > 64;
-      if (p.pre_rows) p.pre = cut(hkv * ((rows + kRowsPerGroup - 1) / kRowsPerGroup), 256, (pb + 3) / 4);
+      if (p.pre_rows) p.pre = cut(hkv * ((rows + 32 * kPrefixWaves - 1) / (32 * kPrefixWaves)), 256, (pb + 3) / 4);
       else p.pre = cut(hkv * ((rows + kColumns - 1) / kColumns), kLive, (pb + 3) / 4);
     }
   } else {
@@ -148,26 +153,27 @@ __device__ __forceinline__ void digits4(const int (&x)[4], uint32_t (&d)[NP]) {
   }
 }
 
-template <int DT, int D, bool PREFIX>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void kv_decode_kernel(KvAttn a, Parts parts, int slot0, int nsplit) {
-  constexpr int NP = DT == WFB_F32 ? 3 : 2;
-  constexpr int HD = D / 2, KS = D / 64, DTL = D / 16;
-  constexpr float QM = Digits<NP>::kMax;
-  __shared__ float qs[kColumns][D];
-  __shared__ __attribute__((aligned(16))) uint8_t qd[NP][kColumns][D];
-  __shared__ float qscale[kColumns];
-  __shared__ float kvn[2][D];        // the new key and value, then what the cache holds for them
-  __shared__ float snew[kColumns];
-  __shared__ float red[4][kColumns][D];
-  __shared__ float mw[4][kColumns], lw[4][kColumns];
+template <int NP, int D>
+struct DecodeShared {
+  uint8_t qd[NP][kColumns][D];  // the queries' digits
+  float red[4][kColumns][D];    // the waves' outputs
+  float mw[4][kColumns], lw[4][kColumns];
+  float qscale[kColumns], snew[kColumns];
+  float vnew[D];  // the new value as the cache holds it
+};
 
-  const int kvh = blockIdx.x, t = threadIdx.x, lane = t & 63;
+template <int DT, int D, bool PREFIX>
+__device__ __forceinline__ void decode_part(const KvAttn& a, const Parts& parts, int slot0, int nsplit, int kvh, int rowblock,
+                                            int split, DecodeShared<DT == WFB_F32 ? 3 : 2, D>& sh) {
+  constexpr int NP = DT == WFB_F32 ? 3 : 2;
+  constexpr int HD = D / 2, KS = D / 64, DTL = D / 16, E = D / 64;
+  constexpr float QM = Digits<NP>::kMax;
+  const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int g = a.hq / a.hkv;
-  const int split = blockIdx.z;
   const int grp = lane >> 4, col = lane & 15;
   // rows of this workgroup: the heads of one sequence, or the next 16 of all sequences' (sequence, head) pairs
-  const int b0 = PREFIX ? 0 : blockIdx.y, r0 = PREFIX ? (int)blockIdx.y * kColumns : 0;
+  const int b0 = PREFIX ? 0 : rowblock, r0 = PREFIX ? rowblock * kColumns : 0;
   const int nrows = PREFIX ? (a.b * g - r0 < kColumns ? a.b * g - r0 : kColumns) : g;
   int64_t pos = 0;
   int n1 = 1;
@@ -215,107 +221,127 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
     for (int n = 0; n < 4; ++n) sv[n] = buf_load16(vsb, off + 16 * n);
   };
+  // ---- a wave's rows w, w + 4, .. and the new key, elements lane and lane + 64, and the first block's loads: these come
+  // last, since loads complete in the order of their issue
+  float x[4][E], xc[4], xs[4], kn[E], vn[E];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = w + 4 * i;  // uniform
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[i][e] = 0.0f;
+    xc[i] = 1.0f;
+    xs[i] = 0.0f;
+    if (r >= nrows) continue;
+    const int sb = PREFIX ? (r0 + r) / g : b0, h = kvh * g + (PREFIX ? (r0 + r) % g : r);
+    int64_t p = pos;
+    if constexpr (PREFIX)
+      if (!kv_span(a.span, sb, p, n1)) continue;  // (its result is not used)
+    const int64_t off = (int64_t)sb * a.ldq + (int64_t)h * D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[i][e] = load_elem<DT>(a.q, off + lane + 64 * e);
+    if (a.rc) {
+      xc[i] = a.rc[(p + a.npre) * HD + lane % HD];
+      xs[i] = a.rs[(p + a.npre) * HD + lane % HD];
+    }
+  }
+  float kc = 1.0f, ks = 0.0f;
+  if (owns_new) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      kn[e] = load_elem<DT>(a.kn, (int64_t)b0 * a.ldk + (int64_t)kvh * D + lane + 64 * e);
+      vn[e] = load_elem<DT>(a.vn, (int64_t)b0 * a.ldv + (int64_t)kvh * D + lane + 64 * e);
+    }
+    if (a.rc) {
+      kc = a.rc[(pos + a.npre) * HD + lane % HD];
+      ks = a.rs[(pos + a.npre) * HD + lane % HD];
+    }
+  }
   int64_t kb = kb0 + w;
   if (kb < kb1) {
     load_k(kb);
     load_s(kb);
     load_v(kb);
   }
-
-  // ---- the rows' queries, the new key and value
-  auto turn_pair = [&](float& x1, float& x2, int64_t p, int j) {
-    if (!a.rc) return;
-    const float cs = a.rc[p * HD + j], sn = a.rs[p * HD + j];
-    const float y1 = __fsub_rn(__fmul_rn(x1, cs), __fmul_rn(x2, sn));
-    x2 = __fadd_rn(__fmul_rn(x2, cs), __fmul_rn(x1, sn));
-    x1 = y1;
+  auto turn = [&](float (&y)[E], float cs, float sn) {  // (tables of ones and zeros where there are none)
+    if constexpr (E == 2) {
+      const float y1 = __fsub_rn(__fmul_rn(y[0], cs), __fmul_rn(y[1], sn));
+      y[1] = __fadd_rn(__fmul_rn(y[1], cs), __fmul_rn(y[0], sn));
+      y[0] = y1;
+    } else {
+      const float other = xor_lanes_f32<32>(y[0]), p = __fmul_rn(y[0], cs), q = __fmul_rn(other, sn);
+      y[0] = lane < 32 ? __fsub_rn(p, q) : __fadd_rn(p, q);
+    }
   };
-  for (int i = t; i < nrows * HD; i += kThreads) {
-    const int r = i / HD, j = i % HD;
-    const int sb = PREFIX ? (r0 + r) / g : b0, h = kvh * g + (PREFIX ? (r0 + r) % g : r);
-    int64_t p = pos;
-    bool fits = true;
-    if constexpr (PREFIX) fits = kv_span(a.span, sb, p, n1);
-    float x1 = 0.0f, x2 = 0.0f;
-    if (fits) {
-      const int64_t off = (int64_t)sb * a.ldq + (int64_t)h * D + j;
-      x1 = load_elem<DT>(a.q, off);
-      x2 = load_elem<DT>(a.q, off + HD);
-      turn_pair(x1, x2, p + a.npre, j);
-    }
-    qs[r][j] = x1;
-    qs[r][j + HD] = x2;
-  }
-  if (owns_new) {
-    if (t < HD) {
-      const int64_t off = (int64_t)b0 * a.ldk + (int64_t)kvh * D + t;
-      float x1 = load_elem<DT>(a.kn, off), x2 = load_elem<DT>(a.kn, off + HD);
-      turn_pair(x1, x2, pos + a.npre, t);
-      kvn[0][t] = x1;
-      kvn[0][t + HD] = x2;
-    } else if (t >= 128 && t - 128 < D) {
-      kvn[1][t - 128] = load_elem<DT>(a.vn, (int64_t)b0 * a.ldv + (int64_t)kvh * D + t - 128);
-    }
-  }
-  __syncthreads();
-  for (int r = w; r < kColumns; r += 4) {  // uniform: a wave takes a row
-    float x[D / 64];
+  auto largest = [&](const float (&y)[E]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      x[e] = r < nrows ? qs[r][lane + 64 * e] : 0.0f;
-      m = umax(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    for (int e = 0; e < E; ++e) m = umax(m, __float_as_uint(y[e]) & 0x7fffffffu);
+    return wave_umax(m);
+  };
+  if (owns_new) {  // every wave forms the key that the cache holds, wave 0 writes it, wave 1 the value
+    if (a.rc) turn(kn, kc, ks);
+    float scale, inv;
+    kv_scale(largest(kn), scale, inv);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int q = kv_code(kn[e], inv);
+      if (w == 0) a.own.k[(base * c.cap + pos) * D + lane + 64 * e] = (int8_t)q;
+      kn[e] = (float)q * scale;
     }
-    m = wave_umax(m);
+    if (w == 0 && lane == 0) a.own.k_scale[base * c.cap + pos] = scale;
+    if (w == 1) {
+      kv_scale(largest(vn), scale, inv);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int q = kv_code(vn[e], inv);
+        a.own.v[(base * c.cap + pos / kKvBlock * kKvBlock) * D + (int64_t)(lane + 64 * e) * kKvBlock + pos % kKvBlock] =
+            (int8_t)q;
+        sh.vnew[lane + 64 * e] = (float)q * scale;
+      }
+      if (lane == 0) a.own.v_scale[base * c.cap + pos] = scale;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = w + 4 * i;
+    if (i > 0 && r >= (nrows + 3) / 4 * 4) {  // uniform: rows of zeros
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+#pragma unroll
+        for (int e = 0; e < E; ++e) sh.qd[n][r][lane + 64 * e] = 0;
+      if (lane == 0) sh.qscale[r] = 0.0f;
+      continue;
+    }
+    if (a.rc) turn(x[i], xc[i], xs[i]);
+    const uint32_t m = largest(x[i]);
     const float mf = __uint_as_float(m);
     const bool some = m < 0x7f800000u && mf >= kKvTiny;
     const float inv = some ? (a.scale < 0.0f ? -QM : QM) / mf : 0.0f;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      const int q = some ? (int)__builtin_rintf(x[e] * inv) : 0;
+    for (int e = 0; e < E; ++e) {
+      const int q = some ? (int)__builtin_rintf(x[i][e] * inv) : 0;
       const uint32_t u = (uint32_t)q + (NP == 2 ? 0x80u : 0x8080u);
 #pragma unroll
       for (int n = 0; n < NP; ++n)
-        qd[n][r][lane + 64 * e] = (uint8_t)((u >> 8 * (NP - 1 - n)) ^ (n == 0 ? 0u : 0x80u));
+        sh.qd[n][r][lane + 64 * e] = (uint8_t)((u >> 8 * (NP - 1 - n)) ^ (n == 0 ? 0u : 0x80u));
     }
     if (lane == 0)  // one step of the digits in units of the exponent of two; NaN for a row with one
-      qscale[r] = m >= 0x7f800000u ? __builtin_nanf("") : some ? mf * (1.0f / QM) * (fabsf(a.scale) * kLog2e) : 0.0f;
-  }
-  if (owns_new && w < 2) {  // wave 0 the key, wave 1 the value: into the cache, and back as the values it stands for
-    float x[D / 64];
-    uint32_t m = 0;
+      sh.qscale[r] = m >= 0x7f800000u ? __builtin_nanf("") : some ? mf * (1.0f / QM) * (fabsf(a.scale) * kLog2e) : 0.0f;
+    if (owns_new) {
+      float p = 0.0f;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      x[e] = kvn[w][lane + 64 * e];
-      m = umax(m, __float_as_uint(x[e]) & 0x7fffffffu);
-    }
-    float scale, inv;
-    kv_scale(wave_umax(m), scale, inv);
-    if (lane == 0) (w == 0 ? a.own.k_scale : a.own.v_scale)[base * c.cap + pos] = scale;
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      const int j = lane + 64 * e, q = kv_code(x[e], inv);
-      if (w == 0) a.own.k[(base * c.cap + pos) * D + j] = (int8_t)q;
-      else a.own.v[(base * c.cap + pos / kKvBlock * kKvBlock) * D + (int64_t)j * kKvBlock + pos % kKvBlock] = (int8_t)q;
-      kvn[w][j] = (float)q * scale;
+      for (int e = 0; e < E; ++e) p += x[i][e] * kn[e];
+      p = wave_sum(p);
+      if (lane == 0) sh.snew[r] = p * (a.scale * kLog2e);
     }
   }
   __syncthreads();
-  if (owns_new) {
-    for (int r = w; r < nrows; r += 4) {
-      float p = 0.0f;
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) p += qs[r][lane + 64 * e] * kvn[0][lane + 64 * e];
-      p = wave_sum(p);
-      if (lane == 0) snew[r] = p * (a.scale * kLog2e);
-    }
-  }
   v4i qf[NP][KS];
 #pragma unroll
   for (int n = 0; n < NP; ++n)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[n][s] = *reinterpret_cast<const v4i*>(&qd[n][col][64 * s + 16 * grp]);
-  const float cq = qscale[col];
+    for (int s = 0; s < KS; ++s) qf[n][s] = *reinterpret_cast<const v4i*>(&sh.qd[n][col][64 * s + 16 * grp]);
+  const float cq = sh.qscale[col];
 
   float o[DTL][4];
 #pragma unroll
@@ -411,36 +437,36 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   l_run += xor_lanes_f32<16>(l_run);
   l_run += xor_lanes_f32<32>(l_run);
   if (grp == 0) {
-    mw[w][col] = m_run;
-    lw[w][col] = l_run;
+    sh.mw[w][col] = m_run;
+    sh.lw[w][col] = l_run;
   }
   if (col < nrows) {
 #pragma unroll
     for (int d = 0; d < DTL; ++d)
-      *reinterpret_cast<float4*>(&red[w][col][16 * d + 4 * grp]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+      *reinterpret_cast<float4*>(&sh.red[w][col][16 * d + 4 * grp]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
   }
   __syncthreads();
   // the four waves and the new key, four elements of a row per thread
   for (int i = t; i < nrows * (D / 4); i += kThreads) {
     const int r = i / (D / 4), j = 4 * (i % (D / 4));
-    float m = fmaxf(fmaxf(mw[0][r], mw[1][r]), fmaxf(mw[2][r], mw[3][r]));
-    if (owns_new) m = fmaxf(m, snew[r]);
+    float m = fmaxf(fmaxf(sh.mw[0][r], sh.mw[1][r]), fmaxf(sh.mw[2][r], sh.mw[3][r]));
+    if (owns_new) m = fmaxf(m, sh.snew[r]);
     float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const float e = __builtin_amdgcn_exp2f(mw[x][r] - m);
-      const float4 f = *reinterpret_cast<const float4*>(&red[x][r][j]);
-      l += lw[x][r] * e;
+      const float e = __builtin_amdgcn_exp2f(sh.mw[x][r] - m);
+      const float4 f = *reinterpret_cast<const float4*>(&sh.red[x][r][j]);
+      l += sh.lw[x][r] * e;
       v[0] += f.x * e;
       v[1] += f.y * e;
       v[2] += f.z * e;
       v[3] += f.w * e;
     }
     if (owns_new) {
-      const float e = __builtin_amdgcn_exp2f(snew[r] - m);
+      const float e = __builtin_amdgcn_exp2f(sh.snew[r] - m);
       l += e;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v[x] += e * kvn[1][j + x];
+      for (int x = 0; x < 4; ++x) v[x] += e * sh.vnew[j + x];
     }
     const int sb = PREFIX ? (r0 + r) / g : b0, h = kvh * g + (PREFIX ? (r0 + r) % g : r);
     if (parts.o) {
@@ -490,9 +516,17 @@ __device__ __forceinline__ void f16_parts(float x0, float x1, uint32_t (&part)[N
 //   O^T[d, row] += V^T W^T        w = p v_scale / (reference of the scales) in fp16 (fp32 rows: two parts)
 // As in the decode kernel the key of a score tile's row is chosen so that a lane holds the keys that it feeds into the
 // second product, 8 consecutive ones per step.
+template <int D>
+struct RowsShared {
+  uint16_t tile[2][2][kKvBlock * D];  // [buffer][keys, values]
+  // scales of a block's keys and values and of the two behind it; svs: as fp16 if kScaled
+  float sks[3][kKvBlock], svs[3][kKvBlock];
+  float vref_s[3];
+};
+
 template <int DT, int D, int W, bool PREFIX>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void kv_rows_kernel(KvAttn a, Parts parts,
-                                                                                                int slot0, int nsplit) {
+__device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, int slot0, int nsplit, int block_id,
+                                          RowsShared<D>& sh) {
   constexpr int NP = DT == WFB_F32 ? 2 : 1;
   constexpr int kRows = 32 * W;
   // With one part the values' scales are multiplied into their codes as these become fp16 (two roundings to 11 bits of a
@@ -510,17 +544,17 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
   constexpr int PT = 2 * KP / (64 * W);    // per thread
   static_assert(PT * 64 * W == 2 * KP && KP % 64 == 0, "whole waves take keys or values");
   static_assert(KP % (64 * W) == 0 || D == kKvBlock, "a round of keys and values needs rows of one length");
-  __shared__ __attribute__((aligned(16))) uint16_t tile[2][2][kKvBlock * D];  // [buffer][keys, values]
-  // scales of a block's keys and values and of the two behind it; svs: as fp16 if kScaled
-  __shared__ __attribute__((aligned(16))) float sks[3][kKvBlock], svs[3][kKvBlock];
-  __shared__ float vref_s[3];
+  auto& tile = sh.tile;
+  auto& sks = sh.sks;
+  auto& svs = sh.svs;
+  auto& vref_s = sh.vref_s;
 
   const int g = a.hq / a.hkv;
   const int nhb = PREFIX ? a.hkv : a.hkv * a.b;
   const int64_t R = PREFIX ? (int64_t)a.b * g : (int64_t)a.t * g;
   const int nrb = (int)((R + kRows - 1) / kRows);
   // the heads' workgroups are nhb apart, so an XCD's L2 holds few heads; the longest rows (the last) come first
-  const int hb = blockIdx.x % nhb, rest = blockIdx.x / nhb;
+  const int hb = block_id % nhb, rest = block_id / nhb;
   const int split = rest % nsplit, rb = nrb - 1 - rest / nsplit;
   const int kvh = hb % a.hkv, b = hb / a.hkv;
   const int t = threadIdx.x, lane = t & 63;
@@ -549,7 +583,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
     if (!fits || tok0 >= n) {  // uniform: no row here
       if (!parts.o && r < R) {
         const float v = fits ? 0.0f : __builtin_nanf("");
-        for (int j = grp; j < D; j += 2) store_elem<DT>(a.out, qrow * a.ldo + (int64_t)h * D + j, v);
+        const float v4[4] = {v, v, v, v};
+        for (int j = 4 * grp; j < D; j += 8) store4<DT>(a.out, qrow * a.ldo + (int64_t)h * D + j, v4);
       }
       return;
     }
@@ -559,6 +594,44 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
   const int64_t pb = (a.npre + kKvBlock - 1) / kKvBlock, nb = pb + (own + kKvBlock - 1) / kKvBlock;
   const int64_t per = (nb + nsplit - 1) / nsplit;
   const int64_t kb0 = split * per, kb1 = kb0 + per < nb ? kb0 + per : nb;
+
+  // ---- staging: K row-major [key][D], V as it is [element][64 keys], 16-byte chunks at chunk ^ (row's swizzle) so that
+  // 16 lanes reading one chunk of 16 rows meet 16 different bank groups
+  auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
+  auto vswz = [](int d) { return (d >> 1) & 7; };
+  v4i raw[2][PT] = {};  // codes of the next block and of the one behind it
+  auto place = [&](int64_t kb, const wfb_kv_i8*& c, int64_t& at, int64_t& left) {  // uniform
+    const bool in_pre = kb < pb;
+    const int64_t k0 = (in_pre ? kb : kb - pb) * kKvBlock;
+    c = in_pre ? &a.pre : &a.own;
+    at = (in_pre ? kvh : (int64_t)b * a.hkv + kvh) * c->cap + k0;
+    left = (in_pre ? a.npre : own) - k0;
+  };
+  auto fetch_codes = [&](int64_t kb, int set) {
+    const wfb_kv_i8* c;
+    int64_t at, left;
+    place(kb, c, at, left);
+    const buf_t kb_ = make_buf(c->k + at * D, kKvBlock * D), vb_ = make_buf(c->v + at * D, kKvBlock * D);
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const int p0 = 64 * (w + i * W);  // uniform
+      raw[set][i] = p0 < KP ? buf_load16(kb_, 16 * (p0 + lane)) : buf_load16(vb_, 16 * (p0 - KP + lane));
+    }
+  };
+  float sk = 0.0f, sv = 0.0f;  // (waves 0 and 1) the scales of key `lane`, zeros behind the last key
+  auto fetch_scales = [&](int64_t kb) {
+    if (w >= 2) return;
+    const wfb_kv_i8* c;
+    int64_t at, left;
+    place(kb, c, at, left);
+    const uint32_t bytes = 4 * (uint32_t)(left < kKvBlock ? left : kKvBlock);
+    sk = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->k_scale + at, bytes), 4 * lane, 0, 0));
+    sv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->v_scale + at, bytes), 4 * lane, 0, 0));
+  };
+  if (kb0 < kb1) {  // under way while the queries are formed
+    fetch_scales(kb0);
+    fetch_codes(kb0, 0);
+  }
 
   // ---- the row's query in fp16 of its largest: lane holds elements 16 s + 8 grp .. + 7
   v4i qf[NP][KS];
@@ -622,39 +695,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float m_ref = kNoMax, l_run = 0.0f, vref = 0x1p-100f;
 
-  // ---- staging: K row-major [key][D], V as it is [element][64 keys], 16-byte chunks at chunk ^ (row's swizzle) so that
-  // 16 lanes reading one chunk of 16 rows meet 16 different bank groups
-  auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
-  auto vswz = [](int d) { return (d >> 1) & 7; };
-  v4i raw[2][PT] = {};  // codes of the next block and of the one behind it
-  auto place = [&](int64_t kb, const wfb_kv_i8*& c, int64_t& at, int64_t& left) {  // uniform
-    const bool in_pre = kb < pb;
-    const int64_t k0 = (in_pre ? kb : kb - pb) * kKvBlock;
-    c = in_pre ? &a.pre : &a.own;
-    at = (in_pre ? kvh : (int64_t)b * a.hkv + kvh) * c->cap + k0;
-    left = (in_pre ? a.npre : own) - k0;
-  };
-  auto fetch_codes = [&](int64_t kb, int set) {
-    const wfb_kv_i8* c;
-    int64_t at, left;
-    place(kb, c, at, left);
-    const buf_t kb_ = make_buf(c->k + at * D, kKvBlock * D), vb_ = make_buf(c->v + at * D, kKvBlock * D);
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int p0 = 64 * (w + i * W);  // uniform
-      raw[set][i] = p0 < KP ? buf_load16(kb_, 16 * (p0 + lane)) : buf_load16(vb_, 16 * (p0 - KP + lane));
-    }
-  };
-  float sk = 0.0f, sv = 0.0f;  // (waves 0 and 1) the scales of key `lane`, zeros behind the last key
-  auto fetch_scales = [&](int64_t kb) {
-    if (w >= 2) return;
-    const wfb_kv_i8* c;
-    int64_t at, left;
-    place(kb, c, at, left);
-    const uint32_t bytes = 4 * (uint32_t)(left < kKvBlock ? left : kKvBlock);
-    sk = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->k_scale + at, bytes), 4 * lane, 0, 0));
-    sv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->v_scale + at, bytes), 4 * lane, 0, 0));
-  };
   float ref = 0x1p-100f;  // (wave 1) reference of the value scales so far
   auto stage_scales = [&](int slot) {
     // a value row that is not finite makes NaN of its key's scores, which a mask can take away, and counts as zeros
@@ -872,8 +912,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
   };
 
   if (kb0 < kb1) {
-    fetch_codes(kb0, 0);
-    fetch_scales(kb0);
     stage_scales(0);
     if (kb0 + 1 < kb1) {
       fetch_scales(kb0 + 1);
@@ -927,6 +965,44 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
       for (int x = 0; x < 4; ++x) v[x] = valid ? o[d][i + x] * f : 0.0f;
       store4<DT>(a.out, qrow * a.ldo + (int64_t)h * D + 32 * d + 2 * i + 4 * grp, v);
     }
+}
+
+// ---- kernels ------------------------------------------------------------------------------------------
+
+enum class Prefix { None, Columns, Rows };
+
+// A decode step: the workgroups of the prefix, if there is one, then those of the sequences' own keys.
+template <int DT, int D, Prefix P>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void kv_decode_kernel(KvAttn a, Parts parts,
+                                                                                                     Plan plan) {
+  using Own = DecodeShared<DT == WFB_F32 ? 3 : 2, D>;
+  constexpr size_t kRowsBytes = P == Prefix::Rows ? sizeof(RowsShared<D>) : 0;
+  __shared__ __attribute__((aligned(16))) char smem[kRowsBytes > sizeof(Own) ? kRowsBytes : sizeof(Own)];
+  const int rows = a.b * (a.hq / a.hkv);
+  int block = blockIdx.x;
+  if constexpr (P != Prefix::None) {
+    constexpr int kEach = P == Prefix::Rows ? 32 * kPrefixWaves : kColumns;
+    const int nrb = (rows + kEach - 1) / kEach, mine = nrb * a.hkv * plan.pre;
+    if (block < mine) {
+      if constexpr (P == Prefix::Rows)
+        rows_part<DT, D, kPrefixWaves, true>(a, parts, plan.own, plan.pre, block, *reinterpret_cast<RowsShared<D>*>(smem));
+      else
+        decode_part<DT, D, true>(a, parts, plan.own, plan.pre, block % a.hkv, block / a.hkv % nrb, block / a.hkv / nrb,
+                                 *reinterpret_cast<Own*>(smem));
+      return;
+    }
+    block -= mine;
+  }
+  decode_part<DT, D, false>(a, parts, 0, plan.own, block % a.hkv, block / a.hkv % a.b, block / a.hkv / a.b,
+                            *reinterpret_cast<Own*>(smem));
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kRowsWaves) __attribute__((amdgpu_waves_per_eu(2))) void kv_rows_kernel(KvAttn a,
+                                                                                                         Parts parts,
+                                                                                                         Plan plan) {
+  __shared__ __attribute__((aligned(16))) RowsShared<D> sh;
+  rows_part<DT, D, kRowsWaves, false>(a, parts, 0, plan.own, blockIdx.x, sh);
 }
 
 // ---- joining ----------------------------------------------------------------------------------------
@@ -1020,25 +1096,22 @@ hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
   const int g = a.hq / a.hkv;
   hipError_t e;
   if (p.decode) {
-    hipLaunchKernelGGL((kv_decode_kernel<DT, D, false>), dim3(a.hkv, a.b, p.own), dim3(kThreads), 0, s, a, parts, 0, p.own);
+    const int rows = a.b * g, each = p.pre_rows ? 32 * kPrefixWaves : kColumns;
+    const int64_t groups = (int64_t)a.hkv * a.b * p.own + (int64_t)(rows + each - 1) / each * a.hkv * p.pre;
+    if (groups > INT32_MAX) return hipErrorInvalidValue;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), 0, s, a, parts, p);
+    };
+    if (p.pre == 0) go(kv_decode_kernel<DT, D, Prefix::None>);
+    else if (p.pre_rows) go(kv_decode_kernel<DT, D, Prefix::Rows>);
+    else go(kv_decode_kernel<DT, D, Prefix::Columns>);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    if (p.pre > 0) {
-      const int rows = a.b * g;
-      if (p.pre_rows)
-        hipLaunchKernelGGL((kv_rows_kernel<DT, D, kRowsWaves, true>),
-                           dim3((unsigned)((rows + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * p.pre)), dim3(64 * kRowsWaves), 0,
-                           s, a, parts, p.own, p.pre);
-      else
-        hipLaunchKernelGGL((kv_decode_kernel<DT, D, true>), dim3(a.hkv, (rows + kColumns - 1) / kColumns, p.pre),
-                           dim3(kThreads), 0, s, a, parts, p.own, p.pre);
-      if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
   } else {
     e = launch_kv_write_i8(a.dt, a.d, a.kn, a.ldk, a.vn, a.ldv, a.rc, a.rs, a.npre, a.own, a.span, a.b, a.hkv, s);
     if (e != hipSuccess) return e;
     const int64_t groups = ((int64_t)a.t * g + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * a.b * p.own;
     if (groups > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((kv_rows_kernel<DT, D, kRowsWaves, false>), dim3((unsigned)groups), dim3(64 * kRowsWaves), 0, s, a, parts, 0, p.own);
+    hipLaunchKernelGGL((kv_rows_kernel<DT, D>), dim3((unsigned)groups), dim3(64 * kRowsWaves), 0, s, a, parts, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!has_parts(p)) return hipSuccess;

@@ -1012,8 +1012,8 @@ def kv_cache_i8(batch: int, kv_heads: int, max_len: int, head_dim: int, device="
                      z(torch.float32, batch, kv_heads, cap))
 
 
-def _cache_i8(name: str, what: str, cache) -> Tuple["_lib.KvI8Struct", int, int, int, int]:
-    """(C struct, batch, kv_heads, cap, head_dim) of the four tensors of an int8 cache."""
+def _cache_i8(name: str, what: str, cache):
+    """(C struct, batch, kv_heads, cap, head_dim, device index) of the four tensors of an int8 cache."""
     if len(cache) != 4:
         raise RuntimeError(f"{name}: {what} must be the four tensors k, k_scale, v, v_scale")
     k, ks, v, vs = cache
@@ -1024,45 +1024,50 @@ def _cache_i8(name: str, what: str, cache) -> Tuple["_lib.KvI8Struct", int, int,
     if cap % WFB_KV_I8_BLOCK or v.shape != (b, h, cap // WFB_KV_I8_BLOCK, d, WFB_KV_I8_BLOCK) \
             or ks.shape != (b, h, cap) or vs.shape != (b, h, cap):
         raise RuntimeError(f"{name}: {what}'s tensors do not belong together: {[tuple(t.shape) for t in cache]}")
-    return _lib.KvI8Struct(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), cap), b, h, cap, d
+    index = k.get_device()
+    if index < 0 or ks.get_device() != index or v.get_device() != index or vs.get_device() != index \
+            or not (k.is_contiguous() and ks.is_contiguous() and v.is_contiguous() and vs.is_contiguous()):
+        _require_gpu(name, k, ks, v, vs)  # says what is wrong
+    return _lib.KvI8Struct(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), cap), b, h, cap, d, index
 
 
-def _per_sequence(name: str, what: str, x, b: int, dev: torch.device) -> Tuple[Optional[int], int]:
+def _per_sequence(name: str, what: str, x, b: int, index: int) -> Tuple[Optional[int], int]:
     """(device pointer or None, host value) of an int or an int64 device tensor [batch]."""
     if not isinstance(x, torch.Tensor):
         return None, int(x)
-    if x.dtype != torch.int64 or x.numel() != b or x.device != dev or not x.is_contiguous():
-        raise RuntimeError(f"{name}: {what} must be an int or contiguous int64 [{b}] on {dev}")
+    if x.dtype != torch.int64 or x.numel() != b or x.get_device() != index or not x.is_contiguous():
+        raise RuntimeError(f"{name}: {what} must be an int or contiguous int64 [{b}] on the cache's device")
     return x.data_ptr(), 0
 
 
-def _rows16(name: str, x: torch.Tensor, rows: int, width: int, dtype: torch.dtype, dev: torch.device):
+def _rows16(name: str, x: torch.Tensor, rows: int, width: int, dtype: torch.dtype, index: int):
     """(view or copy of x as [rows, width], row stride) with rows that start on 16 bytes."""
-    if x.dtype != dtype or x.device != dev or x.numel() != rows * width:
-        raise RuntimeError(f"{name}: expected {rows} x {width} elements of {dtype} on {dev}, got {tuple(x.shape)} "
-                           f"{x.dtype} on {x.device}")
+    if x.dtype != dtype or x.get_device() != index or x.numel() != rows * width:
+        raise RuntimeError(f"{name}: expected {rows} x {width} elements of {dtype} on the cache's device, got "
+                           f"{tuple(x.shape)} {x.dtype} on {x.device}")
     x2 = x if x.dim() == 2 and x.shape[0] == rows else x.reshape(rows, width)
-    per16 = 16 // x2.element_size()
-    ld = x2.stride(0) if rows > 1 else width
-    if x2.stride(1) != 1 or ld % per16 or x2.data_ptr() % 16 or ld < width:
-        x2 = torch.empty((rows, width), dtype=dtype, device=dev).copy_(x2)
+    size = 4 if dtype is torch.float32 else 2
+    inner, ld = x2.stride(1), x2.stride(0) if rows > 1 else width
+    if inner != 1 or ld * size % 16 or ld < width or x2.data_ptr() % 16:
+        x2 = torch.empty((rows, width), dtype=dtype, device=x.device).copy_(x2)
         ld = width
     return x2, ld
 
 
-def _rope_i8(name: str, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], d: int, dev: torch.device):
+def _rope_i8(name: str, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], d: int, index: int):
     """(cos, sin, rows) of the rotary tables, which may be longer than the cache."""
     if cos is None and sin is None:
         return None, None, 0
     if cos is None or sin is None:
         raise RuntimeError(f"{name}: give both rope tables or neither")
-    for x in (cos, sin):
-        if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != d // 2 or x.device != dev \
-                or not x.is_contiguous() or x.shape != cos.shape:
-            raise RuntimeError(f"{name}: rope tables must be contiguous fp32 [positions, {d // 2}] on {dev}")
+    shape = cos.shape
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or shape[1] != d // 2 \
+            or sin.shape != shape or cos.get_device() != index or sin.get_device() != index \
+            or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise RuntimeError(f"{name}: rope tables must be contiguous fp32 [positions, {d // 2}] on the cache's device")
     if cos.data_ptr() % 16 or sin.data_ptr() % 16:
         cos, sin = cos.clone(), sin.clone()
-    return cos, sin, cos.shape[0]
+    return cos, sin, shape[0]
 
 
 def kv_cache_write_i8(
@@ -1078,16 +1083,17 @@ def kv_cache_write_i8(
     sequence that are real (t by default); a sequence whose positions do not fit is not written (a start given as an int
     is checked here).  Position p takes row p + rope_offset of the tables."""
     name = "kv_cache_write_i8"
-    st, b, h, _, d = _cache_i8(name, "cache", cache)
-    dev = _require_gpu(name, *cache)
+    st, b, h, _, d, index = _cache_i8(name, "cache", cache)
+    dev = cache[0].device
     t = int(t)
-    k2, ldk = _rows16(name, k_new, b * t, h * d, k_new.dtype, dev)
-    v2, ldv = _rows16(name, v_new, b * t, h * d, k_new.dtype, dev)
-    cos, sin, n_rope = _rope_i8(name, rope_cos, rope_sin, d, dev)
-    s_dev, s_host = _per_sequence(name, "start", start, b, dev)
-    l_dev = None if lengths is None else _per_sequence(name, "lengths", lengths, b, dev)[0]
+    dt = _float_dtype(name, k_new)
+    k2, ldk = _rows16(name, k_new, b * t, h * d, k_new.dtype, index)
+    v2, ldv = _rows16(name, v_new, b * t, h * d, k_new.dtype, index)
+    cos, sin, n_rope = _rope_i8(name, rope_cos, rope_sin, d, index)
+    s_dev, s_host = _per_sequence(name, "start", start, b, index)
+    l_dev = None if lengths is None else _per_sequence(name, "lengths", lengths, b, index)[0]
     with _on(dev):
-        _lib.call("wfb_kv_write_i8", _p(k2), ldk, _p(v2), ldv, _float_dtype(name, k2), _p(cos), _p(sin), n_rope,
+        _lib.call("wfb_kv_write_i8", k2.data_ptr(), ldk, v2.data_ptr(), ldv, dt, _p(cos), _p(sin), n_rope,
                   int(rope_offset), ctypes.addressof(st), s_dev, s_host, l_dev, b, t, h, d, _stream(dev))
 
 
@@ -1097,60 +1103,63 @@ def kv_cache_read_i8(
     """(k, v) [batch, kv_heads, count, head_dim] of ``dtype`` (float32 or bfloat16): what an int8 cache holds at positions
     start .. start + count - 1 (``start`` an int or int64 [batch] on the device); zeros outside the cache."""
     name = "kv_cache_read_i8"
-    st, b, h, _, d = _cache_i8(name, "cache", cache)
-    dev = _require_gpu(name, *cache)
+    st, b, h, _, d, index = _cache_i8(name, "cache", cache)
+    dev = cache[0].device
     if dtype not in (torch.float32, torch.bfloat16):
         raise RuntimeError(f"{name}: dtype must be float32 or bfloat16, got {dtype}")
-    s_dev, s_host = _per_sequence(name, "start", start, b, dev)
-    k = torch.empty((b, h, int(count), d), dtype=dtype, device=dev)
+    s_dev, s_host = _per_sequence(name, "start", start, b, index)
+    count = int(count)
+    k = torch.empty((b, h, count, d), dtype=dtype, device=dev)
     v = torch.empty_like(k)
     with _on(dev):
-        _lib.call("wfb_kv_read_i8", ctypes.addressof(st), s_dev, s_host, b, int(count), h, d, _p(k), _p(v), _DT[dtype],
-                  _stream(dev))
+        _lib.call("wfb_kv_read_i8", ctypes.addressof(st), s_dev, s_host, b, count, h, d, k.data_ptr(), v.data_ptr(),
+                  _DT[dtype], _stream(dev))
     return k, v
 
 
 def _attention_i8(name, q, k_new, v_new, cache, start, t, rope_cos, rope_sin, scale, out, lengths, prefix, prefix_len):
-    st, b, h, cap, d = _cache_i8(name, "cache", cache)
-    dev = _require_gpu(name, *cache)
+    st, b, h, cap, d, index = _cache_i8(name, "cache", cache)
+    dev = cache[0].device
     rows = b * t
-    prefix_len = int(prefix_len)
-    pst = None
+    p_ptr, prefix_len = None, int(prefix_len)
     if prefix is not None:
-        pst, pb, ph, _, pd = _cache_i8(name, "prefix", prefix)
-        if pb != 1 or ph != h or pd != d or _require_gpu(name, *prefix) != dev:
+        pst, pb, ph, _, pd, p_index = _cache_i8(name, "prefix", prefix)
+        if pb != 1 or ph != h or pd != d or p_index != index:
             raise RuntimeError(f"{name}: prefix must be an int8 cache of one sequence with {h} kv heads of {d} on {dev}")
-    if q.dtype not in (torch.float32, torch.bfloat16):
-        raise RuntimeError(f"{name}: dtype must be float32 or bfloat16, got {q.dtype}")
+        p_ptr = ctypes.addressof(pst)
+    dtype = q.dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{name}: dtype must be float32 or bfloat16, got {dtype}")
     if rows == 0:
         return q.new_empty((0, q.shape[-1])) if out is None else out
-    if q.numel() % (rows * d) != 0:
-        raise RuntimeError(f"{name}: q has {q.numel()} elements, not a multiple of {rows} rows of head_dim")
-    hq = q.numel() // (rows * d)
-    q2, ldq = _rows16(name, q, rows, hq * d, q.dtype, dev)
-    k2, ldk = _rows16(name, k_new, rows, h * d, q.dtype, dev)
-    v2, ldv = _rows16(name, v_new, rows, h * d, q.dtype, dev)
-    cos, sin, n_rope = _rope_i8(name, rope_cos, rope_sin, d, dev)
-    s_dev, s_host = _per_sequence(name, "start", start, b, dev)
-    l_dev = None if lengths is None else _per_sequence(name, "lengths", lengths, b, dev)[0]
-    if out is not None and (out.dtype != q.dtype or out.shape != (rows, hq * d) or out.device != dev):
-        raise RuntimeError(f"{name}: out must be [{rows}, {hq * d}] {q.dtype} on {dev}")
-    o2 = out
-    if out is None or out.stride(1) != 1 or out.data_ptr() % 16 \
-            or (rows > 1 and (out.stride(0) * out.element_size() % 16 or out.stride(0) < hq * d)):
-        o2 = torch.empty((rows, hq * d), dtype=q.dtype, device=dev)
-    ldo = o2.stride(0) if rows > 1 else hq * d
-    size = ctypes.c_int64(0)
-    _lib.call("wfb_gqa_attention_i8_workspace", b, t, hq, h, d, cap, prefix_len, ctypes.addressof(size))
-    work = torch.empty(size.value, dtype=torch.float32, device=dev) if size.value else None
-    sc = 1.0 / float(d) ** 0.5 if scale is None else float(scale)
-    with _on(dev):
-        _lib.call("wfb_gqa_attention_i8", _p(q2), ldq, _p(k2), ldk, _p(v2), ldv, _DT[q.dtype], _p(cos), _p(sin), n_rope,
-                  ctypes.addressof(st), s_dev, s_host, l_dev, None if pst is None else ctypes.addressof(pst),
-                  prefix_len, b, t, hq, h, d, sc, _p(o2), ldo, _p(work), _stream(dev))
+    size = q.numel()
+    if size % (rows * d) != 0:
+        raise RuntimeError(f"{name}: q has {size} elements, not a multiple of {rows} rows of head_dim")
+    width = size // rows
+    q2, ldq = _rows16(name, q, rows, width, dtype, index)
+    k2, ldk = _rows16(name, k_new, rows, h * d, dtype, index)
+    v2, ldv = _rows16(name, v_new, rows, h * d, dtype, index)
+    cos, sin, n_rope = _rope_i8(name, rope_cos, rope_sin, d, index)
+    s_dev, s_host = _per_sequence(name, "start", start, b, index)
+    l_dev = None if lengths is None else _per_sequence(name, "lengths", lengths, b, index)[0]
+    o2, ldo = out, width
     if out is None:
-        return o2
-    return out if o2 is out else out.copy_(o2)
+        o2 = torch.empty((rows, width), dtype=dtype, device=dev)
+    else:
+        if out.dtype != dtype or out.shape != (rows, width) or out.get_device() != index:
+            raise RuntimeError(f"{name}: out must be [{rows}, {width}] {dtype} on {dev}")
+        ldo = out.stride(0) if rows > 1 else width
+        if out.stride(1) != 1 or out.data_ptr() % 16 or ldo * out.element_size() % 16 or ldo < width:
+            o2, ldo = torch.empty((rows, width), dtype=dtype, device=dev), width
+    need = ctypes.c_int64(0)
+    _lib.call("wfb_gqa_attention_i8_workspace", b, t, width // d, h, d, cap, prefix_len, ctypes.addressof(need))
+    work = torch.empty(need.value, dtype=torch.float32, device=dev) if need.value else None
+    with _on(dev):
+        _lib.call("wfb_gqa_attention_i8", q2.data_ptr(), ldq, k2.data_ptr(), ldk, v2.data_ptr(), ldv, _DT[dtype],
+                  _p(cos), _p(sin), n_rope, ctypes.addressof(st), s_dev, s_host, l_dev, p_ptr, prefix_len, b, t,
+                  width // d, h, d, d ** -0.5 if scale is None else float(scale), o2.data_ptr(), ldo, _p(work),
+                  _stream(dev))
+    return o2 if out is None or o2 is out else out.copy_(o2)
 
 
 def gqa_decode_attention_i8(
