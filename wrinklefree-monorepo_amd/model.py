@@ -19,7 +19,8 @@ identical: embedding, residuals, the prefill rotary embedding + cache append + c
 (libwfbitnet's matrix-core kernel for bf16 models, or torch ops with ``prefill_attention="torch"`` and
 for fp32 models), the decode-step rotary embedding + cache append + GQA attention (one libwfbitnet
 kernel, or torch ops with ``decode_attention="torch"``) and the tied LM head with its final norm and
-greedy argmax (one libwfbitnet kernel).
+greedy argmax (one libwfbitnet kernel).  With ``kv_cache="int8"`` the cache holds int8 codes, which the prompt
+and decode attentions of ``gqa_*_attention_i8`` write and read, and ``share_prefix`` lets a batch share a prompt's start.
 """
 
 from __future__ import annotations
@@ -34,7 +35,7 @@ import torch
 from .sglbitnt import SGLBitNetFile, write_sglbitnt
 from .ops import (QK_I2_S, bitnet_linear, bitnet_linear_argmax, bitnet_linear_glu,
                   bitnet_linear_residual, bitnet_linear_segmented, glu_rmsnorm_quantize_i8, gqa_decode_attention,
-                  gqa_prefill_attention,
+                  gqa_decode_attention_i8, gqa_prefill_attention, gqa_prefill_attention_i8, kv_cache_i8,
                   lm_head_argmax, pack_ternary_i2s, rmsnorm_linear, rmsnorm_linear_glu, rmsnorm_linear_glu_supported,
                   rmsnorm_linear_preferred, rmsnorm_quantize_i8, rope_tables)
 
@@ -254,7 +255,7 @@ class BitNetDecoder:
 
     def __init__(self, cfg: BitNetConfig, seed: int = 0, device: str = "cuda", dtype: torch.dtype = torch.float32,
                  backend=None, init_on_device: bool = False, decode_attention: str = "hip",
-                 prefill_attention: str = "hip"):
+                 prefill_attention: str = "hip", kv_cache: str = "model"):
         """``init_on_device``: draw the random weights with a generator on ``device`` (fast for 8B-scale
         models) instead of the host generator (the default, reproducible across devices).
         ``decode_attention``: "hip" runs each decode step's rotary embedding, cache append and GQA attention
@@ -262,8 +263,11 @@ class BitNetDecoder:
         prompt's rotary embedding, cache append and causal attention on libwfbitnet's matrix-core kernel
         (bf16 models with head_dim 64/128 and at most 8 query heads per kv head; other models use torch);
         "steps" runs it as one decode-attention launch per prompt position (any model dtype; the native
-        engine's fp32 prompt path); "torch" always uses torch ops."""
-        self._setup(cfg, device, dtype, backend, decode_attention, prefill_attention)
+        engine's fp32 prompt path); "torch" always uses torch ops.  ``kv_cache``: "model" keeps keys and values
+        in the model dtype; "int8" keeps them as codes with a scale per token and kv head (``kv_cache_i8``), which
+        both attentions read (head_dim 64/128, at most 16 query heads per kv head, "hip" attentions) and a prefix
+        shared by the batch can precede (``share_prefix``)."""
+        self._setup(cfg, device, dtype, backend, decode_attention, prefill_attention, kv_cache)
         gen = torch.Generator(device=self.device if init_on_device else "cpu").manual_seed(seed)
         self.embed = (torch.randn((cfg.vocab_size, cfg.hidden_size), generator=gen, device=gen.device) * 0.02).to(
             self.device, dtype)
@@ -278,9 +282,19 @@ class BitNetDecoder:
         self.head_weight = self.embed
 
     def _setup(self, cfg: BitNetConfig, device, dtype: torch.dtype, backend, decode_attention: str,
-               prefill_attention: str = "hip") -> None:
+               prefill_attention: str = "hip", kv_cache: str = "model") -> None:
         if decode_attention not in ("hip", "torch") or prefill_attention not in ("hip", "torch", "steps"):
             raise ValueError("decode_attention must be 'hip' or 'torch', prefill_attention 'hip', 'steps' or 'torch'")
+        if kv_cache not in ("model", "int8"):
+            raise ValueError("kv_cache must be 'model' or 'int8'")
+        if kv_cache == "int8" and (decode_attention != "hip" or prefill_attention != "hip"
+                                   or cfg.head_dim not in (64, 128) or cfg.num_heads % cfg.num_kv_heads != 0
+                                   or cfg.num_heads // cfg.num_kv_heads > 16
+                                   or dtype not in (torch.float32, torch.bfloat16)):
+            raise ValueError("kv_cache='int8' needs the 'hip' attentions, head_dim 64 or 128, 1 to 16 query heads per "
+                             "kv head and a float32 or bfloat16 model")
+        self.kv_cache = kv_cache
+        self._prefix, self._prefix_len = None, 0
         self.decode_attention = decode_attention
         self.prefill_attention = prefill_attention
         self.fuse_residual = True  # residual adds in the o / down epilogues when the backend offers it
@@ -335,7 +349,7 @@ class BitNetDecoder:
     @classmethod
     def from_float_state(cls, state: Dict[str, torch.Tensor], cfg: BitNetConfig, device="cuda",
                          dtype: torch.dtype = torch.float32, backend=None, decode_attention: str = "hip",
-                         prefill_attention: str = "hip") -> "BitNetDecoder":
+                         prefill_attention: str = "hip", kv_cache: str = "model") -> "BitNetDecoder":
         """Build the model from float weights under HuggingFace Llama names (``model.embed_tokens.weight``,
         ``model.layers.{i}.self_attn.q_proj.weight`` ... ``model.norm.weight``, optional ``lm_head.weight``),
         the names of the stage-1 source model (stage1.py:169-214).  Every projection is absmean-ternarised
@@ -344,7 +358,7 @@ class BitNetDecoder:
         creates them.  A ternary LM head (``cfg.ternary_lm_head``) is packed from ``lm_head.weight``; a
         dense untied head keeps it as floats; a tied head uses the embedding."""
         m = cls.__new__(cls)
-        m._setup(cfg, device, dtype, backend, decode_attention, prefill_attention)
+        m._setup(cfg, device, dtype, backend, decode_attention, prefill_attention, kv_cache)
         dev = m.device
 
         def get(name, shape=None, ones=False):
@@ -382,7 +396,8 @@ class BitNetDecoder:
 
     @classmethod
     def from_sglbitnt(cls, path, device="cuda", dtype: torch.dtype = torch.float32, backend=None,
-                      decode_attention: str = "hip", prefill_attention: str = "hip") -> "BitNetDecoder":
+                      decode_attention: str = "hip", prefill_attention: str = "hip",
+                      kv_cache: str = "model") -> "BitNetDecoder":
         """Build the model from an SGLBITNT file (memory-mapped; tensors go to ``device`` one at a time).
         Packed linears keep their I2_S bytes and scale; a uint8 lm_head.weight is a ternary LM head, a float
         one a dense head, none a head tied to the embedding.  Missing SubLN weights are ones (the engine
@@ -401,7 +416,7 @@ class BitNetDecoder:
                            ternary_lm_head=head_t is not None and head_t.dtype_id == 0,
                            hidden_act=str(c.get("hidden_act", "silu")))
         m = cls.__new__(cls)
-        m._setup(cfg, device, dtype, backend, decode_attention, prefill_attention)
+        m._setup(cfg, device, dtype, backend, decode_attention, prefill_attention, kv_cache)
         dev = m.device
 
         def packed(name, in_features):
@@ -455,10 +470,13 @@ class BitNetDecoder:
 
     def _cache(self, li: int, b: int):
         """Layer li's KV cache in the model dtype: K and V [B, kv, L_max, D] (one key = D contiguous
-        elements, the layout of the decode attention kernel)."""
+        elements, the layout of the decode attention kernel), or the int8 cache's four tensors."""
         cache = self.kv[li]
         if cache is None:
             cfg = self.cfg
+            if self.kv_cache == "int8":
+                self.kv[li] = kv_cache_i8(b, cfg.num_kv_heads, self._max_len, cfg.head_dim, self.device)
+                return self.kv[li]
             shape = (b, cfg.num_kv_heads, self._max_len, cfg.head_dim)
             cache = [torch.zeros(shape, device=self.device, dtype=self.dtype),
                      torch.zeros(shape, device=self.device, dtype=self.dtype)]
@@ -513,6 +531,9 @@ class BitNetDecoder:
         """One decode token per sequence in one kernel: rotary embedding of q and k, cache append at pos[b],
         GQA attention over positions 0..pos[b].  q/k/v are [B, heads*D] rows (possibly column slices of
         one q|k|v output)."""
+        if self.kv_cache == "int8":
+            return gqa_decode_attention_i8(q, k, v, self._cache(li, q.shape[0]), pos, self._rope_cos, self._rope_sin,
+                                           scale=1.0 / math.sqrt(self.cfg.head_dim), **self._prefix_of(li))
         kc, vc = self._cache(li, q.shape[0])
         return gqa_decode_attention(q, k, v, kc, vc, pos, self._rope_cos, self._rope_sin,
                                     scale=1.0 / math.sqrt(self.cfg.head_dim))
@@ -524,8 +545,26 @@ class BitNetDecoder:
         self.kv = [None] * self.cfg.num_layers
         self._key_pos = torch.arange(max_len, device=self.device)
         # cos / sin of every cache position from libwfbitnet's tables (the native engine's values)
-        cos, sin = _rope_tables_cpu(self.cfg.rope_theta, self.cfg.head_dim, max_len)
+        cos, sin = _rope_tables_cpu(self.cfg.rope_theta, self.cfg.head_dim, self._prefix_len + max_len)
         self._rope_cos, self._rope_sin = cos.to(self.device), sin.to(self.device)
+
+    def _prefix_of(self, li: int) -> Dict:
+        return {} if self._prefix is None else {"prefix": self._prefix[li], "prefix_len": self._prefix_len}
+
+    @torch.no_grad()
+    def share_prefix(self, ids: Optional[torch.Tensor]) -> None:
+        """Token ids [P] that precede every sequence from the next ``reset`` (or ``generate``) on: their keys and values
+        are computed once, here, and read once per step for the whole batch; the positions given to ``forward`` and
+        ``decode_step`` keep counting a sequence's own tokens.  ``None`` ends it.  Needs ``kv_cache="int8"``."""
+        if self.kv_cache != "int8":
+            raise ValueError("share_prefix needs kv_cache='int8'")
+        self._prefix, self._prefix_len = None, 0
+        if ids is not None and ids.numel() > 0:
+            n = ids.numel()
+            self.reset(1, n)
+            self._layers(self.embed[ids.reshape(1, n).to(self.device)], self._prefill_attend(1, n, 0))
+            self._prefix, self._prefix_len = self.kv, n
+        self.kv = []
 
     def _layers(self, x: torch.Tensor, attend, first: int = 0, last: Optional[int] = None) -> torch.Tensor:
         cfg, be = self.cfg, self.backend
@@ -580,6 +619,8 @@ class BitNetDecoder:
         quantised groups go to ``backend`` (a host backend holding its own copy of the packed weights);
         the packed weights themselves are shared, not copied."""
         cpu = torch.device("cpu")
+        if self.kv_cache != "model":
+            raise ValueError("on_host needs kv_cache='model': the int8 cache's attentions run on the GPU")
         m = copy.copy(self)
         m.device, m.backend, m.decode_attention, m.prefill_attention = cpu, backend, "torch", "torch"
         m.embed, m.final_norm = self.embed.to(cpu), self.final_norm.to(cpu)
@@ -598,6 +639,9 @@ class BitNetDecoder:
         pos = torch.arange(start, start + t, device=self.device)
 
         def attend(li, q, k, v):
+            if self.kv_cache == "int8":
+                return gqa_prefill_attention_i8(q, k, v, self._cache(li, b), start, t, self._rope_cos, self._rope_sin,
+                                                scale=1.0 / math.sqrt(cfg.head_dim), **self._prefix_of(li))
             if self._hip_prefill():
                 kc, vc = self._cache(li, b)
                 return gqa_prefill_attention(q, k, v, kc, vc, start, t, self._rope_cos, self._rope_sin,
