@@ -254,6 +254,10 @@ DECODES = [
     (2, 20, 5, 128, 64, [3, 63], F32, 500),
     (33, 4, 1, 64, 64, list(range(33)), BF16, 130),
     (5, 32, 8, 128, 256, [200, 0, 13, 64, 255], BF16, 1500),
+    (2, 12, 1, 128, 192, [190, 64], F32, 0),
+    (20, 8, 2, 128, 128, list(range(60, 80)), BF16, 64),   # more than 64 rows against the prefix, whole blocks
+    (20, 8, 2, 128, 64, list(range(20)), F32, 321),
+    (17, 33, 3, 64, 64, list(range(17)), F32, 129),
 ]
 
 
@@ -410,6 +414,8 @@ PROMPTS = [
     (3, 20, 5, 128, 128, [0, 0, 0], [48, 48, 48], 48, BF16, 700),
     (2, 4, 2, 128, 64, [0, 9], [1, 2], 2, F32, 1000),
     (1, 4, 1, 128, 4160, [4000], [100], 100, BF16, 0),  # few rows, a long axis
+    (3, 8, 2, 64, 128, [5, 64, 127], [1, 0, 1], 1, BF16, 0),  # one token a sequence, one of them padding
+    (2, 33, 3, 128, 192, [100, 0], [41, 90], 90, F32, 64),
 ]
 
 

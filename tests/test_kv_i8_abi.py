@@ -28,6 +28,7 @@ def test_write_refusals(pkg):
 
     no("head_dim", d=96)
     no("num_kv_heads", h=0)
+    no("num_kv_heads", h=32768)
     no("batch", batch=65536)
     no("batch", batch=-1)
     no("null cache", cache=0)
@@ -90,9 +91,9 @@ def test_workspace(pkg):
 
 
 def _attend(pkg, cache=None, prefix=None, prefix_len=0, q=0x1000, out=0x5000, ldq=512, ldo=512, hq=8, h=2, d=64, batch=2,
-            t=3, dtype=1, scale=0.125, ws=0x6000, ldk=128, cap=128):
+             t=3, dtype=1, scale=0.125, ws=0x6000, ldk=128, cap=128):
     c = _cache(pkg, cap=cap) if cache is None else cache
-    return pkg._lib.status("wfb_gqa_attention_i8", vp(q), ldq, vp(0x2000), ldk, vp(0x3000), 128, dtype, None, None, 0,
+    return pkg._lib.status("wfb_gqa_attention_i8", vp(q), ldq, vp(0x2000), ldk, vp(0x3000), ldk, dtype, None, None, 0,
                            ctypes.addressof(c), None, 0, None, ctypes.addressof(prefix) if prefix else None, prefix_len,
                            batch, t, hq, h, d, scale, vp(out), ldo, vp(ws) if ws else None, None)
 
@@ -119,7 +120,8 @@ def test_attention_refusals(pkg):
     no("16-byte", q=0x1004)
     no("16-byte", ws=0x6004)
     no("workspace", ws=0, batch=1, t=1, cap=4096)
-    no("2^31", batch=65535, t=1 << 14, cap=1 << 15)
+    no("2^30", batch=65535, t=1 << 14, cap=1 << 15)
+    no("2^21", batch=65535, hq=64, h=32, ldq=64 * 64, ldo=64 * 64, ldk=32 * 64, t=1)
     assert _attend(pkg, batch=0) == 0 and _attend(pkg, t=0, q=0) == 0
 
 

@@ -81,8 +81,8 @@ HOST_ONLY_SOURCES = ("api.hip", "engine.hip")
 def build_asan(verbose: bool = False) -> Path:
     """Host-code AddressSanitizer build for the CPU tests of the C ABI: the host-only sources (argument
     validation, dispatch, the engine's loader and state) compiled with ASan, linked with the kernel objects
-    of the product build (run build() first) into _build/asan/libwfbitnet_asan.so, and the driver
-    tests/asan/abi_driver.cpp linked against it.  Returns the driver's path."""
+    of the product build (run build() first) into _build/asan/libwfbitnet_asan.so, and the drivers
+    tests/asan/abi_driver.cpp and kv_i8_driver.cpp linked against it.  Returns the first driver's path."""
     hipcc = _hipcc()
     ASAN_DIR.mkdir(parents=True, exist_ok=True)
     host = ["--offload-host-only", "-O1", "-g", "-fPIC", "-std=c++17", "-Wno-unused-command-line-argument"]
@@ -102,12 +102,12 @@ def build_asan(verbose: bool = False) -> Path:
         objs.append(obj)
     lib = ASAN_DIR / "libwfbitnet_asan.so"
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *san, *map(str, objs), "-o", str(lib)])
-    driver = ASAN_DIR / "abi_driver"
-    dobj = ASAN_DIR / "abi_driver.o"
-    _run([hipcc, *host, *san, f"-I{PKG_DIR.parent / 'include'}", "-c", str(ASAN_DRIVER_SRC), "-o", str(dobj)])
-    _run([hipcc, "--offload-host-only", *san, str(dobj), f"-L{ASAN_DIR}", "-lwfbitnet_asan",
-          f"-Wl,-rpath,{ASAN_DIR}", "-o", str(driver)])
-    return driver
+    for src in (ASAN_DRIVER_SRC, ASAN_DRIVER_SRC.with_name("kv_i8_driver.cpp")):
+        dobj = ASAN_DIR / (src.stem + ".o")
+        _run([hipcc, *host, *san, f"-I{PKG_DIR.parent / 'include'}", "-c", str(src), "-o", str(dobj)])
+        _run([hipcc, "--offload-host-only", *san, str(dobj), f"-L{ASAN_DIR}", "-lwfbitnet_asan",
+              f"-Wl,-rpath,{ASAN_DIR}", "-o", str(ASAN_DIR / src.stem)])
+    return ASAN_DIR / ASAN_DRIVER_SRC.stem
 
 
 if __name__ == "__main__":

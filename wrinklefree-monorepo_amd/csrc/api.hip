@@ -170,8 +170,8 @@ int check_decode_attention(const char* name, const void* q, int64_t ldq, const v
 // Host checks of the int8 cache's entry points.
 int check_kv_i8(const char* name, const wfb_kv_i8* c, int64_t batch, int64_t num_kv_heads, int64_t head_dim) {
   if (head_dim != 64 && head_dim != 128) return fail(WFB_EINVAL, "%s: head_dim (%lld) must be 64 or 128", name, (long long)head_dim);
-  if (batch < 0 || batch > 65535 || num_kv_heads <= 0 || num_kv_heads > 65535)
-    return fail(WFB_EINVAL, "%s: batch (%lld) must be in 0..65535 and num_kv_heads (%lld) in 1..65535", name,
+  if (batch < 0 || batch > 65535 || num_kv_heads <= 0 || num_kv_heads > 32767)
+    return fail(WFB_EINVAL, "%s: batch (%lld) must be in 0..65535 and num_kv_heads (%lld) in 1..32767", name,
                 (long long)batch, (long long)num_kv_heads);
   if (!c) return fail(WFB_EINVAL, "%s: null cache", name);
   if (c->cap <= 0 || c->cap % WFB_KV_I8_BLOCK != 0 || c->cap > INT32_MAX / head_dim)
@@ -823,8 +823,9 @@ int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t 
   if (ldq < num_heads * head_dim || ldo < num_heads * head_dim || ldq % per16 || ldo % per16)
     return fail(WFB_EINVAL, "%s: q and out row strides must cover num_heads*head_dim and be multiples of 16 bytes", name);
   if (!std::isfinite(scale)) return fail(WFB_EINVAL, "%s: scale must be finite", name);
-  if (batch * t * num_heads > INT32_MAX)
-    return fail(WFB_EINVAL, "%s: batch*T*num_heads (%lld) must be < 2^31", name, (long long)(batch * t * num_heads));
+  if (batch * num_heads >= (1 << 21) || batch * t * num_heads >= (1 << 30))  // (grids of fewer than 2^32 threads)
+    return fail(WFB_EINVAL, "%s: batch*num_heads (%lld) must be < 2^21 and batch*T*num_heads (%lld) < 2^30", name,
+                (long long)(batch * num_heads), (long long)(batch * t * num_heads));
   if (batch == 0 || t == 0) return ok();
   if (!q || !out) return fail(WFB_EINVAL, "%s: null pointer", name);
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16))

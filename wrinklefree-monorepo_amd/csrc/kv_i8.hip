@@ -92,10 +92,11 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const void* __restri
     }
     float scale;
     const uint2 q = quantise8<L>(x[p], scale);
-    if (slot != p * RPP + t / L) continue;
-    if (keys) *reinterpret_cast<uint2*>(c.k + (slice + pos) * D + 8 * l) = q;
-    else *reinterpret_cast<uint2*>(&vt[slot * kPitch + 8 * l]) = q;
-    if (l == 0) (keys ? c.k_scale : c.v_scale)[slice + pos] = scale;
+    if (slot == p * RPP + t / L) {
+      if (keys) *reinterpret_cast<uint2*>(c.k + (slice + pos) * D + 8 * l) = q;
+      else *reinterpret_cast<uint2*>(&vt[slot * kPitch + 8 * l]) = q;
+      if (l == 0) (keys ? c.k_scale : c.v_scale)[slice + pos] = scale;
+    }
   }
   if (keys) return;
   __syncthreads();
