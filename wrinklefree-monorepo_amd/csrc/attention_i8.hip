@@ -591,46 +591,49 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
     const int64_t tok1 = ((int64_t)(rb + 1) * kRows + g - 1) / g;  // past the last row's token
     own = first + (tok1 < n ? tok1 : n);
   }
-  const int64_t pb = (a.npre + kKvBlock - 1) / kKvBlock, nb = pb + (own + kKvBlock - 1) / kKvBlock;
-  const int64_t per = (nb + nsplit - 1) / nsplit;
-  const int64_t kb0 = split * per, kb1 = kb0 + per < nb ? kb0 + per : nb;
+  // (blocks in 32 bits: a comparison of 64 is a vector instruction, and what hangs on it no longer uniform to the compiler)
+  const int pb = (int)((a.npre + kKvBlock - 1) / kKvBlock), nb = pb + (int)((own + kKvBlock - 1) / kKvBlock);
+  const int per = (nb + nsplit - 1) / nsplit;
+  const int kb0 = split * per, kb1 = kb0 + per < nb ? kb0 + per : nb;
 
   // ---- staging: K row-major [key][D], V as it is [element][64 keys], 16-byte chunks at chunk ^ (row's swizzle) so that
   // 16 lanes reading one chunk of 16 rows meet 16 different bank groups
   auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
   auto vswz = [](int d) { return (d >> 1) & 7; };
   v4i raw[2][PT] = {};  // codes of the next block and of the one behind it
-  auto place = [&](int64_t kb, const wfb_kv_i8*& c, int64_t& at, int64_t& left) {  // uniform
-    const bool in_pre = kb < pb;
-    const int64_t k0 = (in_pre ? kb : kb - pb) * kKvBlock;
-    c = in_pre ? &a.pre : &a.own;
-    at = (in_pre ? kvh : (int64_t)b * a.hkv + kvh) * c->cap + k0;
-    left = (in_pre ? a.npre : own) - k0;
-  };
-  auto fetch_codes = [&](int64_t kb, int set) {
-    const wfb_kv_i8* c;
-    int64_t at, left;
-    place(kb, c, at, left);
-    const buf_t kb_ = make_buf(c->k + at * D, kKvBlock * D), vb_ = make_buf(c->v + at * D, kKvBlock * D);
+  const int64_t pre_at = kvh * a.pre.cap, own_at = ((int64_t)b * a.hkv + kvh) * a.own.cap;
+  const int pre_tail = (int)(a.npre - (int64_t)(pb - 1) * kKvBlock), own_tail = (int)(own - (int64_t)(nb - pb - 1) * kKvBlock);
+  // The first key of a block in its cache.  (Members are chosen one by one: a choice between the two structs would have to
+  // be read through a pointer, in every block.)
+  auto first_key = [&](int kb) { return kb < pb ? pre_at + (int64_t)kb * kKvBlock : own_at + (int64_t)(kb - pb) * kKvBlock; };
+  auto fetch_codes = [&](int kb, int set) {
+    const int64_t at = first_key(kb) * D;
+    const buf_t kb_ = make_buf((kb < pb ? a.pre.k : a.own.k) + at, kKvBlock * D);
+    const buf_t vb_ = make_buf((kb < pb ? a.pre.v : a.own.v) + at, kKvBlock * D);
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int p0 = 64 * (w + i * W);  // uniform
-      raw[set][i] = p0 < KP ? buf_load16(kb_, 16 * (p0 + lane)) : buf_load16(vb_, 16 * (p0 - KP + lane));
+      const bool isk = 64 * W * (i + 1) <= KP || (64 * W * i < KP && p0 < KP);
+      raw[set][i] = buf_load16(isk ? kb_ : vb_, 16 * ((isk ? p0 : p0 - KP) + lane));
     }
   };
-  float sk = 0.0f, sv = 0.0f;  // (waves 0 and 1) the scales of key `lane`, zeros behind the last key
-  auto fetch_scales = [&](int64_t kb) {
-    if (w >= 2) return;
-    const wfb_kv_i8* c;
-    int64_t at, left;
-    place(kb, c, at, left);
-    const uint32_t bytes = 4 * (uint32_t)(left < kKvBlock ? left : kKvBlock);
-    sk = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->k_scale + at, bytes), 4 * lane, 0, 0));
-    sv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(make_buf(c->v_scale + at, bytes), 4 * lane, 0, 0));
+  float sk = 0.0f, sv = 0.0f;  // the scales of key `lane`, zeros behind the last key; waves 0 and 1 stage them
+  auto fetch_scales = [&](int kb) {
+    const int64_t at = first_key(kb);
+    const uint32_t bytes = 4 * (kb == pb - 1 ? pre_tail : kb == nb - 1 ? own_tail : kKvBlock);
+    const buf_t ks = make_buf((kb < pb ? a.pre.k_scale : a.own.k_scale) + at, bytes);
+    const buf_t vs = make_buf((kb < pb ? a.pre.v_scale : a.own.v_scale) + at, bytes);
+    sk = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(ks, 4 * lane, 0, 0));
+    sv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(vs, 4 * lane, 0, 0));
   };
+  float sk1 = 0.0f, sv1 = 0.0f;
   if (kb0 < kb1) {  // under way while the queries are formed
+    fetch_scales(kb0 + 1 < kb1 ? kb0 + 1 : kb0);
+    sk1 = sk;
+    sv1 = sv;
     fetch_scales(kb0);
     fetch_codes(kb0, 0);
+    fetch_codes(kb0 + 1 < kb1 ? kb0 + 1 : kb0, 1);
   }
 
   // ---- the row's query in fp16 of its largest: lane holds elements 16 s + 8 grp .. + 7
@@ -766,12 +769,11 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
   const int ka = key * D, kx = kswz(key), va = col * kKvBlock, vx = vswz(col);  // (a tile's 32 rows repeat the swizzle)
   // Block kb, in buffer buf and scale slot `slot`.  Under the first products the next block's codes, fetched during the
   // block before, become fp16 and then go to the other buffer; the scales of the one behind it go to the next slot but one.
-  auto block = [&](int64_t kb, int buf, int slot) {
+  auto block = [&](int kb, int buf, int slot) {
     const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
     const uint16_t* ks = tile[buf][0];
     const uint16_t* vs = tile[buf][1];
-    if (kb + 2 < kb1) fetch_codes(kb + 2, buf);
-    const int64_t k0 = (kb < pb ? kb : kb - pb) * kKvBlock;
+    fetch_codes(kb + 2 < kb1 ? kb + 2 : kb1 - 1, buf);  // (always: with loads in a branch every wait would be for all of them)
     read_factors(0, slot1);
     const float vnew = vref_s[slot];
     if (vnew != vref) {  // uniform
@@ -816,8 +818,8 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (kb + 2 < kb1) stage_scales(slot2);
-    if (kb + 3 < kb1) fetch_scales(kb + 3);
+    stage_scales(slot2);
+    fetch_scales(kb + 3 < kb1 ? kb + 3 : kb1 - 1);
     // register 8 c + j of tile nb2 holds key 32 nb2 + 16 c + 8 grp + j
     float bmax = -__builtin_inff();
 #pragma unroll
@@ -830,9 +832,11 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
         s[nb2][i + 2] *= f.z;
         s[nb2][i + 3] *= f.w;
       }
-    const int64_t seen64 = kb < pb ? a.npre - k0 : pos + 1 - k0, low64 = kb < pb ? a.npre - k0 : pos_low + 1 - k0;
-    if (low64 < kKvBlock) {  // uniform: some row of the wave does not see all keys of the block
-      const int seen = seen64 > kKvBlock ? kKvBlock : (int)seen64;
+    // keys of the block that the row sees, and the wave's first one, if not all of them
+    const int64_t k0 = (int64_t)(kb - pb) * kKvBlock;
+    const int low = kb < pb - 1 ? kKvBlock : kb == pb - 1 ? pre_tail : pos_low + 1 - k0 > kKvBlock ? kKvBlock : (int)(pos_low + 1 - k0);
+    if (low < kKvBlock) {  // uniform
+      const int seen = kb < pb ? pre_tail : pos + 1 - k0 > kKvBlock ? kKvBlock : (int)(pos + 1 - k0);
 #pragma unroll
       for (int nb2 = 0; nb2 < 2; ++nb2)
 #pragma unroll
@@ -913,10 +917,10 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
 
   if (kb0 < kb1) {
     stage_scales(0);
-    if (kb0 + 1 < kb1) {
-      fetch_scales(kb0 + 1);
-      stage_scales(1);
-    }
+    sk = sk1;
+    sv = sv1;
+    stage_scales(1);
+    fetch_scales(kb0 + 2 < kb1 ? kb0 + 2 : kb1 - 1);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
@@ -925,10 +929,8 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
       for (int x = 4 * i; x < 4 * i + 4; ++x) convert(x, 0);
       stage_codes(i, 0);
     }
-    if (kb0 + 1 < kb1) fetch_codes(kb0 + 1, 1);
-    if (kb0 + 2 < kb1) fetch_scales(kb0 + 2);
     int slot = 0;
-    for (int64_t kb = kb0; kb < kb1; kb += 2) {
+    for (int kb = kb0; kb < kb1; kb += 2) {
       __syncthreads();  // block kb and its scales are staged, and everyone is done with block kb - 1
       block(kb, 0, slot);
       slot = slot == 2 ? 0 : slot + 1;
