@@ -441,10 +441,14 @@ int wfb_kv_read_i8(const wfb_kv_i8* cache, const int64_t* start_dev, int64_t sta
 /* wfb_kv_write_i8 of T tokens per sequence, and their attention: token i of sequence b at position p = start[b] + i,
  * query head h: softmax_j(rope(q)_h . k_j * scale) v_j over the prefix_len keys of `prefix` (a cache of one sequence
  * that the whole batch shares, or NULL) and the sequence's own keys 0 .. p, all as the caches hold them, the new
- * tokens' own among them: a result does not depend on how a prompt was cut into calls.  The rotary embedding takes row
- * prefix_len + p.  Scores, softmax and sums are fp32, the products exact integers of the codes with q and the
- * probabilities as fixed-point numbers of 16 bits (dtype WFB_BF16) or 24 (WFB_F32) of their row's largest; the output is
- * rounded once to dtype.  T = 1 with start_dev is a decode step.
+ * tokens' own among them: up to the roundings of its sums a result does not depend on how a prompt was cut into calls.
+ * The rotary embedding takes row prefix_len + p.  Scores, softmax and sums are fp32, the output is rounded once to dtype.
+ * T = 1 without lengths is a decode step: the codes' products with q and with the probabilities are exact integers, these
+ * two being fixed-point numbers of 16 bits (dtype WFB_BF16) or 24 (WFB_F32) of their row's and block's largest.  The
+ * tokens of a prompt, and a prefix that more than 64 rows (batch * num_heads / num_kv_heads) share, take fp16 products
+ * with fp32 sums: q and probabilities in 11 bits (WFB_BF16; the values too, in 11 bits if their scale is above 2^-21 of
+ * the largest in the sequence) or in two parts of 22 bits together (WFB_F32).  A row of q below 2^-100 counts as zeros;
+ * keys of 2^100 and more may leave the range of the scores (NaN).  The prefix must not lie in the cache.
  * q, out [batch*T, ldq / ldo] and k_new, v_new as in wfb_kv_write_i8 (rows 16-byte aligned); num_heads / num_kv_heads
  * in 1..16, head_dim 64 or 128.  Rows at and behind lengths[b] are zeros; a sequence that does not fit (see above) gives
  * NaN rows and is not written.  workspace: the floats that wfb_gqa_attention_i8_workspace (host only) reports, 16-byte

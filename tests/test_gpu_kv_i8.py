@@ -2,14 +2,16 @@
 CPU, and the decode / prompt attentions that read it (with and without a shared prefix) against float64 over the values
 that the cache holds.
 
-Tolerances of the attentions, per output element, are sums of what the arithmetic may lose (``_bound``):
+Tolerances of the attentions, per output element, are sums of what the arithmetic may lose:
   * the output's rounding, half a step of its type (bf16 2^-8, fp32 2^-24 of the value);
   * the query as a fixed-point row of w bits (bf16 16, fp32 24): an element is off by at most 2^-w of its row's largest,
     a score by the sum of that over the key's elements, the output by the weighted sum of (v - out) times that;
   * the weights p * v_scale as fixed-point numbers of w bits, off by at most 2^(2-w) of the largest weight of the row
     (a row's reference may lie up to four times above it), times 127 codes;
   * fp32 scores, exponentials and sums: 2^-20 of sum p |v| (1 + max |s|) covers ten roundings of 2^-24 and the
-    exponent's argument.
+    exponent's argument;
+  * where bf16 rows take fp16 products (prompts, a prefix of more than 64 rows) and ``half`` asks for it: a half step of
+    fp16, 2^-11, of every element of q, and three of them (scale, value, weight) of sum p |v|.
 """
 
 import math
@@ -90,7 +92,7 @@ def _same_cache(cache, host):
             raise AssertionError(f"{name} differs at {bad[:4].tolist()} ({len(bad)} places)")
 
 
-def _attention(q, host, start, lens, t, cos, sin, scale, dtype, prefix=None, npre=0):
+def _attention(q, host, start, lens, t, cos, sin, scale, dtype, prefix=None, npre=0, half=False):
     """(out, bound) float64 [b*t, hq*d]: the definition over the host cache as it is after the write."""
     b, h, _, d = host.k.shape
     hq = q.shape[1] // d
@@ -118,13 +120,17 @@ def _attention(q, host, start, lens, t, cos, sin, scale, dtype, prefix=None, npr
             o = p @ vv
             out[i, :n, j] = o
             ds = 2.0 ** -bits * x[:, j].abs().amax(1, keepdim=True) * abs(scale) * kk.abs().sum(1)[None, :]
+            lost = 0.0
+            if half and dtype == BF16:
+                ds = ds + 2.0 ** -11 * (x[:, j].abs() @ kk.abs().T) * abs(scale)
+                lost = 3 * 2.0 ** -11 * (p @ vv.abs())
             spread = (p * ds) @ vv.abs() + (p * ds).sum(1, keepdim=True) * o.abs()
             w = (p * vc).amax(1) / 127.0
             # a key's weight is off by a step of the fixed-point grid at most, its code by nothing
             fixed = 2.0 ** (2 - bits) * w[:, None] * (kk.shape[0] * 127.0)
             smax = sc.masked_fill(later, 0.0).abs().amax(1, keepdim=True)
             f32 = 2.0 ** -20 * (1.0 + smax) * (p @ vv.abs())
-            tol[i, :n, j] = (2.0 ** -8 if dtype == BF16 else 2.0 ** -23) * o.abs() + spread + fixed + f32
+            tol[i, :n, j] = (2.0 ** -8 if dtype == BF16 else 2.0 ** -23) * o.abs() + spread + fixed + f32 + lost
     return out.reshape(b * t, hq * d), tol.reshape(b * t, hq * d)
 
 
@@ -517,6 +523,112 @@ def test_a_prompt_cut_anywhere_and_decoded_onwards_is_the_same(pkg, dev):
     _check(out, ref[[130, 130]], tol[[130, 130]], "a step behind a prefix")
 
 
+# ---- extremes ------------------------------------------------------------------------------------------
+
+EXTREMES = [
+    # b, hq, hkv, d, t, prefix length (t 0: a decode step)
+    (3, 8, 2, 64, 0, 0),
+    (3, 8, 2, 128, 0, 70),
+    (20, 8, 2, 64, 0, 300),   # the prefix as fp16 products
+    (2, 9, 3, 64, 33, 0),
+    (2, 8, 2, 128, 40, 100),
+]
+
+
+def _call(pkg, dev, case, x, cache, pre, base, **kw):
+    b, hq, h, d, t, npre = case
+    xs = x.to(dev).split([hq * d, h * d, h * d], dim=1)
+    if npre:
+        kw.update(prefix=pre.to(pkg, dev), prefix_len=npre)
+    if t == 0:
+        return pkg.gqa_decode_attention_i8(*xs, cache, torch.full((b,), base, device=dev), **kw)
+    return pkg.gqa_prefill_attention_i8(*xs, cache, base, t, **kw)
+
+
+def _made(case, dtype, seed=5):
+    b, hq, h, d, t, npre = case
+    gen = torch.Generator().manual_seed(seed)
+    host = Host(b, h, 192, d, gen)
+    pre = Host(1, h, (npre + 63) // 64 * 64, d, gen) if npre else None
+    return _qkv(b * max(t, 1), hq, h, d, dtype, gen), host, pre
+
+
+def _wanted(case, x, host, pre, base, dtype):
+    b, hq, h, d, t, npre = case
+    t = max(t, 1)
+    q, k, v = x.split([hq * d, h * d, h * d], dim=1)
+    host.write(k, v, [base] * b, [t] * b, t, None, None)
+    return _attention(q, host, [base] * b, [t] * b, t, None, None, d ** -0.5, dtype, pre, npre, half=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("case", EXTREMES)
+def test_a_query_that_is_not_finite_is_its_own_row_only(pkg, dev, case, dtype):
+    b, hq, h, d, t, npre = case
+    print(f"[kv extremes] {case} {dtype}", flush=True)
+    x, host, pre = _made(case, dtype)
+    cache = host.to(pkg, dev)
+    ref, tol = _wanted(case, x, host, pre, 100, dtype)
+    for row, head, bad in ((0, 1, float("nan")), (x.shape[0] - 1, hq - 1, float("-inf")), (1, 0, float("inf"))):
+        x[row, head * d + 5] = bad
+        ref[row, head * d:(head + 1) * d] = float("nan")
+    _check(_call(pkg, dev, case, x, cache, pre, 100), ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("case", EXTREMES)
+def test_large_keys_under_small_queries_and_large_values(pkg, dev, case, dtype):
+    b, hq, h, d, t, npre = case
+    print(f"[kv extremes] {case} {dtype}", flush=True)
+    x, host, pre = _made(case, dtype)
+    up, down = 2.0 ** 90, 2.0 ** -90
+    x[:, :hq * d] *= down
+    x[:, hq * d:(hq + h) * d] *= up
+    x[:, (hq + h) * d:] *= up
+    for z in (host, pre) if pre else (host,):
+        z.ks *= up
+        z.vs *= up
+    cache = host.to(pkg, dev)
+    ref, tol = _wanted(case, x, host, pre, 100, dtype)
+    _check(_call(pkg, dev, case, x, cache, pre, 100), ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("case", EXTREMES)
+def test_a_value_far_above_the_others_under_no_weight(pkg, dev, case, dtype):
+    """The values that count are 2^-20 of one whose key's weight is nothing."""
+    b, hq, h, d, t, npre = case
+    print(f"[kv extremes] {case} {dtype}", flush=True)
+    x, host, pre = _made(case, dtype)
+    x[:, :hq * d] = 2.0 + x[:, :hq * d].abs() / 8
+    for z in (host, pre) if pre else (host,):
+        z.vs *= 2.0 ** -20
+    x[:, (hq + h) * d:] *= 2.0 ** -20
+    first = pre if pre else host
+    first.k[:, :, 7] = -127
+    first.ks[:, :, 7] = 1.0
+    first.vs[:, :, 7] *= 2.0 ** 20
+    cache = host.to(pkg, dev)
+    ref, tol = _wanted(case, x, host, pre, 100, dtype)
+    _check(_call(pkg, dev, case, x, cache, pre, 100), ref, tol)
+    assert float(ref.abs().max()) < 2.0 ** -10
+
+
+@pytest.mark.parametrize("case", EXTREMES)
+def test_the_output_may_be_the_queries(pkg, dev, case):
+    x, host, pre = _made(case, BF16)
+    want = _call(pkg, dev, case, x, host.to(pkg, dev), pre, 64)
+    b, hq, h, d, t, npre = case
+    q = x[:, :hq * d].to(dev).contiguous()
+    k, v = (z.to(dev) for z in x[:, hq * d:].split([h * d, h * d], dim=1))
+    kw = {"prefix": pre.to(pkg, dev), "prefix_len": npre} if npre else {}
+    if t == 0:
+        got = pkg.gqa_decode_attention_i8(q, k, v, host.to(pkg, dev), torch.full((b,), 64, device=dev), out=q, **kw)
+    else:
+        got = pkg.gqa_prefill_attention_i8(q, k, v, host.to(pkg, dev), 64, t, out=q, **kw)
+    assert got is q and torch.equal(q, want)
+
+
 # ---- where and when the calls run ----------------------------------------------------------------------
 
 
@@ -534,6 +646,25 @@ def test_side_stream_and_unaligned_inputs(pkg, dev):
     s.synchronize()
     _check(out, ref, tol)
     assert torch.equal(res, out) and torch.equal(wide[:, 1:], out) and torch.equal(col, out)
+
+
+def test_two_streams_at_once(pkg, dev):
+    """Calls in flight on two streams, each with a cache and a workspace of its own, over one prefix."""
+    cases = [(20, 8, 2, 64, 0, 300), (2, 9, 3, 64, 33, 0), (3, 8, 2, 128, 0, 0)]
+    made = [_made(c, BF16, seed=i) for i, c in enumerate(cases)]
+    want = [_call(pkg, dev, c, x, host.to(pkg, dev), pre, 100) for c, (x, host, pre) in zip(cases, made)]
+    caches = [[host.to(pkg, dev) for _, host, _ in made] for _ in range(2)]
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for c, (x, host, pre), own in zip(cases, made, zip(*caches)):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_call(pkg, dev, c, x, own[i], pre, 100))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g, w in zip(got[i], want):
+            assert torch.equal(g, w)
 
 
 def test_graphs_replayed_as_positions_advance(pkg, dev):
@@ -679,6 +810,7 @@ def test_refusals(pkg, dev):
     no("out must", dec, q, k, k, cache, pos, out=torch.empty((b, hq * d), device=dev))
     no("prefix", dec, q, k, k, cache, pos, prefix=cache, prefix_len=3)
     no("prefix", dec, q, k, k, cache, pos, prefix_len=3)
+    no("lie in the cache", dec, q, k, k, cache, pos, prefix=tuple(c[1:] for c in cache), prefix_len=3)
     no("capacity", dec, q, k, k, cache, pos, prefix=pre, prefix_len=65)
     no("prefix", dec, q, k, k, cache, pos, prefix=pre, prefix_len=-1)
     no("four tensors", dec, q, k, k, cache[:3], pos)

@@ -110,6 +110,14 @@ def test_attention_refusals(pkg):
     no("capacity", prefix=_cache(pkg), prefix_len=129)
     no("capacity", prefix=_cache(pkg, cap=96), prefix_len=5)
     no("null cache pointer", prefix=_cache(pkg, k=None), prefix_len=5)
+    # the cache's codes span 2 * 2 * 128 * 64 bytes from k and v, the prefix's half of that
+    far = dict(k=0x100000, v=0x200000)
+    no("lie in the cache", prefix=_cache(pkg, k=0x1000, v=0x200000), prefix_len=5)
+    no("lie in the cache", prefix=_cache(pkg, k=0x1000 + 4 * 128 * 64 - 16, v=0x200000), prefix_len=5)
+    no("lie in the cache", cache=_cache(pkg, k=0x100000, v=0x200000),
+       prefix=_cache(pkg, k=0x300000, v=0x200000 - 2 * 128 * 64 + 16), prefix_len=5)
+    assert _attend(pkg, cache=_cache(pkg, **far), prefix=_cache(pkg, k=0x100000 + 4 * 128 * 64, v=0x200000 - 2 * 128 * 64),
+                   prefix_len=5, t=0) == 0
     no("strides", ldq=500)
     no("strides", ldo=516)
     no("strides", ldk=64)

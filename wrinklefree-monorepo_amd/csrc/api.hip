@@ -814,6 +814,15 @@ int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t 
     if (prefix_len > prefix->cap)
       return fail(WFB_EINVAL, "%s: prefix length (%lld) exceeds the prefix's capacity (%lld)", name,
                   (long long)prefix_len, (long long)prefix->cap);
+    // the new tokens are written while the prefix is read
+    const uintptr_t own = (uintptr_t)batch * num_kv_heads * cache->cap * head_dim;
+    const uintptr_t pre = (uintptr_t)num_kv_heads * prefix->cap * head_dim;
+    auto meet = [&](const int8_t* x, const int8_t* y) {
+      const uintptr_t c = reinterpret_cast<uintptr_t>(x), p = reinterpret_cast<uintptr_t>(y);
+      return c < p + pre && p < c + own;
+    };
+    if (batch > 0 && (meet(cache->k, prefix->k) || meet(cache->v, prefix->v)))
+      return fail(WFB_EINVAL, "%s: the prefix must not lie in the cache", name);
   }
   wfb::KvAttn a{};
   st = check_kv_new(name, k_new, ldk, v_new, ldv, dtype, rope_cos, rope_sin, rope_len, prefix_len, cache, start_dev,

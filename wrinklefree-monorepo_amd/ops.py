@@ -1173,8 +1173,8 @@ def gqa_decode_attention_i8(
     q, k_new, v_new float32 or bfloat16, rows as for ``gqa_decode_attention``; up to 16 query heads per kv head; rope
     tables fp32 [positions, head_dim/2], as long as the positions need.  ``prefix``: an int8 cache of one sequence whose
     first ``prefix_len`` keys precede every sequence's own (a shared prompt, read once for the whole batch); ``pos`` stays
-    the position in the sequence's own cache, the rotary embedding takes row prefix_len + pos.  A position outside the
-    cache or the tables gives a NaN row and leaves the cache as it is."""
+    the position in the sequence's own cache, the rotary embedding takes row prefix_len + pos.  The prefix may not be part
+    of ``cache``.  A position outside the cache or the tables gives a NaN row and leaves the cache as it is."""
     name = "gqa_decode_attention_i8"
     if not isinstance(pos, torch.Tensor):
         raise RuntimeError(f"{name}: pos must be int64 [batch] on the device")
