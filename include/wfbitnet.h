@@ -445,7 +445,7 @@ int wfb_kv_read_i8(const wfb_kv_i8* cache, const int64_t* start_dev, int64_t sta
  * The rotary embedding takes row prefix_len + p.  Scores, softmax and sums are fp32, the output is rounded once to dtype.
  * T = 1 without lengths is a decode step: the codes' products with q and with the probabilities are exact integers, these
  * two being fixed-point numbers of 16 bits (dtype WFB_BF16) or 24 (WFB_F32) of their row's and block's largest.  The
- * tokens of a prompt, and a prefix that more than 64 rows (batch * num_heads / num_kv_heads) share, take fp16 products
+ * tokens of a prompt, and a long prefix that more than 32 rows (batch * num_heads / num_kv_heads) share, take fp16 products
  * with fp32 sums: q and probabilities in 11 bits (WFB_BF16; the values too, in 11 bits if their scale is above 2^-21 of
  * the largest in the sequence) or in two parts of 22 bits together (WFB_F32).  A row of q below 2^-100 counts as zeros;
  * keys of 2^100 and more may leave the range of the scores (NaN).  The prefix must not lie in the cache.

@@ -10,7 +10,7 @@ Tolerances of the attentions, per output element, are sums of what the arithmeti
     (a row's reference may lie up to four times above it), times 127 codes;
   * fp32 scores, exponentials and sums: 2^-20 of sum p |v| (1 + max |s|) covers ten roundings of 2^-24 and the
     exponent's argument;
-  * where bf16 rows take fp16 products (prompts, a prefix of more than 64 rows) and ``half`` asks for it: a half step of
+  * where bf16 rows take fp16 products (prompts, a long prefix of more than 32 rows) and ``half`` asks for it: a half step of
     fp16, 2^-11, of every element of q, and three of them (scale, value, weight) of sum p |v|.
 """
 
@@ -261,9 +261,13 @@ DECODES = [
     (33, 4, 1, 64, 64, list(range(33)), BF16, 130),
     (5, 32, 8, 128, 256, [200, 0, 13, 64, 255], BF16, 1500),
     (2, 12, 1, 128, 192, [190, 64], F32, 0),
-    (20, 8, 2, 128, 128, list(range(60, 80)), BF16, 64),   # more than 64 rows against the prefix, whole blocks
+    (20, 8, 2, 128, 128, list(range(60, 80)), BF16, 64),   # several workgroups of rows against the prefix, whole blocks
     (20, 8, 2, 128, 64, list(range(20)), F32, 321),
     (17, 33, 3, 64, 64, list(range(17)), F32, 129),
+    (45, 16, 2, 64, 64, [63 - i for i in range(45)], BF16, 1790),  # from here the prefix as fp16 products
+    (40, 9, 3, 128, 128, list(range(40)), BF16, 3840),
+    (15, 64, 4, 64, 64, list(range(15)), F32, 8800),
+    (9, 120, 8, 128, 64, list(range(9)), F32, 7300),
 ]
 
 
@@ -422,6 +426,8 @@ PROMPTS = [
     (1, 4, 1, 128, 4160, [4000], [100], 100, BF16, 0),  # few rows, a long axis
     (3, 8, 2, 64, 128, [5, 64, 127], [1, 0, 1], 1, BF16, 0),  # one token a sequence, one of them padding
     (2, 33, 3, 128, 192, [100, 0], [41, 90], 90, F32, 64),
+    (2, 8, 2, 64, 128, [0, 28], [90, 100], 300, BF16, 0),  # padded to more than the cache holds
+    (1, 16, 4, 64, 1024, [700], [200], 200, F32, 0),       # long enough to be split
 ]
 
 
@@ -529,7 +535,7 @@ EXTREMES = [
     # b, hq, hkv, d, t, prefix length (t 0: a decode step)
     (3, 8, 2, 64, 0, 0),
     (3, 8, 2, 128, 0, 70),
-    (20, 8, 2, 64, 0, 300),   # the prefix as fp16 products
+    (48, 16, 2, 64, 0, 1790),   # bf16: the prefix as fp16 products
     (2, 9, 3, 64, 33, 0),
     (2, 8, 2, 128, 40, 100),
 ]
@@ -650,7 +656,7 @@ def test_side_stream_and_unaligned_inputs(pkg, dev):
 
 def test_two_streams_at_once(pkg, dev):
     """Calls in flight on two streams, each with a cache and a workspace of its own, over one prefix."""
-    cases = [(20, 8, 2, 64, 0, 300), (2, 9, 3, 64, 33, 0), (3, 8, 2, 128, 0, 0)]
+    cases = [(48, 16, 2, 64, 0, 1790), (2, 9, 3, 64, 33, 0), (3, 8, 2, 128, 0, 0)]
     made = [_made(c, BF16, seed=i) for i, c in enumerate(cases)]
     want = [_call(pkg, dev, c, x, host.to(pkg, dev), pre, 100) for c, (x, host, pre) in zip(cases, made)]
     caches = [[host.to(pkg, dev) for _, host, _ in made] for _ in range(2)]

@@ -71,25 +71,38 @@ int cut(int64_t groups, int64_t target, int64_t most) {
   return (int)(n > most ? (most < 1 ? 1 : most) : n < 1 ? 1 : n);
 }
 
-Plan make_plan(int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t cap, int64_t npre, bool lengths) {
+// keys: how many of their own the sequences of a prompt are expected to see, the host's only guess where positions are on
+// the device.  More keys never mean fewer splits, so cap gives the largest plan.  Times in us: a captured call, fastest third.
+Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t cap, int64_t keys, int64_t npre, bool lengths) {
   const int64_t g = hq / hkv, pb = (npre + kKvBlock - 1) / kKvBlock, cb = cap / kKvBlock;
   Plan p{};
   p.decode = t == 1 && !lengths;
   if (p.decode) {
     // Splits of four blocks (one a wave) or more.  A cache of up to 1024 keys that needs no joining otherwise stays whole:
-    // 3 heads of 64, 32-bit, us in a graph, whole against split at a quarter and at all of 512 keys 5.3, 7.0 against 7.9,
-    // 8.5; of 1024 5.7, 9.3 against 8.5, 8.7; of 2048 8.5, 12.0 (splits of 16 blocks) against 8.6, 9.0.
+    // 3 heads of 64, 32-bit, whole against split at a quarter and at all of 512 keys 5.3, 7.0 against 7.9, 8.5; of 1024
+    // 5.7, 9.3 against 8.5, 8.7; of 2048 8.5, 12.0 (splits of 16 blocks) against 8.6, 9.0.
     p.own = npre == 0 && cb <= 16 ? 1 : cut(b * hkv, kLive, (cb + 3) / 4);
-    if (cb / p.own > 64) p.own = cut(b * hkv, 2 * kLive, cb);  // long splits: sequences of different lengths even out
+    // Splits of more than 64 blocks are halved, so that sequences of different lengths even out: 16 of 16384 to 32768 keys,
+    // 8 heads of 128, 159.6 against 163.7; 16 of 32768 197.5 both; 4 of 131071 194 against 191.
+    if (cb / p.own > 64) p.own = cut(b * hkv, 2 * kLive, cb);
     if (npre > 0) {
-      const int64_t rows = b * g;
-      p.pre_rows = rows > 64;
+      // The rows kernel reads a prefix once for 128 rows, where decode_part reads it for 16, but a block costs it three
+      // times as much (32-bit: more), and converting it is lost on few rows.  8 heads of 128, decode_part against rows:
+      // bf16, 128 rows and 1024 keys 14.5, 19.3; 160 rows 20.1, 19.7; 256 rows 23.5, 20.2; 64 rows and 8192 24.0, 23.3; 256
+      // rows 44.2, 32.7; 32 rows and 8192 20.9, 19.2, and 32768 28.5, 37.7.  fp32, 128 rows and 8192 28.9, 36.2; 256 rows
+      // 45.3, 47.1; 3 heads of 64, 384 rows and 8192 27.4, 25.9.
+      const int64_t rows = b * g, columns = hkv * ((rows + kColumns - 1) / kColumns);
+      p.pre_rows = rows > 32 && columns * pb > (dt == WFB_F32 ? 8192 : 1280);
       if (p.pre_rows) p.pre = cut(hkv * ((rows + 32 * kPrefixWaves - 1) / (32 * kPrefixWaves)), 256, (pb + 3) / 4);
-      else p.pre = cut(hkv * ((rows + kColumns - 1) / kColumns), kLive, (pb + 3) / 4);
+      else p.pre = cut(columns, kLive, (pb + 3) / 4);
     }
   } else {
-    const int64_t groups = b * hkv * ((t * g + kRowsPerGroup - 1) / kRowsPerGroup);
-    p.own = groups >= 96 ? 1 : cut(groups, 256, (pb + cb + 3) / 4);
+    // Split where the GPU is not full and the keys are many: parts of every row go out and come back, 16 us for 65536 rows
+    // of 128, what a workgroup needs for about 7 blocks.  8 heads of 128, whole against split: 512 tokens 30.8, 34.6, behind
+    // 2048 keys 90.1, 50.0; 1024 tokens 46.8, 50.6, behind 2048 keys 105.5, 83.0.
+    const int64_t groups = b * hkv * ((t * g + kRowsPerGroup - 1) / kRowsPerGroup), blocks = pb + (keys + kKvBlock - 1) / kKvBlock;
+    const int64_t n = cut(groups, 256, (blocks + 3) / 4);
+    p.own = blocks * (n - 1) >= 9 * n ? (int)n : 1;
   }
   return p;
 }
@@ -1093,7 +1106,9 @@ __global__ __launch_bounds__(kThreads) void kv_join_kernel(KvAttn a, Parts parts
 
 template <int DT, int D>
 hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
-  const Plan p = make_plan(a.b, a.t, a.hq, a.hkv, a.own.cap, a.npre, a.span.len_dev != nullptr);
+  // where starts are on the device, halfway between the first chunk of a cache and its last
+  const int64_t cap = a.own.cap, keys = !a.span.start_dev ? a.span.start + a.t : a.t < cap ? (a.t + cap) / 2 : cap;
+  const Plan p = make_plan(a.dt, a.b, a.t, a.hq, a.hkv, cap, keys, a.npre, a.span.len_dev != nullptr);
   const Parts parts = parts_of(a, p);
   const int g = a.hq / a.hkv;
   hipError_t e;
@@ -1128,12 +1143,13 @@ hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
 }  // namespace
 
 int64_t kv_attn_workspace_floats(int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t d, int64_t cap, int64_t npre) {
-  // (with lengths a call of one token per sequence takes the rows kernel: room for either)
+  // room for either type, and for one token per sequence with lengths, which takes the rows kernel
   int64_t most = 0;
-  for (int lengths = 0; lengths < 2; ++lengths) {
-    const Plan p = make_plan(b, t, hq, hkv, cap, npre, lengths != 0);
-    if (has_parts(p)) most = most > p.own + p.pre ? most : p.own + p.pre;
-  }
+  for (int dt : {WFB_F32, WFB_BF16})
+    for (bool lengths : {false, true}) {
+      const Plan p = make_plan(dt, b, t, hq, hkv, cap, cap, npre, lengths);
+      if (has_parts(p)) most = most > p.own + p.pre ? most : p.own + p.pre;
+    }
   return most * b * t * hq * (d + 2);
 }
 
