@@ -955,31 +955,49 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
   }
 
   l_run += xor_lanes_f32<32>(l_run);
-  if (r >= R) return;
-  // lane holds O^T[32 d + 8 (i / 4) + 4 grp + i % 4]
-  const float unit = vref * (1.0f / kUp);
+  // A lane holds O^T[32 d + 8 (i / 4) + 4 grp + i % 4] of its row.  Half a row at a time goes through LDS, so that it leaves
+  // in one piece and not 16 bytes (of bf16 8) at a time.
+  constexpr int NC = D / 8, RP = 64 / NC;  // pieces of four elements in half a row, rows that the wave stores at once
+  const float f = parts.o ? vref * (1.0f / kUp) : vref * (1.0f / kUp) / l_run;
+  int64_t at = r < R ? qrow * a.ldo + (int64_t)h * D : -1;
   if (parts.o) {
-    if (!valid) return;
     const int64_t row = (int64_t)(slot0 + split) * parts.rows + qrow * a.hq + h;
-#pragma unroll
-    for (int d = 0; d < DTL; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4*>(parts.o + row * D + 32 * d + 2 * i + 4 * grp) =
-            make_float4(o[d][i] * unit, o[d][i + 1] * unit, o[d][i + 2] * unit, o[d][i + 3] * unit);
-    if (grp == 0) parts.ml[row] = make_float2(m_ref, l_run);
-    return;
+    at = valid ? row * D : -1;
+    if (valid && grp == 0) parts.ml[row] = make_float2(m_ref, l_run);
   }
-  const float f = valid ? unit / l_run : 0.0f;
+  int64_t ats[32 / RP];  // of the rows that the lane stores a piece of
 #pragma unroll
-  for (int d = 0; d < DTL; ++d)
+  for (int p = 0; p < 32 / RP; ++p) ats[p] = __shfl(at, p * RP + lane / NC);
+  __syncthreads();  // no one reads the tiles any more
+  float4* buf = reinterpret_cast<float4*>(tile) + w * 32 * NC;  // [row][piece ^ row]
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      float v[4];
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v[x] = valid ? o[d][i + x] * f : 0.0f;
-      store4<DT>(a.out, qrow * a.ldo + (int64_t)h * D + 32 * d + 2 * i + 4 * grp, v);
+    for (int d = 0; d < DTL / 2; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x16_t& x = o[half * (DTL / 2) + d];
+        buf[col * NC + ((8 * d + i / 2 + grp) ^ (col % NC))] =
+            valid ? make_float4(x[i] * f, x[i + 1] * f, x[i + 2] * f, x[i + 3] * f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < 32 / RP; ++p) {
+      const int row = p * RP + lane / NC, piece = lane % NC;
+      const float4 x = buf[row * NC + (piece ^ (row % NC))];
+      const int64_t to = ats[p] + half * (D / 2) + 4 * piece;
+      if (ats[p] < 0) continue;
+      if (parts.o) {
+        *reinterpret_cast<float4*>(parts.o + to) = x;
+      } else {
+        const float v[4] = {x.x, x.y, x.z, x.w};
+        store4<DT>(a.out, to, v);
+      }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // ---- kernels ------------------------------------------------------------------------------------------
