@@ -428,6 +428,8 @@ PROMPTS = [
     (2, 33, 3, 128, 192, [100, 0], [41, 90], 90, F32, 64),
     (2, 8, 2, 64, 128, [0, 28], [90, 100], 300, BF16, 0),  # padded to more than the cache holds
     (1, 16, 4, 64, 1024, [700], [200], 200, F32, 0),       # long enough to be split
+    (14, 14, 14, 64, 320, [5 * i for i in range(13)] + [0], [257 - i for i in range(13)] + [257], 257, BF16, 0),  # many rows
+    (9, 22, 22, 128, 320, list(range(9)), [300] * 9, 300, BF16, 3),
 ]
 
 

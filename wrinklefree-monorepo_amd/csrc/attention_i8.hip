@@ -58,13 +58,13 @@ struct Plan {
   int own, pre;
   bool decode;    // one token per sequence: decode kernel, else the rows kernel
   bool pre_rows;  // the prefix by the rows kernel
+  int waves;      // of a workgroup of prompt rows, 32 rows each
 };
 
 constexpr int kLive = 512;         // workgroups of four waves that fill the GPU: two per CU by their registers
 constexpr int kColumns = 16;       // rows (token, query head) of a workgroup of decode_part
-constexpr int kRowsWaves = 8;      // of a workgroup of prompt rows, 32 rows each
+constexpr int kRowsWaves = 8;      // of a workgroup of prompt rows at most, 32 rows each
 constexpr int kPrefixWaves = 4;    // of a workgroup of a decode step's rows against the prefix
-constexpr int kRowsPerGroup = 32 * kRowsWaves;
 
 int cut(int64_t groups, int64_t target, int64_t most) {
   const int64_t n = target / groups;
@@ -73,7 +73,8 @@ int cut(int64_t groups, int64_t target, int64_t most) {
 
 // keys: how many of their own the sequences of a prompt are expected to see, the host's only guess where positions are on
 // the device.  More keys never mean fewer splits, so cap gives the largest plan.  Times in us: a captured call, fastest third.
-Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t cap, int64_t keys, int64_t npre, bool lengths) {
+Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t d, int64_t cap, int64_t keys, int64_t npre,
+               bool lengths) {
   const int64_t g = hq / hkv, pb = (npre + kKvBlock - 1) / kKvBlock, cb = cap / kKvBlock;
   Plan p{};
   p.decode = t == 1 && !lengths;
@@ -100,9 +101,15 @@ Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t ca
     // Split where the GPU is not full and the keys are many: parts of every row go out and come back, 16 us for 65536 rows
     // of 128, what a workgroup needs for about 7 blocks.  8 heads of 128, whole against split: 512 tokens 30.8, 34.6, behind
     // 2048 keys 90.1, 50.0; 1024 tokens 46.8, 50.6, behind 2048 keys 105.5, 83.0.
-    const int64_t groups = b * hkv * ((t * g + kRowsPerGroup - 1) / kRowsPerGroup), blocks = pb + (keys + kKvBlock - 1) / kKvBlock;
+    // Four waves, which convert a block for 128 rows instead of 256, where eight would leave rows or CUs empty: 8 heads of
+    // 128, 4 query heads each, eight against four: 512 tokens 29.7, 26.3; 1024 45.7, 40.1; 2048 79.8, 73.5; 3000 114.0,
+    // 111.8; 4096 171.9, 194.8; 16 tokens behind 4000 keys 27.2, 24.6; 48 of 8 sequences behind 4000 45.4, 54.8.  (fp32 rows
+    // of 128 do not fit into the registers of four: 2 x 1587 tokens, 10 / 5 heads, 90.7, 101.7.)
+    const int64_t rows = t * g, groups = b * hkv * ((rows + 32 * kRowsWaves - 1) / (32 * kRowsWaves));
+    const int64_t blocks = pb + (keys + kKvBlock - 1) / kKvBlock;
     const int64_t n = cut(groups, 256, (blocks + 3) / 4);
     p.own = blocks * (n - 1) >= 9 * n ? (int)n : 1;
+    p.waves = (rows <= 128 || (p.own == 1 && groups <= 384)) && (dt == WFB_BF16 || d == 64) ? 4 : kRowsWaves;
   }
   return p;
 }
@@ -1030,12 +1037,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
                             *reinterpret_cast<Own*>(smem));
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(64 * kRowsWaves) __attribute__((amdgpu_waves_per_eu(2))) void kv_rows_kernel(KvAttn a,
-                                                                                                         Parts parts,
-                                                                                                         Plan plan) {
+template <int DT, int D, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void kv_rows_kernel(KvAttn a, Parts parts,
+                                                                                                Plan plan) {
   __shared__ __attribute__((aligned(16))) RowsShared<D> sh;
-  rows_part<DT, D, kRowsWaves, false>(a, parts, 0, plan.own, blockIdx.x, sh);
+  rows_part<DT, D, W, false>(a, parts, 0, plan.own, blockIdx.x, sh);
 }
 
 // ---- joining ----------------------------------------------------------------------------------------
@@ -1126,7 +1132,7 @@ template <int DT, int D>
 hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
   // where starts are on the device, halfway between the first chunk of a cache and its last
   const int64_t cap = a.own.cap, keys = !a.span.start_dev ? a.span.start + a.t : a.t < cap ? (a.t + cap) / 2 : cap;
-  const Plan p = make_plan(a.dt, a.b, a.t, a.hq, a.hkv, cap, keys, a.npre, a.span.len_dev != nullptr);
+  const Plan p = make_plan(a.dt, a.b, a.t, a.hq, a.hkv, a.d, cap, keys, a.npre, a.span.len_dev != nullptr);
   const Parts parts = parts_of(a, p);
   const int g = a.hq / a.hkv;
   hipError_t e;
@@ -1144,9 +1150,14 @@ hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
   } else {
     e = launch_kv_write_i8(a.dt, a.d, a.kn, a.ldk, a.vn, a.ldv, a.rc, a.rs, a.npre, a.own, a.span, a.b, a.hkv, s);
     if (e != hipSuccess) return e;
-    const int64_t groups = ((int64_t)a.t * g + kRowsPerGroup - 1) / kRowsPerGroup * a.hkv * a.b * p.own;
+    const int each = 32 * p.waves;
+    const int64_t groups = ((int64_t)a.t * g + each - 1) / each * a.hkv * a.b * p.own;
     if (groups > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((kv_rows_kernel<DT, D>), dim3((unsigned)groups), dim3(64 * kRowsWaves), 0, s, a, parts, p);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * p.waves), 0, s, a, parts, p);
+    };
+    if (p.waves == kRowsWaves) go(kv_rows_kernel<DT, D, kRowsWaves>);
+    else if constexpr (DT == WFB_BF16 || D == 64) go(kv_rows_kernel<DT, D, 4>);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!has_parts(p)) return hipSuccess;
@@ -1165,7 +1176,7 @@ int64_t kv_attn_workspace_floats(int64_t b, int64_t t, int64_t hq, int64_t hkv, 
   int64_t most = 0;
   for (int dt : {WFB_F32, WFB_BF16})
     for (bool lengths : {false, true}) {
-      const Plan p = make_plan(dt, b, t, hq, hkv, cap, cap, npre, lengths);
+      const Plan p = make_plan(dt, b, t, hq, hkv, d, cap, cap, npre, lengths);
       if (has_parts(p)) most = most > p.own + p.pre ? most : p.own + p.pre;
     }
   return most * b * t * hq * (d + 2);
