@@ -71,8 +71,8 @@ int cut(int64_t groups, int64_t target, int64_t most) {
   return (int)(n > most ? (most < 1 ? 1 : most) : n < 1 ? 1 : n);
 }
 
-// keys: how many of their own the sequences of a prompt are expected to see, the host's only guess where positions are on
-// the device.  More keys never mean fewer splits, so cap gives the largest plan.  Times in us: a captured call, fastest third.
+// keys: how many of their own the sequences of a prompt are expected to see (positions may be known on the device only).
+// More keys never mean fewer splits, so cap gives the largest plan.  Times in us, of one call in a graph.
 Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t d, int64_t cap, int64_t keys, int64_t npre,
                bool lengths) {
   const int64_t g = hq / hkv, pb = (npre + kKvBlock - 1) / kKvBlock, cb = cap / kKvBlock;
@@ -145,6 +145,11 @@ __device__ __forceinline__ int64_t split_blocks(int64_t nb, int n) { return ((nb
 // The products are exact; a block's sums of V^T W^T come to less than 2^31 (127 * 2^15 * 64 < 2^28) and are added up in fp32.
 // The key that row R of score tile n stands for is chosen as 16 (R / 4) + 4 n + R % 4: a lane then holds 16 consecutive
 // keys, the ones that it feeds into the second product.
+// What bounds it: HBM where the cache is large (16 sequences of 16384 to 32768 keys, 8 heads of 128, 32 query heads, bf16:
+// 0.7 GB in 143 us, 4.9 TB/s; one of 131071 keys and 5 heads 36 us, 4.8 TB/s), else the chain of one block's loads, products
+// and exponentials (8 sequences of 1000 to 4096 keys: 44 MB in 15.2 us).  A wave's next block is fetched under the products
+// of the one before; splits are sized so that two workgroups a CU are at work.  No conversion of codes and no LDS on the
+// way: one key at a time in fp32, as the plain kernel had it, took 3.6 ms for the first of these.
 template <int NP>
 struct Digits;
 template <>
@@ -528,14 +533,19 @@ __device__ __forceinline__ void f16_parts(float x0, float x1, uint32_t (&part)[N
   part[0] = h;
 }
 
-// Rows r of one kv head (row r: token r / G, query head r % G), 32 per wave, 128 per workgroup, against blocks of 64 keys
-// that the workgroup converts to fp16 (exactly) into LDS.  PREFIX: the rows of all sequences of a decode step against the
+// Rows r of one kv head (row r: token r / G, query head r % G), 32 per wave of W, against blocks of 64 keys that the
+// workgroup converts to fp16 (exactly) into LDS.  PREFIX: the rows of all sequences of a decode step against the
 // shared prefix; else the prefix first, if there is one, then the sequence's own keys, causal.
 //   S^T[key, row] = K Q^T         v_mfma_f32_32x32x16_f16; q in fp16 of its row's largest (fp32 rows: two parts)
 //   p = exp2(s k_scale c - m)     fp32, a reference m that follows the row's maximum in steps of 2^8 or more
 //   O^T[d, row] += V^T W^T        w = p v_scale / (reference of the scales) in fp16 (fp32 rows: two parts)
 // As in the decode kernel the key of a score tile's row is chosen so that a lane holds the keys that it feeds into the
 // second product, 8 consecutive ones per step.
+// What bounds it: nothing alone.  4096 tokens, 32 / 8 heads of 128, bf16: 137 GFLOP in 172 to 182 us (0.8 PFLOP/s); the
+// matrix cores are busy 34% of the cycles, vector instructions 43%, LDS about half, since a product of 32 x 32 x 16 reads 16
+// bytes a lane of it; two waves a SIMD (by their registers) leave the rest to latency.  A block costs 256 rows 2.0 to 2.8 us.
+// Tried without gain: the two waves of a SIMD half a block apart (197 against 187 us), 64 rows a wave and one wave a SIMD
+// (331: 100 spilled registers), the exponentials a block ahead of their products (5% slower).
 template <int D>
 struct RowsShared {
   uint16_t tile[2][2][kKvBlock * D];  // [buffer][keys, values]
@@ -554,14 +564,14 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
   // factors of the scores in both: a score may be large, and 11 bits of it too few.
   constexpr bool kScaled = NP == 1;
   constexpr int HD = D / 2, KS = D / 16, DTL = D / 32;
-  // (a scale is at most half its reference.)  One part: weights reach 2^kSlack, so their reference rarely moves, and values
+  // A scale is at most half its reference.  One part: weights reach 2^kSlack, so their reference rarely moves, and values
   // 127 kUp / 2 < 2^14.  Two parts: weights reach 2^(kSlack - 1) kUp = 2^15, which keeps the lower part of weights down to
   // 2^-16 of the row's largest out of the subnormal numbers.
   constexpr float kSlack = NP == 1 ? 8.0f : 1.0f, kUp = NP == 1 ? 0x1p8f : 0x1p15f;
-  constexpr int kRingK = 4, kRingV = 4;                           // fragments read ahead of their products
-  constexpr int CK = D / 16;               // pieces of 16 codes of a key
-  constexpr int KP = kKvBlock * CK;        // of a block's keys; as many of its values
-  constexpr int PT = 2 * KP / (64 * W);    // per thread
+  constexpr int kRingK = 4, kRingV = 4;  // fragments read ahead of their products
+  constexpr int CK = D / 16;             // pieces of 16 codes of a key
+  constexpr int KP = kKvBlock * CK;      // of a block's keys; as many of its values
+  constexpr int PT = 2 * KP / (64 * W);  // per thread
   static_assert(PT * 64 * W == 2 * KP && KP % 64 == 0, "whole waves take keys or values");
   static_assert(KP % (64 * W) == 0 || D == kKvBlock, "a round of keys and values needs rows of one length");
   auto& tile = sh.tile;
@@ -622,7 +632,8 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
   auto vswz = [](int d) { return (d >> 1) & 7; };
   v4i raw[2][PT] = {};  // codes of the next block and of the one behind it
   const int64_t pre_at = kvh * a.pre.cap, own_at = ((int64_t)b * a.hkv + kvh) * a.own.cap;
-  const int pre_tail = (int)(a.npre - (int64_t)(pb - 1) * kKvBlock), own_tail = (int)(own - (int64_t)(nb - pb - 1) * kKvBlock);
+  const int pre_tail = (int)(a.npre - (int64_t)(pb - 1) * kKvBlock);  // keys of the last blocks
+  const int own_tail = (int)(own - (int64_t)(nb - pb - 1) * kKvBlock);
   // The first key of a block in its cache.  (Members are chosen one by one: a choice between the two structs would have to
   // be read through a pointer, in every block.)
   auto first_key = [&](int kb) { return kb < pb ? pre_at + (int64_t)kb * kKvBlock : own_at + (int64_t)(kb - pb) * kKvBlock; };
@@ -793,7 +804,7 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
     const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
     const uint16_t* ks = tile[buf][0];
     const uint16_t* vs = tile[buf][1];
-    fetch_codes(kb + 2 < kb1 ? kb + 2 : kb1 - 1, buf);  // (always: with loads in a branch every wait would be for all of them)
+    fetch_codes(kb + 2 < kb1 ? kb + 2 : kb1 - 1, buf);  // (always: behind a branch every wait would be for all loads)
     read_factors(0, slot1);
     const float vnew = vref_s[slot];
     if (vnew != vref) {  // uniform
@@ -854,9 +865,10 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
       }
     // keys of the block that the row sees, and the wave's first one, if not all of them
     const int64_t k0 = (int64_t)(kb - pb) * kKvBlock;
-    const int low = kb < pb - 1 ? kKvBlock : kb == pb - 1 ? pre_tail : pos_low + 1 - k0 > kKvBlock ? kKvBlock : (int)(pos_low + 1 - k0);
+    auto sees = [&](int64_t p) { return p + 1 - k0 > kKvBlock ? kKvBlock : (int)(p + 1 - k0); };
+    const int low = kb < pb - 1 ? kKvBlock : kb == pb - 1 ? pre_tail : sees(pos_low);
     if (low < kKvBlock) {  // uniform
-      const int seen = kb < pb ? pre_tail : pos + 1 - k0 > kKvBlock ? kKvBlock : (int)(pos + 1 - k0);
+      const int seen = kb < pb ? pre_tail : sees(pos);
 #pragma unroll
       for (int nb2 = 0; nb2 < 2; ++nb2)
 #pragma unroll
@@ -1047,7 +1059,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
 // ---- joining ----------------------------------------------------------------------------------------
 
 // out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the slots that were written, W waves per row: D / 4 lanes take
-// four elements each, the groups of lanes the slots in turn.
+// four elements each, the groups of lanes the slots in turn.  Bound by latency (4 to 8 us for 1 to 30 MB).
 template <int DT, int D, int W>
 __global__ __launch_bounds__(kThreads) void kv_join_kernel(KvAttn a, Parts parts, Plan plan) {
   constexpr int L = D / 4, G = 64 * W / L;  // lanes of a group, groups of a row
@@ -1161,7 +1173,8 @@ hipError_t launch_dd(const KvAttn& a, hipStream_t s) {
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!has_parts(p)) return hipSuccess;
-  // a row's slots by one wave, or by four where they are many
+  // a row's slots by one wave, or by four where they are many: a whole call of 2 sequences of 8192 keys (32 splits of 64
+  // rows) 16.0, 14.1 us; one of 4096 keys and 3 heads (16 splits) 9.5, 9.9; 4 of 8192 (16 splits of 128 rows) 20.5 both
   if (p.own + p.pre <= 16)
     hipLaunchKernelGGL((kv_join_kernel<DT, D, 1>), dim3((unsigned)((parts.rows + 3) / 4)), dim3(kThreads), 0, s, a, parts, p);
   else
