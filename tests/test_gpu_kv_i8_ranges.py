@@ -1,0 +1,76 @@
+"""The attentions over the int8 cache where a number comes near the end of what holds it: value scales that double from
+one block of keys to the next, one key that takes nearly all the weight, scores far outside the exponential's range.
+
+Every case runs as a decode step over a sequence's own keys, as a prompt, and as a decode step behind a long prefix that
+more than 32 rows share (the matrix-core form of prompts), so each softmax meets it.
+"""
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv_i8 import BF16, F32, Host, _attention, _check
+
+pytestmark = pytest.mark.gpu
+
+D = 64
+
+
+def _empty(b, h, cap):
+    return Host(b, h, cap, D, torch.Generator().manual_seed(0), empty=True)
+
+
+class Keys:
+    """``n`` keys and values, the same for every kv head, met by queries ``q`` [rows, D] in one of three ways; each row sees
+    all of them, and new keys of zeros with values of zeros that ``n`` does not count."""
+
+    FORMS = ["step", "prompt", "shared"]
+
+    def __init__(self, form, n, heads, kv_heads, dtype):
+        self.form, self.n, self.hq, self.h, self.dtype = form, n, heads, kv_heads, dtype
+        # rows of the call: a step and a prompt's last token take one sequence; the prefix is shared by 40 sequences or more
+        self.b, self.t = {"step": (3, 1), "prompt": (1, 33), "shared": (45, 1)}[form]
+        self.cap = (n + self.t + 63) // 64 * 64
+        self.held = _empty(1 if form == "shared" else self.b, kv_heads, self.cap)
+
+    def run(self, pkg, dev, q, scale):
+        """Outputs of the rows q [b * t, hq * D] and the definition with its bound."""
+        b, t, hq, h, n = self.b, self.t, self.hq, self.h, self.n
+        zeros = torch.zeros((b * t, h * D), dtype=self.dtype)
+        own, start, kw, pre, npre = self.held, n, {}, None, 0
+        if self.form == "shared":
+            pre, npre, own, start = self.held, n, _empty(b, h, 64), 0
+            kw = {"prefix": pre.to(pkg, dev), "prefix_len": n}
+        cache = own.to(pkg, dev)
+        args = (q.to(dev), zeros.to(dev), zeros.to(dev), cache)
+        if self.form == "prompt":
+            out = pkg.gqa_prefill_attention_i8(*args, start, t, scale=scale, **kw)
+        else:
+            out = pkg.gqa_decode_attention_i8(*args, torch.full((b,), start, device=dev), scale=scale, **kw)
+        own.write(zeros, zeros, [start] * b, [t] * b, t, None, None)
+        ref, tol = _attention(q, own, [start] * b, [t] * b, t, None, None, scale, self.dtype, pre, npre,
+                              half=self.form != "step")
+        return out.cpu(), ref, tol
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", Keys.FORMS)
+def test_a_value_scale_that_doubles_under_a_growing_maximum(pkg, dev, form, dtype):
+    """Values of scale 1, then one of scale 2 whose key's weight lies just under twice the maximum before it: weight and
+    scale at the ends of their ranges at once (scores of 0, then of 0.9990 to 1.0001 in powers of two)."""
+    print(f"[kv ranges] doubling {form} {dtype}", flush=True)
+    m = Keys(form, 8800, 32, 4, dtype)
+    m.held.v[:, :, :m.n] = torch.randint(-127, 128, (1, 4, m.n, D), generator=torch.Generator().manual_seed(1),
+                                         dtype=torch.int8)
+    m.held.vs[:, :, :m.n] = 1.0
+    for j in range(70, m.n, 128):  # in every second block
+        m.held.k[:, :, j, 0] = 127
+        m.held.ks[:, :, j] = 1.0 / 127
+        m.held.v[:, :, j, ::2] = 127
+        m.held.vs[:, :, j] = 2.0
+    rows = m.b * m.t * 32
+    q = torch.zeros((rows, D))
+    q[:, 0] = math.log(2.0) * torch.linspace(0.9990, 1.0001, rows)
+    out, ref, tol = m.run(pkg, dev, q.reshape(-1, 32 * D).to(dtype), 1.0)
+    _check(out, ref, tol, form)

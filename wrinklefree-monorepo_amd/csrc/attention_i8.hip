@@ -564,9 +564,10 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
   // factors of the scores in both: a score may be large, and 11 bits of it too few.
   constexpr bool kScaled = NP == 1;
   constexpr int HD = D / 2, KS = D / 16, DTL = D / 32;
-  // A scale is at most half its reference.  One part: weights reach 2^kSlack, so their reference rarely moves, and values
-  // 127 kUp / 2 < 2^14.  Two parts: weights reach 2^(kSlack - 1) kUp = 2^15, which keeps the lower part of weights down to
-  // 2^-16 of the row's largest out of the subnormal numbers.
+  // A scale is at most half its reference, in every block.  One part: weights reach 2^kSlack, so their reference rarely
+  // moves, and values 127 kUp / 2 < 2^14.  Two parts: weights reach 2^(kSlack - 1) kUp = 2^15, which keeps the lower part of
+  // weights down to 2^-16 of the row's largest out of the subnormal numbers; a scale above half its reference would take
+  // them past 65504.
   constexpr float kSlack = NP == 1 ? 8.0f : 1.0f, kUp = NP == 1 ? 0x1p8f : 0x1p15f;
   constexpr int kRingK = 4, kRingV = 4;  // fragments read ahead of their products
   constexpr int CK = D / 16;             // pieces of 16 codes of a key
@@ -743,7 +744,7 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
       mx = fmaxf(mx, xor_lanes_f32<4>(mx));
       mx = fmaxf(mx, xor_lanes_f32<2>(mx));
       mx = fmaxf(mx, xor_lanes_f32<1>(mx));
-      if (mx > ref)  // twice the next power of two: growth below it costs nothing
+      if (2.0f * mx > ref)  // twice the power of two at or above it: growth up to that power costs nothing
         ref = __uint_as_float(((__float_as_uint(mx) + 0x7fffffu) & 0x7f800000u) + 0x800000u);
       const float y = x * (kUp * __uint_as_float(0x7f000000u - __float_as_uint(ref)));
       if constexpr (kScaled) reinterpret_cast<_Float16*>(svs[slot])[lane] = (_Float16)y;
