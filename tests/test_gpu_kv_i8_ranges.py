@@ -34,8 +34,9 @@ class Keys:
         self.cap = (n + self.t + 63) // 64 * 64
         self.held = _empty(1 if form == "shared" else self.b, kv_heads, self.cap)
 
-    def run(self, pkg, dev, q, scale):
-        """Outputs of the rows q [b * t, hq * D] and the definition with its bound."""
+    def run(self, pkg, dev, q, scale, half=True):
+        """Outputs of the rows q [b * t, hq * D] and the definition with its bound (``half``: with the terms of fp16
+        products, where there are any)."""
         b, t, hq, h, n = self.b, self.t, self.hq, self.h, self.n
         zeros = torch.zeros((b * t, h * D), dtype=self.dtype)
         own, start, kw, pre, npre = self.held, n, {}, None, 0
@@ -50,7 +51,7 @@ class Keys:
             out = pkg.gqa_decode_attention_i8(*args, torch.full((b,), start, device=dev), scale=scale, **kw)
         own.write(zeros, zeros, [start] * b, [t] * b, t, None, None)
         ref, tol = _attention(q, own, [start] * b, [t] * b, t, None, None, scale, self.dtype, pre, npre,
-                              half=self.form != "step")
+                              half=half and self.form != "step")
         return out.cpu(), ref, tol
 
 
@@ -73,4 +74,31 @@ def test_a_value_scale_that_doubles_under_a_growing_maximum(pkg, dev, form, dtyp
     q = torch.zeros((rows, D))
     q[:, 0] = math.log(2.0) * torch.linspace(0.9990, 1.0001, rows)
     out, ref, tol = m.run(pkg, dev, q.reshape(-1, 32 * D).to(dtype), 1.0)
+    _check(out, ref, tol, form)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", Keys.FORMS)
+def test_keys_far_below_one_that_takes_the_weight(pkg, dev, form, dtype):
+    """A key in every 128 with a value of zeros and a score of 10 to 16 above the rest (fp32: 14), whose equal weights make
+    the whole output: they are as exact as the large one.  All values are positive, so the output's sum loses nothing and
+    an error that the equal weights share shows in full.  The queries are exact in fp16; three roundings of 2^-11 are the
+    weight's, the value scale's and the scaled value's."""
+    print(f"[kv ranges] sink {form} {dtype}", flush=True)
+    m = Keys(form, {"prompt": 500}.get(form, 1790), 32, 4, dtype)
+    m.held.v[:, :, :m.n] = torch.randint(64, 128, (1, 4, m.n, D), generator=torch.Generator().manual_seed(2),
+                                         dtype=torch.int8)
+    m.held.vs[:, :, :m.n] = 1.0 / 127
+    sinks = torch.arange(5, m.n, 128)
+    m.held.k[:, :, sinks, 0] = 127
+    m.held.ks[:, :, sinks] = 1.0 / 127
+    m.held.v[:, :, sinks] = 0
+    m.held.vs[:, :, sinks] = 0.0
+    rows = m.b * m.t * 32
+    q = torch.zeros((rows, D))
+    q[:, 0] = torch.linspace(10.0, 16.0 if dtype == BF16 else 14.0, rows)
+    out, ref, tol = m.run(pkg, dev, q.reshape(-1, 32 * D).to(dtype), 1.0, half=False)
+    if dtype == BF16:
+        tol = tol + 3 * 2.0 ** -11 * ref.abs()
+    assert float(ref.min()) > 0.0 and float((tol / ref).max()) < 0.01
     _check(out, ref, tol, form)
