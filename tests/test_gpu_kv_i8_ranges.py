@@ -34,25 +34,31 @@ class Keys:
         self.cap = (n + self.t + 63) // 64 * 64
         self.held = _empty(1 if form == "shared" else self.b, kv_heads, self.cap)
 
-    def run(self, pkg, dev, q, scale, half=True):
-        """Outputs of the rows q [b * t, hq * D] and the definition with its bound (``half``: with the terms of fp16
-        products, where there are any)."""
-        b, t, hq, h, n = self.b, self.t, self.hq, self.h, self.n
-        zeros = torch.zeros((b * t, h * D), dtype=self.dtype)
-        own, start, kw, pre, npre = self.held, n, {}, None, 0
+    def call(self, pkg, dev, q, k_new, scale):
+        """Outputs of the rows q [b * t, hq * D] with new keys k_new [b * t, h * D] and values of zeros."""
+        own, start, kw = self.held, self.n, {}
         if self.form == "shared":
-            pre, npre, own, start = self.held, n, _empty(b, h, 64), 0
-            kw = {"prefix": pre.to(pkg, dev), "prefix_len": n}
+            own, start = _empty(self.b, self.h, 64), 0
+            kw = {"prefix": self.held.to(pkg, dev), "prefix_len": self.n}
         cache = own.to(pkg, dev)
-        args = (q.to(dev), zeros.to(dev), zeros.to(dev), cache)
+        args = (q.to(dev), k_new.to(dev), torch.zeros_like(k_new, device=dev), cache)
         if self.form == "prompt":
-            out = pkg.gqa_prefill_attention_i8(*args, start, t, scale=scale, **kw)
+            out = pkg.gqa_prefill_attention_i8(*args, start, self.t, scale=scale, **kw)
         else:
-            out = pkg.gqa_decode_attention_i8(*args, torch.full((b,), start, device=dev), scale=scale, **kw)
+            out = pkg.gqa_decode_attention_i8(*args, torch.full((self.b,), start, device=dev), scale=scale, **kw)
+        return out.cpu()
+
+    def run(self, pkg, dev, q, scale, half=True):
+        """The outputs under new keys of zeros and the definition with its bound (``half``: with the terms of fp16
+        products, where there are any)."""
+        b, t, h, n = self.b, self.t, self.h, self.n
+        zeros = torch.zeros((b * t, h * D), dtype=self.dtype)
+        out = self.call(pkg, dev, q, zeros, scale)
+        own, start, pre, npre = (_empty(b, h, 64), 0, self.held, n) if self.form == "shared" else (self.held, n, None, 0)
         own.write(zeros, zeros, [start] * b, [t] * b, t, None, None)
         ref, tol = _attention(q, own, [start] * b, [t] * b, t, None, None, scale, self.dtype, pre, npre,
                               half=half and self.form != "step")
-        return out.cpu(), ref, tol
+        return out, ref, tol
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -102,3 +108,33 @@ def test_keys_far_below_one_that_takes_the_weight(pkg, dev, form, dtype):
         tol = tol + 3 * 2.0 ** -11 * ref.abs()
     assert float(ref.min()) > 0.0 and float((tol / ref).max()) < 0.01
     _check(out, ref, tol, form)
+
+
+def _one_takes_all(pkg, dev, form, dtype, size, sign):
+    """Keys that are multiples of one direction, of elements up to ``size``, under queries of ``size``: the scores lie so
+    far apart that the output is the value of the largest, the last key (sign 1) or the first (-1).  Roundings of q turn
+    all scores alike; what remains is that of the output, and of fp16 the value's two."""
+    print(f"[kv ranges] one takes all {form} {dtype} {size} {sign}", flush=True)
+    m = Keys(form, 8800 if form == "shared" else 300, 32, 4, dtype)
+    gen = torch.Generator().manual_seed(3)
+    m.held.v[:, :, :m.n] = torch.randint(-127, 128, (1, 4, m.n, D), generator=gen, dtype=torch.int8)
+    m.held.vs[:, :, :m.n] = 1.0 / 127
+    m.held.k[:, :, :m.n] = 127 * sign
+    m.held.ks[:, :, :m.n] = size / 127 * torch.arange(1, m.n + 1) / m.n
+    rows = m.b * m.t
+    q = (size * (1.0 + 0.5 * torch.rand((rows, 32 * D), generator=gen))).to(dtype)
+    new = torch.full((rows, 4 * D), -2.0 * size if sign < 0 else 0.0, dtype=dtype)
+    out = m.call(pkg, dev, q, new, D ** -0.5).double().reshape(rows, 4, 8, D)
+    _, vals = m.held.held(0)
+    ref = vals[None, :, None, m.n - 1 if sign > 0 else 0].expand_as(out)
+    tol = (2.0 ** -8 + 2 * 2.0 ** -11 if dtype == BF16 else 2.0 ** -20) * ref.abs()
+    _check(out, ref, tol, f"{form} {size} {sign}")
+
+
+@pytest.mark.parametrize("size", [1e3, 2.5e3, 3e3, 4e3, 5e3, 1e4, 1e6, 1e10, 1e14])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", Keys.FORMS)
+def test_scores_of_very_large_magnitude(pkg, dev, form, dtype, size):
+    """Scores of 1e7 to 1e29, whose rounding alone is many powers of two."""
+    for sign in (1, -1):
+        _one_takes_all(pkg, dev, form, dtype, size, sign)

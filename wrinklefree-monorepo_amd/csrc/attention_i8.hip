@@ -733,6 +733,11 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float m_ref = kNoMax, l_run = 0.0f, vref = 0x1p-100f;
+  // A weight's exponent is s cq - m_ref with one rounding, where m_ref comes from a rounded product: the two may differ by
+  // half a unit of m_ref's last place, which is nothing below kFar and, far above it, whole powers of two.  A wave with such a
+  // reference multiplies first (and takes the maximum itself, since one kDown below it need not be a number).
+  constexpr float kFar = 0x1p20f;
+  bool far = false;
 
   float ref = 0x1p-100f;  // (wave 1) reference of the value scales so far
   auto stage_scales = [&](int slot) {
@@ -885,12 +890,22 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
 #pragma unroll
       for (int i = 0; i < 16; ++i) bmax = fmaxf(bmax, s[nb2][i]);
     bmax = fmaxf(bmax, xor_lanes_f32<32>(bmax)) * cq;
-    if (__any(bmax > m_ref + kSlack)) {
-      const float m_new = fmaxf(m_ref, bmax - kDown), alpha = __builtin_amdgcn_exp2f(m_ref - m_new);
+    if (__any(bmax - m_ref > kSlack)) {
+      const float m_new = fmaxf(m_ref, fabsf(bmax) < kFar ? bmax - kDown : bmax);
+      const float alpha = __builtin_amdgcn_exp2f(m_ref - m_new);
       m_ref = m_new;
+      far = __any(m_ref > kNoMax && fabsf(m_ref) >= kFar);
       l_run *= alpha;
 #pragma unroll
       for (int d = 0; d < DTL; ++d) o[d] *= alpha;
+    }
+    float c2 = cq;
+    if (far) {  // uniform
+      c2 = 1.0f;
+#pragma unroll
+      for (int nb2 = 0; nb2 < 2; ++nb2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[nb2][i] *= cq;
     }
     // O^T over 4 steps of 16 keys, 8 of them this lane's; a step's weights are formed under the products of the one before
     float psum = 0.0f;
@@ -904,8 +919,8 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
       }
     };
     auto weights = [&](int c, int j) {  // keys j and j + 1 of step c
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j], cq, -m_ref));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j + 1], cq, -m_ref));
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j], c2, -m_ref));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j + 1], c2, -m_ref));
       uint32_t part[NP];
       if constexpr (kScaled) {
         f16_parts<NP>(p0, p1, part);
