@@ -447,10 +447,11 @@ int wfb_kv_read_i8(const wfb_kv_i8* cache, const int64_t* start_dev, int64_t sta
  * two being fixed-point numbers of 16 bits (dtype WFB_BF16) or 24 (WFB_F32) of their row's and block's largest.  The
  * tokens of a prompt, and a long prefix that more than 32 rows (batch * num_heads / num_kv_heads) share, take fp16 products
  * with fp32 sums.  WFB_BF16: q, probabilities and values in 11 bits; a probability below 2^-24 of the row's largest is off by
- * up to 2^-35 of that instead, a value whose scale is below 2^-21 of the largest in the sequence has fewer bits.  WFB_F32: q
- * and the probabilities times value scales in two parts of 22 bits together; a product below 2^-16 of the largest is off by up
- * to 2^-38 of that instead.  (Largest: of the keys up to the end of the block of 64 that holds the row's last one.)  A row of
- * q below 2^-100 counts as zeros; keys of 2^100 and more may leave the range of the scores (NaN).  The prefix must not lie in the cache.
+ * up to 2^-35 of that instead, a value whose scale is below 2^-20 of the largest in the sequence has fewer bits.  WFB_F32: q
+ * and the probabilities times value scales in two parts of 22 bits together; a product below 2^-16 of the largest probability
+ * times the largest scale is off by up to 2^-38 of that instead.  (Largest: of the keys up to the end of the block of 64 that
+ * holds the row's last one.)  A row of q below 2^-100 counts as zeros; keys of 2^100 and more, and scores near the end of
+ * fp32's range and past it (2^126, in powers of two), may give NaN.  The prefix must not lie in the cache.
  * q, out [batch*T, ldq / ldo] and k_new, v_new as in wfb_kv_write_i8 (rows 16-byte aligned); num_heads / num_kv_heads
  * in 1..16, head_dim 64 or 128.  Rows at and behind lengths[b] are zeros; a sequence that does not fit (see above) gives
  * NaN rows and is not written.  workspace: the floats that wfb_gqa_attention_i8_workspace (host only) reports, 16-byte

@@ -138,3 +138,40 @@ def test_scores_of_very_large_magnitude(pkg, dev, form, dtype, size):
     """Scores of 1e7 to 1e29, whose rounding alone is many powers of two."""
     for sign in (1, -1):
         _one_takes_all(pkg, dev, form, dtype, size, sign)
+
+
+@pytest.mark.parametrize("size", [1e15, 1e16, 3e17, 1e18])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", Keys.FORMS)
+def test_scores_close_to_the_end_of_fp32(pkg, dev, form, dtype, size):
+    """Scores of 10^31 to 10^37 in powers of two, of either sign: a softmax is defined for all that are finite."""
+    for sign in (1, -1):
+        _one_takes_all(pkg, dev, form, dtype, size, sign)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens", [1, 2])
+@pytest.mark.parametrize("npre", [0, 1])
+def test_a_first_key_of_any_score_returns_its_value(pkg, dev, dtype, tokens, npre):
+    """The first token of a sequence sees one key (and a prefix of one key that lies further below): its output is that
+    key's value whatever the score."""
+    print(f"[kv ranges] first key {dtype} {tokens} {npre}", flush=True)
+    gen = torch.Generator().manual_seed(4)
+    q = torch.full((tokens, 2 * D), 1e16, dtype=dtype)
+    v = torch.randn((tokens, D), generator=gen).to(dtype)
+    pre = _empty(1, 1, 64)
+    pre.k[:, :, 0], pre.ks[:, :, 0], pre.v[:, :, 0], pre.vs[:, :, 0] = -127, 1e20 / 127, 127, 1.0
+    kw = {"prefix": pre.to(pkg, dev), "prefix_len": 1} if npre else {}
+    for size in (-1e16, -1.0, 0.0, 1e16):
+        host = _empty(1, 1, 64)
+        cache = host.to(pkg, dev)
+        k = torch.full((tokens, D), size, dtype=dtype)
+        args = (q.to(dev), k.to(dev), v.to(dev), cache)
+        if tokens == 1:
+            out = pkg.gqa_decode_attention_i8(*args, torch.zeros(1, dtype=torch.int64, device=dev), **kw)
+        else:
+            out = pkg.gqa_prefill_attention_i8(*args, 0, tokens, **kw)
+        host.write(k, v, [0], [tokens], tokens, None, None)
+        ref = host.held(0)[1][0, 0].repeat(2)[None]
+        tol = (2.0 ** -8 + 2 * 2.0 ** -11 if dtype == BF16 else 2.0 ** -20) * ref.abs()
+        _check(out[:1], ref, tol, f"score of {size}")

@@ -11,7 +11,8 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kThreads = 256;
-constexpr float kNoMax = -1e30f;  // running maximum of a row that has met no key: finite, so that no difference is NaN
+// Running maximum of a row that has met no key: finite, so that no difference is NaN, and not above any score.
+constexpr float kNoMax = -3.40282347e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DT>
