@@ -159,3 +159,14 @@ def test_model_refuses_what_the_int8_cache_does_not_take(pkg):
                     (dict(ok, head_dim=32), dict(kv_cache="int8")), (dict(ok, num_heads=17), dict(kv_cache="int8"))):
         with pytest.raises(ValueError, match="kv_cache"):
             M.BitNetDecoder(M.BitNetConfig(**cfg), device="cpu", **kw)
+
+
+@pytest.mark.parametrize("lengths", [1, 0, [1, 1], (1, 1), 1.0])
+def test_lengths_that_are_no_tensor_are_refused(pkg, lengths):
+    """A length for the whole batch is not a form of the call: dropped, all t tokens would be written and attended."""
+    c = pkg.kv_cache_i8(2, 2, 100, 64, "cpu")
+    x = torch.zeros((2, 128), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="lengths"):
+        pkg.kv_cache_write_i8(x, x, c, 0, 1, lengths=lengths)
+    with pytest.raises(RuntimeError, match="lengths"):
+        pkg.gqa_prefill_attention_i8(x, x, x, c, 0, 1, lengths=lengths)

@@ -1040,6 +1040,11 @@ def _per_sequence(name: str, what: str, x, b: int, index: int) -> Tuple[Optional
     return x.data_ptr(), 0
 
 
+def _check_lengths(name: str, lengths) -> None:
+    if lengths is not None and not isinstance(lengths, torch.Tensor):
+        raise RuntimeError(f"{name}: lengths must be None or int64 [batch] on the cache's device, got {type(lengths).__name__}")
+
+
 def _rows16(name: str, x: torch.Tensor, rows: int, width: int, dtype: torch.dtype, index: int):
     """(view or copy of x as [rows, width], row stride) with rows that start on 16 bytes."""
     if x.dtype != dtype or x.get_device() != index or x.numel() != rows * width:
@@ -1083,6 +1088,7 @@ def kv_cache_write_i8(
     sequence that are real (t by default); a sequence whose positions do not fit is not written (a start given as an int
     is checked here).  Position p takes row p + rope_offset of the tables."""
     name = "kv_cache_write_i8"
+    _check_lengths(name, lengths)
     st, b, h, _, d, index = _cache_i8(name, "cache", cache)
     dev = cache[0].device
     t = int(t)
@@ -1118,6 +1124,7 @@ def kv_cache_read_i8(
 
 
 def _attention_i8(name, q, k_new, v_new, cache, start, t, rope_cos, rope_sin, scale, out, lengths, prefix, prefix_len):
+    _check_lengths(name, lengths)
     st, b, h, cap, d, index = _cache_i8(name, "cache", cache)
     dev = cache[0].device
     rows = b * t
