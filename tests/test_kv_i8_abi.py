@@ -170,3 +170,13 @@ def test_lengths_that_are_no_tensor_are_refused(pkg, lengths):
         pkg.kv_cache_write_i8(x, x, c, 0, 1, lengths=lengths)
     with pytest.raises(RuntimeError, match="lengths"):
         pkg.gqa_prefill_attention_i8(x, x, x, c, 0, 1, lengths=lengths)
+
+
+def test_a_prefix_without_its_length_is_refused(pkg):
+    """Taken as a length of zero, the prefix would not be attended to at all."""
+    c, pre = pkg.kv_cache_i8(2, 2, 100, 64, "cpu"), pkg.kv_cache_i8(1, 2, 100, 64, "cpu")
+    x = torch.zeros((2, 128), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="prefix_len"):
+        pkg.gqa_decode_attention_i8(x, x, x, c, torch.zeros(2, dtype=torch.int64), prefix=pre)
+    with pytest.raises(RuntimeError, match="prefix_len"):
+        pkg.gqa_prefill_attention_i8(x, x, x, c, 0, 1, prefix=pre)

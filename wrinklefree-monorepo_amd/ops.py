@@ -1125,10 +1125,13 @@ def kv_cache_read_i8(
 
 def _attention_i8(name, q, k_new, v_new, cache, start, t, rope_cos, rope_sin, scale, out, lengths, prefix, prefix_len):
     _check_lengths(name, lengths)
+    if prefix is not None and prefix_len is None:
+        raise RuntimeError(f"{name}: give prefix_len, the keys of prefix that count")
+    prefix_len = 0 if prefix_len is None else int(prefix_len)
     st, b, h, cap, d, index = _cache_i8(name, "cache", cache)
     dev = cache[0].device
     rows = b * t
-    p_ptr, prefix_len = None, int(prefix_len)
+    p_ptr = None
     if prefix is not None:
         pst, pb, ph, _, pd, p_index = _cache_i8(name, "prefix", prefix)
         if pb != 1 or ph != h or pd != d or p_index != index:
@@ -1172,7 +1175,7 @@ def _attention_i8(name, q, k_new, v_new, cache, start, t, rope_cos, rope_sin, sc
 def gqa_decode_attention_i8(
     q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: Sequence[torch.Tensor], pos: torch.Tensor,
     rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-    out: Optional[torch.Tensor] = None, prefix: Optional[Sequence[torch.Tensor]] = None, prefix_len: int = 0,
+    out: Optional[torch.Tensor] = None, prefix: Optional[Sequence[torch.Tensor]] = None, prefix_len: Optional[int] = None,
 ) -> torch.Tensor:
     """``gqa_decode_attention`` over an int8 cache (``kv_cache_i8``): rotary embedding of q / k_new, quantising append at
     pos[b], attention over positions 0..pos[b] as the cache holds them.  Returns out [batch, num_heads * head_dim].
@@ -1192,7 +1195,7 @@ def gqa_prefill_attention_i8(
     q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: Sequence[torch.Tensor],
     start: Union[int, torch.Tensor], t: int, rope_cos: Optional[torch.Tensor] = None,
     rope_sin: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-    lengths: Optional[torch.Tensor] = None, prefix: Optional[Sequence[torch.Tensor]] = None, prefix_len: int = 0,
+    lengths: Optional[torch.Tensor] = None, prefix: Optional[Sequence[torch.Tensor]] = None, prefix_len: Optional[int] = None,
 ) -> torch.Tensor:
     """``gqa_prefill_attention`` over an int8 cache: a chunk of t tokens per sequence, appended at positions start ..
     start + t - 1 and causal over what the cache then holds, so a prompt gives the same cut into any chunks.  Returns
