@@ -180,3 +180,12 @@ def test_a_prefix_without_its_length_is_refused(pkg):
         pkg.gqa_decode_attention_i8(x, x, x, c, torch.zeros(2, dtype=torch.int64), prefix=pre)
     with pytest.raises(RuntimeError, match="prefix_len"):
         pkg.gqa_prefill_attention_i8(x, x, x, c, 0, 1, prefix=pre)
+
+
+def test_share_prefix_takes_one_sequence(pkg):
+    """Prompts of several sequences are not joined to one; the prefix that is there stays."""
+    model = pkg.model.BitNetDecoder.__new__(pkg.model.BitNetDecoder)
+    model.kv_cache, model._prefix, model._prefix_len = "int8", "held", 7
+    with pytest.raises(ValueError, match="one sequence"):
+        model.share_prefix(torch.zeros((2, 3), dtype=torch.long))
+    assert (model._prefix, model._prefix_len) == ("held", 7)

@@ -558,6 +558,8 @@ class BitNetDecoder:
         ``decode_step`` keep counting a sequence's own tokens.  ``None`` ends it.  Needs ``kv_cache="int8"``."""
         if self.kv_cache != "int8":
             raise ValueError("share_prefix needs kv_cache='int8'")
+        if ids is not None and ids.dim() > 0 and ids.shape[-1] != ids.numel():
+            raise ValueError(f"share_prefix takes the ids of one sequence, got {tuple(ids.shape)}")
         self._prefix, self._prefix_len = None, 0
         if ids is not None and ids.numel() > 0:
             n = ids.numel()
