@@ -1,0 +1,168 @@
+"""How far an attention over the int8 cache may be off in the norm: the roundings that its arithmetic makes, as independent
+errors, and CPU checks that a bound made of them rejects what is wrong by little.
+
+``expected`` gives, per row and head, the definition in float64 and the root mean square of the error's norm in two parts:
+
+  * ``e_out``, the output's rounding: u |o| / sqrt(3) with u = 2^-8 (bf16), 2^-23 (fp32: the division and the rounding), an
+    error spread evenly over half a step that is at most u of the value;
+  * ``e_in``, what is lost before it.  Of the fixed-point form (one token a sequence): the query's elements by a step of their
+    row's largest / 32512 (fp32: 8323072) spread evenly, through the softmax; a weight by a step of its block's largest
+    p v_scale / 32512, times its codes.  Of the fp16 form (prompts, long shared prefixes): 2^-11 of q, and of p v three
+    times (weight, scale, scaled value), with weights below 2^-24 of the largest off by 2^-35 of it; fp32 rows 2^-22 of q and of
+    p v, and 2^-38 of the largest probability times the largest scale.  Of both: 2^-22 (1 + |s|) of a weight, s the score
+    in powers of two, of which 2^-23 |s| alike for the row; 16 roundings of 2^-24 a block of 64 keys of the partial sums,
+    32 of the sum of weights.
+Roundings with a bound c that are not spread evenly count as c; even ones as c / sqrt(3), and a step as step / sqrt(12).
+
+A row may be off by 1.4 e_out + 4 e_in, all rows of a case together by 1.1 e_out + 3 e_in: e_out is the most that an even
+spread gives, at the low end of a power of two, and has 64 terms a row or more; e_in has few that matter.
+"""
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv_i8 import BF16, DECODES, F32, PROMPTS, Host, _qkv, _rope, _tables
+
+DRAWS = 4  # of the query's error
+
+
+class Case:
+    """An entry of DECODES or PROMPTS as tensors on the CPU, the cache before the write."""
+
+    def __init__(self, entry, seed=0):
+        self.step = not isinstance(entry[6], list)
+        if self.step:
+            self.b, self.hq, self.h, self.d, self.cap, self.start, self.dtype, self.npre = entry
+            self.t, self.lens = 1, [1] * self.b
+        else:
+            self.b, self.hq, self.h, self.d, self.cap, self.start, self.lens, self.t, self.dtype, self.npre = entry
+        gen = torch.Generator().manual_seed(1000 + seed + self.cap + self.b + self.t)
+        self.x = _qkv(self.b * self.t, self.hq, self.h, self.d, self.dtype, gen)
+        self.q, self.k, self.v = self.x.split([self.hq * self.d, self.h * self.d, self.h * self.d], dim=1)
+        self.cos, self.sin = _tables(self.cap + self.npre, self.d)
+        self.host = Host(self.b, self.h, self.cap, self.d, gen)
+        self.pre = Host(1, self.h, (self.npre + 63) // 64 * 64, self.d, gen) if self.npre else None
+
+    def write(self):
+        self.host.write(self.k, self.v, self.start, self.lens, self.t, self.cos, self.sin, turn=self.npre)
+
+    def heads(self, i, device="cpu"):
+        """Of sequence i: queries [hq, n, d], keys, values [h, keys, d], value scales [h, keys], the block that a key lies
+        in [keys] and the keys that a row does not see [n, keys]; float64."""
+        s, n, p = self.start[i], self.lens[i], self.npre
+        x = self.q[i * self.t:i * self.t + n].reshape(n, self.hq, self.d).double()
+        x = _rope(x, self.cos[p + s:p + s + n].double(), self.sin[p + s:p + s + n].double()).transpose(0, 1)
+        keys, vals = (z[:, :s + n] for z in self.host.held(i))
+        scales, block = self.host.vs[i, :, :s + n].double(), torch.arange(s + n) // 64
+        if p:
+            pk, pv = (z[:, :p] for z in self.pre.held(0))
+            keys, vals = torch.cat([pk, keys], 1), torch.cat([pv, vals], 1)
+            scales = torch.cat([self.pre.vs[0, :, :p].double(), scales], 1)
+            block = torch.cat([torch.arange(p) // 64, block + (p + 63) // 64])
+        later = torch.arange(p + s + n)[None, :] - p > s + torch.arange(n)[:, None]
+        return tuple(z.to(device) for z in (x, keys, vals, scales, block, later))
+
+    def softmax(self, x, keys, later):
+        sc = (x @ keys.T * self.d ** -0.5).masked_fill(later, -math.inf)
+        return sc.masked_fill(later, 0.0), torch.softmax(sc, 1)
+
+
+def expected(case, device="cpu"):
+    """(out [b, t, hq, d], e_out, e_in [b, t, hq]) in float64 on the CPU, after the write."""
+    c, r = case, case.hq // case.h
+    out = torch.zeros((c.b, c.t, c.hq, c.d), dtype=torch.float64, device=device)
+    e_out, e_in = (torch.zeros((c.b, c.t, c.hq), dtype=torch.float64, device=device) for _ in range(2))
+    gen = torch.Generator(device=device).manual_seed(9)
+    fixed, half = c.step, not c.step or c.npre > 0  # the arithmetic that a case may take (behind a prefix, one for each part)
+    grid = 32512.0 if c.dtype == BF16 else 8323072.0
+    bf = c.dtype == BF16
+    for i in range(c.b):
+        n = c.lens[i]
+        if n == 0:
+            continue
+        xs, keys, vals, scales, block, later = c.heads(i, device)
+        nb = int(block[-1]) + 1
+        where = block[None, :].expand(n, -1)
+        for j in range(c.hq):
+            x, kk, vv, vs = xs[j], keys[j // r], vals[j // r], scales[j // r]
+            sc, p = c.softmax(x, kk, later)
+            o = p @ vv
+            codes2, vals2 = (vv / vs[:, None]).square().sum(1), vv.square().sum(1)
+            top = p.amax(1, keepdim=True)
+            apart = (vals2[None, :] - 2 * (o @ vv.T) + o.square().sum(1, keepdim=True)).clamp(min=0.0)  # |v - o|^2
+            # the query, through the softmax
+            var = (2 * 2.0 ** -24 * x).square()
+            if fixed:
+                var = var + (x.abs().amax(1, keepdim=True) / grid).square() / 12
+            if half:
+                var = var + (2.0 ** (-11 if bf else -22) * x).square() / 3
+            err = torch.zeros(n, dtype=torch.float64, device=device)
+            for _ in range(DRAWS):
+                dx = torch.randn(x.shape, generator=gen, dtype=torch.float64, device=device) * var.sqrt()
+                pd = p * (dx @ kk.T * c.d ** -0.5)
+                err += ((pd @ vv) - pd.sum(1, keepdim=True) * o).square().sum(1) / DRAWS
+            # weights and values
+            w2 = (3 * 2.0 ** -24 * p).square() @ vals2
+            if fixed:
+                wmax = torch.zeros((n, nb), dtype=torch.float64, device=device).scatter_reduce(1, where, p * vs, "amax")
+                w2 = w2 + (wmax / grid).square().gather(1, where) @ codes2 / 12
+            if half and bf:
+                w2 = w2 + (2.0 ** -11 * p).square() @ vals2 + (2.0 ** -35 * top[:, 0]).square() * vals2.sum() / 3
+            elif half:
+                w2 = w2 + (2.0 ** -22 * p).square() @ vals2 / 3 \
+                    + (2.0 ** -38 * top[:, 0] * vs.max()).square() * codes2.sum() / 3
+            # fp32: scores, exponentials, sums
+            s = sc.abs() * math.log2(math.e)
+            f2 = ((2.0 ** -22 * (1.0 + s) * p).square() * apart).sum(1)
+            ps = p * s * torch.sign(sc)
+            f2 = f2 + (2.0 ** -23) ** 2 * ((ps @ vv) - ps.sum(1, keepdim=True) * o).square().sum(1)
+            sums = torch.zeros((nb, c.d), dtype=torch.float64, device=device)
+            parts = torch.stack([sums.index_add(0, block, p[y, :, None] * vv).square().sum(1).sum().sqrt() for y in range(n)]) \
+                if n * kk.numel() < 1 << 22 else (p.square() @ vals2).sqrt() * 8.0  # (64 keys a block: at most 8 times)
+            size = parts + o.norm(dim=1)
+            f2 = f2 + 16 * nb * 2.0 ** -48 / 3 * size.square() + 32 * nb * 2.0 ** -48 / 3 * o.square().sum(1)
+            out[i, :n, j] = o
+            e_out[i, :n, j] = (2.0 ** -8 if bf else 2.0 ** -23) / math.sqrt(3.0) * o.norm(dim=1)
+            e_in[i, :n, j] = (err + w2 + f2).sqrt()
+    return out.cpu(), e_out.cpu(), e_in.cpu()
+
+
+def beyond(got, out, e_out, e_in):
+    """(worst row, whole case) as shares of what they may be off by; got [b * t, hq * d]."""
+    off = (got.cpu().double().reshape(out.shape) - out).norm(dim=-1)
+    rows = off / (1.4 * e_out + 4 * e_in).clamp(min=1e-300)
+    whole = off.square().sum().sqrt() / (1.1 * e_out.square().sum().sqrt() + 3 * e_in.square().sum().sqrt())
+    return float(rows.max()), float(whole)
+
+
+LONG = [DECODES[6], PROMPTS[11], DECODES[18], DECODES[4], PROMPTS[15]]
+
+
+@pytest.mark.parametrize("entry", LONG, ids=["decode_4100", "prompt_4000", "prefix_3840", "decode_2100_fp32", "prompt_700_fp32"])
+def test_the_bound_rejects_what_is_wrong_by_little(entry):
+    """On long axes: the rounded definition passes; 2% more, a query of 8 bits, weights of 8 bits and a block of 64 keys
+    left out (of those, one with an average share of the weights) do not."""
+    c = Case(entry)
+    c.write()
+    out, e_out, e_in = expected(c)
+    flat = out.reshape(c.b * c.t, -1)
+    assert max(beyond(flat.to(c.dtype), out, e_out, e_in)) <= 1.0
+    assert max(beyond((1.02 * flat).to(c.dtype), out, e_out, e_in)) > 1.0
+    wrong = {"query": torch.zeros_like(out), "weights": torch.zeros_like(out), "block": torch.zeros_like(out)}
+    r = c.hq // c.h
+    for i in range(c.b):
+        xs, keys, vals, _, block, later = c.heads(i)
+        n = c.lens[i]
+        for j in range(c.hq):
+            step = xs[j].abs().amax(1, keepdim=True) / 127
+            wrong["query"][i, :n, j] = c.softmax((xs[j] / step).round() * step, keys[j // r], later)[1] @ vals[j // r]
+            p0 = c.softmax(xs[j], keys[j // r], later)[1]
+            step = p0.amax(1, keepdim=True) / 127
+            wrong["weights"][i, :n, j] = (p0 / step).round() * step @ vals[j // r]
+            share = torch.zeros(int(block[-1]) + 1, dtype=torch.float64).index_add(0, block, p0.mean(0))
+            gone = later | (block == int((share - 1 / len(share)).abs().argmin()))[None, :] if len(share) > 1 else later
+            wrong["block"][i, :n, j] = c.softmax(xs[j], keys[j // r], gone)[1] @ vals[j // r]
+    for what, x in wrong.items():
+        assert beyond(x.reshape(c.b * c.t, -1).to(c.dtype), out, e_out, e_in)[1] > 1.0, what
