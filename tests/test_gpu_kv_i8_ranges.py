@@ -29,8 +29,8 @@ class Keys:
 
     def __init__(self, form, n, heads, kv_heads, dtype):
         self.form, self.n, self.hq, self.h, self.dtype = form, n, heads, kv_heads, dtype
-        # rows of the call: a step and a prompt's last token take one sequence; the prefix is shared by 40 sequences or more
-        self.b, self.t = {"step": (3, 1), "prompt": (1, 33), "shared": (45, 1)}[form]
+        # rows of the call: a step and a prompt's last token take one sequence; the prefix is shared by many sequences
+        self.b, self.t = {"step": (3, 1), "prompt": (1, 33), "shared": (64, 1)}[form]
         self.cap = (n + self.t + 63) // 64 * 64
         self.held = _empty(1 if form == "shared" else self.b, kv_heads, self.cap)
 

@@ -69,8 +69,8 @@ class Case:
         return sc.masked_fill(later, 0.0), torch.softmax(sc, 1)
 
 
-def expected(case, device="cpu"):
-    """(out [b, t, hq, d], e_out, e_in [b, t, hq]) in float64 on the CPU, after the write."""
+def expected(case, device="cpu", every=1):
+    """(out [b, t, hq, d], e_out, e_in [b, t, hq]) in float64 on the CPU, after the write; of every ``every``-th head."""
     c, r = case, case.hq // case.h
     out = torch.zeros((c.b, c.t, c.hq, c.d), dtype=torch.float64, device=device)
     e_out, e_in = (torch.zeros((c.b, c.t, c.hq), dtype=torch.float64, device=device) for _ in range(2))
@@ -85,7 +85,7 @@ def expected(case, device="cpu"):
         xs, keys, vals, scales, block, later = c.heads(i, device)
         nb = int(block[-1]) + 1
         where = block[None, :].expand(n, -1)
-        for j in range(c.hq):
+        for j in range(0, c.hq, every):
             x, kk, vv, vs = xs[j], keys[j // r], vals[j // r], scales[j // r]
             sc, p = c.softmax(x, kk, later)
             o = p @ vv
@@ -126,12 +126,12 @@ def expected(case, device="cpu"):
             out[i, :n, j] = o
             e_out[i, :n, j] = (2.0 ** -8 if bf else 2.0 ** -23) / math.sqrt(3.0) * o.norm(dim=1)
             e_in[i, :n, j] = (err + w2 + f2).sqrt()
-    return out.cpu(), e_out.cpu(), e_in.cpu()
+    return tuple(z[:, :, ::every].cpu() for z in (out, e_out, e_in))
 
 
-def beyond(got, out, e_out, e_in):
+def beyond(got, out, e_out, e_in, every=1):
     """(worst row, whole case) as shares of what they may be off by; got [b * t, hq * d]."""
-    off = (got.cpu().double().reshape(out.shape) - out).norm(dim=-1)
+    off = (got.cpu().double().reshape(*out.shape[:2], -1, out.shape[3])[:, :, ::every] - out).norm(dim=-1)
     rows = off / (1.4 * e_out + 4 * e_in).clamp(min=1e-300)
     whole = off.square().sum().sqrt() / (1.1 * e_out.square().sum().sqrt() + 3 * e_in.square().sum().sqrt())
     return float(rows.max()), float(whole)

@@ -89,12 +89,15 @@ Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t d,
     if (cb / p.own > 64) p.own = cut(b * hkv, 2 * kLive, cb);
     if (npre > 0) {
       // The rows kernel reads a prefix once for 128 rows, where decode_part reads it for 16, but a block costs it three
-      // times as much (32-bit: more), and converting it is lost on few rows.  8 heads of 128, decode_part against rows:
-      // bf16, 128 rows and 1024 keys 14.5, 19.3; 160 rows 20.1, 19.7; 256 rows 23.5, 20.2; 64 rows and 8192 24.0, 23.3; 256
-      // rows 44.2, 32.7; 32 rows and 8192 20.9, 19.2, and 32768 28.5, 37.7.  fp32, 128 rows and 8192 28.9, 36.2; 256 rows
-      // 45.3, 47.1; 3 heads of 64, 384 rows and 8192 27.4, 25.9.
+      // times as much (32-bit: more), and converting it is lost on few rows.  decode_part against rows, c = columns * pb:
+      // bf16, 8 heads of 128: 128 rows and 1024 keys (c 1024) 14.6, 19.7; 256 rows (2048) 23.9, 21.1; 64 rows and 4096 (2048)
+      // 21.7, 21.2; 128 rows (4096) 22.9, 25.6; 128 rows and 16384 (16384) 40.1, 33.4; 512 rows (65536) 120.6, 69.4.
+      // fp32 of 128: 256 rows and 8192 (16384) 45.2, 48.0; 512 rows and 4096 (16384) 52.5, 50.4; 1024 rows of 2 heads and
+      // 16384 (32768) 65.9, 68.2; 256 rows of 8 (32768) 71.1 both; 512 rows and 8192 (32768) 78.9, 71.5; 16384 (65536) 123.9,
+      // 116.2.  fp32 of 64: 256 rows and 4096 (8192) 24.2, 25.7; 8192 (16384) 30.3, 31.8; 16384 (32768) 44.2, 43.8; 512 rows
+      // and 8192 (32768) 50.8, 42.0; 510 rows of 3 heads and 16384 (24576) 39.9, 38.4.
       const int64_t rows = b * g, columns = hkv * ((rows + kColumns - 1) / kColumns);
-      p.pre_rows = rows > 32 && columns * pb > (dt == WFB_F32 ? 8192 : 1280);
+      p.pre_rows = rows > 32 && columns * pb > (dt == WFB_BF16 ? 1280 : d == 64 ? 16384 : 24576);
       if (p.pre_rows) p.pre = cut(hkv * ((rows + 32 * kPrefixWaves - 1) / (32 * kPrefixWaves)), 256, (pb + 3) / 4);
       else p.pre = cut(columns, kLive, (pb + 3) / 4);
     }
