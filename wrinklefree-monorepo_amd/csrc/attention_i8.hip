@@ -81,11 +81,11 @@ Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t d,
   p.decode = t == 1 && !lengths;
   if (p.decode) {
     // Splits of four blocks (one a wave) or more.  A cache of up to 1024 keys that needs no joining otherwise stays whole:
-    // 3 heads of 64, 32-bit, whole against split at a quarter and at all of 512 keys 5.3, 7.0 against 7.9, 8.5; of 1024
-    // 5.7, 9.3 against 8.5, 8.7; of 2048 8.5, 12.0 (splits of 16 blocks) against 8.6, 9.0.
+    // 3 heads of 64, 32-bit, whole against split at a quarter and at all of 512 keys 6.1, 7.8 against 8.6, 9.5; of 1024
+    // 6.5, 10.1 against 9.3, 9.4; of 2048 7.7, 14.8 against 9.4, 10.0.
     p.own = npre == 0 && cb <= 16 ? 1 : cut(b * hkv, kLive, (cb + 3) / 4);
     // Splits of more than 64 blocks are halved, so that sequences of different lengths even out: 16 of 16384 to 32768 keys,
-    // 8 heads of 128, 159.6 against 163.7; 16 of 32768 197.5 both; 4 of 131071 194 against 191.
+    // 8 heads of 128, 159.7 against 164.2; 16 of 32768 197.6, 198.3; 4 of 131071 195.9 against 192.3.
     if (cb / p.own > 64) p.own = cut(b * hkv, 2 * kLive, cb);
     if (npre > 0) {
       // The rows kernel reads a prefix once for 128 rows, where decode_part reads it for 16, but a block costs it three
@@ -103,12 +103,12 @@ Plan make_plan(int dt, int64_t b, int64_t t, int64_t hq, int64_t hkv, int64_t d,
     }
   } else {
     // Split where the GPU is not full and the keys are many: parts of every row go out and come back, 16 us for 65536 rows
-    // of 128, what a workgroup needs for about 7 blocks.  8 heads of 128, whole against split: 512 tokens 30.8, 34.6, behind
-    // 2048 keys 90.1, 50.0; 1024 tokens 46.8, 50.6, behind 2048 keys 105.5, 83.0.
+    // of 128, what a workgroup needs for about 7 blocks.  8 heads of 128, whole against split: 512 tokens 26.9, 33.9, behind
+    // 2048 keys 78.5, 51.2; 1024 tokens 41.2, 49.9, behind 2048 keys 91.9, 83.5.
     // Four waves, which convert a block for 128 rows instead of 256, where eight would leave rows or CUs empty: 8 heads of
-    // 128, 4 query heads each, eight against four: 512 tokens 29.7, 26.3; 1024 45.7, 40.1; 2048 79.8, 73.5; 3000 114.0,
-    // 111.8; 4096 171.9, 194.8; 16 tokens behind 4000 keys 27.2, 24.6; 48 of 8 sequences behind 4000 45.4, 54.8.  (fp32 rows
-    // of 128 do not fit into the registers of four: 2 x 1587 tokens, 10 / 5 heads, 90.7, 101.7.)
+    // 128, 4 query heads each, eight against four: 512 tokens 30.5, 27.0; 1024 46.1, 41.3; 2048 81.9, 74.5; 3000 114.5,
+    // 112.3; 4096 182.8, 199.8; 16 tokens behind 4000 keys 27.6, 25.1; 8 x 48 behind 4000 shared keys, 5 heads, 46.7, 49.9.
+    // (fp32 rows of 128 do not fit into the registers of four: 2 x 1587 tokens, 10 / 5 heads, 90.7, 101.7.)
     const int64_t rows = t * g, groups = b * hkv * ((rows + 32 * kRowsWaves - 1) / (32 * kRowsWaves));
     const int64_t blocks = pb + (keys + kKvBlock - 1) / kKvBlock;
     const int64_t n = cut(groups, 256, (blocks + 3) / 4);
@@ -545,8 +545,8 @@ __device__ __forceinline__ void f16_parts(float x0, float x1, uint32_t (&part)[N
 //   O^T[d, row] += V^T W^T        w = p v_scale / (reference of the scales) in fp16 (fp32 rows: two parts)
 // As in the decode kernel the key of a score tile's row is chosen so that a lane holds the keys that it feeds into the
 // second product, 8 consecutive ones per step.
-// What bounds it: nothing alone.  4096 tokens, 32 / 8 heads of 128, bf16: 137 GFLOP in 172 to 182 us (0.8 PFLOP/s); the
-// matrix cores are busy 34% of the cycles, vector instructions 43%, LDS about half, since a product of 32 x 32 x 16 reads 16
+// What bounds it: nothing alone.  4096 tokens, 32 / 8 heads of 128, bf16: 137 GFLOP in 188 to 190 us (0.73 PFLOP/s); the
+// matrix cores are busy 34% of the cycles, vector instructions 44%, LDS about half, since a product of 32 x 32 x 16 reads 16
 // bytes a lane of it; two waves a SIMD (by their registers) leave the rest to latency.  A block costs 256 rows 2.0 to 2.8 us.
 // Tried without gain: the two waves of a SIMD half a block apart (197 against 187 us), 64 rows a wave and one wave a SIMD
 // (331: 100 spilled registers), the exponentials a block ahead of their products (5% slower).

@@ -42,7 +42,9 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& scale) {
 // One workgroup per (64-key block of the cache, kv head, sequence, keys or values): the new tokens that fall into the block.
 // A row is read by D / 8 lanes, 8 elements each (the rotary partner D / 2 away sits in the lane half a group away); the
 // value codes pass through LDS, row by row in and 4 x 4 bytes transposed out, 8 keys of 4 elements per thread.
-// What bounds it: HBM.  8 x 2048 tokens of 8 heads of 128, bf16: 67 MB in and 35 MB out in 29 us (3.5 TB/s).  With
+// What bounds it, at 8 x 2048 tokens of 8 heads of 128: bf16, 67 MB in and 35 MB out in 29 us (3.5 TB/s; a copy of as many
+// bytes takes 21), 27 without rotary tables; fp32, 134 MB in, 40 us (4.2 TB/s; a copy 33).  The 7 to 8 us over a copy are a
+// workgroup's one chain of loads, maximum, codes and stores, in which only the CU's other workgroups keep memory busy.  With
 // one workgroup for the keys and the values of a block, here and in the read back, the two calls took 58 us together, now 51.
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const void* __restrict__ kn, int64_t ldk,
@@ -150,7 +152,8 @@ __device__ __forceinline__ void store4(void* p, int64_t i, const float (&v)[4]) 
 // k / v [batch, kv_heads, count, D].  One workgroup per (64-key block, kv head, sequence, keys or values), the blocks counted
 // from the one that holds the first position; positions outside the cache read as zeros.  A value block passes through
 // LDS as it is stored and is read 4 keys x 4 elements at a time.
-// What bounds it: HBM.  8 x 2048 tokens of 8 heads of 128: 35 MB in and 67 MB out in 17 us (6.0 TB/s).
+// What bounds it: memory.  8 x 2048 tokens of 8 heads of 128 that were just written: 35 MB in and 67 MB out as bf16 in 17 us
+// (6.0 TB/s, above a copy's 4.9: part of the codes still lies in the last cache), 134 MB out as fp32 in 32 us (5.3 TB/s).
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(wfb_kv_i8 c, const int64_t* __restrict__ start_dev, int64_t start,
                                                            int64_t count, int hkv, void* __restrict__ k,

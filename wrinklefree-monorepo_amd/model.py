@@ -554,8 +554,9 @@ class BitNetDecoder:
     @torch.no_grad()
     def share_prefix(self, ids: Optional[torch.Tensor]) -> None:
         """Token ids [P] that precede every sequence from the next ``reset`` (or ``generate``) on: their keys and values
-        are computed once, here, and read once per step for the whole batch; the positions given to ``forward`` and
-        ``decode_step`` keep counting a sequence's own tokens.  ``None`` ends it.  Needs ``kv_cache="int8"``."""
+        are computed and held once, here, and a ``decode_step`` reads them for all sequences together (``forward`` for
+        each of them); the positions given to ``forward`` and ``decode_step`` keep counting a sequence's own tokens.
+        ``None`` ends it.  Needs ``kv_cache="int8"``."""
         if self.kv_cache != "int8":
             raise ValueError("share_prefix needs kv_cache='int8'")
         if ids is not None and ids.dim() > 0 and ids.shape[-1] != ids.numel():

@@ -1182,7 +1182,8 @@ def gqa_decode_attention_i8(
 
     q, k_new, v_new float32 or bfloat16, rows as for ``gqa_decode_attention``; up to 16 query heads per kv head; rope
     tables fp32 [positions, head_dim/2], as long as the positions need.  ``prefix``: an int8 cache of one sequence whose
-    first ``prefix_len`` keys precede every sequence's own (a shared prompt, read once for the whole batch); ``pos`` stays
+    first ``prefix_len`` keys precede every sequence's own (a shared prompt, read for 16 or 128 rows at a time of all the
+    sequences', not once for each of them); ``prefix_len`` has to be given with it, 0 for none of its keys; ``pos`` stays
     the position in the sequence's own cache, the rotary embedding takes row prefix_len + pos.  The prefix may not be part
     of ``cache``.  A position outside the cache or the tables gives a NaN row and leaves the cache as it is."""
     name = "gqa_decode_attention_i8"
@@ -1204,7 +1205,9 @@ def gqa_prefill_attention_i8(
     ``start``: an int, or int64 [batch] on the device; ``lengths``: int64 [batch] on the device for a batch padded to t
     tokens: sequence b has lengths[b] of them, the rows behind are zeros and nothing is written for them.  A sequence
     that does not fit the cache or the rope tables gives NaN rows and is not written (a ``start`` given as an int is
-    checked here instead).  ``prefix`` / ``prefix_len`` and the types as for ``gqa_decode_attention_i8``."""
+    checked here instead).  ``prefix`` / ``prefix_len`` and the types as for ``gqa_decode_attention_i8``, but every sequence
+    of a prompt reads the prefix for itself: it is held once, not read once.  Over a long cache a chunk of two tokens costs
+    what one of eight does; one token without ``lengths`` takes the decode step's form."""
     return _attention_i8("gqa_prefill_attention_i8", q, k_new, v_new, cache, start, int(t), rope_cos, rope_sin, scale,
                          out, lengths, prefix, prefix_len)
 
