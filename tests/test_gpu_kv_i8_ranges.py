@@ -175,3 +175,21 @@ def test_a_first_key_of_any_score_returns_its_value(pkg, dev, dtype, tokens, npr
         ref = host.held(0)[1][0, 0].repeat(2)[None]
         tol = (2.0 ** -8 + 2 * 2.0 ** -11 if dtype == BF16 else 2.0 ** -20) * ref.abs()
         _check(out[:1], ref, tol, f"score of {size}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", Keys.FORMS)
+def test_values_whose_sum_over_the_keys_is_just_within_fp32(pkg, dev, form, dtype):
+    """8800 values of up to 2^113 on a split axis: their sum under weights of one stays below 2^127, and so do the parts
+    of a row that are joined."""
+    print(f"[kv ranges] large values {form} {dtype}", flush=True)
+    m = Keys(form, 8800, 32, 4, dtype)
+    gen = torch.Generator().manual_seed(6)
+    m.held.v[:, :, :m.n] = torch.randint(64, 128, (1, 4, m.n, D), generator=gen, dtype=torch.int8)
+    m.held.vs[:, :, :m.n] = 2.0 ** 106
+    m.held.k[:, :, :m.n] = torch.randint(-127, 128, (1, 4, m.n, D), generator=gen, dtype=torch.int8)
+    m.held.ks[:, :, :m.n] = 0.01
+    q = torch.randn((m.b * m.t, 32 * D), generator=gen).to(dtype)
+    out, ref, tol = m.run(pkg, dev, q, D ** -0.5, half=True)
+    assert float((tol / ref).max()) < 0.1
+    _check(out, ref, tol, form)

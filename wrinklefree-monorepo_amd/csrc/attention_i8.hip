@@ -1001,12 +1001,17 @@ __device__ __forceinline__ void rows_part(const KvAttn& a, const Parts& parts, i
   // A lane holds O^T[32 d + 8 (i / 4) + 4 grp + i % 4] of its row.  Half a row at a time goes through LDS, so that it leaves
   // in one piece and not 16 bytes (of bf16 8) at a time.
   constexpr int NC = D / 8, RP = 64 / NC;  // pieces of four elements in half a row, rows that the wave stores at once
-  const float f = parts.o ? vref * (1.0f / kUp) : vref * (1.0f / kUp) / l_run;
+  // A part leaves as if its weights were at most one, so that a sum over values near the end of fp32 does not pass it (but
+  // for far scores, where the shift need not be exact).
+  constexpr float kOne = kSlack == 15.0f ? 0x1p-15f : 0x1p-1f;
+  static_assert(kSlack == 15.0f || kSlack == 1.0f);
+  const float down = far ? 1.0f : kOne;
+  const float f = parts.o ? vref * (1.0f / kUp) * down : vref * (1.0f / kUp) / l_run;
   int64_t at = r < R ? qrow * a.ldo + (int64_t)h * D : -1;
   if (parts.o) {
     const int64_t row = (int64_t)(slot0 + split) * parts.rows + qrow * a.hq + h;
     at = valid ? row * D : -1;
-    if (valid && grp == 0) parts.ml[row] = make_float2(m_ref, l_run);
+    if (valid && grp == 0) parts.ml[row] = make_float2(far ? m_ref : m_ref + kSlack, l_run * down);
   }
   int64_t ats[32 / RP];  // of the rows that the lane stores a piece of
 #pragma unroll
