@@ -6,8 +6,8 @@ errors, and CPU checks that a bound made of them rejects what is wrong by little
   * ``e_out``, the output's rounding: u |o| / sqrt(3) with u = 2^-8 (bf16), 2^-23 (fp32: the division and the rounding), an
     error spread evenly over half a step that is at most u of the value;
   * ``e_in``, what is lost before it.  Of the fixed-point form (one token a sequence): the query's elements by a step of their
-    row's largest / 32512 (fp32: 8323072) spread evenly, through the softmax; a weight by a step of its block's largest
-    p v_scale / 32512, times its codes.  Of the fp16 form (prompts, long shared prefixes): 2^-11 of q, and of p v three
+    row's largest / (127 * 256) (fp32: 127 * 2^16) spread evenly, through the softmax; a weight by a step of its block's largest
+    p v_scale by the same, times its codes.  Of the fp16 form (prompts, long shared prefixes): 2^-11 of q, and of p v three
     times (weight, scale, scaled value), with weights below 2^-24 of the largest off by 2^-35 of it; fp32 rows 2^-22 of q and of
     p v, and 2^-38 of the largest probability times the largest scale.  Of both: 2^-22 (1 + |s|) of a weight, s the score
     in powers of two, of which 2^-23 |s| alike for the row; 16 roundings of 2^-24 a block of 64 keys of the partial sums,
@@ -76,7 +76,7 @@ def expected(case, device="cpu", every=1):
     e_out, e_in = (torch.zeros((c.b, c.t, c.hq), dtype=torch.float64, device=device) for _ in range(2))
     gen = torch.Generator(device=device).manual_seed(9)
     fixed, half = c.step, not c.step or c.npre > 0  # the arithmetic that a case may take (behind a prefix, one for each part)
-    grid = 32512.0 if c.dtype == BF16 else 8323072.0
+    grid = 127.0 * (256 if c.dtype == BF16 else 65536)
     bf = c.dtype == BF16
     for i in range(c.b):
         n = c.lens[i]
