@@ -19,9 +19,9 @@ AdamW (kind "adamw"), step t, every operation rounded to fp32:
     p = p (1 - lr wd) - (m (lr / (1 - b1^t))) / (r (1 / sqrt(1 - b2^t)) + eps)
 The states of all tensors lie in one flat array each, every tensor from a multiple of 256 on.  In 8 bits, a block of 256
 holds a = max|m|, s = max r (0 where below 2^-100) and
-    m code c = sign(m) min(127, floor(127 sqrt(|m| / a) + z)),
-    r code u = min(255, floor(255 sqrt(r / s) + z)), 1 at least where r > 0
-standing for m = c |c| (a / 127^2), r = u u (s / 255^2), v = r r (each quotient a product with the rounded inverse);
+    m code c = sign(m) min(127, floor(sqrt(|m| (127^2 / a)) + z)),
+    r code u = min(255, floor(sqrt(r (255^2 / s)) + z)), 1 at least where r > 0
+standing for m = c |c| (a (1 / 127^2)), r = u u (s (1 / 255^2)), v = r r;
 z = ((i 0x9E3779B1 + t 0x6A09E667) mod 2^32 >> 8) 2^-24 for element i of the flat array.
 
 ``own`` chooses the package's operators; else ``run`` computes the same with elementary torch operations.
@@ -348,8 +348,8 @@ def _codes(x, top, z):
     x = x.view(-1, _BLOCK)
     scale = x.amax(1)
     scale = torch.where(scale < 2.0 ** -100, 0.0, scale)
-    q = torch.sqrt(x / torch.where(scale == 0.0, 1.0, scale)[:, None]) * float(top)
-    q = torch.floor(q + z.view(-1, _BLOCK)).clamp_(max=float(top))
+    k = torch.full_like(scale, float(top * top)) / torch.where(scale == 0.0, 1.0, scale)
+    q = torch.floor(torch.sqrt(x * k[:, None]) + z.view(-1, _BLOCK)).clamp_(max=float(top))
     return torch.where(scale[:, None] == 0.0, 0.0, q).view(-1), scale
 
 
@@ -491,7 +491,7 @@ def _exact_adamw(c, s):
             big = x.view(-1, _BLOCK).max(dim=1).values
             big[big < 2.0 ** -100] = 0.0
             wide = big.repeat_interleave(_BLOCK)
-            q = step(step(torch.sqrt(step(x / wide.masked_fill(wide == 0, 1.0)))) * top)
+            q = step(torch.sqrt(step(x * step(top * top / wide.masked_fill(wide == 0, 1.0)))))
             q = step(q + z).floor().clamp(max=top)
             if least:
                 q = torch.where(x > 0, q.clamp(min=1.0), q)
