@@ -465,6 +465,102 @@ int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t 
                          int64_t num_kv_heads, int64_t head_dim, float scale, void* out, int64_t ldo, float* workspace,
                          void* stream);
 
+/* ---- training step: gated feed-forward product ------------------------------------------------- */
+
+/* h [M, F] (h_dtype, rows contiguous) = act(gate) * up, gate|up = acc * w_scale * a_scale of the F gate rows and the F up
+ * rows of qweight [2F, K/4] (scales_dev: their two fp32 scales), act WFB_ACT_SILU or WFB_ACT_RELU2, every product
+ * rounded to fp32 as in wfb_linear_i2s and the gated activation as in wfb_linear_i2s_glu, then once to h_dtype.
+ * gate_up fp32 [M, 2F] receives both products, which wfb_gated_grad takes; it may be NULL where
+ * wfb_gated_i2s_workspace(M, F, K) is 0 (it holds that many floats otherwise).  act_codes int8 [M, lda], K % 128 == 0, rows
+ * and bases 16-byte aligned.  The float product: WF/models/ffn.py:10-45. */
+int wfb_gated_i2s_workspace(int64_t m, int64_t f, int64_t k, int64_t* floats);
+int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* act_codes, int64_t m, int64_t lda,
+                  const float* a_scale, const float* scales_dev, int act, void* h, int h_dtype, float* gate_up,
+                  void* stream);
+
+/* The straight-through gradients of wfb_gated_i2s: with d = [grad_h * up * act'(gate) | grad_h * act(gate)] [M, 2F],
+ *   grad_x [M, K] = (d * w_scale) t,   grad_w [2F, K] = d^T (codes * a_scale)       (gate's rows before up's)
+ * t the ternary weights, in fp32 arithmetic, each result rounded once to its type.  gate_up as wfb_gated_i2s left it;
+ * grad_h [M, ldg]; qweight [2F, k_pad/4] 8-byte aligned; codes [M, lda].  grad_x or grad_w may be NULL.
+ * Products run on the matrix cores: an fp32 operand enters in parts that hold 24 bits of it (grad_x of type fp32, grad_w
+ * of type fp32), see csrc/gated.hip for the 16-bit results.  work: wfb_gated_grad_workspace bytes (host only; the
+ * same sizes, types and wanted results), 256-byte aligned. */
+int wfb_gated_grad_workspace(int64_t m, int64_t f, int64_t k, int gx_dtype, int want_x, int gw_dtype, int want_w,
+                             int64_t* bytes);
+int wfb_gated_grad(const float* gate_up, const void* grad_h, int gh_dtype, int64_t ldg, int64_t m, int64_t f, int act,
+                   const uint8_t* qweight, int64_t k, int64_t k_pad, const float* scales_dev, const int8_t* codes,
+                   int64_t lda, const float* a_scale, void* grad_x, int gx_dtype, void* grad_w, int gw_dtype, void* work,
+                   void* stream);
+
+/* ---- training step: norm of query and key heads with the rotary embedding ---------------------- */
+
+/* One side of the call: heads of x [batch, T, heads, head_dim] (strides in elements, the last dimension contiguous), the
+ * norm's weight [head_dim] or NULL for no norm, and where the result goes (contiguous).  g: the gradient at the output
+ * (wfb_qk_norm_rope_grad only, out then takes the gradient of x or is NULL; grad_weight [head_dim] of weight_dtype or
+ * NULL). */
+typedef struct wfb_heads {
+  const void* x;
+  int64_t stride_b, stride_t, stride_h;
+  const void* g;
+  int64_t g_stride_b, g_stride_t, g_stride_h;
+  const void* weight;
+  int64_t weight_dtype;
+  void* out;
+  void* grad_weight;
+  int64_t heads;
+} wfb_heads;
+
+/* Where the tokens stand: rope_cos / rope_sin fp32 [rope_len, rotary_dim / 2] (rows contiguous); position of token (b, t)
+ * start + t, or pos[b * pos_stride_b + t * pos_stride_t], int32 or int64 (pos_bytes 4 or 8) on the device.  interleaved:
+ * pairs (2i, 2i + 1) of the first rotary_dim elements are turned, else pairs (i, i + rotary_dim / 2).  A position outside the
+ * tables gives NaN rows and reads nothing. */
+typedef struct wfb_rope {
+  const float* cos;
+  const float* sin;
+  int64_t rope_len, rotary_dim, interleaved;
+  const void* pos;
+  int64_t pos_bytes, pos_stride_b, pos_stride_t, start;
+} wfb_rope;
+
+/* out = rotate(x * rsqrt(mean(x^2) + eps) * weight) of every query and key head, fp32 arithmetic, rounded once to dtype
+ * (that of x, g and out).  head_dim even, 2..WFB_QK_MAX_DIM; rotary_dim even, 0..head_dim.  The rotation: WF/models/
+ * attention.py:14-64 (interleaved), the stage-1 model's (halves). */
+#define WFB_QK_MAX_DIM 256
+int wfb_qk_norm_rope(const wfb_heads* q, const wfb_heads* k, const wfb_rope* rope, int dtype, int64_t batch, int64_t t,
+                     int64_t head_dim, float eps, void* stream);
+/* Its gradients; work: wfb_qk_norm_rope_grad_workspace floats (host only), needed where a grad_weight is. */
+int wfb_qk_norm_rope_grad_workspace(int64_t batch, int64_t t, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                    int64_t* floats);
+int wfb_qk_norm_rope_grad(const wfb_heads* q, const wfb_heads* k, const wfb_rope* rope, int dtype, int64_t batch, int64_t t,
+                          int64_t head_dim, float eps, float* work, void* stream);
+
+/* ---- training step: AdamW --------------------------------------------------------------------- */
+
+/* One AdamW step (decoupled weight decay) over n_tensors tensors of p_dtype with gradients of g_dtype, every operation one
+ * fp32 operation in this order, parameters rounded once to p_dtype:
+ *   m = m b1 + g (1 - b1),  v = v b2 + (g g)(1 - b2),  r = sqrt(v)
+ *   p = p (1 - lr wd) - (m (lr / (1 - b1^step))) / (r (1 / sqrt(1 - b2^step)) + eps)
+ * The states lie in flat arrays of state_elements (a multiple of WFB_ADAMW_BLOCK); tensor i takes elements first ..
+ * first + n - 1 of them, first a multiple of WFB_ADAMW_BLOCK, no two tensors the same block.  bits 32: m, v fp32.
+ * bits 8: m int8, v uint8 codes with m_scale, v_scale fp32 [state_elements / WFB_ADAMW_BLOCK], see csrc/adamw.hip.
+ * step >= 1 on the host, or step_dev int64 [1] on the device (a captured graph's replays count it up there), for which
+ * scalars holds WFB_ADAMW_SCALARS floats of device memory; lr_dev fp32 [1] or NULL goes with step_dev only.
+ * Pointers of p and g are multiples of their element's size; states 16-byte aligned. */
+#define WFB_ADAMW_BLOCK 256
+#define WFB_ADAMW_SCALARS 16
+typedef struct wfb_adamw_tensor {
+  void* p;
+  const void* g;
+  int64_t n, first;
+} wfb_adamw_tensor;
+int wfb_adamw_step(const wfb_adamw_tensor* tensors, int64_t n_tensors, int p_dtype, int g_dtype, void* m, void* v,
+                   float* m_scale, float* v_scale, int64_t state_elements, int bits, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, int64_t step, const int64_t* step_dev,
+                   const float* lr_dev, float* scalars, void* stream);
+/* The values m, v fp32 [state_elements] that a state in 8 bits stands for. */
+int wfb_adamw_values(const void* m, const void* v, const float* m_scale, const float* v_scale, int64_t state_elements,
+                     float* m_out, float* v_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,6 +45,9 @@ from .ops import (
 from . import engine, model, sglbitnt
 from .engine import NativeEngine
 from .sglbitnt import SGLBitNetFile, write_sglbitnt
+from .gated import GatedBitLinear, PackedGated, gated_bitlinear, pack_gated
+from .optim import AdamW, AdamWState, adamw_state, adamw_state_values, adamw_step
+from .rotary import qk_norm_rope
 from .bitlinear import (
     BitLinear,
     BitNetLinearMethod,
@@ -63,6 +66,8 @@ __all__ = [
     "pack_ternary_i2s",
     "quantize_activations_i8", "quantize_activations_i8_per_token", "rmsnorm_linear", "rmsnorm_linear_glu", "rmsnorm_linear_glu_supported", "rmsnorm_linear_preferred", "rmsnorm_linear_supported",
     "rmsnorm_quantize_i8", "rope_tables", "unpack_i2s",
+    "AdamW", "AdamWState", "adamw_state", "adamw_state_values", "adamw_step", "GatedBitLinear", "PackedGated",
+    "gated_bitlinear", "pack_gated", "qk_norm_rope",
     "BitLinear", "BitNetLinearMethod", "BitNetLinearNative", "SubLNBitLinear", "convert_linear_to_bitlinear",
     "patch_model_with_native_kernels", "set_lambda_source", "engine", "NativeEngine", "model", "sglbitnt", "SGLBitNetFile", "write_sglbitnt",
 ]

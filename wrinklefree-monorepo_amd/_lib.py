@@ -25,6 +25,9 @@ WFB_MAX_SEGMENTS = 8
 WFB_SCALE_REFERENCE = 0
 WFB_SCALE_CHECKPOINT = 1
 WFB_KV_I8_BLOCK = 64
+WFB_QK_MAX_DIM = 256
+WFB_ADAMW_BLOCK = 256
+WFB_ADAMW_SCALARS = 16
 WFB_ACT_SILU = 1
 WFB_ACT_RELU2 = 2
 
@@ -32,6 +35,7 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 
 
@@ -39,6 +43,21 @@ class KvI8Struct(ctypes.Structure):
     """wfb_kv_i8: the four tensors of an int8 key/value cache and its keys per sequence."""
 
     _fields_ = [("k", _vp), ("k_scale", _vp), ("v", _vp), ("v_scale", _vp), ("cap", _i64)]
+
+
+class HeadsStruct(ctypes.Structure):
+    """wfb_heads: the query or the key side of wfb_qk_norm_rope."""
+
+    _fields_ = [("x", _vp), ("stride_b", _i64), ("stride_t", _i64), ("stride_h", _i64), ("g", _vp), ("g_stride_b", _i64),
+                ("g_stride_t", _i64), ("g_stride_h", _i64), ("weight", _vp), ("weight_dtype", _i64), ("out", _vp),
+                ("grad_weight", _vp), ("heads", _i64)]
+
+
+class RopeStruct(ctypes.Structure):
+    """wfb_rope: rotary tables, layout and positions of wfb_qk_norm_rope."""
+
+    _fields_ = [("cos", _vp), ("sin", _vp), ("rope_len", _i64), ("rotary_dim", _i64), ("interleaved", _i64), ("pos", _vp),
+                ("pos_bytes", _i64), ("pos_stride_b", _i64), ("pos_stride_t", _i64), ("start", _i64)]
 
 
 # name -> argtypes (restype is int for all but the two queries)
@@ -82,6 +101,17 @@ SIGNATURES = {
     "wfb_rmsnorm_linear_i2s": [_vp, _int, _i64, _vp, _int, _f32, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _vp,
                                _int, _i64, _vp, _int, _i64, _vp],
     "wfb_rope_tables": [ctypes.c_double, _i64, _i64, _vp, _vp],
+    "wfb_gated_i2s_workspace": [_i64, _i64, _i64, _vp],
+    "wfb_gated_i2s": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _int, _vp, _int, _vp, _vp],
+    "wfb_gated_grad_workspace": [_i64, _i64, _i64, _int, _int, _int, _int, _vp],
+    "wfb_gated_grad": [_vp, _vp, _int, _i64, _i64, _i64, _int, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _int,
+                       _vp, _vp],
+    "wfb_qk_norm_rope": [_vp, _vp, _vp, _int, _i64, _i64, _i64, _f32, _vp],
+    "wfb_qk_norm_rope_grad_workspace": [_i64, _i64, _i64, _i64, _i64, _vp],
+    "wfb_qk_norm_rope_grad": [_vp, _vp, _vp, _int, _i64, _i64, _i64, _f32, _vp, _vp],
+    "wfb_adamw_step": [_vp, _i64, _int, _int, _vp, _vp, _vp, _vp, _i64, _int, _f64, _f64, _f64, _f64, _f64, _i64, _vp,
+                       _vp, _vp, _vp],
+    "wfb_adamw_values": [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
     "wfb_rmsnorm_linear_i2s_glu": [_vp, _int, _i64, _vp, _int, _f32, _i64, _i64, _vp, _i64, _i64, _vp, _int, _int, _vp,
                                    _i64, _vp],
 }

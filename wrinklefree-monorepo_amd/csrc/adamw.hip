@@ -1,0 +1,288 @@
+// AdamW over many tensors in one launch, its states in fp32 or in 8 bits.
+//
+// Step t, every operation one correctly rounded fp32 operation, in this order:
+//   m = m b1 + g (1 - b1),  v = v b2 + (g g)(1 - b2),  r = sqrt(v)
+//   p = p (1 - lr wd) - (m (lr / (1 - b1^t))) / (r (1 / sqrt(1 - b2^t)) + eps)
+// In 8 bits a block of 256 elements holds a = max|m|, s = max r and codes on quadratic grids, which keep 1 / 127^2 and
+// 1 / 255^2 of the largest apart from zero:
+//   c = sign(m) min(127, floor(sqrt(|m| (127^2 / a)) + z)) for m = c |c| (a (1 / 127^2))
+//   u = min(255, floor(sqrt(r (255^2 / s)) + z)), 1 at least where r > 0, for r = u u (s (1 / 255^2))
+// The second moment is held as r: what the step divides by, with half of v's range to cover, and no r > 0 is held as 0,
+// so an element's step never grows because its r went below the grid.  z in [0, 1) runs through a Weyl sequence over
+// steps and elements: a moment that moves by less than a code's distance in a step still moves on average, which with
+// rounding to the nearest it would not (b2 = 0.999 moves r by 0.05% a step, neighbouring codes lie 0.8% apart at best).
+// Blocks whose largest is below 2^-100 are held as zeros; one with an infinity or a NaN has scale NaN.
+#include <cmath>
+
+#include "train_ops.h"
+
+namespace wfb {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = WFB_ADAMW_BLOCK;          // elements of a block: a wave's 64 x 4
+constexpr int kTileBlocks = 16;                  // blocks of one workgroup
+constexpr int kMaxTensors = 64;                  // of one launch: the table travels with the kernel's arguments
+
+struct Table {
+  int n;
+  uint32_t tile[kMaxTensors + 1];  // first workgroup of each tensor
+  void* p[kMaxTensors];
+  const void* g[kMaxTensors];
+  int64_t len[kMaxTensors];
+  int64_t first[kMaxTensors];  // of its elements in the state
+};
+static_assert(sizeof(Table) + sizeof(AdamWState) + sizeof(AdamWScalars) + 16 <= 4096, "kernel arguments");
+
+// Four elements from any address that is a multiple of the element's size: gfx950 takes unaligned vectors.
+struct __attribute__((packed, aligned(4))) F4 { float v[4]; };
+struct __attribute__((packed, aligned(2))) H4 { uint16_t v[4]; };
+
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, int64_t i, int n, float (&v)[4]) {
+  if (n >= 4) {
+    if constexpr (DT == WFB_F32) {
+      const F4 x = *reinterpret_cast<const F4*>(reinterpret_cast<const float*>(p) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = x.v[e];
+    } else {
+      const H4 x = *reinterpret_cast<const H4*>(reinterpret_cast<const uint16_t*>(p) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = DT == WFB_BF16 ? bf16_bits_to_f32(x.v[e]) : f16_bits_to_f32(x.v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? load_elem<DT>(p, i + e) : 0.0f;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store4(void* p, int64_t i, int n, const float (&v)[4]) {
+  if constexpr (DT == WFB_F32) {
+    float* q = reinterpret_cast<float*>(p) + i;
+    if (n >= 4) {
+      F4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.v[e] = v[e];
+      *reinterpret_cast<F4*>(q) = x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) q[e] = v[e];
+    }
+  } else {
+    uint16_t* q = reinterpret_cast<uint16_t*>(p) + i;
+    H4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.v[e] = DT == WFB_BF16 ? f32_to_bf16_rne(v[e]) : __builtin_bit_cast(uint16_t, (_Float16)v[e]);
+    if (n >= 4) {
+      *reinterpret_cast<H4*>(q) = x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) q[e] = x.v[e];
+    }
+  }
+}
+
+// The largest of the wave's non-negative values; a NaN is the largest of all (its bits are).
+__device__ __forceinline__ float wave_top(float v) {
+  uint32_t u = __float_as_uint(v);
+  auto up = [&](int o) { u = max(u, (uint32_t)o); };
+  up(xor_lanes<1>((int)u));
+  up(xor_lanes<2>((int)u));
+  up(xor_lanes<4>((int)u));
+  up(xor_lanes<8>((int)u));
+  up(xor_lanes<16>((int)u));
+  up(xor_lanes<32>((int)u));
+  return __uint_as_float(u);
+}
+
+// Scale of a block whose largest is v.
+__device__ __forceinline__ float scale_of(float v) {
+  if (!(v <= 3.402823466e38f)) return __builtin_nanf("");
+  return v < 7.888609052210118e-31f ? 0.0f : v;  // 2^-100
+}
+
+// Code of x >= 0 on the grid of `top` steps with k = top^2 / scale; k = 0: no scale, no code.
+__device__ __forceinline__ int code_of(float x, float k, float top, float z) {
+  return k > 0.0f ? (int)fminf(floorf(__fadd_rn(sqrtf(__fmul_rn(x, k)), z)), top) : 0;
+}
+
+template <int PDT, int GDT, int BITS>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(Table tb, AdamWState st, AdamWScalars host,
+                                                         const AdamWScalars* __restrict__ dev) {
+  int k = 0;  // the tensor of this workgroup
+  for (int step = kMaxTensors / 2; step; step /= 2)
+    if (k + step < tb.n && tb.tile[k + step] <= blockIdx.x) k += step;
+  const AdamWScalars c = dev ? *dev : host;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  void* const p = tb.p[k];
+  const void* const g = tb.g[k];
+  const int64_t len = tb.len[k], first = tb.first[k];
+  const int64_t e0 = (int64_t)(blockIdx.x - tb.tile[k]) * (kTileBlocks * kBlock);
+  for (int b = w; b < kTileBlocks; b += kThreads / 64) {
+    const int64_t base = e0 + b * kBlock;
+    if (base >= len) break;
+    const int64_t i = base + 4 * lane, s = first + i;
+    const int n = (int)min((int64_t)4, max((int64_t)0, len - i));
+    float pv[4], gv[4], m[4], r[4];
+    load4<PDT>(p, i, n, pv);
+    load4<GDT>(g, i, n, gv);
+    float v[4];
+    if constexpr (BITS == 32) {
+      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(st.m) + s);
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(st.v) + s);
+      m[0] = x.x, m[1] = x.y, m[2] = x.z, m[3] = x.w;
+      v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+    } else {
+      const uint32_t mc = reinterpret_cast<const uint32_t*>(st.m)[s / 4], vc = reinterpret_cast<const uint32_t*>(st.v)[s / 4];
+      const float ma = __fmul_rn(st.m_scale[s / kBlock], 1.0f / 16129.0f);
+      const float va = __fmul_rn(st.v_scale[s / kBlock], 1.0f / 65025.0f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float q = (float)(int8_t)(mc >> (8 * e)), u = (float)((vc >> (8 * e)) & 255u);
+        m[e] = __fmul_rn(q * fabsf(q), ma);
+        const float x = __fmul_rn(u * u, va);
+        v[e] = __fmul_rn(x, x);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      m[e] = __fadd_rn(__fmul_rn(m[e], c.b1), __fmul_rn(gv[e], c.omb1));
+      v[e] = __fadd_rn(__fmul_rn(v[e], c.b2), __fmul_rn(__fmul_rn(gv[e], gv[e]), c.omb2));
+      if (e >= n) m[e] = v[e] = 0.0f;  // behind the tensor's end
+      r[e] = sqrtf(v[e]);
+      pv[e] = __fsub_rn(__fmul_rn(pv[e], c.decay),
+                        __fdiv_rn(__fmul_rn(m[e], c.rate), __fadd_rn(__fmul_rn(r[e], c.ib2), c.eps)));
+    }
+    store4<PDT>(p, i, n, pv);
+    if constexpr (BITS == 32) {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(st.m) + s) = make_float4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(st.v) + s) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      auto top4 = [](float a, float b, float c, float d) {  // (bits: a NaN is the largest)
+        return __uint_as_float(max(max(__float_as_uint(fabsf(a)), __float_as_uint(fabsf(b))),
+                                   max(__float_as_uint(fabsf(c)), __float_as_uint(fabsf(d)))));
+      };
+      const float a = scale_of(wave_top(top4(m[0], m[1], m[2], m[3]))), t = scale_of(wave_top(top4(r[0], r[1], r[2], r[3])));
+      const float ka = a > 0.0f ? __fdiv_rn(16129.0f, a) : 0.0f, kt = t > 0.0f ? __fdiv_rn(65025.0f, t) : 0.0f;
+      uint32_t mc = 0, vc = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = (float)((((uint32_t)s + e) * 0x9E3779B1u + c.turn) >> 8) * 0x1p-24f;
+        int q = code_of(fabsf(m[e]), ka, 127.0f, z), u = code_of(r[e], kt, 255.0f, z);
+        if (m[e] < 0.0f) q = -q;
+        if (kt > 0.0f && r[e] > 0.0f && u < 1) u = 1;
+        mc |= (uint32_t)(q & 255) << (8 * e);
+        vc |= (uint32_t)u << (8 * e);
+      }
+      reinterpret_cast<uint32_t*>(st.m)[s / 4] = mc;
+      reinterpret_cast<uint32_t*>(st.v)[s / 4] = vc;
+      if (lane == 0) {
+        st.m_scale[s / kBlock] = a;
+        st.v_scale[s / kBlock] = t;
+      }
+    }
+  }
+}
+
+// The scalars of a step that is counted on the device, in double as the host computes them.
+__global__ void adamw_scalars_kernel(double lr, const float* __restrict__ lr_dev, double b1, double b2, double wd,
+                                     float eps, const int64_t* __restrict__ step_dev, AdamWScalars* __restrict__ out) {
+  if (threadIdx.x) return;
+  if (lr_dev) lr = (double)lr_dev[0];
+  const int64_t t = step_dev[0];
+  AdamWScalars c;
+  c.b1 = (float)b1, c.omb1 = (float)(1.0 - b1), c.b2 = (float)b2, c.omb2 = (float)(1.0 - b2), c.eps = eps;
+  c.decay = (float)(1.0 - lr * wd);
+  c.rate = (float)(lr / (1.0 - pow(b1, (double)t)));
+  c.ib2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+  c.turn = (uint32_t)t * 0x6A09E667u;
+  *out = c;
+}
+
+// What the codes stand for, 4 elements a thread.
+__global__ __launch_bounds__(kThreads) void adamw_values_kernel(AdamWState st, int64_t quads, float* __restrict__ m,
+                                                                float* __restrict__ v) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < quads; i += (int64_t)gridDim.x * kThreads) {
+    const uint32_t mc = reinterpret_cast<const uint32_t*>(st.m)[i], vc = reinterpret_cast<const uint32_t*>(st.v)[i];
+    const float ma = __fmul_rn(st.m_scale[4 * i / kBlock], 1.0f / 16129.0f);
+    const float va = __fmul_rn(st.v_scale[4 * i / kBlock], 1.0f / 65025.0f);
+    float x[4], y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float q = (float)(int8_t)(mc >> (8 * e)), u = (float)((vc >> (8 * e)) & 255u);
+      x[e] = __fmul_rn(q * fabsf(q), ma);
+      const float r = __fmul_rn(u * u, va);
+      y[e] = __fmul_rn(r, r);
+    }
+    reinterpret_cast<float4*>(m)[i] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(v)[i] = make_float4(y[0], y[1], y[2], y[3]);
+  }
+}
+
+template <int PDT, int GDT>
+void launch_bits(const Table& tb, unsigned grid, const AdamWState& st, const AdamWScalars& host, const AdamWScalars* dev,
+                 hipStream_t s) {
+  if (st.bits == 32)
+    hipLaunchKernelGGL((adamw_kernel<PDT, GDT, 32>), dim3(grid), dim3(kThreads), 0, s, tb, st, host, dev);
+  else
+    hipLaunchKernelGGL((adamw_kernel<PDT, GDT, 8>), dim3(grid), dim3(kThreads), 0, s, tb, st, host, dev);
+}
+
+template <int PDT>
+void launch_grad_type(const Table& tb, unsigned grid, int gdt, const AdamWState& st, const AdamWScalars& host,
+                      const AdamWScalars* dev, hipStream_t s) {
+  if (gdt == WFB_F32) launch_bits<PDT, WFB_F32>(tb, grid, st, host, dev, s);
+  else if (gdt == WFB_BF16) launch_bits<PDT, WFB_BF16>(tb, grid, st, host, dev, s);
+  else launch_bits<PDT, WFB_F16>(tb, grid, st, host, dev, s);
+}
+
+}  // namespace
+
+hipError_t launch_adamw(const wfb_adamw_tensor* tensors, int64_t n, int pdt, int gdt, const AdamWState& st,
+                        const AdamWScalars& host, const AdamWScalars* dev, hipStream_t s) {
+  constexpr int64_t kTile = (int64_t)kTileBlocks * kBlock, kMostTiles = INT32_MAX / 2;
+  Table tb;
+  tb.n = 0;
+  tb.tile[0] = 0;
+  auto flush = [&]() -> hipError_t {
+    if (tb.n == 0) return hipSuccess;
+    const unsigned grid = tb.tile[tb.n];
+    if (pdt == WFB_F32) launch_grad_type<WFB_F32>(tb, grid, gdt, st, host, dev, s);
+    else if (pdt == WFB_BF16) launch_grad_type<WFB_BF16>(tb, grid, gdt, st, host, dev, s);
+    else launch_grad_type<WFB_F16>(tb, grid, gdt, st, host, dev, s);
+    tb.n = 0;
+    return hipGetLastError();
+  };
+  for (int64_t i = 0; i < n; ++i) {
+    if (tensors[i].n == 0) continue;
+    const int64_t tiles = (tensors[i].n + kTile - 1) / kTile;
+    if (tb.n == kMaxTensors || tb.tile[tb.n] + tiles > kMostTiles)
+      if (const hipError_t e = flush(); e != hipSuccess) return e;
+    tb.p[tb.n] = tensors[i].p;
+    tb.g[tb.n] = tensors[i].g;
+    tb.len[tb.n] = tensors[i].n;
+    tb.first[tb.n] = tensors[i].first;
+    tb.tile[tb.n + 1] = tb.tile[tb.n] + (uint32_t)tiles;
+    ++tb.n;
+  }
+  return flush();
+}
+
+hipError_t launch_adamw_scalars(double lr, const float* lr_dev, double b1, double b2, double wd, float eps,
+                                const int64_t* step_dev, AdamWScalars* out, hipStream_t s) {
+  hipLaunchKernelGGL(adamw_scalars_kernel, dim3(1), dim3(64), 0, s, lr, lr_dev, b1, b2, wd, eps, step_dev, out);
+  return hipGetLastError();
+}
+
+hipError_t launch_adamw_values(const AdamWState& st, int64_t elements, float* m, float* v, hipStream_t s) {
+  const int64_t quads = elements / 4, groups = (quads + kThreads - 1) / kThreads;
+  hipLaunchKernelGGL(adamw_values_kernel, dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20)), dim3(kThreads), 0, s,
+                     st, quads, m, v);
+  return hipGetLastError();
+}
+
+}  // namespace wfb

@@ -11,6 +11,7 @@
 #include <string>
 
 #include "kv_i8.h"
+#include "train_ops.h"
 #include "wfb_common.h"
 
 namespace {
@@ -849,6 +850,214 @@ int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t 
   a.b = (int)batch, a.t = (int)t, a.hq = (int)num_heads, a.hkv = (int)num_kv_heads, a.d = (int)head_dim, a.dt = dtype;
   a.scale = scale, a.out = out, a.ldo = ldo, a.ws = workspace;
   return hip_status(wfb::launch_kv_attention(a, as_stream(stream)), name);
+}
+
+
+// ---- training step ----------------------------------------------------------------------------
+
+static int check_gated(const char* name, int64_t m, int64_t f, int64_t k) {
+  if (m < 0 || f <= 0 || k <= 0) return fail(WFB_EINVAL, "%s: bad sizes m=%lld f=%lld k=%lld", name, (long long)m, (long long)f, (long long)k);
+  if (m >= 1 << 20 || 2 * f >= 1 << 20 || k >= 1 << 20)
+    return fail(WFB_EINVAL, "%s: M, 2F and K must be below 2^20 (got %lld, %lld, %lld)", name, (long long)m, (long long)(2 * f), (long long)k);
+  return WFB_OK;
+}
+
+int wfb_gated_i2s_workspace(int64_t m, int64_t f, int64_t k, int64_t* floats) {
+  const char* name = "wfb_gated_i2s_workspace";
+  if (const int st = check_gated(name, m, f, k)) return st;
+  if (!floats) return fail(WFB_EINVAL, "%s: null pointer", name);
+  *floats = wfb::gated_workspace_floats(m, f, k);
+  return ok();
+}
+
+int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* act_codes, int64_t m, int64_t lda,
+                  const float* a_scale, const float* scales_dev, int act, void* h, int h_dtype, float* gate_up,
+                  void* stream) {
+  const char* name = "wfb_gated_i2s";
+  if (const int st = check_gated(name, m, f, k)) return st;
+  if (k % WFB_QK_I2S != 0) return fail(WFB_EINVAL, "%s: K (%lld) must be multiple of %d", name, (long long)k, WFB_QK_I2S);
+  if (act != WFB_ACT_SILU && act != WFB_ACT_RELU2) return fail(WFB_EINVAL, "%s: bad activation %d", name, act);
+  if (!valid_dtype(h_dtype)) return fail(WFB_EINVAL, "%s: bad dtype %d", name, h_dtype);
+  if (m == 0) return ok();
+  if (!qweight || !act_codes || !a_scale || !scales_dev || !h || (!gate_up && wfb::gated_workspace_floats(m, f, k)))
+    return fail(WFB_EINVAL, "%s: null pointer", name);
+  if (!aligned(qweight, 16) || !aligned(act_codes, 16) || !aligned(gate_up, 16) || !aligned(h, 16))
+    return fail(WFB_EINVAL, "%s: qweight, codes, h and gate_up must be 16-byte aligned", name);
+  if (lda < k || lda % 16 != 0 || 127 * lda + k > INT32_MAX)
+    return fail(WFB_EINVAL, "%s: activation row stride (%lld) must be >= K, a multiple of 16 and 127 * lda + K below 2^31", name, (long long)lda);
+  wfb::GatedForward p{qweight, f, k, act_codes, m, lda, a_scale, scales_dev, act, h, h_dtype, gate_up};
+  return hip_status(wfb::launch_gated(p, as_stream(stream)), name);
+}
+
+int wfb_gated_grad_workspace(int64_t m, int64_t f, int64_t k, int gx_dtype, int want_x, int gw_dtype, int want_w,
+                             int64_t* bytes) {
+  const char* name = "wfb_gated_grad_workspace";
+  if (const int st = check_gated(name, m, f, k)) return st;
+  if (!valid_dtype(gx_dtype) || !valid_dtype(gw_dtype)) return fail(WFB_EINVAL, "%s: bad dtype", name);
+  if (!bytes) return fail(WFB_EINVAL, "%s: null pointer", name);
+  wfb::GatedGrad p{};
+  p.m = m, p.f = f, p.k = k, p.gx_dtype = gx_dtype, p.gw_dtype = gw_dtype;
+  p.gx = want_x ? bytes : nullptr;  // (only whether they are null counts)
+  p.gw = want_w ? bytes : nullptr;
+  *bytes = m == 0 ? 0 : wfb::gated_grad_workspace(p);
+  return ok();
+}
+
+int wfb_gated_grad(const float* gate_up, const void* grad_h, int gh_dtype, int64_t ldg, int64_t m, int64_t f, int act,
+                   const uint8_t* qweight, int64_t k, int64_t k_pad, const float* scales_dev, const int8_t* codes,
+                   int64_t lda, const float* a_scale, void* grad_x, int gx_dtype, void* grad_w, int gw_dtype, void* work,
+                   void* stream) {
+  const char* name = "wfb_gated_grad";
+  if (const int st = check_gated(name, m, f, k)) return st;
+  if (m == 0) return fail(WFB_EINVAL, "%s: no rows", name);
+  if (act != WFB_ACT_SILU && act != WFB_ACT_RELU2) return fail(WFB_EINVAL, "%s: bad activation %d", name, act);
+  if (!valid_dtype(gh_dtype) || !valid_dtype(gx_dtype) || !valid_dtype(gw_dtype)) return fail(WFB_EINVAL, "%s: bad dtype", name);
+  if (!gate_up || !grad_h || !qweight || !scales_dev || !codes || !a_scale || !work || (!grad_x && !grad_w))
+    return fail(WFB_EINVAL, "%s: null pointer", name);
+  if (k_pad < k || k_pad % WFB_QK_I2S != 0 || !aligned(qweight, 8))
+    return fail(WFB_EINVAL, "%s: packed rows must be 8-byte aligned and hold k_pad >= K weights, a multiple of %d", name, WFB_QK_I2S);
+  if (ldg < f || lda < k) return fail(WFB_EINVAL, "%s: row strides below the rows' length", name);
+  if (!aligned(gate_up, 16) || !aligned(work, 256)) return fail(WFB_EINVAL, "%s: gate_up must be 16-byte, work 256-byte aligned", name);
+  wfb::GatedGrad p{gate_up, grad_h, gh_dtype, ldg, m, f, act, qweight, k, k_pad, scales_dev, codes, lda, a_scale,
+                   grad_x, gx_dtype, grad_w, gw_dtype};
+  return hip_status(wfb::launch_gated_grad(p, work, as_stream(stream)), name);
+}
+
+// The call as the kernels take it; a status other than WFB_OK refuses it.
+static int qk_rope_args(const char* name, const wfb_heads* q, const wfb_heads* k, const wfb_rope* rope, int dtype,
+                        int64_t batch, int64_t t, int64_t head_dim, float eps, bool grad, wfb::QkRope& p) {
+  if (!q || !k || !rope) return fail(WFB_EINVAL, "%s: null argument", name);
+  if (!valid_dtype(dtype)) return fail(WFB_EINVAL, "%s: bad dtype %d", name, dtype);
+  if (head_dim < 2 || head_dim > WFB_QK_MAX_DIM || head_dim % 2 != 0)
+    return fail(WFB_EINVAL, "%s: head_dim (%lld) must be even and in 2..%d", name, (long long)head_dim, WFB_QK_MAX_DIM);
+  if (rope->rotary_dim < 0 || rope->rotary_dim > head_dim || rope->rotary_dim % 2 != 0)
+    return fail(WFB_EINVAL, "%s: rotary_dim (%lld) must be even and in 0..head_dim", name, (long long)rope->rotary_dim);
+  if (batch < 0 || t < 0 || batch > INT32_MAX || t > INT32_MAX || q->heads < 0 || k->heads < 0 || q->heads > 65535 || k->heads > 65535)
+    return fail(WFB_EINVAL, "%s: bad sizes", name);
+  if (rope->rotary_dim > 0 && (!rope->cos || !rope->sin || rope->rope_len < 1))
+    return fail(WFB_EINVAL, "%s: rotary tables missing", name);
+  if (!aligned(rope->cos, 4) || !aligned(rope->sin, 4)) return fail(WFB_EINVAL, "%s: rotary tables must be 4-byte aligned", name);
+  if (rope->pos && rope->pos_bytes != 4 && rope->pos_bytes != 8)
+    return fail(WFB_EINVAL, "%s: positions must be int32 or int64", name);
+  if (!rope->pos && rope->rotary_dim > 0 && (rope->start < 0 || rope->start > rope->rope_len - t))
+    return fail(WFB_EINVAL, "%s: positions %lld.. leave the rotary tables of %lld rows", name, (long long)rope->start, (long long)rope->rope_len);
+  const wfb_heads* in[2] = {q, k};
+  const size_t esz = dtype == WFB_F32 ? 4 : 2;
+  for (int i = 0; i < 2; ++i) {
+    const wfb_heads& h = *in[i];
+    if (h.weight && !valid_dtype((int)h.weight_dtype)) return fail(WFB_EINVAL, "%s: bad weight dtype", name);
+    const bool some = batch * t > 0 && h.heads > 0;
+    if (some && (!h.x || (!grad && !h.out) || (grad && !h.g))) return fail(WFB_EINVAL, "%s: null pointer", name);
+    if (!aligned(h.x, esz) || !aligned(h.g, esz) || !aligned(h.out, esz)) return fail(WFB_EINVAL, "%s: pointers must be aligned to their elements", name);
+    if (h.grad_weight && !h.weight) return fail(WFB_EINVAL, "%s: a weight's gradient without the weight", name);
+    p.side[i] = wfb::HeadRows{h.x, h.stride_b, h.stride_t, h.stride_h, h.g, h.g_stride_b, h.g_stride_t, h.g_stride_h,
+                              h.weight, (int)h.weight_dtype, h.out, (int)h.heads};
+  }
+  p.cos = rope->cos, p.sin = rope->sin, p.rope_len = rope->rope_len, p.rotary = (int)rope->rotary_dim;
+  p.interleaved = rope->interleaved != 0;
+  p.pos = rope->pos, p.pos64 = rope->pos_bytes == 8, p.pb = rope->pos_stride_b, p.pt = rope->pos_stride_t;
+  p.start = rope->start, p.batch = batch, p.t = t, p.head_dim = (int)head_dim, p.eps = eps;
+  if (batch * t > INT32_MAX || wfb::qk_tasks(p) > INT32_MAX)
+    return fail(WFB_EINVAL, "%s: more than 2^31 groups of heads", name);
+  return WFB_OK;
+}
+
+int wfb_qk_norm_rope(const wfb_heads* q, const wfb_heads* k, const wfb_rope* rope, int dtype, int64_t batch, int64_t t,
+                     int64_t head_dim, float eps, void* stream) {
+  const char* name = "wfb_qk_norm_rope";
+  wfb::QkRope p{};
+  if (const int st = qk_rope_args(name, q, k, rope, dtype, batch, t, head_dim, eps, false, p)) return st;
+  if (wfb::qk_tasks(p) == 0) return ok();
+  return hip_status(wfb::launch_qk_rope(p, dtype, as_stream(stream)), name);
+}
+
+int wfb_qk_norm_rope_grad_workspace(int64_t batch, int64_t t, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                    int64_t* floats) {
+  const char* name = "wfb_qk_norm_rope_grad_workspace";
+  if (batch < 0 || t < 0 || q_heads < 0 || k_heads < 0 || head_dim < 2 || head_dim > WFB_QK_MAX_DIM || batch > INT32_MAX ||
+      t > INT32_MAX || q_heads > 65535 || k_heads > 65535 || batch * t > INT32_MAX)
+    return fail(WFB_EINVAL, "%s: bad sizes", name);
+  if (!floats) return fail(WFB_EINVAL, "%s: null pointer", name);
+  wfb::QkRope p{};
+  p.batch = batch, p.t = t, p.side[0].heads = (int)q_heads, p.side[1].heads = (int)k_heads;
+  *floats = (int64_t)wfb::qk_grad_parts(p) * 2 * head_dim;
+  return ok();
+}
+
+int wfb_qk_norm_rope_grad(const wfb_heads* q, const wfb_heads* k, const wfb_rope* rope, int dtype, int64_t batch, int64_t t,
+                          int64_t head_dim, float eps, float* work, void* stream) {
+  const char* name = "wfb_qk_norm_rope_grad";
+  wfb::QkRope p{};
+  if (const int st = qk_rope_args(name, q, k, rope, dtype, batch, t, head_dim, eps, true, p)) return st;
+  if ((q->grad_weight || k->grad_weight) && wfb::qk_tasks(p) > 0 && !work)
+    return fail(WFB_EINVAL, "%s: null workspace", name);
+  if (!aligned(work, 4)) return fail(WFB_EINVAL, "%s: workspace must be 4-byte aligned", name);
+  return hip_status(wfb::launch_qk_rope_grad(p, dtype, q->grad_weight, (int)q->weight_dtype, k->grad_weight,
+                                             (int)k->weight_dtype, work, as_stream(stream)), name);
+}
+
+static int check_adamw_state(const char* name, const void* m, const void* v, const float* m_scale, const float* v_scale,
+                             int64_t elements, int bits) {
+  if (bits != 32 && bits != 8) return fail(WFB_EINVAL, "%s: states have 32 or 8 bits, not %d", name, bits);
+  if (elements < 0 || elements % WFB_ADAMW_BLOCK != 0)
+    return fail(WFB_EINVAL, "%s: the state's elements (%lld) must be a multiple of %d", name, (long long)elements, WFB_ADAMW_BLOCK);
+  if (elements > 0 && (!m || !v || (bits == 8 && (!m_scale || !v_scale)))) return fail(WFB_EINVAL, "%s: null state", name);
+  if (!aligned(m, 16) || !aligned(v, 16) || !aligned(m_scale, 4) || !aligned(v_scale, 4))
+    return fail(WFB_EINVAL, "%s: states must be 16-byte aligned, scales 4-byte aligned", name);
+  return WFB_OK;
+}
+
+int wfb_adamw_step(const wfb_adamw_tensor* tensors, int64_t n_tensors, int p_dtype, int g_dtype, void* m, void* v,
+                   float* m_scale, float* v_scale, int64_t state_elements, int bits, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, int64_t step, const int64_t* step_dev,
+                   const float* lr_dev, float* scalars, void* stream) {
+  const char* name = "wfb_adamw_step";
+  if (const int st = check_adamw_state(name, m, v, m_scale, v_scale, state_elements, bits)) return st;
+  if (!valid_dtype(p_dtype) || !valid_dtype(g_dtype)) return fail(WFB_EINVAL, "%s: bad dtype", name);
+  if (n_tensors < 0 || (n_tensors > 0 && !tensors)) return fail(WFB_EINVAL, "%s: bad tensor list", name);
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return fail(WFB_EINVAL, "%s: betas must lie in [0, 1)", name);
+  if (!(eps >= 0.0) || !(weight_decay >= 0.0) || (!lr_dev && !(lr >= 0.0)))
+    return fail(WFB_EINVAL, "%s: lr, eps and weight_decay must not be negative", name);
+  if (!step_dev && step < 1) return fail(WFB_EINVAL, "%s: steps count from 1", name);
+  if (lr_dev && !step_dev) return fail(WFB_EINVAL, "%s: a device learning rate goes with a device step", name);
+  if (step_dev && (!scalars || !aligned(scalars, 4))) return fail(WFB_EINVAL, "%s: null scalars", name);
+  const size_t ps = p_dtype == WFB_F32 ? 4 : 2, gs = g_dtype == WFB_F32 ? 4 : 2;
+  for (int64_t i = 0; i < n_tensors; ++i) {
+    const wfb_adamw_tensor& t = tensors[i];
+    if (t.n < 0 || t.first < 0 || t.first % WFB_ADAMW_BLOCK != 0 || t.n > state_elements - t.first)
+      return fail(WFB_EINVAL, "%s: tensor %lld leaves the state (elements %lld from %lld of %lld)", name, (long long)i,
+                  (long long)t.n, (long long)t.first, (long long)state_elements);
+    if (t.n > 0 && (!t.p || !t.g || !aligned(t.p, ps) || !aligned(t.g, gs)))
+      return fail(WFB_EINVAL, "%s: tensor %lld: null or misaligned pointer", name, (long long)i);
+  }
+  const wfb::AdamWState st{m, v, m_scale, v_scale, bits};
+  wfb::AdamWScalars c{};
+  const wfb::AdamWScalars* dev = nullptr;
+  static_assert(sizeof(wfb::AdamWScalars) <= 4 * WFB_ADAMW_SCALARS, "scalars");
+  if (step_dev) {
+    auto* out = reinterpret_cast<wfb::AdamWScalars*>(scalars);
+    const hipError_t e = wfb::launch_adamw_scalars(lr, lr_dev, beta1, beta2, weight_decay, (float)eps, step_dev, out, as_stream(stream));
+    if (e != hipSuccess) return hip_status(e, name);
+    dev = out;
+  } else {
+    c.b1 = (float)beta1, c.omb1 = (float)(1.0 - beta1), c.b2 = (float)beta2, c.omb2 = (float)(1.0 - beta2), c.eps = (float)eps;
+    c.decay = (float)(1.0 - lr * weight_decay);
+    c.rate = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+    c.ib2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+    c.turn = (uint32_t)step * 0x6A09E667u;
+  }
+  return hip_status(wfb::launch_adamw(tensors, n_tensors, p_dtype, g_dtype, st, c, dev, as_stream(stream)), name);
+}
+
+int wfb_adamw_values(const void* m, const void* v, const float* m_scale, const float* v_scale, int64_t state_elements,
+                     float* m_out, float* v_out, void* stream) {
+  const char* name = "wfb_adamw_values";
+  if (const int st = check_adamw_state(name, m, v, m_scale, v_scale, state_elements, 8)) return st;
+  if (state_elements == 0) return ok();
+  if (!m_out || !v_out || !aligned(m_out, 16) || !aligned(v_out, 16))
+    return fail(WFB_EINVAL, "%s: outputs must be 16-byte aligned", name);
+  const wfb::AdamWState st{const_cast<void*>(m), const_cast<void*>(v), const_cast<float*>(m_scale), const_cast<float*>(v_scale), 8};
+  return hip_status(wfb::launch_adamw_values(st, state_elements, m_out, v_out, as_stream(stream)), name);
 }
 
 }  // extern "C"

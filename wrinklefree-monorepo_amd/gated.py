@@ -1,0 +1,218 @@
+"""The gated feed-forward product of two ternary projections, act(gate(x)) * up(x), with its backward pass.
+
+The float block is the reference's FFN (WF/models/ffn.py:10-45, WF = packages/training/src/wrinklefree); each projection
+is a BitLinear (WF/models/bitlinear.py:36-113) under the straight-through estimator at lambda = 1, as
+:class:`~.bitlinear.BitLinear` trains it: int8 codes of the tokens, shared by both projections, ternary weights, exact
+integer sums.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import WFB_ABSMEAN_WS_DOUBLES
+from .bitlinear import BitLinear, _check_lambda
+from .ops import _ACTS, _DT, QK_I2_S, _on, _p, _require_gpu, _stream, quantize_activations_i8_per_token
+
+_NAME = "gated_bitlinear"
+
+
+class PackedGated(NamedTuple):
+    """Gate over up as they are multiplied with: I2_S uint8 [2 * hidden, k_pad / 4] and their two fp32 scales."""
+
+    qweight: torch.Tensor
+    scales: torch.Tensor
+
+
+def _check_pair(name: str, gate: torch.Tensor, up: torch.Tensor) -> None:
+    if gate.dim() != 2 or gate.shape != up.shape or gate.dtype != up.dtype:
+        raise RuntimeError(f"{name}: gate and up must be 2D [hidden, in_features] of one shape and type")
+    if gate.dtype not in _DT:
+        raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {gate.dtype}")
+
+
+@torch.no_grad()
+def pack_gated(gate_weight: torch.Tensor, up_weight: torch.Tensor) -> PackedGated:
+    """Both matrices [hidden, in_features] ternarised and packed, each with its own absmean scale, as
+    :func:`pack_ternary_i2s` packs one; in_features is padded to a multiple of 128 with zero weights."""
+    name = "pack_gated"
+    _check_pair(name, gate_weight, up_weight)
+    dev = _require_gpu(name, gate_weight, up_weight)
+    f, k = gate_weight.shape
+    if f == 0 or k == 0:
+        raise RuntimeError(f"{name}: empty weights")
+    kp = (k + QK_I2_S - 1) // QK_I2_S * QK_I2_S
+    dt = _DT[gate_weight.dtype]
+    qweight = torch.empty((2 * f, kp // 4), dtype=torch.uint8, device=dev)
+    scales = torch.empty(2, dtype=torch.float32, device=dev)
+    ws = torch.empty(WFB_ABSMEAN_WS_DOUBLES, dtype=torch.float64, device=dev)
+    with _on(dev):
+        s = _stream(dev)
+        for i, w in enumerate((gate_weight, up_weight)):
+            _lib.call("wfb_weight_absmean", _p(w), dt, w.numel(), scales.data_ptr() + 4 * i, _p(ws), s)
+            if kp != k:
+                w = nn.functional.pad(w, (0, kp - k))
+            _lib.call("wfb_pack_i2s", _p(w), dt, f, kp, kp, scales.data_ptr() + 4 * i,
+                      qweight.data_ptr() + i * f * (kp // 4), s)
+    return PackedGated(qweight, scales)
+
+
+def _forward(x2: torch.Tensor, packed: PackedGated, act: str, keep: bool):
+    """(h, gate|up or None, codes, a_scale) of the rows x2."""
+    n, kb = packed.qweight.shape
+    f, kp, m, dev = n // 2, 4 * kb, x2.shape[0], x2.device
+    q, a_scale = quantize_activations_i8_per_token(x2, k_pad=kp)
+    h = torch.empty((m, f), dtype=x2.dtype, device=dev)
+    floats = 2 * f * m
+    if not keep and m:
+        size = ctypes.c_int64(0)
+        _lib.call("wfb_gated_i2s_workspace", m, f, kp, ctypes.addressof(size))
+        floats = size.value
+    gate_up = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    with _on(dev):
+        _lib.call("wfb_gated_i2s", _p(packed.qweight), f, kp, _p(q), m, kp, _p(a_scale), _p(packed.scales), _ACTS[act],
+                  _p(h), _DT[h.dtype], _p(gate_up), _stream(dev))
+    return h, gate_up, q, a_scale
+
+
+class _GatedSTE(torch.autograd.Function):
+    """Straight through both quantisers, as BitLinear: the forward's value is the kernels', the backward is the gradient of
+    act(x~ gate~^T) * (x~ up~^T) at the quantised operands, from the two products that the forward kept."""
+
+    @staticmethod
+    def forward(ctx, x2, gate_weight, up_weight, qweight, scales, act):
+        h, gate_up, q, a_scale = _forward(x2, PackedGated(qweight, scales), act, True)
+        ctx.save_for_backward(gate_up, q, a_scale, qweight, scales)
+        ctx.meta = (act, x2.dtype, gate_weight.dtype, x2.shape[1])
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gh):
+        # (contiguous: a saved-tensor hook may give them back otherwise)
+        gate_up, q, a_scale, qweight, scales = (t.contiguous() for t in ctx.saved_tensors)
+        act, xdt, wdt, k = ctx.meta
+        need_x, need_gate, need_up = ctx.needs_input_grad[:3]
+        f, m, dev = qweight.shape[0] // 2, q.shape[0], q.device
+        if gh.stride(-1) != 1 or gh.stride(0) < f or gh.is_neg():
+            gh = gh.contiguous()
+        need_w = need_gate or need_up
+        gx = torch.empty((m, k), dtype=xdt, device=dev) if need_x else None
+        gw = torch.empty((2 * f, k), dtype=wdt, device=dev) if need_w else None
+        if m == 0:
+            return gx, *([gw[:f].zero_(), gw[f:].zero_()] if need_w else [None, None]), None, None, None
+        size = ctypes.c_int64(0)
+        _lib.call("wfb_gated_grad_workspace", m, f, k, _DT[xdt], int(need_x), _DT[wdt], int(need_w),
+                  ctypes.addressof(size))
+        work = torch.empty(size.value, dtype=torch.uint8, device=dev)
+        kp = 4 * qweight.shape[1]
+        with _on(dev):
+            _lib.call("wfb_gated_grad", _p(gate_up), _p(gh), _DT[gh.dtype], gh.stride(0) if m > 1 else f, m, f, _ACTS[act],
+                      _p(qweight), k, kp, _p(scales), _p(q), kp, _p(a_scale), _p(gx), _DT[xdt], _p(gw), _DT[wdt], _p(work),
+                      _stream(dev))
+        return gx, gw[:f] if need_gate else None, gw[f:] if need_up else None, None, None, None
+
+
+def gated_bitlinear(
+    x: torch.Tensor, gate_weight: Optional[torch.Tensor] = None, up_weight: Optional[torch.Tensor] = None,
+    act: str = "silu", packed: Optional[PackedGated] = None,
+) -> torch.Tensor:
+    """act(gate) * up, [..., hidden] in x's type, of x [..., in_features] (fp32, bf16 or fp16) through two ternary
+    projections; ``act`` is "silu" or "relu2" (relu squared).  Products and activation are those of
+    :func:`bitnet_linear_glu` with ``mid_dtype=float32``, rounded once.
+
+    ``packed`` (of :func:`pack_gated`) saves packing the float weights; without them the call serves only.  With autograd on
+    and x or a weight requiring a gradient, the result is differentiable once, straight through both quantisers, and the
+    products are kept for it (8 bytes per token and hidden feature); x, gate_weight and up_weight get gradients in their
+    types.  ``packed`` must then be the weights' own pack."""
+    if act not in _ACTS:
+        raise ValueError(f"{_NAME}: act must be one of {sorted(_ACTS)}")
+    if (gate_weight is None) != (up_weight is None):
+        raise RuntimeError(f"{_NAME}: gate_weight and up_weight go together")
+    if gate_weight is None and packed is None:
+        raise RuntimeError(f"{_NAME}: weights or their pack are needed")
+    if x.dtype not in _DT or x.dim() < 1:
+        raise RuntimeError(f"{_NAME}: x must be float32, bfloat16 or float16 with a feature dimension")
+    if x.device.type != "cuda":
+        raise RuntimeError(f"{_NAME}: tensors must be on a HIP device (got {x.device})")
+    k = x.shape[-1]
+    if gate_weight is not None:
+        _check_pair(_NAME, gate_weight, up_weight)
+        if gate_weight.shape[1] != k:
+            raise RuntimeError(f"{_NAME}: x has {k} features, the weights {gate_weight.shape[1]}")
+        if gate_weight.device != x.device or up_weight.device != x.device:
+            raise RuntimeError(f"{_NAME}: weights must be on {x.device}")
+    if packed is None:
+        packed = pack_gated(gate_weight.detach().contiguous(), up_weight.detach().contiguous())
+    else:
+        qw, scales = packed
+        _require_gpu(_NAME, qw, scales)
+        if qw.dtype != torch.uint8 or qw.dim() != 2 or qw.shape[0] % 2 or qw.shape[0] == 0 or qw.device != x.device \
+                or scales.dtype != torch.float32 or scales.numel() != 2 or scales.device != x.device:
+            raise RuntimeError(f"{_NAME}: packed must be uint8 [2 * hidden, k_pad / 4] and fp32 [2] on {x.device}")
+        if 4 * qw.shape[1] != (k + QK_I2_S - 1) // QK_I2_S * QK_I2_S:
+            raise RuntimeError(f"{_NAME}: x has {k} features, packed rows hold {4 * qw.shape[1]}")
+        if gate_weight is not None and gate_weight.shape[0] != qw.shape[0] // 2:
+            raise RuntimeError(f"{_NAME}: packed has {qw.shape[0] // 2} hidden features, the weights {gate_weight.shape[0]}")
+    f = packed.qweight.shape[0] // 2
+    x2 = x.reshape(-1, k) if k else x.new_empty((0, 0))
+    if not x2.is_contiguous() or x2.is_neg():
+        x2 = x2.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, gate_weight, up_weight)):
+        if gate_weight is None:
+            raise RuntimeError(f"{_NAME}: packed weights alone have no float weights to train")
+        h = _GatedSTE.apply(x2, gate_weight, up_weight, packed.qweight, packed.scales, act)
+    else:
+        h = _forward(x2, packed, act, False)[0]
+    return h.view(*x.shape[:-1], f)
+
+
+class GatedBitLinear(nn.Module):
+    """act(gate_proj(x)) * up_proj(x) of two bias-free ternary projections, on one set of activation codes; in front of a
+    :class:`SubLNBitLinear` it is the feed-forward block of the converted models
+    (packages/training/src/wrinklefree/training/stage1.py:93-166).  ``gate_proj`` and ``up_proj`` hold the float weights under
+    the names of the linears that they replace; the pack of both is rebuilt when either has changed."""
+
+    def __init__(self, in_features: int, hidden_features: int, act: str = "silu", device=None, dtype=None):
+        super().__init__()
+        if act not in _ACTS:
+            raise ValueError(f"GatedBitLinear: act must be one of {sorted(_ACTS)}")
+        self.act = act
+        self.gate_proj = BitLinear(in_features, hidden_features, device=device, dtype=dtype)
+        self.up_proj = BitLinear(in_features, hidden_features, device=device, dtype=dtype)
+        self._packed: Optional[PackedGated] = None
+        self._packed_from = None
+
+    @classmethod
+    def from_linears(cls, gate_proj: nn.Linear, up_proj: nn.Linear, act: str = "silu") -> "GatedBitLinear":
+        """A module that shares the weights of two linears."""
+        if gate_proj.bias is not None or up_proj.bias is not None:
+            raise RuntimeError("GatedBitLinear: projections with a bias are not gated in one product")
+        _check_pair("GatedBitLinear", gate_proj.weight, up_proj.weight)
+        mod = cls(gate_proj.in_features, gate_proj.out_features, act, device="meta", dtype=gate_proj.weight.dtype)
+        mod.gate_proj.weight, mod.up_proj.weight = gate_proj.weight, up_proj.weight
+        return mod
+
+    def packed(self) -> PackedGated:
+        """The weights' pack, rebuilt if a weight changed since the last one."""
+        stamp = (self.gate_proj._weight_stamp(), self.up_proj._weight_stamp())
+        if self._packed is None or self._packed_from != stamp:
+            self._packed = pack_gated(self.gate_proj.weight.detach().contiguous(), self.up_proj.weight.detach().contiguous())
+            self._packed_from = stamp
+        return self._packed
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _check_lambda("GatedBitLinear")
+        return gated_bitlinear(x, self.gate_proj.weight, self.up_proj.weight, self.act, self.packed())
+
+    def __getstate__(self):
+        return {**self.__dict__, "_packed": None, "_packed_from": None}
+
+    def extra_repr(self) -> str:
+        return f"act={self.act}"

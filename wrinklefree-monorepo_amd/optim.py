@@ -1,0 +1,226 @@
+"""AdamW over many tensors in one launch, with states in fp32 or in 8 bits.
+
+The reference trains its float weights with torch's and 8-bit AdamW; here one kernel walks every tensor of a group, and
+the states of a group lie in one flat array each, so that a state in 8 bits (codes and one scale for 256 elements, about
+a quarter of the bytes) needs no bookkeeping per tensor.  The arithmetic is in csrc/adamw.hip's first lines.  Weights
+change in place and their version counters with them, so that a BitLinear over them repacks.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from array import array
+from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from ._lib import WFB_ADAMW_BLOCK, WFB_ADAMW_SCALARS
+from .ops import _DT, _on, _stream
+
+
+class AdamWState(NamedTuple):
+    """The moments of a list of tensors, flat: tensor i starts at a multiple of 256 elements, behind tensor i - 1.  In 32
+    bits ``m`` and ``v`` are fp32 and the scales None; in 8 bits int8 and uint8 codes with fp32 scales, one for each 256.
+    Elements behind a tensor's end are 0."""
+
+    m: torch.Tensor
+    v: torch.Tensor
+    m_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+
+def _blocks(n: int) -> int:
+    return (n + WFB_ADAMW_BLOCK - 1) // WFB_ADAMW_BLOCK
+
+
+def adamw_state(params: Iterable[torch.Tensor], bits: int = 32) -> AdamWState:
+    """A zero state in 32 or 8 bits for these tensors, on their device."""
+    params = list(params)
+    if bits not in (8, 32):
+        raise ValueError(f"adamw_state: states have 32 or 8 bits, not {bits}")
+    if not params:
+        raise ValueError("adamw_state: no tensors")
+    blocks, dev = sum(_blocks(p.numel()) for p in params), params[0].device
+    n = blocks * WFB_ADAMW_BLOCK
+    if bits == 32:
+        return AdamWState(*(torch.zeros(n, dtype=torch.float32, device=dev) for _ in range(2)))
+    return AdamWState(torch.zeros(n, dtype=torch.int8, device=dev), torch.zeros(n, dtype=torch.uint8, device=dev),
+                      *(torch.zeros(blocks, dtype=torch.float32, device=dev) for _ in range(2)))
+
+
+def _check_state(name: str, state: AdamWState) -> Tuple[int, torch.device]:
+    """(bits, device) of a state."""
+    m, v, ms, vs = state
+    if m.device.type != "cuda":
+        raise RuntimeError(f"{name}: the state must be on a HIP device (got {m.device})")
+    n = m.numel()
+    if m.dtype == v.dtype == torch.float32 and ms is None and vs is None:
+        bits, rest = 32, (v,)
+    elif m.dtype == torch.int8 and v.dtype == torch.uint8 and ms is not None and vs is not None:
+        bits, rest = 8, (v, ms, vs)
+        if ms.dtype != torch.float32 or vs.dtype != torch.float32 or ms.numel() * WFB_ADAMW_BLOCK != n \
+                or vs.numel() * WFB_ADAMW_BLOCK != n:
+            raise RuntimeError(f"{name}: scales must be fp32, one for each {WFB_ADAMW_BLOCK} elements")
+    else:
+        raise RuntimeError(f"{name}: a state is fp32 m and v, or int8 m and uint8 v with their scales")
+    if v.numel() != n or n % WFB_ADAMW_BLOCK:
+        raise RuntimeError(f"{name}: m and v must have as many elements, a multiple of {WFB_ADAMW_BLOCK}")
+    for t in (m, *rest):
+        if not t.is_contiguous() or t.device != m.device:
+            raise RuntimeError(f"{name}: the state must be contiguous and on one device")
+    return bits, m.device
+
+
+@torch.no_grad()
+def adamw_step(
+    params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]], state: AdamWState,
+    step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+    eps: float = 1e-8, weight_decay: float = 1e-2,
+) -> None:
+    """AdamW step number ``step`` (from 1) of every tensor that has a gradient (None: left as it is), in place.
+
+    params fp32, bf16 or fp16 and their gradients, each of any of these types, contiguous, on one device; ``state`` of
+    :func:`adamw_state` for the same list.  Decoupled weight decay; arithmetic in fp32, parameters rounded once.
+    For a captured graph ``step`` is an int64 device tensor of one element, which the caller counts up, and ``lr`` may be an
+    fp32 one.  A gradient that is not finite spoils its own element, and in 8 bits the moments of its block of 256."""
+    name = "adamw_step"
+    bits, dev = _check_state(name, state)
+    if len(params) != len(grads):
+        raise RuntimeError(f"{name}: {len(params)} tensors, {len(grads)} gradients")
+    kinds: dict = {}  # (p type, g type) -> rows of wfb_adamw_tensor
+    first, seen, written = 0, set(), []
+    for p, g in zip(params, grads):
+        n = p.numel()
+        if g is not None and n:
+            if p.device != dev or g.device != dev or g.shape != p.shape:
+                raise RuntimeError(f"{name}: a gradient has its tensor's shape, both are on {dev}")
+            if not p.is_contiguous() or g.is_neg():
+                raise RuntimeError(f"{name}: tensors must be contiguous")
+            if not g.is_contiguous():
+                g = g.contiguous()
+            at = p.data_ptr()
+            if at in seen:
+                raise RuntimeError(f"{name}: a tensor is given twice")
+            seen.add(at)
+            written.append(p)
+            rows = kinds.get((p.dtype, g.dtype))
+            if rows is None:
+                if p.dtype not in _DT or g.dtype not in _DT:
+                    raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {p.dtype} and {g.dtype}")
+                rows = kinds[(p.dtype, g.dtype)] = (array("q"), [])
+            rows[0].extend((at, g.data_ptr(), n, first))
+            rows[1].append(g)  # (a copy lives until the launch is in the stream)
+        first += _blocks(n) * WFB_ADAMW_BLOCK
+    if first != state.m.numel():
+        raise RuntimeError(f"{name}: the state has {state.m.numel()} elements, the tensors take {first}")
+    step_dev = lr_dev = scalars = None
+    if isinstance(step, torch.Tensor):
+        if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
+            raise RuntimeError(f"{name}: a step tensor must be one int64 element on {dev}")
+        step_dev, step = step.data_ptr(), 0
+        scalars = torch.empty(WFB_ADAMW_SCALARS, dtype=torch.float32, device=dev)
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev or step_dev is None:
+            raise RuntimeError(f"{name}: a lr tensor must be one fp32 element on {dev} and goes with a step tensor")
+        lr_dev, lr = lr.data_ptr(), 0.0
+    m, v, ms, vs = state
+    with _on(dev):
+        for (pdt, gdt), (rows, _) in kinds.items():
+            _lib.call("wfb_adamw_step", rows.buffer_info()[0], len(rows) // 4, _DT[pdt], _DT[gdt], m.data_ptr(),
+                      v.data_ptr(), None if ms is None else ms.data_ptr(), None if vs is None else vs.data_ptr(),
+                      m.numel(), bits, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+                      int(step), step_dev, lr_dev, None if scalars is None else scalars.data_ptr(), _stream(dev))
+    if written:
+        torch.autograd.graph.increment_version(written)
+
+
+def adamw_state_values(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(m, v) fp32 of a state, flat: of 32 bits its own arrays, of 8 bits new ones with what the codes stand for."""
+    name = "adamw_state_values"
+    bits, dev = _check_state(name, state)
+    if bits == 32:
+        return state.m, state.v
+    m, v = (torch.empty(state.m.numel(), dtype=torch.float32, device=dev) for _ in range(2))
+    with _on(dev):
+        _lib.call("wfb_adamw_values", state.m.data_ptr(), state.v.data_ptr(), state.m_scale.data_ptr(),
+                  state.v_scale.data_ptr(), m.numel(), m.data_ptr(), v.data_ptr(), _stream(dev))
+    return m, v
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW``'s arguments and step over :func:`adamw_step`, ``state_bits`` 32 or 8.
+
+    A group has one state and one count of steps; its tensors are of one device.  With ``capturable`` the count lies on the
+    device and :meth:`step` can be captured into a graph (``lr`` may then be an fp32 device tensor); the first step, which makes
+    the state, comes before the capture.  The state dict holds the states as they are."""
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32, capturable: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 32 or 8, not {state_bits}")
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"AdamW: bad lr {lr}")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("AdamW: a lr tensor needs capturable=True")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"AdamW: bad betas {betas}, eps {eps} or weight_decay {weight_decay}")
+        self._flat: List[Optional[dict]] = []
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      capturable=capturable))
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        self._flat.append(None)
+
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "_flat": self._flat}
+
+    def group_state(self, index: int = 0) -> Optional[AdamWState]:
+        """The state of a group, None before its first step."""
+        return None if self._flat[index] is None else self._flat[index]["state"]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for i, group in enumerate(self.param_groups):
+            params = group["params"]
+            grads = [p.grad for p in params]
+            if all(g is None for g in grads):
+                continue
+            if any(g is not None and g.is_sparse for g in grads):
+                raise RuntimeError("AdamW: sparse gradients are not supported")
+            flat = self._flat[i]
+            if flat is None:
+                count = torch.zeros(1, dtype=torch.int64, device=params[0].device) if group["capturable"] else 0
+                flat = self._flat[i] = {"state": adamw_state(params, group["state_bits"]), "step": count}
+            flat["step"] += 1
+            adamw_step(params, grads, flat["state"], flat["step"], group["lr"], group["betas"], group["eps"],
+                       group["weight_decay"])
+        return loss
+
+    def state_dict(self) -> dict:
+        d = super().state_dict()
+        d["flat"] = [None if f is None else {"state": tuple(f["state"]), "step": f["step"]} for f in self._flat]
+        return d
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        flat = state_dict["flat"]
+        super().load_state_dict({k: v for k, v in state_dict.items() if k != "flat"})
+        self._flat = []
+        for group, f in zip(self.param_groups, flat):
+            if f is None:
+                self._flat.append(None)
+                continue
+            dev = group["params"][0].device
+            state = AdamWState(*(None if t is None else t.detach().to(dev, copy=True) for t in f["state"]))
+            need = sum(_blocks(p.numel()) for p in group["params"]) * WFB_ADAMW_BLOCK
+            if state.m.numel() != need:
+                raise ValueError(f"AdamW: the state has {state.m.numel()} elements, the group's tensors take {need}")
+            step = f["step"]
+            if group["capturable"]:
+                step = torch.as_tensor(step, dtype=torch.int64).reshape(1).to(dev, copy=True)
+            self._flat.append({"state": state, "step": step if group["capturable"] else int(step)})
