@@ -470,8 +470,8 @@ int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t 
 /* h [M, F] (h_dtype, rows contiguous) = act(gate) * up, gate|up = acc * w_scale * a_scale of the F gate rows and the F up
  * rows of qweight [2F, K/4] (scales_dev: their two fp32 scales), act WFB_ACT_SILU or WFB_ACT_RELU2, every product
  * rounded to fp32 as in wfb_linear_i2s and the gated activation as in wfb_linear_i2s_glu, then once to h_dtype.
- * gate_up fp32 [M, 2F] receives both products, which wfb_gated_grad takes; it may be NULL where
- * wfb_gated_i2s_workspace(M, F, K) is 0 (it holds that many floats otherwise).  act_codes int8 [M, lda], K % 128 == 0, rows
+ * gate_up fp32 [M, 2 Fp], Fp = F rounded up to a multiple of 64, receives both products (gate in columns 0 .. F - 1, up in
+ * Fp .. Fp + F - 1), which wfb_gated_grad takes; it may be NULL where wfb_gated_i2s_workspace(M, F, K) is 0.  act_codes int8 [M, lda], K % 128 == 0, rows
  * and bases 16-byte aligned.  The float product: WF/models/ffn.py:10-45. */
 int wfb_gated_i2s_workspace(int64_t m, int64_t f, int64_t k, int64_t* floats);
 int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* act_codes, int64_t m, int64_t lda,
@@ -482,8 +482,8 @@ int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* ac
  *   grad_x [M, K] = (d * w_scale) t,   grad_w [2F, K] = d^T (codes * a_scale)       (gate's rows before up's)
  * t the ternary weights, in fp32 arithmetic, each result rounded once to its type.  gate_up as wfb_gated_i2s left it;
  * grad_h [M, ldg]; qweight [2F, k_pad/4] 8-byte aligned; codes [M, lda].  grad_x or grad_w may be NULL.
- * Products run on the matrix cores: an fp32 operand enters in parts that hold 24 bits of it (grad_x of type fp32, grad_w
- * of type fp32), see csrc/gated.hip for the 16-bit results.  work: wfb_gated_grad_workspace bytes (host only; the
+ * d times its scale enters the products in 22 bits (11 where the result is bf16) down to 2^-18 (2^-28) of the largest of its
+ * row, see csrc/gated.hip.  work: wfb_gated_grad_workspace bytes (host only; the
  * same sizes, types and wanted results), 256-byte aligned. */
 int wfb_gated_grad_workspace(int64_t m, int64_t f, int64_t k, int gx_dtype, int want_x, int gw_dtype, int want_w,
                              int64_t* bytes);

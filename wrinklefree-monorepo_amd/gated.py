@@ -69,7 +69,7 @@ def _forward(x2: torch.Tensor, packed: PackedGated, act: str, keep: bool):
     f, kp, m, dev = n // 2, 4 * kb, x2.shape[0], x2.device
     q, a_scale = quantize_activations_i8_per_token(x2, k_pad=kp)
     h = torch.empty((m, f), dtype=x2.dtype, device=dev)
-    floats = 2 * f * m
+    floats = 2 * m * ((f + 63) // 64 * 64)
     if not keep and m:
         size = ctypes.c_int64(0)
         _lib.call("wfb_gated_i2s_workspace", m, f, kp, ctypes.addressof(size))
