@@ -248,6 +248,9 @@ int wfb_lm_head_argmax(const void* x, int x_dtype, int64_t ldx, const void* gamm
  * The angles of the stage-1 HF model's rotary embedding (WF/training/stage1.py:169-214; the reference
  * C engine has none, SGB/sgl-kernel/csrc/inference/bitnet_engine.cpp:381-441). */
 int wfb_rope_tables(double theta, int64_t head_dim, int64_t max_len, float* cos_out, float* sin_out);
+/* The same for any frequencies: cos / sin of p * inv_freq[i], i < pairs, times factor (contexts longer than trained). */
+int wfb_rope_tables_scaled(const double* inv_freq, int64_t pairs, double factor, int64_t max_len, float* cos_out,
+                           float* sin_out);
 
 /* ---- GQA decode attention over a KV cache (one new token per sequence) --------------------- */
 

@@ -741,6 +741,20 @@ int wfb_rope_tables(double theta, int64_t head_dim, int64_t max_len, float* cos_
   return ok();
 }
 
+int wfb_rope_tables_scaled(const double* inv_freq, int64_t pairs, double factor, int64_t max_len, float* cos_out,
+                           float* sin_out) {
+  const char* name = "wfb_rope_tables_scaled";
+  if (pairs < 1 || max_len < 1 || !(factor > 0.0)) return fail(WFB_EINVAL, "%s: bad pairs / max_len / factor", name);
+  if (!inv_freq || !cos_out || !sin_out) return fail(WFB_EINVAL, "%s: null pointer", name);
+  for (int64_t i = 0; i < pairs; ++i)
+    for (int64_t p = 0; p < max_len; ++p) {
+      const double a = (double)p * inv_freq[i];
+      cos_out[p * pairs + i] = (float)(std::cos(a) * factor);
+      sin_out[p * pairs + i] = (float)(std::sin(a) * factor);
+    }
+  return ok();
+}
+
 int wfb_kv_write_i8(const void* k_new, int64_t ldk, const void* v_new, int64_t ldv, int dtype, const float* rope_cos,
                     const float* rope_sin, int64_t rope_len, int64_t turn, const wfb_kv_i8* cache,
                     const int64_t* start_dev, int64_t start, const int64_t* lengths_dev, int64_t batch, int64_t t,
@@ -939,7 +953,7 @@ static int qk_rope_args(const char* name, const wfb_heads* q, const wfb_heads* k
   if (!aligned(rope->cos, 4) || !aligned(rope->sin, 4)) return fail(WFB_EINVAL, "%s: rotary tables must be 4-byte aligned", name);
   if (rope->pos && rope->pos_bytes != 4 && rope->pos_bytes != 8)
     return fail(WFB_EINVAL, "%s: positions must be int32 or int64", name);
-  if (!rope->pos && rope->rotary_dim > 0 && (rope->start < 0 || rope->start > rope->rope_len - t))
+  if (batch > 0 && t > 0 && !rope->pos && rope->rotary_dim > 0 && (rope->start < 0 || rope->start > rope->rope_len - t))
     return fail(WFB_EINVAL, "%s: positions %lld.. leave the rotary tables of %lld rows", name, (long long)rope->start, (long long)rope->rope_len);
   const wfb_heads* in[2] = {q, k};
   const size_t esz = dtype == WFB_F32 ? 4 : 2;

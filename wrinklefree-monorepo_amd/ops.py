@@ -17,8 +17,9 @@ from __future__ import annotations
 import collections
 import contextlib
 import ctypes
+import math
 import weakref
-from typing import NamedTuple, Optional, Sequence, Tuple, Union
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -855,16 +856,60 @@ def _rows2d(name: str, t: torch.Tensor, b: int, width: int) -> Tuple[torch.Tenso
     return t2, (t2.stride(0) if b > 1 else width)
 
 
-def rope_tables(theta: float, head_dim: int, max_len: int) -> Tuple[torch.Tensor, torch.Tensor]:
+def _scaled_frequencies(theta: float, head_dim: int, scaling: dict) -> Tuple[List[float], float]:
+    """(inverse frequencies, factor of the tables) of a rotary embedding scaled for longer contexts, in double precision."""
+    name = "rope_tables"
+    kind = scaling.get("rope_type", scaling.get("type"))
+    factor = float(scaling.get("factor", 1.0))
+    if not factor >= 1.0:
+        raise ValueError(f"{name}: scaling factor must be at least 1, not {factor}")
+    inv = [1.0 / theta ** (2 * i / head_dim) for i in range(head_dim // 2)]
+    if kind == "linear":  # positions divided by the factor
+        return [f / factor for f in inv], 1.0
+    length = float(scaling.get("original_max_position_embeddings", 0))
+    if kind in ("llama3", "yarn") and not length > 0:
+        raise ValueError(f"{name}: {kind} scaling needs original_max_position_embeddings")
+    if kind == "llama3":
+        # by the turns that a pair makes over the original length: few are slowed by the factor, many are left, and the
+        # weight runs linearly between
+        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        if not 0 < low < high:
+            raise ValueError(f"{name}: low_freq_factor must be positive and below high_freq_factor")
+        keep = [min(1.0, max(0.0, (length * f / (2 * math.pi) - low) / (high - low))) for f in inv]
+        return [f * w + f / factor * (1.0 - w) for f, w in zip(inv, keep)], 1.0
+    if kind == "yarn":
+        # the same by the pair's index, between the pairs that turn beta_fast and beta_slow times; the tables grow with
+        # the factor's logarithm
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        if not 0 < slow < fast:
+            raise ValueError(f"{name}: beta_slow must be positive and below beta_fast")
+        index = [head_dim * math.log(length / (b * 2 * math.pi)) / (2 * math.log(theta)) for b in (fast, slow)]
+        first, last = max(math.floor(index[0]), 0), min(math.ceil(index[1]), head_dim - 1)
+        span = max(last - first, 1e-3)
+        keep = [1.0 - min(1.0, max(0.0, (i - first) / span)) for i in range(head_dim // 2)]
+        mscale = scaling.get("attention_factor")
+        mscale = 0.1 * math.log(factor) + 1.0 if mscale is None else float(mscale)
+        return [f * w + f / factor * (1.0 - w) for f, w in zip(inv, keep)], mscale
+    raise ValueError(f"{name}: scaling type must be linear, llama3 or yarn, not {kind!r}")
+
+
+def rope_tables(theta: float, head_dim: int, max_len: int,
+                scaling: Optional[dict] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """cos / sin fp32 CPU tensors [max_len, head_dim/2] of the HF rotate-half rotary embedding at positions
     0..max_len-1 (angle p * theta^(-2i/head_dim) in double precision, rounded once to float): the tables
-    the decode / prefill attention kernels take, the same values the native engine computes."""
+    the decode / prefill attention kernels take, the same values the native engine computes.  ``head_dim`` is the number of
+    elements turned where that is only a part of a head (qk_norm_rope).  ``scaling`` is a model configuration's
+    ``rope_scaling`` of type linear, llama3 or yarn."""
     name = "rope_tables"
     if head_dim < 2 or head_dim % 2 != 0 or max_len < 1 or not theta > 0:
         raise ValueError(f"{name}: bad theta / head_dim / max_len")
     cos = torch.empty((max_len, head_dim // 2), dtype=torch.float32)
     sin = torch.empty_like(cos)
-    _lib.call("wfb_rope_tables", float(theta), head_dim, max_len, _p(cos), _p(sin))
+    if scaling is None:
+        _lib.call("wfb_rope_tables", float(theta), head_dim, max_len, _p(cos), _p(sin))
+    else:
+        inv, factor = _scaled_frequencies(float(theta), head_dim, scaling)
+        _lib.call("wfb_rope_tables_scaled", (ctypes.c_double * len(inv))(*inv), len(inv), factor, max_len, _p(cos), _p(sin))
     return cos, sin
 
 
