@@ -474,9 +474,8 @@ int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t 
  * rows of qweight [2F, K/4] (scales_dev: their two fp32 scales), act WFB_ACT_SILU or WFB_ACT_RELU2, every product
  * rounded to fp32 as in wfb_linear_i2s and the gated activation as in wfb_linear_i2s_glu, then once to h_dtype.
  * gate_up fp32 [M, 2 Fp], Fp = F rounded up to a multiple of 64, receives both products (gate in columns 0 .. F - 1, up in
- * Fp .. Fp + F - 1), which wfb_gated_grad takes; it may be NULL where wfb_gated_i2s_workspace(M, F, K) is 0.  act_codes int8 [M, lda], K % 128 == 0, rows
+ * Fp .. Fp + F - 1), which wfb_gated_grad takes, or is NULL.  act_codes int8 [M, lda], K % 128 == 0, rows
  * and bases 16-byte aligned.  The float product: WF/models/ffn.py:10-45. */
-int wfb_gated_i2s_workspace(int64_t m, int64_t f, int64_t k, int64_t* floats);
 int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* act_codes, int64_t m, int64_t lda,
                   const float* a_scale, const float* scales_dev, int act, void* h, int h_dtype, float* gate_up,
                   void* stream);

@@ -43,7 +43,6 @@ def test_gated_refusals(pkg):
 def test_gated_workspaces(pkg):
     n = ctypes.c_int64(-1)
     at = ctypes.addressof(n)
-    assert pkg._lib.status("wfb_gated_i2s_workspace", 100, 65, 256, at) == 0 and n.value in (0, 100 * 2 * 128)
     sizes = {}
     for want in ((1, 0), (0, 1), (1, 1)):
         assert pkg._lib.status("wfb_gated_grad_workspace", 100, 65, 200, 1, want[0], 0, want[1], at) == 0
@@ -52,7 +51,7 @@ def test_gated_workspaces(pkg):
     # two planes of d^T, 2 F rows of 128 tokens, and the codes at the least
     assert sizes[0, 1] >= 2 * 2 * 130 * 128 + 2 * 200 * 128
     assert pkg._lib.status("wfb_gated_grad_workspace", 0, 65, 200, 1, 1, 0, 1, at) == 0 and n.value == 0
-    _no(pkg, "null", pkg._lib.status("wfb_gated_i2s_workspace", 1, 1, 128, None))
+    _no(pkg, "null", pkg._lib.status("wfb_gated_grad_workspace", 1, 1, 1, 1, 1, 0, 1, None))
     _no(pkg, "dtype", pkg._lib.status("wfb_gated_grad_workspace", 1, 1, 1, 9, 1, 0, 1, at))
 
 

@@ -876,14 +876,6 @@ static int check_gated(const char* name, int64_t m, int64_t f, int64_t k) {
   return WFB_OK;
 }
 
-int wfb_gated_i2s_workspace(int64_t m, int64_t f, int64_t k, int64_t* floats) {
-  const char* name = "wfb_gated_i2s_workspace";
-  if (const int st = check_gated(name, m, f, k)) return st;
-  if (!floats) return fail(WFB_EINVAL, "%s: null pointer", name);
-  *floats = wfb::gated_workspace_floats(m, f, k);
-  return ok();
-}
-
 int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* act_codes, int64_t m, int64_t lda,
                   const float* a_scale, const float* scales_dev, int act, void* h, int h_dtype, float* gate_up,
                   void* stream) {
@@ -893,7 +885,7 @@ int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* ac
   if (act != WFB_ACT_SILU && act != WFB_ACT_RELU2) return fail(WFB_EINVAL, "%s: bad activation %d", name, act);
   if (!valid_dtype(h_dtype)) return fail(WFB_EINVAL, "%s: bad dtype %d", name, h_dtype);
   if (m == 0) return ok();
-  if (!qweight || !act_codes || !a_scale || !scales_dev || !h || (!gate_up && wfb::gated_workspace_floats(m, f, k)))
+  if (!qweight || !act_codes || !a_scale || !scales_dev || !h)
     return fail(WFB_EINVAL, "%s: null pointer", name);
   if (!aligned(qweight, 16) || !aligned(act_codes, 16) || !aligned(gate_up, 16) || !aligned(h, 16))
     return fail(WFB_EINVAL, "%s: qweight, codes, h and gate_up must be 16-byte aligned", name);

@@ -28,21 +28,6 @@ namespace {
 
 constexpr int64_t gated_pad(int64_t f) { return (f + 63) / 64 * 64; }  // columns of one product in gate_up
 
-__device__ __forceinline__ void store_as(void* o, int dt, int64_t i, float y) {
-  if (dt == WFB_F32) reinterpret_cast<float*>(o)[i] = y;
-  else if (dt == WFB_BF16) reinterpret_cast<uint16_t*>(o)[i] = f32_to_bf16_rne(y);
-  else reinterpret_cast<uint16_t*>(o)[i] = __builtin_bit_cast(uint16_t, (_Float16)y);
-}
-
-template <int ACT>
-__global__ __launch_bounds__(256) void gated_kernel(const float* __restrict__ gu, int64_t m, int64_t f,
-                                                    void* __restrict__ h, int h_dtype) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= m * f) return;
-  const int64_t row = i / f, col = i - row * f, fp = gated_pad(f);
-  store_as(h, h_dtype, i, glu<ACT>(gu[row * 2 * fp + col], gu[row * 2 * fp + fp + col]));
-}
-
 // ---- backward: what the layout kernels share -------------------------------------------------------
 
 struct GradSrc {
@@ -382,30 +367,23 @@ hipError_t launch_layouts(const GradSrc& src, const GradLayout& l, char* ws, hip
 
 }  // namespace
 
-int64_t gated_workspace_floats(int64_t m, int64_t f, int64_t k) { return m * 2 * gated_pad(f); }
-
+// Decode batches whose products nobody keeps take the decode kernels' gated epilogue, all else pair tiles.
 hipError_t launch_gated(const GatedForward& p, hipStream_t s) {
-  const int64_t fp = gated_pad(p.f);
-  for (int i = 0; i < 2; ++i) {
-    Epilogue e{};
-    e.nseg = 1;
-    e.a_scale = p.a_scale;
-    e.ws_dev = p.scales + i;
-    e.out = p.gate_up + i * fp;
-    e.out_dtype = WFB_F32;
-    e.ldo = 2 * fp;
-    const uint8_t* w = p.qw + i * p.f * (p.k / 4);
-    const bool gemv = p.m <= 2 && p.k <= 32768 && p.f * (p.k / 4) <= INT32_MAX && (p.m - 1) * p.lda + p.k <= INT32_MAX;
-    const hipError_t st = gemv ? launch_gemv_i2s(w, (int)p.f, (int)p.k, p.codes, (int)p.m, p.lda, e, s)
-                               : launch_gemm_i2s(w, (int)p.f, (int)p.k, p.codes, (int)p.m, p.lda, e, s);
-    if (st != hipSuccess) return st;
-  }
-  const unsigned grid = (unsigned)((p.m * p.f + 255) / 256);
-  if (p.act == WFB_ACT_SILU)
-    hipLaunchKernelGGL(gated_kernel<WFB_ACT_SILU>, dim3(grid), dim3(256), 0, s, p.gate_up, p.m, p.f, p.h, p.h_dtype);
-  else
-    hipLaunchKernelGGL(gated_kernel<WFB_ACT_RELU2>, dim3(grid), dim3(256), 0, s, p.gate_up, p.m, p.f, p.h, p.h_dtype);
-  return hipGetLastError();
+  Epilogue e{};
+  e.nseg = 2;
+  e.seg_end[0] = (int)p.f;
+  e.a_scale = p.a_scale;
+  e.ws_dev = p.scales;
+  e.out = p.h;
+  e.out_dtype = p.h_dtype;
+  e.ldo = p.f;
+  e.mid_dtype = WFB_F32;
+  e.gate_up = p.gate_up;
+  e.ldgu = 2 * gated_pad(p.f);
+  const int n = (int)(2 * p.f), k = (int)p.k, m = (int)p.m;
+  if (m <= 64 && !p.gate_up && p.f % 32 == 0 && (int64_t)n * (k / 4) <= INT32_MAX && (m - 1) * p.lda + k <= INT32_MAX)
+    return launch_gemm_i2s_glu(p.qw, n, k, p.codes, m, p.lda, p.act, e, s);
+  return launch_gemm_i2s_pair(p.qw, n, k, p.codes, m, p.lda, p.act, e, s);
 }
 
 int64_t gated_grad_workspace(const GatedGrad& p) { return grad_layout(p).bytes; }

@@ -235,7 +235,7 @@ __global__ __launch_bounds__(64 * S) void gemm_i2s_skinny_kernel(const uint8_t* 
           yg = bf16_bits_to_f32(f32_to_bf16_rne(yg));
           yu = bf16_bits_to_f32(f32_to_bf16_rne(yu));
         }
-        reinterpret_cast<float*>(ep.out)[(int64_t)tok * ep.ldo + n] = glu<GLUE>(yg, yu);
+        store_glu(ep, (int64_t)tok * ep.ldo + n, glu<GLUE>(yg, yu));
       }
     return;
   }
@@ -351,8 +351,11 @@ hipError_t launch_skinny(const uint8_t* W, int n, int C, const int8_t* A, int m,
 //    added after a coalesced 16-byte load, whole-line stores.  EPI = 0: any output type, bias,
 //    accumulator copy, stored from registers.
 //  * KSPL = 2..4: groups of four waves split the tile's K stages, their int32 partials added in LDS.
-//  * GL (gated gate|up, with KSPL = 2): 64 gate rows and their 64 up rows per tile; the fp32 output is
+//  * GL (gated gate|up) with TN = 1 and KSPL = 2: 64 gate rows and their 64 up rows per tile; the fp32 output is
 //    act(gate) * up, the up products handed to the gate waves through LDS.
+//  * GL with TN = 2 (pair tiles): a wave's two weight tiles are 32 gate rows and their 32 up rows, so a lane holds both
+//    products of an output.  They pass through the wave's LDS to lie in rows (as for EPI = 2); act(gate) * up is computed
+//    and stored in the output's type and, for a backward pass, both products are stored fp32 as well.
 constexpr int kGroupM = 8;
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -383,7 +386,10 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
   // GL (1 SiLU, 2 relu^2): W is gate|up (N = 2 * half); a tile's 128 weight rows are 64 gate rows n0 .. and
   // their up rows half + n0 .., loaded and multiplied by waves 0-1 and 2-3 (one wave's load instructions
   // cover the 32 rows it multiplies), and the epilogue stores act(gate) * up fp32 for 64 output columns
-  static_assert(GL == 0 || (TN == 1 && EPI == 0 && BI * (64 / BLPR) == 32), "gated tiles: 128 rows, 32 loaded per wave");
+  // (TN = 2: every wave has 32 gate rows as its first MFMA tile of columns and their up rows as its second)
+  constexpr bool PAIR = GL != 0 && TN == 2;
+  static_assert(GL == 0 || PAIR || (TN == 1 && EPI == 0 && BI * (64 / BLPR) == 32), "gated tiles: 128 rows, 32 loaded per wave");
+  static_assert(!PAIR || BI * (64 / BLPR) == 64, "pair tiles: a wave loads the rows that it multiplies");
   __shared__ __attribute__((aligned(16))) int8_t lds_a0s[KSPL][ASZ];
   __shared__ __attribute__((aligned(16))) int8_t lds_a1s[KSPL][ASZ];
   __shared__ __attribute__((aligned(16))) uint8_t lds_b0s[KSPL][BSZ];
@@ -415,8 +421,9 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
   const int mrows = min(BM, M - m0), nrows = GL ? min(BN / 2, half - n0) : min(BN, N - n0);
   const uint32_t a_end = (uint32_t)((int64_t)(mrows - 1) * lda + K), b_end = (uint32_t)nrows * row_bytes;
   const buf_t ab = make_buf(A + (int64_t)m0 * lda, a_end);
-  const int wrow0 = GL && wn >= 2 ? half + n0 : n0;  // first weight row this wave loads from (gated: up rows)
+  const int wrow0 = GL && !PAIR && wn >= 2 ? half + n0 : n0;  // first weight row this wave loads from (gated: up rows)
   const buf_t wb = make_buf(W + (int64_t)wrow0 * row_bytes, b_end);
+  const buf_t wb_up = PAIR ? make_buf(W + (int64_t)(half + n0) * row_bytes, b_end) : wb;
 
   // LDS position p of activation row r holds chunk p ^ aswz(r); position q of weight row R holds
   // 16-byte piece q ^ bswz(R).  (16 consecutive rows then fall on 16 distinct 16-byte bank groups.)
@@ -436,7 +443,8 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
 #pragma unroll
   for (int jj = 0; jj < BI; ++jj) {
     const int R = (64 / BLPR) * (BI * wn + jj) + l / BLPR;
-    const int Rl = GL && wn >= 2 ? R - BN / 2 : R;  // row within the block this wave loads from
+    // row within the block this wave loads from
+    const int Rl = PAIR ? 32 * wn + R % 32 : GL && wn >= 2 ? R - BN / 2 : R;
     b_row[jj] = (uint32_t)min(Rl, nrows - 1) * row_bytes;
     b_col[jj] = 16 * ((l % BLPR) ^ bswz(R));
   }
@@ -449,7 +457,7 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
 #pragma unroll
     for (int jj = 0; jj < BI; ++jj) {
       const uint32_t kb = (uint32_t)BROW * kt + b_col[jj];
-      lds_load16(wb, lb + (BI * wn + jj) * 1024, kb < row_bytes ? b_row[jj] + kb : b_end);
+      lds_load16(PAIR && 2 * jj >= BI ? wb_up : wb, lb + (BI * wn + jj) * 1024, kb < row_bytes ? b_row[jj] + kb : b_end);
     }
   };
 
@@ -628,7 +636,60 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
     }
   };
 
-  if constexpr (GL != 0) {
+  if constexpr (PAIR) {
+    // per 32-row MFMA tile: both products (32 rows x 32 columns fp32, 16-byte chunks XOR-swizzled by row) through this
+    // wave's own LDS buffer; a lane then takes 4 consecutive columns of a row of each
+    static_assert(ASZ >= 8192 && BSZ >= 8192, "both staged products fit one buffer");
+    float* st = wn == 0 ? reinterpret_cast<float*>(lds_a0)
+              : wn == 1 ? reinterpret_cast<float*>(lds_a1)
+              : wn == 2 ? reinterpret_cast<float*>(lds_b0) : reinterpret_cast<float*>(lds_b1);
+    const float ws[2] = {ep.ws_dev[0], ep.ws_dev[1]};
+    const int64_t up0 = ep.ldgu / 2;
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+      const int rs = rsum(tm * 32 + i);
+      const float as = epi_ascale(ep, min(m0 + tm * 32 + i, M - 1));
+#pragma unroll
+      for (int tn = 0; tn < 2; ++tn)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(__fmul_rn((float)(acc[tn][tm][4 * q + e] - rs), ws[tn]), as);
+          *reinterpret_cast<float4*>(st + tn * 1024 + i * 32 + (((2 * q + g) ^ (i & 7)) * 4)) =
+              make_float4(y[0], y[1], y[2], y[3]);
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 8 * j + (l >> 3), c = l & 7;
+        const float4 a = *reinterpret_cast<const float4*>(st + r * 32 + ((c ^ (r & 7)) * 4));
+        const float4 b = *reinterpret_cast<const float4*>(st + 1024 + r * 32 + ((c ^ (r & 7)) * 4));
+        const int m = m0 + tm * 32 + r, n = n0 + wn * 32 + 4 * c;
+        if (m >= M || n >= half) continue;
+        if (ep.gate_up) {  // (its rows are padded to whole groups of 4 columns)
+          float* gu = ep.gate_up + (int64_t)m * ep.ldgu + n;
+          *reinterpret_cast<float4*>(gu) = a;
+          *reinterpret_cast<float4*>(gu + up0) = b;
+        }
+        const float h[4] = {glu<GL>(a.x, b.x), glu<GL>(a.y, b.y), glu<GL>(a.z, b.z), glu<GL>(a.w, b.w)};
+        const int64_t off = (int64_t)m * ep.ldo + n;
+        if (!vec_out) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < half) store_glu(ep, off + e, h[e]);
+        } else if (ep.out_dtype == WFB_F32) {
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(ep.out) + off) = make_float4(h[0], h[1], h[2], h[3]);
+        } else {
+          union { uint16_t s[4]; uint2 q; } o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o.s[e] = ep.out_dtype == WFB_BF16 ? f32_to_bf16_rne(h[e]) : __builtin_bit_cast(uint16_t, (_Float16)h[e]);
+          *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(ep.out) + off) = o.q;
+        }
+      }
+    }
+    return;
+  } else if constexpr (GL != 0) {
     // up waves 2, 3 hand their rescaled products (rounded to ep.mid_dtype, as a plain linear stores them)
     // to gate waves 0, 1 through LDS; the gate waves store act(gate) * up (fp32) -- the skinny kernels'
     // gated epilogue, element for element
@@ -669,13 +730,13 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
           const float yg = mid(__fmul_rn(__fmul_rn((float)(acc[0][tm][4 * q + e] - rs), wsg), as));
           o4[e] = glu<GL>(yg, xf[((tm * 4 + q) * 4 + e) * 64 + l]);
         }
-        float* o = reinterpret_cast<float*>(ep.out) + (int64_t)m * ep.ldo + n;
+        const int64_t off = (int64_t)m * ep.ldo + n;
         if (vec_out && n + 3 < half) {
-          *reinterpret_cast<float4*>(o) = make_float4(o4[0], o4[1], o4[2], o4[3]);
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(ep.out) + off) = make_float4(o4[0], o4[1], o4[2], o4[3]);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (n + e < half) o[e] = o4[e];
+            if (n + e < half) store_glu(ep, off + e, o4[e]);
         }
       }
     }
@@ -857,9 +918,27 @@ hipError_t launch_tile_glu(const uint8_t* W, int n, int k, const int8_t* A, int 
   const int tiles_n = (half + 63) / 64, tiles_m = (m + 31) / 32;
   const int nwg = tiles_n * tiles_m;
   const int grid = ((nwg + 7) / 8) * 8;
-  const bool vec_out = e.ldo % 4 == 0 && (uintptr_t)e.out % 16 == 0;
+  const bool vec_out = e.out_dtype == WFB_F32 && e.ldo % 4 == 0 && (uintptr_t)e.out % 16 == 0;
   hipLaunchKernelGGL((gemm_i2s_tile_kernel<1, 2, 4, 0, 1, 2, GL>), dim3(grid), dim3(512), 0, s, W, A, lda, m, n, k,
                      tiles_m, tiles_n, nwg, vec_out, e);
+  return hipGetLastError();
+}
+
+// Gated gate|up as pair tiles: 32 TM tokens x 128 outputs.
+template <int TM, int KB, int OCC, int KSPL>
+hipError_t launch_tile_pair(const uint8_t* W, int n, int k, const int8_t* A, int m, int64_t lda, int act,
+                            const Epilogue& e, hipStream_t s) {
+  const int half = n / 2;
+  const int tiles_n = (half + 127) / 128, tiles_m = (m + 32 * TM - 1) / (32 * TM);
+  const int nwg = tiles_n * tiles_m;
+  const int grid = ((nwg + 7) / 8) * 8;
+  const bool vec_out = half % 4 == 0 && e.ldo % 4 == 0 && (uintptr_t)e.out % (e.out_dtype == WFB_F32 ? 16 : 8) == 0;
+  if (act == WFB_ACT_SILU)
+    hipLaunchKernelGGL((gemm_i2s_tile_kernel<TM, KB, OCC, 0, 2, KSPL, WFB_ACT_SILU>), dim3(grid), dim3(256 * KSPL), 0, s, W,
+                       A, lda, m, n, k, tiles_m, tiles_n, nwg, vec_out, e);
+  else
+    hipLaunchKernelGGL((gemm_i2s_tile_kernel<TM, KB, OCC, 0, 2, KSPL, WFB_ACT_RELU2>), dim3(grid), dim3(256 * KSPL), 0, s, W,
+                       A, lda, m, n, k, tiles_m, tiles_n, nwg, vec_out, e);
   return hipGetLastError();
 }
 
@@ -885,8 +964,7 @@ static hipError_t launch_token_halves(const uint8_t* W, int n, int k, const int8
   if (st != hipSuccess) return st;
   Epilogue e2 = e;
   if (e2.a_scale) e2.a_scale += 32;
-  // the gated product is stored fp32
-  if (e2.out) e2.out = static_cast<char*>(e2.out) + 32 * e2.ldo * (act || e2.out_dtype == WFB_F32 ? 4 : 2);
+  if (e2.out) e2.out = static_cast<char*>(e2.out) + 32 * e2.ldo * (e2.out_dtype == WFB_F32 ? 4 : 2);
   if (e2.acc_out) e2.acc_out += 32 * e2.ldo;
   if (e2.res) e2.res = static_cast<const char*>(e2.res) + 32 * e2.ldr * (e2.res_dtype == WFB_F32 ? 4 : 2);
   const hipError_t st2 = launch_skinny_lds(W, n, k, A + 32 * lda, m - 32, lda, e2, act, s);
@@ -941,6 +1019,17 @@ hipError_t launch_gemm_i2s_glu(const uint8_t* W, int n, int k, const int8_t* A, 
   if (m <= 16) WFB_GLU(1);
   WFB_GLU(2);
 #undef WFB_GLU
+}
+
+// The gated product of any number of tokens, with or without both products kept: the rules of launch_gemm_i2s for the same
+// 256 weight rows a tile.
+hipError_t launch_gemm_i2s_pair(const uint8_t* W, int n, int k, const int8_t* A, int m, int64_t lda, int act,
+                                const Epilogue& e, hipStream_t s) {
+  const int64_t tn = (n / 2 + 127) / 128, t128 = tn * ((m + 127) / 128), t64 = tn * ((m + 63) / 64), t32 = tn * ((m + 31) / 32);
+  if (t128 >= 320) return launch_tile_pair<4, 1, 2, 1>(W, n, k, A, m, lda, act, e, s);
+  if (t64 >= 160) return launch_tile_pair<2, 2, 2, 1>(W, n, k, A, m, lda, act, e, s);
+  if (t32 <= 256) return launch_tile_pair<1, 2, 3, 3>(W, n, k, A, m, lda, act, e, s);
+  return launch_tile_pair<1, 2, 3, 1>(W, n, k, A, m, lda, act, e, s);
 }
 
 hipError_t launch_gemm_i2s(const uint8_t* W, int n, int k, const int8_t* A, int m, int64_t lda, const Epilogue& e,

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(64 * S) void kernel(const uint8_t* __restrict__ W, 
       A += (int64_t)t0 * lda;
       M = min(MR, M - t0);
       if (ep.a_scale) ep.a_scale += t0;
-      if (ep.out) ep.out = static_cast<char*>(ep.out) + (int64_t)t0 * ep.ldo * (GLUE || ep.out_dtype == WFB_F32 ? 4 : 2);
+      if (ep.out) ep.out = static_cast<char*>(ep.out) + (int64_t)t0 * ep.ldo * (ep.out_dtype == WFB_F32 ? 4 : 2);
       if (ep.acc_out) ep.acc_out += (int64_t)t0 * ep.ldo;
       if (ep.res) ep.res = static_cast<const char*>(ep.res) + (int64_t)t0 * ep.ldr * (ep.res_dtype == WFB_F32 ? 4 : 2);
     }
@@ -541,7 +541,7 @@ __global__ __launch_bounds__(64 * S) void kernel(const uint8_t* __restrict__ W, 
         yg = bf16_bits_to_f32(f32_to_bf16_rne(yg));
         yu = bf16_bits_to_f32(f32_to_bf16_rne(yu));
       }
-      reinterpret_cast<float*>(ep.out)[(int64_t)tok * ep.ldo + n] = glu<GLUE>(yg, yu);
+      store_glu(ep, (int64_t)tok * ep.ldo + n, glu<GLUE>(yg, yu));
     }
     return;
   } else if constexpr (!STAGED) {

@@ -63,7 +63,7 @@ hipError_t launch_adamw_scalars(double lr, const float* lr_dev, double b1, doubl
                                 const int64_t* step_dev, AdamWScalars* out, hipStream_t s);
 hipError_t launch_adamw_values(const AdamWState& st, int64_t elements, float* m, float* v, hipStream_t s);
 
-// h [m, f] = act(gate) * up of the gate|up product of int8 codes; gate_up fp32 [m, 2f] takes both products.
+// h [m, f] = act(gate) * up of the gate|up product of int8 codes; gate_up takes both products, or is null.
 struct GatedForward {
   const uint8_t* qw;  // [2f, k / 4]
   int64_t f, k;
@@ -76,7 +76,6 @@ struct GatedForward {
   int h_dtype;
   float* gate_up;
 };
-int64_t gated_workspace_floats(int64_t m, int64_t f, int64_t k);
 hipError_t launch_gated(const GatedForward& p, hipStream_t s);
 
 struct GatedGrad {

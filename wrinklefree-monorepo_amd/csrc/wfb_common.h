@@ -194,6 +194,9 @@ struct Epilogue {
   int64_t ldr;
   // Gated (gate|up) epilogue only: the type the two products are rounded to before the activation.
   int mid_dtype;
+  // Gated pair tiles only: where both products go as well, [M][ldgu] fp32 with up at column ldgu / 2, or null.
+  float* gate_up;
+  int64_t ldgu;
 };
 
 __device__ __forceinline__ float epi_res(const Epilogue& e, int m, int n) {
@@ -230,6 +233,13 @@ __device__ __forceinline__ float glu(float g, float u) {
     const float r = fmaxf(g, 0.0f);
     return __fmul_rn(__fmul_rn(r, r), u);
   }
+}
+
+// Store of a gated product, rounded once to the output's type.
+__device__ __forceinline__ void store_glu(const Epilogue& e, int64_t off, float y) {
+  if (e.out_dtype == WFB_F32) reinterpret_cast<float*>(e.out)[off] = y;
+  else if (e.out_dtype == WFB_BF16) reinterpret_cast<uint16_t*>(e.out)[off] = f32_to_bf16_rne(y);
+  else reinterpret_cast<uint16_t*>(e.out)[off] = __builtin_bit_cast(uint16_t, (_Float16)y);
 }
 
 // Orderable 64-bit key of (value y, row n): larger y wins, and among equal values the smaller row
@@ -615,8 +625,11 @@ hipError_t launch_gemm_i2s_skinny(const uint8_t* W, int n, int k, const int8_t* 
 hipError_t launch_gemm_i2s(const uint8_t* W, int n, int k, const int8_t* A, int m, int64_t lda,
                            const Epilogue& e, hipStream_t s);
 // gate|up linear with the gated activation in its epilogue (M <= 64; n = 2 * half, half % 32 == 0;
-// fp32 output [M, half] at e.out / e.ldo)
+// output [M, half] of e.out_dtype at e.out / e.ldo)
 hipError_t launch_gemm_i2s_glu(const uint8_t* W, int n, int k, const int8_t* A, int m, int64_t lda, int act,
                                const Epilogue& e, hipStream_t s);
+// the same for any M and any half, the output in any type, with e.gate_up both products too; 127 * lda + K below 2^31
+hipError_t launch_gemm_i2s_pair(const uint8_t* W, int n, int k, const int8_t* A, int m, int64_t lda, int act,
+                                const Epilogue& e, hipStream_t s);
 
 }  // namespace wfb

@@ -69,12 +69,7 @@ def _forward(x2: torch.Tensor, packed: PackedGated, act: str, keep: bool):
     f, kp, m, dev = n // 2, 4 * kb, x2.shape[0], x2.device
     q, a_scale = quantize_activations_i8_per_token(x2, k_pad=kp)
     h = torch.empty((m, f), dtype=x2.dtype, device=dev)
-    floats = 2 * m * ((f + 63) // 64 * 64)
-    if not keep and m:
-        size = ctypes.c_int64(0)
-        _lib.call("wfb_gated_i2s_workspace", m, f, kp, ctypes.addressof(size))
-        floats = size.value
-    gate_up = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    gate_up = torch.empty(2 * m * ((f + 63) // 64 * 64), dtype=torch.float32, device=dev) if keep and m else None
     with _on(dev):
         _lib.call("wfb_gated_i2s", _p(packed.qweight), f, kp, _p(q), m, kp, _p(a_scale), _p(packed.scales), _ACTS[act],
                   _p(h), _DT[h.dtype], _p(gate_up), _stream(dev))
