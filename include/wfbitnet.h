@@ -470,6 +470,12 @@ int wfb_gqa_attention_i8(const void* q, int64_t ldq, const void* k_new, int64_t 
 
 /* ---- training step: gated feed-forward product ------------------------------------------------- */
 
+/* Both weight matrices [F, K] (w_dtype, rows contiguous) of a gated product ternarised and packed, each as
+ * wfb_weight_absmean and wfb_pack_i2s do: qweight uint8 [2F, k_pad/4], gate's rows first, k_pad = K rounded up to a multiple
+ * of 128 (zero weights), scales_dev fp32 [2].  workspace: 2 * WFB_ABSMEAN_WS_DOUBLES doubles. */
+int wfb_pack_gated(const void* gate, const void* up, int w_dtype, int64_t f, int64_t k, float* scales_dev, uint8_t* qweight,
+                   double* workspace, void* stream);
+
 /* h [M, F] (h_dtype, rows contiguous) = act(gate) * up, gate|up = acc * w_scale * a_scale of the F gate rows and the F up
  * rows of qweight [2F, K/4] (scales_dev: their two fp32 scales), act WFB_ACT_SILU or WFB_ACT_RELU2, every product
  * rounded to fp32 as in wfb_linear_i2s and the gated activation as in wfb_linear_i2s_glu, then once to h_dtype.

@@ -27,6 +27,14 @@ def test_gated_refusals(pkg):
         _no(pkg, match, fwd(**kw))
     assert fwd(m=0, qw=None) == 0
 
+    def pack(g=0x1000, u=0x2000, dt=0, f=64, k=200, s=0x100, q=0x3000, ws=0x4000):
+        return pkg._lib.status("wfb_pack_gated", vp(g), vp(u), dt, f, k, vp(s), vp(q), vp(ws), None)
+
+    for match, kw in (("sizes", dict(f=0)), ("sizes", dict(k=0)), ("2^20", dict(k=1 << 20)), ("dtype", dict(dt=3)),
+                      ("null", dict(u=None)), ("null", dict(ws=None)), ("misaligned", dict(q=0x3001)),
+                      ("misaligned", dict(ws=0x4004))):
+        _no(pkg, match, pack(**kw))
+
     def bwd(gu=0x1000, gh=0x2000, ghdt=1, ldg=64, m=4, f=64, act=1, qw=0x3000, k=200, kp=256, s=0x100, c=0x4000, lda=256,
             a=0x200, gx=0x5000, gxdt=1, gw=0x6000, gwdt=0, work=0x10000):
         return pkg._lib.status("wfb_gated_grad", vp(gu), vp(gh), ghdt, ldg, m, f, act, vp(qw), k, kp, vp(s), vp(c), lda, vp(a),

@@ -102,6 +102,7 @@ SIGNATURES = {
                                _int, _i64, _vp, _int, _i64, _vp],
     "wfb_rope_tables_scaled": [_vp, _i64, _f64, _i64, _vp, _vp],
     "wfb_rope_tables": [ctypes.c_double, _i64, _i64, _vp, _vp],
+    "wfb_pack_gated": [_vp, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp],
     "wfb_gated_i2s": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _int, _vp, _int, _vp, _vp],
     "wfb_gated_grad_workspace": [_i64, _i64, _i64, _int, _int, _int, _int, _vp],
     "wfb_gated_grad": [_vp, _vp, _int, _i64, _i64, _i64, _int, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _int,

@@ -876,6 +876,17 @@ static int check_gated(const char* name, int64_t m, int64_t f, int64_t k) {
   return WFB_OK;
 }
 
+int wfb_pack_gated(const void* gate, const void* up, int w_dtype, int64_t f, int64_t k, float* scales_dev, uint8_t* qweight,
+                   double* workspace, void* stream) {
+  const char* name = "wfb_pack_gated";
+  if (const int st = check_gated(name, 0, f, k)) return st;
+  if (!valid_dtype(w_dtype)) return fail(WFB_EINVAL, "%s: bad dtype %d", name, w_dtype);
+  if (!gate || !up || !scales_dev || !qweight || !workspace) return fail(WFB_EINVAL, "%s: null pointer", name);
+  if (!aligned(qweight, 4) || !aligned(workspace, 8)) return fail(WFB_EINVAL, "%s: misaligned qweight or workspace", name);
+  const int64_t kp = (k + WFB_QK_I2S - 1) / WFB_QK_I2S * WFB_QK_I2S;
+  return hip_status(wfb::launch_pack_pair(gate, up, w_dtype, f, k, kp, scales_dev, qweight, workspace, as_stream(stream)), name);
+}
+
 int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* act_codes, int64_t m, int64_t lda,
                   const float* a_scale, const float* scales_dev, int act, void* h, int h_dtype, float* gate_up,
                   void* stream) {

@@ -93,10 +93,9 @@ __device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0
 constexpr int kTopRows = 256;
 
 template <int ACT, int GDT>
-__global__ __launch_bounds__(256) void gated_top_kernel(GradSrc p, uint32_t* __restrict__ row_part,
-                                                        uint32_t* __restrict__ col_part) {
-  __shared__ uint32_t red[2][16][64];
-  const int cq = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = blockIdx.x * 64 + 4 * cq, m0 = blockIdx.y * kTopRows;
+__device__ __forceinline__ void gated_top(const GradSrc& p, int bx, int by, uint32_t* __restrict__ row_part,
+                                          uint32_t* __restrict__ col_part, uint32_t (&red)[2][16][64]) {
+  const int cq = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = bx * 64 + 4 * cq, m0 = by * kTopRows;
   const float w0 = p.scales[0], w1 = p.scales[1];
   uint32_t cg[4] = {0, 0, 0, 0}, cu[4] = {0, 0, 0, 0};
 #pragma unroll 4
@@ -116,18 +115,81 @@ __global__ __launch_bounds__(256) void gated_top_kernel(GradSrc p, uint32_t* __r
     top = max(top, (uint32_t)xor_lanes<2>((int)top));
     top = max(top, (uint32_t)xor_lanes<4>((int)top));
     top = max(top, (uint32_t)xor_lanes<8>((int)top));
-    if (cq == 0 && row < p.m) row_part[(int64_t)blockIdx.x * p.m + row] = top;
+    if (cq == 0 && row < p.m) row_part[(int64_t)bx * p.m + row] = top;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) red[0][r0][4 * cq + e] = cg[e], red[1][r0][4 * cq + e] = cu[e];
   __syncthreads();
   if (threadIdx.x < 128) {
-    const int half = threadIdx.x >> 6, i = threadIdx.x & 63, f = blockIdx.x * 64 + i;
+    const int half = threadIdx.x >> 6, i = threadIdx.x & 63, f = bx * 64 + i;
     uint32_t v = 0;
 #pragma unroll
     for (int k = 0; k < 16; ++k) v = max(v, red[half][k][i]);
-    if (f < p.f) col_part[(int64_t)blockIdx.y * 2 * p.f + half * p.f + f] = v;
+    if (f < p.f) col_part[(int64_t)by * 2 * p.f + half * p.f + f] = v;
   }
+}
+
+// I2_S codes of the 2f weight rows as fp16 {-1, 0, 1}, dst[k][2 fp]: row n of gate in column n, of up in column fp + n,
+// zeros between.  One 128-weight block of 64 rows per workgroup.
+__device__ __forceinline__ void gated_weights_t(const uint8_t* __restrict__ qw, int64_t row_bytes, int f, int fp, int K,
+                                                int bx, int b, uint16_t* __restrict__ dst, uint8_t (&tile)[64][36]) {
+  const int n0 = bx * 64;  // columns n0 .. n0 + 63 of dst lie in one half (fp % 64 == 0)
+  const int up = n0 >= fp, first = up ? n0 - fp : n0;
+  {
+    const int r = threadIdx.x >> 2, c8 = threadIdx.x & 3;  // 8 bytes of one row per thread
+    const int n = first + r;
+    const uint2 w = *reinterpret_cast<const uint2*>(qw + (int64_t)(up * f + min(n, f - 1)) * row_bytes + 32 * b + 8 * c8);
+    uint32_t* t = reinterpret_cast<uint32_t*>(&tile[r][8 * c8]);  // (code 1 = weight 0)
+    t[0] = n < f ? w.x : 0x55555555u;
+    t[1] = n < f ? w.y : 0x55555555u;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int idx = threadIdx.x + 256 * it, ch = idx & 7, kl = idx >> 3;  // 8 rows n of column kl
+    const int k = 128 * b + kl;
+    if (k >= K) continue;
+    const int j = kl & 31, sh = 6 - 2 * (kl >> 5);
+    union { uint16_t h[8]; uint4 q; } o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int code = (tile[8 * ch + e][j] >> sh) & 3;
+      o.h[e] = code == 0 ? 0xbc00u : code == 1 ? 0u : 0x3c00u;  // -1, 0, 1 in fp16
+    }
+    *reinterpret_cast<uint4*>(dst + (int64_t)k * 2 * fp + n0 + 8 * ch) = o.q;
+  }
+}
+
+// The first launch of the backward pass: the largest of d's rows and columns, and the operands that do not wait for
+// them, the transposed weights (columns x 64 by blocks of 128) and codes (tokens x 64 by columns x 64).
+struct Operands {
+  const uint8_t* qw;
+  int64_t row_bytes;
+  const int8_t* codes;
+  int64_t lda;
+  bool vec;  // codes' rows 16-byte aligned
+  int K, mp;
+  uint16_t *wt, *ct;  // null: not wanted
+  int tops, top_tiles, weights, weight_tiles, code_tiles;  // workgroups of each part, tiles of its first dimension
+};
+
+template <int ACT, int GDT>
+__global__ __launch_bounds__(256) void gated_top_kernel(GradSrc p, Operands o, uint32_t* __restrict__ row_part,
+                                                        uint32_t* __restrict__ col_part) {
+  __shared__ union {
+    uint32_t red[2][16][64];
+    __attribute__((aligned(4))) uint8_t w[64][36];
+    __attribute__((aligned(4))) int8_t c[64][68];
+  } lds;
+  int b = blockIdx.x;
+  if (b < o.tops) return gated_top<ACT, GDT>(p, b % o.top_tiles, b / o.top_tiles, row_part, col_part, lds.red);
+  b -= o.tops;
+  if (b < o.weights)
+    return gated_weights_t(o.qw, o.row_bytes, p.f, p.fp, o.K, b % o.weight_tiles, b / o.weight_tiles, o.wt, lds.w);
+  b -= o.weights;
+  const int m0 = b % o.code_tiles, k0 = b / o.code_tiles;
+  if (o.vec) codes_t<true, true>(o.codes, o.lda, p.m, o.K, o.mp, m0, k0, o.ct, lds.c);
+  else codes_t<false, true>(o.codes, o.lda, p.m, o.K, o.mp, m0, k0, o.ct, lds.c);
 }
 
 // What a row whose largest is `top` is multiplied by: the power of two that brings it into [2^14, 2^15), 2^126 at most; 1
@@ -238,38 +300,6 @@ __global__ __launch_bounds__(256) void gated_planes_kernel(GradSrc p, const floa
   }
 }
 
-// I2_S codes of the 2f weight rows as fp16 {-1, 0, 1}, dst[k][2 fp]: row n of gate in column n, of up in column fp + n,
-// zeros between.  One 128-weight block of 64 rows per workgroup.
-__global__ __launch_bounds__(256) void gated_weights_t_kernel(const uint8_t* __restrict__ qw, int64_t row_bytes, int f,
-                                                              int fp, int K, uint16_t* __restrict__ dst) {
-  __shared__ __attribute__((aligned(4))) uint8_t tile[64][36];
-  const int n0 = blockIdx.x * 64, b = blockIdx.y;  // columns n0 .. n0 + 63 of dst lie in one half (fp % 64 == 0)
-  const int up = n0 >= fp, first = up ? n0 - fp : n0;
-  {
-    const int r = threadIdx.x >> 2, c8 = threadIdx.x & 3;  // 8 bytes of one row per thread
-    const int n = first + r;
-    const uint2 w = *reinterpret_cast<const uint2*>(qw + (int64_t)(up * f + min(n, f - 1)) * row_bytes + 32 * b + 8 * c8);
-    uint32_t* t = reinterpret_cast<uint32_t*>(&tile[r][8 * c8]);  // (code 1 = weight 0)
-    t[0] = n < f ? w.x : 0x55555555u;
-    t[1] = n < f ? w.y : 0x55555555u;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int idx = threadIdx.x + 256 * it, ch = idx & 7, kl = idx >> 3;  // 8 rows n of column kl
-    const int k = 128 * b + kl;
-    if (k >= K) continue;
-    const int j = kl & 31, sh = 6 - 2 * (kl >> 5);
-    union { uint16_t h[8]; uint4 q; } o;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int code = (tile[8 * ch + e][j] >> sh) & 3;
-      o.h[e] = code == 0 ? 0xbc00u : code == 1 ? 0u : 0x3c00u;  // -1, 0, 1 in fp16
-    }
-    *reinterpret_cast<uint4*>(dst + (int64_t)k * 2 * fp + n0 + 8 * ch) = o.q;
-  }
-}
-
 constexpr Variant kVariants16[] = {{1, 256, 256, 64, 1, 1.20, 8},   {1, 128, 128, 64, 2, 1.05, 5},
                                    {1, 64, 128, 64, 3, 0.80, 3},    {2, 256, 256, 32, 1, 1.15, 8},
                                    {2, 128, 256, 32, 2, 1.10, 8},   {2, 64, 128, 32, 4, 0.85, 2.5}};
@@ -332,13 +362,13 @@ GradLayout grad_layout(const GatedGrad& p) {
 }
 
 template <int ACT, int GDT>
-hipError_t launch_layouts(const GradSrc& src, const GradLayout& l, char* ws, hipStream_t s) {
+hipError_t launch_layouts(const GradSrc& src, const Operands& ops, const GradLayout& l, char* ws, hipStream_t s) {
   auto* row_part = reinterpret_cast<uint32_t*>(ws + l.row_part);
   auto* col_part = reinterpret_cast<uint32_t*>(ws + l.col_part);
   auto* scale = reinterpret_cast<float*>(ws + l.scale);
   auto* inverse = reinterpret_cast<float*>(ws + l.inverse);
-  hipLaunchKernelGGL((gated_top_kernel<ACT, GDT>), dim3((unsigned)l.row_tiles, (unsigned)l.col_tiles), dim3(256), 0, s, src,
-                     row_part, col_part);
+  const int grid0 = ops.tops + ops.weights + (ops.ct ? ops.code_tiles * ((ops.K + 63) / 64) : 0);
+  hipLaunchKernelGGL((gated_top_kernel<ACT, GDT>), dim3(grid0), dim3(256), 0, s, src, ops, row_part, col_part);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int n = src.m + 2 * src.f;
@@ -394,20 +424,26 @@ hipError_t launch_gated_grad(const GatedGrad& p, void* work, hipStream_t s) {
   const int64_t esz = p.gh_dtype == WFB_F32 ? 16 : 8;
   const GradSrc src{p.gate_up, p.gh, p.ldg, (uintptr_t)p.gh % esz == 0 && p.ldg % 4 == 0, (int)p.m, (int)p.f, (int)l.fp,
                     p.scales, p.a_scale};
+  auto* bx = reinterpret_cast<uint16_t*>(ws + l.bx);
+  auto* bw = reinterpret_cast<uint16_t*>(ws + l.bw);
+  Operands ops{};
+  ops.qw = p.qw, ops.row_bytes = p.k_pad / 4;
+  ops.codes = p.codes, ops.lda = p.lda, ops.vec = (uintptr_t)p.codes % 16 == 0 && p.lda % 16 == 0;
+  ops.K = (int)p.k, ops.mp = (int)l.mp;
+  ops.wt = l.px ? bx : nullptr, ops.ct = l.pw ? bw : nullptr;
+  ops.top_tiles = (int)l.row_tiles, ops.tops = (int)(l.row_tiles * l.col_tiles);
+  ops.weight_tiles = (int)(2 * l.fp / 64), ops.weights = l.px ? ops.weight_tiles * (int)((p.k + 127) / 128) : 0;
+  ops.code_tiles = (int)(l.mp / 64);
   hipError_t e;
 #define WFB_LAYOUTS(ACT)                                                               \
-  (p.gh_dtype == WFB_F32    ? launch_layouts<ACT, WFB_F32>(src, l, ws, s)             \
-   : p.gh_dtype == WFB_BF16 ? launch_layouts<ACT, WFB_BF16>(src, l, ws, s)            \
-                            : launch_layouts<ACT, WFB_F16>(src, l, ws, s))
+  (p.gh_dtype == WFB_F32    ? launch_layouts<ACT, WFB_F32>(src, ops, l, ws, s)        \
+   : p.gh_dtype == WFB_BF16 ? launch_layouts<ACT, WFB_BF16>(src, ops, l, ws, s)       \
+                            : launch_layouts<ACT, WFB_F16>(src, ops, l, ws, s))
   e = p.act == WFB_ACT_SILU ? WFB_LAYOUTS(WFB_ACT_SILU) : WFB_LAYOUTS(WFB_ACT_RELU2);
 #undef WFB_LAYOUTS
   if (e != hipSuccess) return e;
   const float* inverse = reinterpret_cast<const float*>(ws + l.inverse);
   if (l.px) {
-    auto* bx = reinterpret_cast<uint16_t*>(ws + l.bx);
-    hipLaunchKernelGGL(gated_weights_t_kernel, dim3((unsigned)(2 * l.fp / 64), (unsigned)((p.k + 127) / 128)), dim3(256), 0,
-                       s, p.qw, p.k_pad / 4, (int)p.f, (int)l.fp, (int)p.k, bx);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
     GradGemm g{};
     g.a = reinterpret_cast<const uint16_t*>(ws + l.ax);
     g.lda = g.ldb = 2 * l.fp;
@@ -423,13 +459,6 @@ hipError_t launch_gated_grad(const GatedGrad& p, void* work, hipStream_t s) {
     if ((e = run_gemm16(g, l.plan_x, 2 * l.fp, reinterpret_cast<float*>(ws + l.parts_x), s)) != hipSuccess) return e;
   }
   if (l.pw) {
-    auto* bw = reinterpret_cast<uint16_t*>(ws + l.bw);
-    const dim3 gq((unsigned)(l.mp / 64), (unsigned)((p.k + 63) / 64));
-    if ((uintptr_t)p.codes % 16 == 0 && p.lda % 16 == 0)
-      hipLaunchKernelGGL((codes_t_kernel<true, true>), gq, dim3(256), 0, s, p.codes, p.lda, p.m, p.k, l.mp, bw);
-    else
-      hipLaunchKernelGGL((codes_t_kernel<false, true>), gq, dim3(256), 0, s, p.codes, p.lda, p.m, p.k, l.mp, bw);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
     GradGemm g{};
     g.a = reinterpret_cast<const uint16_t*>(ws + l.aw);
     g.lda = g.ldb = l.mp;

@@ -266,9 +266,9 @@ hipError_t launch_grad_w(const void* g, int gdt, int64_t ldg, int64_t m, int64_t
   if (bias_out && (e = launch_column_sum(sums, (int)(mp / 64), n, bias_out, bdt, s)) != hipSuccess) return e;
   const dim3 gq((unsigned)(mp / 64), (unsigned)((k + 63) / 64));
   if ((uintptr_t)q % 16 == 0 && ldq % 16 == 0)
-    hipLaunchKernelGGL((codes_t_kernel<true, false>), gq, dim3(256), 0, s, q, ldq, m, k, mp, qt);
+    hipLaunchKernelGGL((codes_t_kernel<true>), gq, dim3(256), 0, s, q, ldq, m, k, mp, qt);
   else
-    hipLaunchKernelGGL((codes_t_kernel<false, false>), gq, dim3(256), 0, s, q, ldq, m, k, mp, qt);
+    hipLaunchKernelGGL((codes_t_kernel<false>), gq, dim3(256), 0, s, q, ldq, m, k, mp, qt);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   GradGemm p{};
   p.a = gt;

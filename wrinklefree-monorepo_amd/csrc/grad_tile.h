@@ -38,10 +38,9 @@ __device__ __forceinline__ float scale_unit(float s) {
 // int8 codes q[m][k] as bf16 or fp16 (both exact) dst[k][m], rows of mp elements (m >= M: zeros).  VEC: 16 codes per load (rows 16-byte
 // aligned); a row's last codes, fewer than 16, one at a time: nothing has to lie behind the last row's.
 template <bool VEC, bool F16>
-__global__ __launch_bounds__(256) void codes_t_kernel(const int8_t* __restrict__ q, int64_t ldq, int64_t M, int64_t K,
-                                                      int64_t mp, uint16_t* __restrict__ dst) {
-  __shared__ __attribute__((aligned(4))) int8_t tile[64][68];
-  const int64_t m0 = (int64_t)blockIdx.x * 64, k0 = (int64_t)blockIdx.y * 64;
+__device__ __forceinline__ void codes_t(const int8_t* __restrict__ q, int64_t ldq, int64_t M, int64_t K, int64_t mp, int bx,
+                                        int by, uint16_t* __restrict__ dst, int8_t (&tile)[64][68]) {
+  const int64_t m0 = (int64_t)bx * 64, k0 = (int64_t)by * 64;
   const int r = threadIdx.x >> 2, c = 16 * (threadIdx.x & 3);  // 16 codes of row r
   const int64_t m = m0 + r, row = (m < M ? m : M - 1) * ldq;
   uint32_t v[4] = {0, 0, 0, 0};
@@ -74,6 +73,13 @@ __global__ __launch_bounds__(256) void codes_t_kernel(const int8_t* __restrict__
     }
     *reinterpret_cast<uint4*>(dst + k * mp + mo) = o.q4;
   }
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(256) void codes_t_kernel(const int8_t* __restrict__ q, int64_t ldq, int64_t M, int64_t K,
+                                                      int64_t mp, uint16_t* __restrict__ dst) {
+  __shared__ __attribute__((aligned(4))) int8_t tile[64][68];
+  codes_t<VEC, false>(q, ldq, M, K, mp, blockIdx.x, blockIdx.y, dst, tile);
 }
 
 typedef __attribute__((address_space(3))) void lds_void;

@@ -23,9 +23,8 @@ constexpr int kAbsBatch = 16, kAbsTail = 4;
 constexpr int64_t kStride = (int64_t)kAbsBlocks * 256;
 
 template <int DT, bool SMALL>
-__global__ __launch_bounds__(256) void absmean_partial_kernel(const void* __restrict__ w, int64_t numel,
-                                                              double* __restrict__ partial) {
-  __shared__ double red[256];
+__device__ __forceinline__ void absmean_partial(const void* __restrict__ w, int64_t numel, double* __restrict__ partial,
+                                                double (&red)[256]) {
   double acc = 0.0;
   int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if constexpr (SMALL) {
@@ -58,9 +57,23 @@ __global__ __launch_bounds__(256) void absmean_partial_kernel(const void* __rest
   if (threadIdx.x == 0) partial[blockIdx.x] = red[0];
 }
 
-__global__ __launch_bounds__(256) void absmean_final_kernel(const double* __restrict__ partial, int64_t numel,
-                                                            float* __restrict__ scale) {
+template <int DT, bool SMALL>
+__global__ __launch_bounds__(256) void absmean_partial_kernel(const void* __restrict__ w, int64_t numel,
+                                                              double* __restrict__ partial) {
   __shared__ double red[256];
+  absmean_partial<DT, SMALL>(w, numel, partial, red);
+}
+
+// The same of two matrices of one size, blockIdx.y.
+template <int DT, bool SMALL>
+__global__ __launch_bounds__(256) void absmean_pair_kernel(const void* __restrict__ w0, const void* __restrict__ w1,
+                                                           int64_t numel, double* __restrict__ partial) {
+  __shared__ double red[256];
+  absmean_partial<DT, SMALL>(blockIdx.y ? w1 : w0, numel, partial + blockIdx.y * kAbsBlocks, red);
+}
+
+// Stage 2, in one workgroup; the scale is thread 0's.
+__device__ __forceinline__ float absmean_final(const double* __restrict__ partial, int64_t numel, double (&red)[256]) {
   double acc = 0.0;
   for (int i = threadIdx.x; i < kAbsBlocks; i += 256) acc += partial[i];
   red[threadIdx.x] = acc;
@@ -69,11 +82,15 @@ __global__ __launch_bounds__(256) void absmean_final_kernel(const double* __rest
     if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    float s = numel > 0 ? (float)(red[0] / (double)numel) : 0.0f;
-    if ((double)s < 1e-8) s = 1.0f;
-    scale[0] = s;
-  }
+  const float s = numel > 0 ? (float)(red[0] / (double)numel) : 0.0f;
+  return (double)s < 1e-8 ? 1.0f : s;
+}
+
+__global__ __launch_bounds__(256) void absmean_final_kernel(const double* __restrict__ partial, int64_t numel,
+                                                            float* __restrict__ scale) {
+  __shared__ double red[256];
+  const float s = absmean_final(partial, numel, red);
+  if (threadIdx.x == 0) scale[0] = s;
 }
 
 // clamp(rint(w / s), -1, 1) + 1 of the correctly rounded quotient; NaN gives 0.
@@ -127,6 +144,50 @@ __global__ __launch_bounds__(256) void pack_i2s_kernel(const void* __restrict__ 
   qw[first + threadIdx.x] = out;
 }
 
+// Two matrices [n, k] at once (blockIdx.y), each behind its own stage 2 (every workgroup repeats that over 1024 partial
+// sums, 8 KB from L2, instead of a launch between), rows padded with zero weights from k to kp.  gate and up of 6912 x 2560
+// fp32 together with stage 1: PACKPAIRFIG.
+template <int DT>
+__global__ __launch_bounds__(256) void pack_pair_kernel(const void* __restrict__ w0, const void* __restrict__ w1, int64_t n,
+                                                        int64_t k, int64_t kp, const double* __restrict__ partial,
+                                                        float* __restrict__ scales, uint32_t* __restrict__ qw) {
+  __shared__ double red[256];
+  const int64_t dw_per_row = kp / 16, total = n * dw_per_row;
+  const void* w = blockIdx.y ? w1 : w0;
+  const int64_t first = (int64_t)blockIdx.x * 256, row0 = first / dw_per_row;
+  int64_t row = row0, p = first - row0 * dw_per_row + threadIdx.x;
+  if (dw_per_row < 256) {
+    row += (uint32_t)p / (uint32_t)dw_per_row;
+    p = (uint32_t)p % (uint32_t)dw_per_row;
+  } else if (p >= dw_per_row) {
+    row += 1;
+    p -= dw_per_row;
+  }
+  const int64_t c = 128 * (p >> 3) + (p & 7) * 4, base = (row < n ? row : n - 1) * k;
+  float v[4][4];  // requested before the sums, needed behind them
+#pragma unroll
+  for (int f = 0; f < 4; ++f)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int64_t col = c + 32 * f + t;
+      v[f][t] = load_elem<DT>(w, base + (col < k ? col : k - 1));
+    }
+  const float s = absmean_final(partial + blockIdx.y * kAbsBlocks, n * k, red);
+  if (blockIdx.x == 0 && threadIdx.x == 0) scales[blockIdx.y] = s;
+  if (row >= n) return;
+  const bool plain = s >= 0x1p-125f && s <= 0x1.fffffep127f;
+  const float h = 0.5f * s;
+  uint32_t out = 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const uint32_t code = plain ? ternary_code_half(v[f][t], h) : ternary_code(v[f][t], s);
+      out |= (c + 32 * f + t < k ? code : 1u) << (8 * t + 6 - 2 * f);
+    }
+  qw[blockIdx.y * total + first + threadIdx.x] = out;
+}
+
 __global__ __launch_bounds__(256) void unpack_i2s_kernel(const uint8_t* __restrict__ qw, int64_t n, int64_t k,
                                                          int8_t* __restrict__ out) {
   const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;  // one packed byte
@@ -161,7 +222,28 @@ hipError_t pack_t(const void* w, int64_t n, int64_t k, int64_t ldw, const float*
   return hipGetLastError();
 }
 
+template <int DT>
+hipError_t pack_pair_t(const void* w0, const void* w1, int64_t n, int64_t k, int64_t kp, float* scales, uint8_t* qw,
+                       double* ws, hipStream_t s) {
+  if (n * k <= 2 * kStride)
+    hipLaunchKernelGGL((absmean_pair_kernel<DT, true>), dim3(kAbsBlocks, 2), dim3(256), 0, s, w0, w1, n * k, ws);
+  else
+    hipLaunchKernelGGL((absmean_pair_kernel<DT, false>), dim3(kAbsBlocks, 2), dim3(256), 0, s, w0, w1, n * k, ws);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((pack_pair_kernel<DT>), dim3((unsigned)((n * (kp / 16) + 255) / 256), 2), dim3(256), 0, s, w0, w1, n, k,
+                     kp, ws, scales, reinterpret_cast<uint32_t*>(qw));
+  return hipGetLastError();
+}
+
 }  // namespace
+
+hipError_t launch_pack_pair(const void* w0, const void* w1, int dt, int64_t n, int64_t k, int64_t kp, float* scales,
+                            uint8_t* qw, double* ws, hipStream_t s) {
+  if (dt == WFB_F32) return pack_pair_t<WFB_F32>(w0, w1, n, k, kp, scales, qw, ws, s);
+  if (dt == WFB_BF16) return pack_pair_t<WFB_BF16>(w0, w1, n, k, kp, scales, qw, ws, s);
+  return pack_pair_t<WFB_F16>(w0, w1, n, k, kp, scales, qw, ws, s);
+}
 
 hipError_t launch_weight_absmean(const void* w, int dt, int64_t numel, float* scale, double* ws, hipStream_t s) {
   if (dt == WFB_F32) return absmean_t<WFB_F32>(w, numel, scale, ws, s);

@@ -487,6 +487,9 @@ __device__ __forceinline__ void epi_store4(const Epilogue& e, float ws, float as
 hipError_t launch_weight_absmean(const void* w, int dt, int64_t numel, float* scale, double* ws, hipStream_t s);
 hipError_t launch_pack_i2s(const void* w, int dt, int64_t n, int64_t k, int64_t ldw, const float* scale,
                            uint8_t* qw, hipStream_t s);
+// both matrices [n, k] of a gated product into qw [2n, kp / 4] with their own scales; ws: 2 WFB_ABSMEAN_WS_DOUBLES
+hipError_t launch_pack_pair(const void* w0, const void* w1, int dt, int64_t n, int64_t k, int64_t kp, float* scales,
+                            uint8_t* qw, double* ws, hipStream_t s);
 hipError_t launch_unpack_i2s(const uint8_t* qw, int64_t n, int64_t k, int8_t* out, hipStream_t s);
 // Straight-through gradients (grad.hip); workspace bytes of each.
 int64_t grad_x_workspace(int64_t m, int64_t n, int64_t k, int gdt);

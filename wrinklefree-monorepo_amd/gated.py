@@ -51,15 +51,9 @@ def pack_gated(gate_weight: torch.Tensor, up_weight: torch.Tensor) -> PackedGate
     dt = _DT[gate_weight.dtype]
     qweight = torch.empty((2 * f, kp // 4), dtype=torch.uint8, device=dev)
     scales = torch.empty(2, dtype=torch.float32, device=dev)
-    ws = torch.empty(WFB_ABSMEAN_WS_DOUBLES, dtype=torch.float64, device=dev)
+    ws = torch.empty(2 * WFB_ABSMEAN_WS_DOUBLES, dtype=torch.float64, device=dev)
     with _on(dev):
-        s = _stream(dev)
-        for i, w in enumerate((gate_weight, up_weight)):
-            _lib.call("wfb_weight_absmean", _p(w), dt, w.numel(), scales.data_ptr() + 4 * i, _p(ws), s)
-            if kp != k:
-                w = nn.functional.pad(w, (0, kp - k))
-            _lib.call("wfb_pack_i2s", _p(w), dt, f, kp, kp, scales.data_ptr() + 4 * i,
-                      qweight.data_ptr() + i * f * (kp // 4), s)
+        _lib.call("wfb_pack_gated", _p(gate_weight), _p(up_weight), dt, f, k, _p(scales), _p(qweight), _p(ws), _stream(dev))
     return PackedGated(qweight, scales)
 
 

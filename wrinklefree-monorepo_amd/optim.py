@@ -8,8 +8,8 @@ change in place and their version counters with them, so that a BitLinear over t
 
 from __future__ import annotations
 
-import ctypes
 from array import array
+from itertools import accumulate
 from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -88,32 +88,30 @@ def adamw_step(
     bits, dev = _check_state(name, state)
     if len(params) != len(grads):
         raise RuntimeError(f"{name}: {len(params)} tensors, {len(grads)} gradients")
-    kinds: dict = {}  # (p type, g type) -> rows of wfb_adamw_tensor
-    first, seen, written = 0, set(), []
-    for p, g in zip(params, grads):
-        n = p.numel()
-        if g is not None and n:
-            if p.device != dev or g.device != dev or g.shape != p.shape:
-                raise RuntimeError(f"{name}: a gradient has its tensor's shape, both are on {dev}")
-            if not p.is_contiguous() or g.is_neg():
-                raise RuntimeError(f"{name}: tensors must be contiguous")
-            if not g.is_contiguous():
-                g = g.contiguous()
-            at = p.data_ptr()
-            if at in seen:
-                raise RuntimeError(f"{name}: a tensor is given twice")
-            seen.add(at)
-            written.append(p)
-            rows = kinds.get((p.dtype, g.dtype))
-            if rows is None:
-                if p.dtype not in _DT or g.dtype not in _DT:
-                    raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {p.dtype} and {g.dtype}")
-                rows = kinds[(p.dtype, g.dtype)] = (array("q"), [])
-            rows[0].extend((at, g.data_ptr(), n, first))
-            rows[1].append(g)  # (a copy lives until the launch is in the stream)
-        first += _blocks(n) * WFB_ADAMW_BLOCK
-    if first != state.m.numel():
-        raise RuntimeError(f"{name}: the state has {state.m.numel()} elements, the tensors take {first}")
+    sizes = [p.numel() for p in params]
+    firsts = list(accumulate(((n + WFB_ADAMW_BLOCK - 1) // WFB_ADAMW_BLOCK * WFB_ADAMW_BLOCK for n in sizes), initial=0))
+    if firsts[-1] != state.m.numel():
+        raise RuntimeError(f"{name}: the state has {state.m.numel()} elements, the tensors take {firsts[-1]}")
+    live = [t for t in zip(params, grads, sizes, firsts) if t[1] is not None and t[2]]
+    # (a few calls a tensor are what a step over small tensors costs: 121 norms 138 us with attributes compared one by one,
+    # ADAMHOSTFIG so)
+    at = dev.index
+    if not all([p.is_same_size(g) and p.get_device() == at and g.get_device() == at for p, g, _, _ in live]):
+        raise RuntimeError(f"{name}: a gradient has its tensor's shape, both are on {dev}")
+    if not all([p.is_contiguous() and not p.is_neg() for p, _, _, _ in live]):
+        raise RuntimeError(f"{name}: tensors must be contiguous")
+    if not all([g.is_contiguous() and not g.is_neg() for _, g, _, _ in live]):
+        live = [(p, g.resolve_neg().contiguous(), n, f) for p, g, n, f in live]  # (copies live until the launch)
+    kinds = {(p.dtype, g.dtype) for p, g, _, _ in live}
+    tables = []
+    for pdt, gdt in kinds:
+        if pdt not in _DT or gdt not in _DT:
+            raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {pdt} and {gdt}")
+        rows = live if len(kinds) == 1 else [t for t in live if t[0].dtype == pdt and t[1].dtype == gdt]
+        # rows of wfb_adamw_tensor
+        tables.append((_DT[pdt], _DT[gdt], array("q", [x for p, g, n, f in rows for x in (p.data_ptr(), g.data_ptr(), n, f)])))
+    if sum(len(set(t[2][::4])) for t in tables) != len(live):
+        raise RuntimeError(f"{name}: a tensor is given twice")
     step_dev = lr_dev = scalars = None
     if isinstance(step, torch.Tensor):
         if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
@@ -126,13 +124,13 @@ def adamw_step(
         lr_dev, lr = lr.data_ptr(), 0.0
     m, v, ms, vs = state
     with _on(dev):
-        for (pdt, gdt), (rows, _) in kinds.items():
-            _lib.call("wfb_adamw_step", rows.buffer_info()[0], len(rows) // 4, _DT[pdt], _DT[gdt], m.data_ptr(),
+        for pdt, gdt, rows in tables:
+            _lib.call("wfb_adamw_step", rows.buffer_info()[0], len(rows) // 4, pdt, gdt, m.data_ptr(),
                       v.data_ptr(), None if ms is None else ms.data_ptr(), None if vs is None else vs.data_ptr(),
                       m.numel(), bits, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
                       int(step), step_dev, lr_dev, None if scalars is None else scalars.data_ptr(), _stream(dev))
-    if written:
-        torch.autograd.graph.increment_version(written)
+    if live:
+        torch.autograd.graph.increment_version([t[0] for t in live])
 
 
 def adamw_state_values(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -9,6 +9,7 @@ halves of a head, ``layout="half"``.  Tables come from :func:`rope_tables` or fr
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -25,25 +26,18 @@ Positions = Union[None, int, torch.Tensor]
 
 
 def _side(x: torch.Tensor, weight: Optional[torch.Tensor]) -> HeadsStruct:
-    s = HeadsStruct()
-    s.x = x.data_ptr()
-    s.stride_b, s.stride_t, s.stride_h = x.stride()[:3]
-    s.heads = x.shape[2]
-    if weight is not None:
-        s.weight, s.weight_dtype = weight.data_ptr(), _DT[weight.dtype]
-    return s
+    sb, st, sh, _ = x.stride()
+    w, wdt = (None, 0) if weight is None else (weight.data_ptr(), _DT[weight.dtype])
+    return HeadsStruct(x.data_ptr(), sb, st, sh, None, 0, 0, 0, w, wdt, None, None, x.shape[2])
 
 
 def _rope(cos: torch.Tensor, sin: torch.Tensor, positions: Positions, layout: str) -> RopeStruct:
-    r = RopeStruct()
-    r.cos, r.sin = cos.data_ptr(), sin.data_ptr()
-    r.rope_len, r.rotary_dim, r.interleaved = cos.shape[0], 2 * cos.shape[1], _LAYOUTS[layout]
+    n, half = cos.shape
     if isinstance(positions, torch.Tensor):
-        r.pos, r.pos_bytes = positions.data_ptr(), positions.element_size()
-        r.pos_stride_b, r.pos_stride_t = positions.stride()
+        where = (positions.data_ptr(), positions.element_size(), *positions.stride(), 0)
     else:
-        r.start = positions
-    return r
+        where = (None, 0, 0, 0, positions)
+    return RopeStruct(cos.data_ptr(), sin.data_ptr(), n, 2 * half, _LAYOUTS[layout], *where)
 
 
 def _forward(q, k, cos, sin, positions, wq, wk, eps, layout):
@@ -55,6 +49,14 @@ def _forward(q, k, cos, sin, positions, wq, wk, eps, layout):
         _lib.call("wfb_qk_norm_rope", ctypes.addressof(sq), ctypes.addressof(sk), ctypes.addressof(rope), _DT[q.dtype],
                   b, t, d, eps, _stream(q.device))
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _grad_workspace(*sizes: int) -> int:
+    """Floats that wfb_qk_norm_rope_grad works with at these sizes."""
+    n = ctypes.c_int64(0)
+    _lib.call("wfb_qk_norm_rope_grad_workspace", *sizes, ctypes.addressof(n))
+    return n.value
 
 
 class _QkNormRope(torch.autograd.Function):
@@ -90,9 +92,7 @@ class _QkNormRope(torch.autograd.Function):
             weights.append(gw)
         work = None
         if any(w is not None for w in weights):
-            size = ctypes.c_int64(0)
-            _lib.call("wfb_qk_norm_rope_grad_workspace", b, t, q.shape[2], k.shape[2], d, ctypes.addressof(size))
-            work = torch.empty(size.value, dtype=torch.float32, device=dev)
+            work = torch.empty(_grad_workspace(b, t, q.shape[2], k.shape[2], d), dtype=torch.float32, device=dev)
         with _on(dev):
             _lib.call("wfb_qk_norm_rope_grad", ctypes.addressof(sides[0][0]), ctypes.addressof(sides[1][0]),
                       ctypes.addressof(rope), _DT[q.dtype], b, t, d, eps, None if work is None else work.data_ptr(),
