@@ -182,7 +182,12 @@ __global__ __launch_bounds__(256) void gated_top_kernel(GradSrc p, Operands o, u
     __attribute__((aligned(4))) int8_t c[64][68];
   } lds;
   int b = blockIdx.x;
-  if (b < o.tops) return gated_top<ACT, GDT>(p, b % o.top_tiles, b / o.top_tiles, row_part, col_part, lds.red);
+  // (last tokens first: the products written last, the forward pass's, are still in the memory-side cache; the planes'
+  // kernel then begins with the first tokens, read last here)
+  if (b < o.tops) {
+    const int back = o.tops - 1 - b;
+    return gated_top<ACT, GDT>(p, back % o.top_tiles, back / o.top_tiles, row_part, col_part, lds.red);
+  }
   b -= o.tops;
   if (b < o.weights)
     return gated_weights_t(o.qw, o.row_bytes, p.f, p.fp, o.K, b % o.weight_tiles, b / o.weight_tiles, o.wt, lds.w);

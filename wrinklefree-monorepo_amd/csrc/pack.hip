@@ -144,48 +144,75 @@ __global__ __launch_bounds__(256) void pack_i2s_kernel(const void* __restrict__ 
   qw[first + threadIdx.x] = out;
 }
 
-// Two matrices [n, k] at once (blockIdx.y), each behind its own stage 2 (every workgroup repeats that over 1024 partial
-// sums, 8 KB from L2, instead of a launch between), rows padded with zero weights from k to kp.  gate and up of 6912 x 2560
-// fp32 together with stage 1: PACKPAIRFIG.
-template <int DT>
+// Two matrices [n, k] at once (blockIdx.y), rows padded with zero weights from k to kp, each behind its own stage 2: every
+// workgroup repeats that over the 1024 partial sums, 8 KB from L2, instead of a launch between, and packs `chunks` times 256
+// dwords behind it.  VEC: k % 4 == 0 and rows aligned to groups of four weights, one load each.
+template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void pack_pair_kernel(const void* __restrict__ w0, const void* __restrict__ w1, int64_t n,
                                                         int64_t k, int64_t kp, const double* __restrict__ partial,
-                                                        float* __restrict__ scales, uint32_t* __restrict__ qw) {
+                                                        float* __restrict__ scales, uint32_t* __restrict__ qw, int chunks) {
   __shared__ double red[256];
   const int64_t dw_per_row = kp / 16, total = n * dw_per_row;
   const void* w = blockIdx.y ? w1 : w0;
-  const int64_t first = (int64_t)blockIdx.x * 256, row0 = first / dw_per_row;
-  int64_t row = row0, p = first - row0 * dw_per_row + threadIdx.x;
-  if (dw_per_row < 256) {
-    row += (uint32_t)p / (uint32_t)dw_per_row;
-    p = (uint32_t)p % (uint32_t)dw_per_row;
-  } else if (p >= dw_per_row) {
-    row += 1;
-    p -= dw_per_row;
-  }
-  const int64_t c = 128 * (p >> 3) + (p & 7) * 4, base = (row < n ? row : n - 1) * k;
-  float v[4][4];  // requested before the sums, needed behind them
-#pragma unroll
-  for (int f = 0; f < 4; ++f)
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int64_t col = c + 32 * f + t;
-      v[f][t] = load_elem<DT>(w, base + (col < k ? col : k - 1));
+  float v[4][4];
+  int64_t c = 0;
+  auto load = [&](int64_t first) {  // (rows past the last one read it again)
+    const int64_t row0 = first / dw_per_row;
+    int64_t row = row0, p = first - row0 * dw_per_row + threadIdx.x;
+    if (dw_per_row < 256) {
+      row += (uint32_t)p / (uint32_t)dw_per_row;
+      p = (uint32_t)p % (uint32_t)dw_per_row;
+    } else if (p >= dw_per_row) {
+      row += 1;
+      p -= dw_per_row;
     }
-  const float s = absmean_final(partial + blockIdx.y * kAbsBlocks, n * k, red);
-  if (blockIdx.x == 0 && threadIdx.x == 0) scales[blockIdx.y] = s;
-  if (row >= n) return;
-  const bool plain = s >= 0x1p-125f && s <= 0x1.fffffep127f;
-  const float h = 0.5f * s;
-  uint32_t out = 0;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
+    c = 128 * (p >> 3) + (p & 7) * 4;
+    const int64_t base = (row < n ? row : n - 1) * k;
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
-      const uint32_t code = plain ? ternary_code_half(v[f][t], h) : ternary_code(v[f][t], s);
-      out |= (c + 32 * f + t < k ? code : 1u) << (8 * t + 6 - 2 * f);
+      const int64_t col = c + 32 * f;
+      if constexpr (VEC) {
+        const int64_t at = base + (col < k ? col : 0);
+        if constexpr (DT == WFB_F32) {
+          const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + at);
+          v[f][0] = x.x, v[f][1] = x.y, v[f][2] = x.z, v[f][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(w) + at);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint16_t b = (uint16_t)((t < 2 ? x.x : x.y) >> (16 * (t & 1)));
+            v[f][t] = DT == WFB_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[f][t] = load_elem<DT>(w, base + (col + t < k ? col + t : k - 1));
+      }
     }
-  qw[blockIdx.y * total + first + threadIdx.x] = out;
+  };
+  int64_t first = (int64_t)blockIdx.x * chunks * 256;
+  if (first >= total) return;
+  load(first);  // requested before the sums, needed behind them
+  const float s = absmean_final(partial + blockIdx.y * kAbsBlocks, n * k, red);
+  if (blockIdx.x == 0 && threadIdx.x == 0) scales[blockIdx.y] = s;
+  const bool plain = s >= 0x1p-125f && s <= 0x1.fffffep127f;
+  const float h = 0.5f * s;
+  for (int i = 0;;) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const uint32_t code = plain ? ternary_code_half(v[f][t], h) : ternary_code(v[f][t], s);
+        out |= (c + 32 * f + t < k ? code : 1u) << (8 * t + 6 - 2 * f);
+      }
+    const int64_t at = first + threadIdx.x;
+    first += 256;
+    const bool more = ++i < chunks && first < total;
+    if (more) load(first);
+    if (at < total) qw[blockIdx.y * total + at] = out;
+    if (!more) return;
+  }
 }
 
 __global__ __launch_bounds__(256) void unpack_i2s_kernel(const uint8_t* __restrict__ qw, int64_t n, int64_t k,
@@ -231,8 +258,17 @@ hipError_t pack_pair_t(const void* w0, const void* w1, int64_t n, int64_t k, int
     hipLaunchKernelGGL((absmean_pair_kernel<DT, false>), dim3(kAbsBlocks, 2), dim3(256), 0, s, w0, w1, n * k, ws);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((pack_pair_kernel<DT>), dim3((unsigned)((n * (kp / 16) + 255) / 256), 2), dim3(256), 0, s, w0, w1, n, k,
-                     kp, ws, scales, reinterpret_cast<uint32_t*>(qw));
+  // one chunk a workgroup while that leaves the chip room, else enough to have the sums repeated by about 2048 only
+  const int64_t all = (n * (kp / 16) + 255) / 256;
+  const int chunks = (int)(all <= 1024 ? 1 : (all + 1023) / 1024);
+  const unsigned grid = (unsigned)((all + chunks - 1) / chunks);
+  const int64_t bytes = DT == WFB_F32 ? 16 : 8;
+  if (k % 4 == 0 && (uintptr_t)w0 % bytes == 0 && (uintptr_t)w1 % bytes == 0)
+    hipLaunchKernelGGL((pack_pair_kernel<DT, true>), dim3(grid, 2), dim3(256), 0, s, w0, w1, n, k, kp, ws, scales,
+                       reinterpret_cast<uint32_t*>(qw), chunks);
+  else
+    hipLaunchKernelGGL((pack_pair_kernel<DT, false>), dim3(grid, 2), dim3(256), 0, s, w0, w1, n, k, kp, ws, scales,
+                       reinterpret_cast<uint32_t*>(qw), chunks);
   return hipGetLastError();
 }
 
