@@ -182,12 +182,7 @@ __global__ __launch_bounds__(256) void gated_top_kernel(GradSrc p, Operands o, u
     __attribute__((aligned(4))) int8_t c[64][68];
   } lds;
   int b = blockIdx.x;
-  // (last tokens first: the products written last, the forward pass's, are still in the memory-side cache; the planes'
-  // kernel then begins with the first tokens, read last here)
-  if (b < o.tops) {
-    const int back = o.tops - 1 - b;
-    return gated_top<ACT, GDT>(p, back % o.top_tiles, back / o.top_tiles, row_part, col_part, lds.red);
-  }
+  if (b < o.tops) return gated_top<ACT, GDT>(p, b % o.top_tiles, b / o.top_tiles, row_part, col_part, lds.red);
   b -= o.tops;
   if (b < o.weights)
     return gated_weights_t(o.qw, o.row_bytes, p.f, p.fp, o.K, b % o.weight_tiles, b / o.weight_tiles, o.wt, lds.w);
@@ -305,21 +300,23 @@ __global__ __launch_bounds__(256) void gated_planes_kernel(GradSrc p, const floa
   }
 }
 
-constexpr Variant kVariants16[] = {{1, 256, 256, 64, 1, 1.20, 8},   {1, 128, 128, 64, 2, 1.05, 5},
-                                   {1, 64, 128, 64, 3, 0.80, 3},    {2, 256, 256, 32, 1, 1.15, 8},
-                                   {2, 128, 256, 32, 2, 1.10, 8},   {2, 64, 128, 32, 4, 0.85, 2.5}};
+constexpr Variant kVariants16[] = {{1, 256, 256, 32, 1, 1.25, 12, 0.66}, {1, 256, 128, 64, 1, 1.25, 12, 0.66},
+                                   {1, 128, 128, 64, 2, 1.05, 5},         {1, 64, 128, 64, 3, 0.80, 3},
+                                   {2, 256, 256, 32, 1, 1.25, 10, 0.66},  {2, 128, 256, 32, 2, 1.10, 8},
+                                   {2, 64, 128, 32, 4, 0.85, 2.5}};
 constexpr int kNumVariants16 = sizeof(kVariants16) / sizeof(kVariants16[0]);
 
-Plan plan16(int planes, int64_t I, int64_t J, int64_t C) { return plan_of(kVariants16, kNumVariants16, planes, I, J, C); }
+Plan plan16(int planes, int64_t I, int64_t J, int64_t C) { return plan_of(kVariants16, kNumVariants16, planes, I, J, C, 0.45); }
 
 hipError_t run_gemm16(GradGemm p, const Plan& pl, int64_t C, float* parts, hipStream_t s) {
   set_plan(p, pl, kVariants16, C, parts);
   switch (pl.variant) {  // kVariants16
-    case 0: return launch_tiles<true, 1, 4, 2, 2, 4, 64, 2>(p, pl, s);
-    case 1: return launch_tiles<true, 1, 2, 2, 2, 2, 64, 2>(p, pl, s);
-    case 2: return launch_tiles<true, 1, 1, 2, 2, 2, 64, 3>(p, pl, s);
-    case 3: return launch_tiles<true, 2, 4, 2, 2, 4, 32, 2>(p, pl, s);
-    case 4: return launch_tiles<true, 2, 2, 4, 2, 2, 32, 2>(p, pl, s);
+    case 0: return launch_tiles<true, 1, 4, 2, 2, 4, 32, 2, 4>(p, pl, s);
+    case 1: return launch_tiles<true, 1, 4, 2, 2, 2, 64, 1, 3>(p, pl, s);
+    case 2: return launch_tiles<true, 1, 2, 2, 2, 2, 64, 2>(p, pl, s);
+    case 3: return launch_tiles<true, 1, 1, 2, 2, 2, 64, 3>(p, pl, s);
+    case 4: return launch_tiles<true, 2, 4, 2, 2, 4, 32, 2, 3>(p, pl, s);
+    case 5: return launch_tiles<true, 2, 2, 4, 2, 2, 32, 2>(p, pl, s);
     default: return launch_tiles<true, 2, 1, 2, 2, 2, 32, 4>(p, pl, s);
   }
 }

@@ -145,7 +145,8 @@ __device__ __forceinline__ void store8(const GradGemm& p, int64_t off, int col, 
 // index advances in stages of BK: the P planes' rows and the B rows of a stage go from global memory straight
 // into one of two LDS buffers (whole 64- or 128-byte row pieces, 16-byte chunks XOR-swizzled by row so that 16
 // rows at one chunk meet 16 distinct bank groups), the next stage's loads in flight while a stage is multiplied.
-template <bool F16, int P, int TI, int TJ, int WI, int WJ, int BK, int WPE>
+// ST = 3, 4: a ring of so many buffers instead, ST - 1 stages in flight; see below.
+template <bool F16, int P, int TI, int TJ, int WI, int WJ, int BK, int WPE, int ST = 2>
 __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void grad_tile_kernel(
     GradGemm p, int tiles_i, int tiles_j) {
   constexpr int W = WI * WJ, BI = 32 * TI * WI, BJ = 32 * TJ * WJ;
@@ -157,6 +158,8 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
   static_assert((P * BI / RPI / W) * W * RPI == P * BI && BI % RPI == 0, "a load stays in one plane");
   __shared__ __attribute__((aligned(16))) uint8_t lds0[SZ];
   __shared__ __attribute__((aligned(16))) uint8_t lds1[SZ];
+  __shared__ __attribute__((aligned(16))) uint8_t lds2[ST > 2 ? SZ : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t lds3[ST > 3 ? SZ : 16];
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = w / WJ, wj = w % WJ, i = l & 31, g = l >> 5;
 
@@ -169,9 +172,10 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
   constexpr int kGroup = 8;
   const int gsz = kGroup * tiles_j, grp = tt / gsz, rr = tt - grp * gsz;
   const int gm = min(kGroup, tiles_i - grp * kGroup);
-  const int i0 = (grp * kGroup + rr % gm) * BI, j0 = (rr / gm) * BJ;
+  const int i0 = __builtin_amdgcn_readfirstlane((grp * kGroup + rr % gm) * BI);
+  const int j0 = __builtin_amdgcn_readfirstlane((rr / gm) * BJ);
   const int per = whole ? p.stages : (p.stages + p.nsplit - 1) / p.nsplit;
-  const int s0 = split * per, s1 = min(s0 + per, p.stages);
+  const int s0 = __builtin_amdgcn_readfirstlane(split * per), s1 = __builtin_amdgcn_readfirstlane(min(s0 + per, p.stages));
 
   const int irows = min(BI, p.I - i0), jrows = min(BJ, p.J - j0);
   const uint32_t a_row = 2u * (uint32_t)p.lda, b_row = 2u * (uint32_t)p.ldb;
@@ -229,7 +233,7 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
       for (int ti = 0; ti < TI; ++ti)
         af[x & 1][q][ti] = *reinterpret_cast<const v8*>(lds + afr + (q * BI + ti * 32) * ROW + c);
   };
-  auto multiply = [&](int x, bool reads) {
+  auto multiply = [&](int x, bool reads, int loads = 0) {
 #pragma unroll
     for (int q = 0; q < P; ++q)
 #pragma unroll
@@ -243,6 +247,8 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
     for (int k = 0; k < P * TI * TJ; ++k) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       if (reads && k < TJ + P * TI) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (loads && k * loads / (P * TI * TJ) != (k + 1) * loads / (P * TI * TJ))
+        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -263,7 +269,89 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
     multiply(KS - 1, true);
   };
   static_assert(KS % 2 == 0, "a stage starts with fragment set 0");
-  if (s0 < s1) {
+  if constexpr (ST > 2) {
+    // Stage s: the loads of stage s + ST - 1 go into the buffer of stage s - 1, which every wave had read before the
+    // barrier at that stage's end.  Its own end waits, in every wave, until its reads of cur are done and all but the
+    // last ST - 2 stages' loads of this wave have landed, then for the others.  The count is fixed: stages past s1 are
+    // issued too, from past the operands' ends (zeros, no traffic).
+    constexpr int kOpen = (ST - 2) * (AI + NB), kWait = (kOpen & 15) | 0x70 | (kOpen >> 4 << 14);  // vmcnt, lgkmcnt(0)
+    static_assert(kOpen < 64, "vmcnt's range");
+    // loads [from, to) of a stage's AI + NB
+    auto load = [&](int s, uint8_t* lds, int from, int to) {
+      const bool on = s < s1;
+#pragma unroll
+      for (int jj = 0; jj < AI; ++jj) {
+        if (jj < from || jj >= to) continue;
+        const uint32_t col = (uint32_t)ROW * s + acol[jj];
+        lds_load16(ab[jj], lds + (AI * w + jj) * 1024, on && col < a_cols ? arow[jj] + col : a_end);
+      }
+#pragma unroll
+      for (int jj = 0; jj < NB; ++jj) {
+        if (AI + jj < from || AI + jj >= to) continue;
+        lds_load16(bb, lds + ASZ + (NB * w + jj) * 1024, on ? boff[jj] + (uint32_t)ROW * s : b_end);
+      }
+    };
+    constexpr int LP = (AI + NB + KS - 1) / KS;  // loads that go with one step's MFMAs
+    auto meet = [&] {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (orders the LDS accesses for the compiler)
+      __builtin_amdgcn_s_waitcnt(kWait);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    // stage s from cur, behind the last step of stage s - 1
+    auto ring = [&](int s, uint8_t* cur, uint8_t* last) {
+      meet();
+      read(cur, 0);
+      load(s + ST - 1, last, 0, LP);
+      multiply(KS - 1, true, LP);
+#pragma unroll
+      for (int x = 0; x + 1 < KS; ++x) {
+        read(cur, x + 1);
+        load(s + ST - 1, last, LP * (x + 1), LP * (x + 2));
+        multiply(x, true, min(AI + NB - LP * (x + 1), LP));
+      }
+    };
+    uint8_t* const b2 = ST > 2 ? lds2 : lds0;
+    uint8_t* const b3 = ST > 3 ? lds3 : lds0;
+    if (s0 < s1) {
+      load(s0, lds0, 0, AI + NB);
+      load(s0 + 1, lds1, 0, AI + NB);
+      if constexpr (ST > 3) load(s0 + 2, b2, 0, AI + NB);
+      meet();
+      read(lds0, 0);
+      load(s0 + ST - 1, ST > 3 ? b3 : b2, 0, AI + NB);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x + 1 < KS; ++x) {
+        read(lds0, x + 1);
+        multiply(x, true);
+      }
+      // (whole turns of the ring, then what is left: a loop that could end within a turn would have the compiler lose
+      // count of the loads in flight and wait for all of them once a turn)
+      int s = s0 + 1;
+      if constexpr (ST == 3) {
+        for (; s + 3 <= s1; s += 3) {
+          ring(s, lds1, lds0);
+          ring(s + 1, b2, lds1);
+          ring(s + 2, lds0, b2);
+        }
+        if (s < s1) ring(s, lds1, lds0);
+        if (s + 1 < s1) ring(s + 1, b2, lds1);
+      } else {
+        for (; s + 4 <= s1; s += 4) {
+          ring(s, lds1, lds0);
+          ring(s + 1, b2, lds1);
+          ring(s + 2, b3, b2);
+          ring(s + 3, lds0, b3);
+        }
+        if (s < s1) ring(s, lds1, lds0);
+        if (s + 1 < s1) ring(s + 1, b2, lds1);
+        if (s + 2 < s1) ring(s + 2, b3, b2);
+      }
+      multiply(KS - 1, false);
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // the last stages' zeros: the buffers are the epilogue's from here on
+    }
+  } else if (s0 < s1) {
     issue(s0, lds0);
     __builtin_amdgcn_s_waitcnt(0x0F70);
     __syncthreads();
@@ -281,10 +369,10 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
   // every wave) through this wave's LDS, 16-byte chunks XOR-swizzled by row; then 8 consecutive outputs of a row
   // per lane, whole lines per instruction
   constexpr int TS = 2 * (SZ / (4096 * TJ)) >= W ? TJ : TJ / 2;
-  constexpr int CPR = 8 * TS, ST = 32 * CPR * 16;  // chunks of a staged row, bytes a wave stages
-  constexpr int WPB = SZ / ST;                     // waves whose staging fits one buffer
+  constexpr int CPR = 8 * TS, STG = 32 * CPR * 16;  // chunks of a staged row, bytes a wave stages
+  constexpr int WPB = SZ / STG;                     // waves whose staging fits one buffer
   static_assert(TJ % TS == 0 && WPB >= 1 && 2 * WPB >= W, "staging fits the two operand buffers");
-  uint8_t* st = w < WPB ? lds0 + w * ST : lds1 + (w - WPB) * ST;
+  uint8_t* st = w < WPB ? lds0 + w * STG : lds1 + (w - WPB) * STG;
   float alpha = whole ? alpha_of(p) : 1.0f;
   constexpr int LPR = CPR / 2, RP = 64 / LPR;
   float* const part = whole ? nullptr : p.parts + (int64_t)u * (BI * BJ);
@@ -308,7 +396,8 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
               make_float4(v[4 * q] * alpha, v[4 * q + 1] * alpha, v[4 * q + 2] * alpha, v[4 * q + 3] * alpha);
         }
       wave_sync();
-#pragma unroll
+      constexpr int kStores = F16 ? 2 : 32 / RP;  // unrolled: whole, the stores' code is several times the products'
+#pragma unroll kStores
       for (int jj = 0; jj < 32 / RP; ++jj) {
         const int r = RP * jj + l / LPR, c8 = l % LPR;
         const float4 ya = *reinterpret_cast<const float4*>(st + (r * CPR + ((2 * c8) ^ (r & (CPR - 1)))) * 16);
@@ -356,6 +445,7 @@ constexpr int64_t pad_to(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 struct Variant {
   int planes, bi, bj, bk, per_cu;
   double rate, round_us;
+  double partial = 0.85;  // (one workgroup a CU) a round that leaves CUs idle, of a full one's time
 };
 
 // The first `full` tiles whole, the others in nsplit parts of the summed index, each a workgroup of its own.
@@ -371,7 +461,8 @@ struct Plan {
 // every (variant, split of all tiles) of 18 shapes from 1 x 576 x 576 to 4096^3, both products: the estimate's pick
 // is within 8% of the fastest on all but four, within 15% there.  Splitting only the tiles past the last full round
 // (28 of 540 at 2048 x 6912 x 2560) took grad_w there from 200 us and 26 for all tiles' sums to 180-189 and 7.
-inline Plan plan_of(const Variant* variants, int count, int planes, int64_t I, int64_t J, int64_t C) {
+// split_us: what each further part costs beside its traffic, the summing kernel's chain of loads.
+inline Plan plan_of(const Variant* variants, int count, int planes, int64_t I, int64_t J, int64_t C, double split_us = 0) {
   Plan best{-1, 0, 0, 1};
   double best_us = 0;
   for (int v = 0; v < count; ++v) {
@@ -383,7 +474,7 @@ inline Plan plan_of(const Variant* variants, int count, int planes, int64_t I, i
     auto rounds_us = [&](int64_t wgs, int64_t n) {  // wgs workgroups of n stages each
       const int64_t full = wgs / slots;
       const double r = (double)(wgs % slots) / slots;
-      const double last = r == 0 ? 0 : t.per_cu == 1 ? 0.85 : r * t.per_cu <= 1 ? 0.6 : 0.6 + 0.4 * r;
+      const double last = r == 0 ? 0 : t.per_cu == 1 ? t.partial : r * t.per_cu <= 1 ? 0.6 : 0.6 + 0.4 * r;
       return (full + last) * 2.0 * planes * t.bi * t.bj * n * t.bk / rate + t.round_us * (full + (r > 0));
     };
     auto consider = [&](int64_t full, int64_t ns, double us) {
@@ -396,7 +487,7 @@ inline Plan plan_of(const Variant* variants, int count, int planes, int64_t I, i
       for (const int64_t full : {(int64_t)0, tiles / slots * slots}) {
         const int64_t rest = tiles - full;
         if (rest == 0 || rest * ns > 4 * slots) continue;  // (no rest, or enough workgroups without so many parts)
-        const double sums = 4.0 + 8.0 * ns * rest * t.bi * t.bj / 8e6;
+        const double sums = 4.0 + split_us * ns + 8.0 * ns * rest * t.bi * t.bj / 8e6;
         consider(full, ns, (full ? rounds_us(full, stages) : 0) + rounds_us(rest * ns, per) + sums);
       }
     }
@@ -404,13 +495,13 @@ inline Plan plan_of(const Variant* variants, int count, int planes, int64_t I, i
   return best;
 }
 
-template <bool F16, int P, int TI, int TJ, int WI, int WJ, int BK, int WPE>
+template <bool F16, int P, int TI, int TJ, int WI, int WJ, int BK, int WPE, int ST = 2>
 hipError_t launch_tiles(const GradGemm& p, const Plan& pl, hipStream_t s) {
   constexpr int BI = 32 * TI * WI, BJ = 32 * TJ * WJ;
   const int ti = (p.I + BI - 1) / BI, tj = (p.J + BJ - 1) / BJ;
   const int64_t rest = pl.tiles - pl.full, grid = pad_to(pl.full, 8) + rest * pl.nsplit;
   if (grid > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((grad_tile_kernel<F16, P, TI, TJ, WI, WJ, BK, WPE>), dim3((unsigned)grid), dim3(64 * WI * WJ), 0, s, p,
+  hipLaunchKernelGGL((grad_tile_kernel<F16, P, TI, TJ, WI, WJ, BK, WPE, ST>), dim3((unsigned)grid), dim3(64 * WI * WJ), 0, s, p,
                      ti, tj);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || rest == 0) return e;

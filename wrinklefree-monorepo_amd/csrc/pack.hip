@@ -154,23 +154,22 @@ __global__ __launch_bounds__(256) void pack_pair_kernel(const void* __restrict__
   __shared__ double red[256];
   const int64_t dw_per_row = kp / 16, total = n * dw_per_row;
   const void* w = blockIdx.y ? w1 : w0;
+  int64_t first = (int64_t)blockIdx.x * chunks * 256;
+  if (first >= total) return;
+  // this thread's dword: p of `row`, and how far the next chunk's lies
+  const uint32_t dw = (uint32_t)dw_per_row, rows = 256u / dw, rest = 256u % dw;
+  const int64_t row0 = first / dw_per_row;
+  uint32_t p = (uint32_t)(first - row0 * dw_per_row) + threadIdx.x;
+  int64_t row = row0 + p / dw;
+  p %= dw;
   float v[4][4];
-  int64_t c = 0;
-  auto load = [&](int64_t first) {  // (rows past the last one read it again)
-    const int64_t row0 = first / dw_per_row;
-    int64_t row = row0, p = first - row0 * dw_per_row + threadIdx.x;
-    if (dw_per_row < 256) {
-      row += (uint32_t)p / (uint32_t)dw_per_row;
-      p = (uint32_t)p % (uint32_t)dw_per_row;
-    } else if (p >= dw_per_row) {
-      row += 1;
-      p -= dw_per_row;
-    }
-    c = 128 * (p >> 3) + (p & 7) * 4;
+  int c = 0;
+  auto load = [&] {  // (rows past the last one read it again)
+    c = 128 * (int)(p >> 3) + (int)(p & 7) * 4;
     const int64_t base = (row < n ? row : n - 1) * k;
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
-      const int64_t col = c + 32 * f;
+      const int col = c + 32 * f;
       if constexpr (VEC) {
         const int64_t at = base + (col < k ? col : 0);
         if constexpr (DT == WFB_F32) {
@@ -190,9 +189,7 @@ __global__ __launch_bounds__(256) void pack_pair_kernel(const void* __restrict__
       }
     }
   };
-  int64_t first = (int64_t)blockIdx.x * chunks * 256;
-  if (first >= total) return;
-  load(first);  // requested before the sums, needed behind them
+  load();  // requested before the sums, needed behind them
   const float s = absmean_final(partial + blockIdx.y * kAbsBlocks, n * k, red);
   if (blockIdx.x == 0 && threadIdx.x == 0) scales[blockIdx.y] = s;
   const bool plain = s >= 0x1p-125f && s <= 0x1.fffffep127f;
@@ -200,16 +197,25 @@ __global__ __launch_bounds__(256) void pack_pair_kernel(const void* __restrict__
   for (int i = 0;;) {
     uint32_t out = 0;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int f = 0; f < 4; ++f) {
+      uint32_t field = 0;
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
+      for (int t = 0; t < 4; ++t) {
         const uint32_t code = plain ? ternary_code_half(v[f][t], h) : ternary_code(v[f][t], s);
-        out |= (c + 32 * f + t < k ? code : 1u) << (8 * t + 6 - 2 * f);
+        field |= (VEC || c + 32 * f + t < k ? code : 1u) << (8 * t);
       }
+      if (VEC && c + 32 * f >= k) field = 0x01010101u;
+      out |= field << (6 - 2 * f);
+    }
     const int64_t at = first + threadIdx.x;
     first += 256;
     const bool more = ++i < chunks && first < total;
-    if (more) load(first);
+    if (more) {
+      row += rows;
+      p += rest;
+      if (p >= dw) p -= dw, row += 1;
+      load();
+    }
     if (at < total) qw[blockIdx.y * total + at] = out;
     if (!more) return;
   }
