@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void gated_planes_kernel(GradSrc p, const floa
   }
 }
 
-constexpr Variant kVariants16[] = {{1, 256, 256, 32, 1, 1.25, 12, 0.66}, {1, 256, 128, 64, 1, 1.25, 12, 0.66},
+constexpr Variant kVariants16[] = {{1, 256, 256, 32, 1, 1.22, 14, 0.95}, {1, 256, 128, 64, 1, 1.25, 12, 0.7},
                                    {1, 128, 128, 64, 2, 1.05, 5},         {1, 64, 128, 64, 3, 0.80, 3},
                                    {2, 256, 256, 32, 1, 1.25, 10, 0.66},  {2, 128, 256, 32, 2, 1.10, 8},
                                    {2, 64, 128, 32, 4, 0.85, 2.5}};
