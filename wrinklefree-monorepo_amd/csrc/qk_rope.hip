@@ -17,57 +17,54 @@ namespace {
 // Elements travel in chunks of V (one load each, 16 bytes where the sizes allow it).  Item j of a row is two chunks
 // that hold V whole pairs, chunk j of each half of the rotated part or two neighbours (interleaved layout); behind the
 // rotated part, two neighbours that pass.  A row takes L lanes (a power of two), IT items each.  A group of lanes walks
-// kHeads heads of one token, which share the angles.
+// kHeads heads of one token, which share the angles; all their loads are requested before the first is used, and stay as
+// they were loaded until they are.
 constexpr int kThreads = 256;
 constexpr int kHeads = 4;
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// V elements of type DT as the words they are loaded in (V = 1 of 16 bits: one half of a word).
 template <int DT, int V>
-__device__ __forceinline__ void load_chunk(const void* p, int64_t i, float* v) {
-  if constexpr (DT == WFB_F32) {
-    const float* q = reinterpret_cast<const float*>(p) + i;
-    if constexpr (V % 4 == 0) {
-#pragma unroll
-      for (int e = 0; e < V; e += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(q + e);
-        v[e] = x.x, v[e + 1] = x.y, v[e + 2] = x.z, v[e + 3] = x.w;
-      }
-    } else if constexpr (V == 2) {
-      const float2 x = *reinterpret_cast<const float2*>(q);
-      v[0] = x.x, v[1] = x.y;
+struct Chunk {
+  static constexpr int N = DT == WFB_F32 ? V : (V + 1) / 2;
+  uint32_t w[N];
+
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if constexpr (DT != WFB_F32 && V == 1) {
+      w[0] = reinterpret_cast<const uint16_t*>(p)[i];
     } else {
-      v[0] = q[0];
-    }
-  } else if constexpr (V == 1) {
-    v[0] = load_elem<DT>(p, i);
-  } else {
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + i;
-    uint32_t w[V / 2];
-    if constexpr (V == 8) {
-      const uint4 x = *reinterpret_cast<const uint4*>(q);
-      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    } else if constexpr (V == 4) {
-      const uint2 x = *reinterpret_cast<const uint2*>(q);
-      w[0] = x.x, w[1] = x.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(q);
-    }
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(p) + i * (DT == WFB_F32 ? 4 : 2));
+      if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int e = 0; e < V / 2; ++e) {
-      if constexpr (DT == WFB_BF16) {
-        v[2 * e] = __uint_as_float(w[e] << 16);
-        v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        for (int e = 0; e < N; e += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(q + e);
+          w[e] = x.x, w[e + 1] = x.y, w[e + 2] = x.z, w[e + 3] = x.w;
+        }
+      } else if constexpr (N == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(q);
+        w[0] = x.x, w[1] = x.y;
       } else {
-        v[2 * e] = f16_bits_to_f32((uint16_t)(w[e] & 0xffffu));
-        v[2 * e + 1] = f16_bits_to_f32((uint16_t)(w[e] >> 16));
+        w[0] = q[0];
       }
     }
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = 0;
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (DT == WFB_F32) return __uint_as_float(w[e]);
+    else if constexpr (DT == WFB_BF16) return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    else return f16_bits_to_f32((uint16_t)(w[e / 2] >> (16 * (e & 1))));
+  }
+};
 
 template <int DT>
-__device__ __forceinline__ uint32_t half_bits(float v) {
-  if constexpr (DT == WFB_BF16) return f32_to_bf16_rne(v);
-  else return __builtin_bit_cast(uint16_t, (_Float16)v);
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == WFB_BF16) return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+  else return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
 }
 
 template <int DT, int V>
@@ -83,21 +80,48 @@ __device__ __forceinline__ void store_chunk(void* p, int64_t i, const float* v) 
       q[0] = v[0];
     }
   } else if constexpr (V == 1) {
-    reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)half_bits<DT>(v[0]);
+    reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)pack2<DT>(v[0], 0.0f);
   } else {
     uint16_t* q = reinterpret_cast<uint16_t*>(p) + i;
     uint32_t w[V / 2];
 #pragma unroll
-    for (int e = 0; e < V / 2; ++e) w[e] = half_bits<DT>(v[2 * e]) | half_bits<DT>(v[2 * e + 1]) << 16;
+    for (int e = 0; e < V / 2; ++e) w[e] = pack2<DT>(v[2 * e], v[2 * e + 1]);
     if constexpr (V == 8) *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
     else if constexpr (V == 4) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(q) = w[0];
   }
 }
 
-__device__ __forceinline__ float load_weight(const void* w, int wdt, int i) {
-  if (wdt == WFB_F32) return load_elem<WFB_F32>(w, i);
-  return wdt == WFB_BF16 ? load_elem<WFB_BF16>(w, i) : load_elem<WFB_F16>(w, i);
+template <int WDT, int V>
+__device__ __forceinline__ void load_weight(const void* w, int ea, int eb, float (&v)[2 * V]) {
+  Chunk<WDT, V> a, b;
+  a.load(w, ea);
+  b.load(w, eb);
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = a.get(e), v[V + e] = b.get(e);
+}
+
+// The norm's weight for an item, ones without a norm.
+template <int V>
+__device__ __forceinline__ void item_weight(const HeadRows& s, bool on, int ea, int eb, float (&v)[2 * V]) {
+#pragma unroll
+  for (int e = 0; e < 2 * V; ++e) v[e] = 1.0f;
+  if (!s.w || !on) return;
+  if (s.wdt == WFB_F32) load_weight<WFB_F32, V>(s.w, ea, eb, v);
+  else if (s.wdt == WFB_BF16) load_weight<WFB_BF16, V>(s.w, ea, eb, v);
+  else load_weight<WFB_F16, V>(s.w, ea, eb, v);
+}
+
+// Sum over a row's L lanes, in every one of them.  (Lanes of other rows may be elsewhere: their side has no norm.)
+template <int L>
+__device__ __forceinline__ float row_sum(float v) {
+  if constexpr (L <= 16) {
+    return group_sum_f32<L>(v);
+  } else {
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+  }
 }
 
 // Where item j lies: its two chunks' first elements and its first pair, -1 behind the rotated part.
@@ -115,44 +139,40 @@ __device__ __forceinline__ void item_place(const QkRope& p, int j, int& ea, int&
   }
 }
 
-// The 2V elements x (chunk a, then chunk b) turned by the angles c, s; back: by their negatives.
+// The 2V elements x (chunk a, then chunk b) turned by the angles c, s (of the opposite sign to turn back).
 template <int V>
-__device__ __forceinline__ void turn(float (&x)[2 * V], const float (&c)[V], const float (&s)[V], bool interleaved,
-                                     bool back) {
+__device__ __forceinline__ void turn(float (&x)[2 * V], const float (&c)[V], const float (&s)[V], bool interleaved) {
   if (interleaved) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float sn = back ? -s[e] : s[e], a = x[2 * e], b = x[2 * e + 1];
-      x[2 * e] = a * c[e] - b * sn;
-      x[2 * e + 1] = b * c[e] + a * sn;
+      const float a = x[2 * e], b = x[2 * e + 1];
+      x[2 * e] = __builtin_fmaf(a, c[e], -(b * s[e]));
+      x[2 * e + 1] = __builtin_fmaf(b, c[e], a * s[e]);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float sn = back ? -s[e] : s[e], a = x[e], b = x[V + e];
-      x[e] = a * c[e] - b * sn;
-      x[V + e] = b * c[e] + a * sn;
+      const float a = x[e], b = x[V + e];
+      x[e] = __builtin_fmaf(a, c[e], -(b * s[e]));
+      x[V + e] = __builtin_fmaf(b, c[e], a * s[e]);
     }
   }
 }
 
 // What a group of lanes works on: kHeads heads from `head` on of one side at token (b, t).
 struct Task {
-  int side, head, count;
+  int head, count;
   int64_t b, t;
 };
 
-// (fewer than 2^31 tasks, host-checked: 32-bit divisions)
-__device__ __forceinline__ Task task_of(const QkRope& p, uint32_t i) {
-  const int cq = (p.side[0].heads + kHeads - 1) / kHeads, ck = (p.side[1].heads + kHeads - 1) / kHeads;
-  const uint32_t token = i / (uint32_t)(cq + ck), bi = token / (uint32_t)p.t;
-  const int c = (int)(i - token * (uint32_t)(cq + ck));
+// Task i of the tokens' groups of heads, `chunks` of them a token.  (fewer than 2^31 tasks, host-checked: 32-bit divisions)
+__device__ __forceinline__ Task task_of(uint32_t i, uint32_t chunks, int heads, uint32_t tokens) {
+  const uint32_t token = i / chunks, bi = token / tokens;
   Task k;
-  k.side = c >= cq;
-  k.head = (k.side ? c - cq : c) * kHeads;
-  k.count = min(kHeads, (k.side ? p.side[1].heads : p.side[0].heads) - k.head);
+  k.head = (int)(i - token * chunks) * kHeads;
+  k.count = min(kHeads, heads - k.head);
   k.b = bi;
-  k.t = token - bi * (uint32_t)p.t;
+  k.t = token - bi * tokens;
   return k;
 }
 
@@ -162,31 +182,36 @@ __device__ __forceinline__ int64_t position_of(const QkRope& p, const Task& k) {
   return p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[i] : reinterpret_cast<const int32_t*>(p.pos)[i];
 }
 
+// cos and sin of an item's pairs (1, 0 behind the rotated part).  A position that the tables do not hold reads nothing.
 template <int V>
-__device__ __forceinline__ void load_angles(const QkRope& p, int64_t at, int pair, float (&c)[V], float (&s)[V]) {
+__device__ __forceinline__ void load_angles(const QkRope& p, bool in, int64_t at, int pair, float (&c)[V], float (&s)[V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) c[e] = 1.0f, s[e] = 0.0f;
-  if (pair < 0) return;
-  if (at < 0 || at >= p.rope_len) {  // no such position: the row becomes NaN, and nothing is read
+  if (pair < 0 || !in) return;
+  Chunk<WFB_F32, V> x, y;
+  x.load(p.cos, at * (p.rotary / 2) + pair);
+  y.load(p.sin, at * (p.rotary / 2) + pair);
 #pragma unroll
-    for (int e = 0; e < V; ++e) c[e] = s[e] = __builtin_nanf("");
-    return;
-  }
-  load_chunk<WFB_F32, V>(p.cos, at * (p.rotary / 2) + pair, c);
-  load_chunk<WFB_F32, V>(p.sin, at * (p.rotary / 2) + pair, s);
+  for (int e = 0; e < V; ++e) c[e] = x.get(e), s[e] = y.get(e);
 }
 
+// Forward, both sides' tasks in one range, a token's queries before its keys.  655k heads of 128 in bf16 (16384 tokens, 32/8
+// heads): QKFWDFIG, against 70 us for a copy of the same bytes.
 template <int DT, int V, int L, int IT>
 __global__ __launch_bounds__(kThreads) void qk_rope_kernel(QkRope p, uint32_t tasks) {
   const int lane = threadIdx.x % L;
   const uint32_t i = blockIdx.x * (kThreads / L) + threadIdx.x / L;
   const bool live = i < tasks;
-  const Task k = task_of(p, live ? i : 0);
-  const HeadRows sd = k.side ? p.side[1] : p.side[0];
+  const uint32_t cq = (uint32_t)(p.side[0].heads + kHeads - 1) / kHeads, ck = (uint32_t)(p.side[1].heads + kHeads - 1) / kHeads;
+  Task k = task_of(live ? i : 0, cq + ck, INT32_MAX, (uint32_t)p.t);
+  const bool keys = (uint32_t)k.head >= cq * kHeads;
+  const HeadRows sd = keys ? p.side[1] : p.side[0];
+  k.head -= keys ? (int)cq * kHeads : 0;
+  k.count = min(kHeads, sd.heads - k.head);
   const int D = p.head_dim, items = D / (2 * V);
   const int64_t at = position_of(p, k);
-  const bool lost = p.rotary > 0 && (at < 0 || at >= p.rope_len);
-  float x[IT][kHeads][2 * V];
+  const bool in = at >= 0 && at < p.rope_len, lost = p.rotary > 0 && !in;
+  Chunk<DT, V> xa[IT][kHeads], xb[IT][kHeads];
   int ea[IT], eb[IT], pair[IT];
   bool on[IT];
   const int64_t row = k.b * sd.xb + k.t * sd.xt + k.head * sd.xh;
@@ -197,27 +222,19 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(QkRope p, uint32_t ta
     item_place<V>(p, on[it] ? j : 0, ea[it], eb[it], pair[it]);
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
-#pragma unroll
-      for (int e = 0; e < 2 * V; ++e) x[it][h][e] = 0.0f;
+      xa[it][h].zero();
+      xb[it][h].zero();
       if (on[it] && h < k.count) {
-        load_chunk<DT, V>(sd.x, row + h * sd.xh + ea[it], &x[it][h][0]);
-        load_chunk<DT, V>(sd.x, row + h * sd.xh + eb[it], &x[it][h][V]);
+        xa[it][h].load(sd.x, row + h * sd.xh + ea[it]);
+        xb[it][h].load(sd.x, row + h * sd.xh + eb[it]);
       }
     }
   }
   float w[IT][2 * V], c[IT][V], s[IT][V];
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
-    load_angles<V>(p, at, on[it] ? pair[it] : -1, c[it], s[it]);
-#pragma unroll
-    for (int e = 0; e < 2 * V; ++e) w[it][e] = 1.0f;
-    if (sd.w && on[it]) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        w[it][e] = load_weight(sd.w, sd.wdt, ea[it] + e);
-        w[it][V + e] = load_weight(sd.w, sd.wdt, eb[it] + e);
-      }
-    }
+    load_angles<V>(p, in, at, on[it] ? pair[it] : -1, c[it], s[it]);
+    item_weight<V>(sd, on[it], ea[it], eb[it], w[it]);
   }
 #pragma unroll
   for (int h = 0; h < kHeads; ++h) {
@@ -227,18 +244,22 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(QkRope p, uint32_t ta
 #pragma unroll
       for (int it = 0; it < IT; ++it)
 #pragma unroll
-        for (int e = 0; e < 2 * V; ++e) ss += x[it][h][e] * x[it][h][e];
-#pragma unroll
-      for (int o = 1; o < L; o <<= 1) ss += __shfl_xor(ss, o, 64);
-      r = 1.0f / sqrtf(ss / (float)D + p.eps);
+        for (int e = 0; e < V; ++e) {
+          ss = __builtin_fmaf(xa[it][h].get(e), xa[it][h].get(e), ss);
+          ss = __builtin_fmaf(xb[it][h].get(e), xb[it][h].get(e), ss);
+        }
+      r = __builtin_amdgcn_rsqf(row_sum<L>(ss) / (float)D + p.eps);
     }
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       if (!on[it] || h >= k.count) continue;
       float y[2 * V];
 #pragma unroll
-      for (int e = 0; e < 2 * V; ++e) y[e] = x[it][h][e] * r * w[it][e];
-      if (pair[it] >= 0) turn<V>(y, c[it], s[it], p.interleaved, false);
+      for (int e = 0; e < V; ++e) {
+        y[e] = xa[it][h].get(e) * r * w[it][e];
+        y[V + e] = xb[it][h].get(e) * r * w[it][V + e];
+      }
+      if (pair[it] >= 0) turn<V>(y, c[it], s[it], p.interleaved);
       if (lost) {
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) y[e] = __builtin_nanf("");
@@ -250,111 +271,111 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(QkRope p, uint32_t ta
   }
 }
 
+// Backward: the workgroups walk the queries' tasks, then the keys', and leave each side's part of the weight's gradient.
+// 205k heads of 128 in bf16 (8192 tokens, 20/5 heads): QKBWDFIG.
 template <int DT, int V, int L, int IT>
-__global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, uint32_t tasks, float* __restrict__ part) {
+__global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, float* __restrict__ part) {
   __shared__ float red[kThreads / L][2 * V * IT * L];
+  constexpr int G = kThreads / L;
   const int lane = threadIdx.x % L, grp = threadIdx.x / L;
   const int D = p.head_dim, items = D / (2 * V);
-  float acc[2][IT][2 * V];
-#pragma unroll
-  for (int sdx = 0; sdx < 2; ++sdx)
-#pragma unroll
-    for (int it = 0; it < IT; ++it)
-#pragma unroll
-      for (int e = 0; e < 2 * V; ++e) acc[sdx][it][e] = 0.0f;
   int ea[IT], eb[IT], pair[IT];
 #pragma unroll
   for (int it = 0; it < IT; ++it) item_place<V>(p, min(lane + L * it, items - 1), ea[it], eb[it], pair[it]);
 
-  // every group of the workgroup takes the same number of turns, so that the lanes of a wave stay together
-  constexpr int G = kThreads / L;
-  for (uint32_t i0 = blockIdx.x * G; i0 < tasks; i0 += gridDim.x * G) {
-    const bool live = i0 + grp < tasks;
-    const Task k = task_of(p, live ? i0 + grp : 0);
-    const HeadRows sd = k.side ? p.side[1] : p.side[0];
-    const int64_t at = position_of(p, k);
-    const bool lost = p.rotary > 0 && (at < 0 || at >= p.rope_len);
-    const int64_t row = k.b * sd.xb + k.t * sd.xt + k.head * sd.xh, grow = k.b * sd.gb + k.t * sd.gt + k.head * sd.gh;
-    float c[IT][V], s[IT][V], w[IT][2 * V];
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const HeadRows sd = side ? p.side[1] : p.side[0];
+    const uint32_t chunks = (uint32_t)(sd.heads + kHeads - 1) / kHeads, tasks = (uint32_t)(p.batch * p.t) * chunks;
+    float acc[IT][2 * V], w[IT][2 * V];
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
-      const bool on = live && lane + L * it < items;
-      load_angles<V>(p, at, on ? pair[it] : -1, c[it], s[it]);
+      item_weight<V>(sd, true, ea[it], eb[it], w[it]);
 #pragma unroll
-      for (int e = 0; e < 2 * V; ++e) w[it][e] = 1.0f;
-      if (sd.w && on) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          w[it][e] = load_weight(sd.w, sd.wdt, ea[it] + e);
-          w[it][V + e] = load_weight(sd.w, sd.wdt, eb[it] + e);
-        }
-      }
+      for (int e = 0; e < 2 * V; ++e) acc[it][e] = 0.0f;
     }
-#pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      float x[IT][2 * V], g[IT][2 * V];
-      float ss = 0.0f, sg = 0.0f;
+    // every group of the workgroup takes the same number of turns, so that the lanes of a wave stay together
+    for (uint32_t i0 = blockIdx.x * G; i0 < tasks; i0 += gridDim.x * G) {
+      const bool live = i0 + grp < tasks;
+      const Task k = task_of(live ? i0 + grp : 0, chunks, sd.heads, (uint32_t)p.t);
+      const int64_t at = position_of(p, k);
+      const bool in = at >= 0 && at < p.rope_len, lost = p.rotary > 0 && !in;
+      const int64_t row = k.b * sd.xb + k.t * sd.xt + k.head * sd.xh, grow = k.b * sd.gb + k.t * sd.gt + k.head * sd.gh;
+      Chunk<DT, V> xa[IT][kHeads], xb[IT][kHeads], ga[IT][kHeads], gb[IT][kHeads];
+      float c[IT][V], s[IT][V];
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
-        const bool on = live && lane + L * it < items && h < k.count;
+        const bool on = live && lane + L * it < items;
 #pragma unroll
-        for (int e = 0; e < 2 * V; ++e) x[it][e] = g[it][e] = 0.0f;
-        if (on) {
-          load_chunk<DT, V>(sd.g, grow + h * sd.gh + ea[it], &g[it][0]);
-          load_chunk<DT, V>(sd.g, grow + h * sd.gh + eb[it], &g[it][V]);
-          if (sd.w) {
-            load_chunk<DT, V>(sd.x, row + h * sd.xh + ea[it], &x[it][0]);
-            load_chunk<DT, V>(sd.x, row + h * sd.xh + eb[it], &x[it][V]);
+        for (int h = 0; h < kHeads; ++h) {
+          ga[it][h].zero(), gb[it][h].zero(), xa[it][h].zero(), xb[it][h].zero();
+          if (on && h < k.count) {
+            ga[it][h].load(sd.g, grow + h * sd.gh + ea[it]);
+            gb[it][h].load(sd.g, grow + h * sd.gh + eb[it]);
+            if (sd.w) {
+              xa[it][h].load(sd.x, row + h * sd.xh + ea[it]);
+              xb[it][h].load(sd.x, row + h * sd.xh + eb[it]);
+            }
           }
-          if (pair[it] >= 0) turn<V>(g[it], c[it], s[it], p.interleaved, true);
+        }
+        load_angles<V>(p, in, at, on ? pair[it] : -1, c[it], s[it]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[it][e] = -s[it][e];  // turned back
+      }
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        float g[IT][2 * V], ss = 0.0f, sg = 0.0f;
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) g[it][e] = ga[it][h].get(e), g[it][V + e] = gb[it][h].get(e);
+          if (pair[it] >= 0) turn<V>(g[it], c[it], s[it], p.interleaved);
           if (lost) {
 #pragma unroll
             for (int e = 0; e < 2 * V; ++e) g[it][e] = __builtin_nanf("");
           }
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float a = xa[it][h].get(e), b = xb[it][h].get(e);
+            ss = __builtin_fmaf(a, a, __builtin_fmaf(b, b, ss));
+            sg = __builtin_fmaf(g[it][e] * w[it][e], a, __builtin_fmaf(g[it][V + e] * w[it][V + e], b, sg));
+          }
+        }
+        float r = 1.0f, m = 0.0f;
+        if (sd.w) {
+          r = __builtin_amdgcn_rsqf(row_sum<L>(ss) / (float)D + p.eps);
+          m = r * (row_sum<L>(sg) / (float)D);
         }
 #pragma unroll
-        for (int e = 0; e < 2 * V; ++e) {
-          ss += x[it][e] * x[it][e];
-          sg += g[it][e] * w[it][e] * x[it][e];
-        }
-      }
-      float r = 1.0f, m = 0.0f;
-      if (sd.w) {
+        for (int it = 0; it < IT; ++it) {
+          const bool on = live && lane + L * it < items && h < k.count;
+          float y[2 * V];
+          if (sd.w) {
 #pragma unroll
-        for (int o = 1; o < L; o <<= 1) {
-          ss += __shfl_xor(ss, o, 64);
-          sg += __shfl_xor(sg, o, 64);
-        }
-        r = 1.0f / sqrtf(ss / (float)D + p.eps);
-        m = r * (sg / (float)D);
-      }
+            for (int e = 0; e < 2 * V; ++e) {
+              const float n = (e < V ? xa[it][h].get(e) : xb[it][h].get(e - V)) * r;
+              // (a row past the last one has g = x = 0; one without a position adds its NaN)
+              acc[it][e] = __builtin_fmaf(on ? g[it][e] : 0.0f, n, acc[it][e]);
+              y[e] = r * __builtin_fmaf(g[it][e], w[it][e], -(n * m));
+            }
+          } else {
 #pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        const bool on = live && lane + L * it < items && h < k.count;
-        float y[2 * V];
-#pragma unroll
-        for (int e = 0; e < 2 * V; ++e) {
-          const float n = x[it][e] * r, d = g[it][e] * n;
-          y[e] = sd.w ? r * (g[it][e] * w[it][e] - n * m) : g[it][e];
-          acc[0][it][e] += k.side ? 0.0f : d;
-          acc[1][it][e] += k.side ? d : 0.0f;
-        }
-        if (on && sd.out) {
-          const int64_t o = ((k.b * p.t + k.t) * sd.heads + k.head + h) * D;
-          store_chunk<DT, V>(sd.out, o + ea[it], &y[0]);
-          store_chunk<DT, V>(sd.out, o + eb[it], &y[V]);
+            for (int e = 0; e < 2 * V; ++e) y[e] = g[it][e];
+          }
+          if (on && sd.out) {
+            const int64_t o = ((k.b * p.t + k.t) * sd.heads + k.head + h) * D;
+            store_chunk<DT, V>(sd.out, o + ea[it], &y[0]);
+            store_chunk<DT, V>(sd.out, o + eb[it], &y[V]);
+          }
         }
       }
     }
-  }
-  if (!part) return;
-#pragma unroll
-  for (int sdx = 0; sdx < 2; ++sdx) {
-    if (sdx) __syncthreads();
+    if (!part) continue;
+    if (side) __syncthreads();  // the first side's sums are read
 #pragma unroll
     for (int it = 0; it < IT; ++it)
 #pragma unroll
-      for (int e = 0; e < 2 * V; ++e) red[grp][(it * 2 * V + e) * L + lane] = acc[sdx][it][e];
+      for (int e = 0; e < 2 * V; ++e) red[grp][(it * 2 * V + e) * L + lane] = acc[it][e];
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * V * IT * L; i += kThreads) {
       float v = 0.0f;
@@ -363,12 +384,12 @@ __global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, uint32
       if (j >= items) continue;
       int a, b, pr;
       item_place<V>(p, j, a, b, pr);
-      part[((int64_t)blockIdx.x * 2 + sdx) * D + (e < V ? a + e : b + e - V)] = v;
+      part[((int64_t)blockIdx.x * 2 + side) * D + (e < V ? a + e : b + e - V)] = v;
     }
   }
 }
 
-constexpr int kGradGroups = 512;
+constexpr int kGradGroups = 768;
 
 // The widest chunk that the sizes, strides and addresses allow: whole pairs on either side of the rotated part's end,
 // chunks that start at multiples of their length in every row, and in the tables' rows.
@@ -382,6 +403,8 @@ int chunk_of(const QkRope& p, int dtype, bool grad) {
     for (const HeadRows& s : p.side) {
       if (!whole(s.x, s.xb, s.xt, s.xh) || !whole(s.out, 0, 0, 0)) return false;
       if (grad && !whole(s.g, s.gb, s.gt, s.gh)) return false;
+      const int wv = v * (s.wdt == WFB_F32 ? 4 : 2);
+      if (s.w && (uintptr_t)s.w % (wv < 16 ? wv : 16) != 0) return false;
     }
     const int tv = v >= 4 ? 16 : 4 * v;
     return p.rotary == 0 || ((uintptr_t)p.cos % tv == 0 && (uintptr_t)p.sin % tv == 0);
@@ -393,12 +416,12 @@ int chunk_of(const QkRope& p, int dtype, bool grad) {
 
 template <int DT, int V, int L, int IT>
 hipError_t launch(const QkRope& p, bool grad, float* part, int groups, hipStream_t s) {
-  const int64_t tasks = qk_tasks(p);
   if (!grad) {
+    const int64_t tasks = qk_tasks(p);
     const int64_t grid = (tasks + kThreads / L - 1) / (kThreads / L);
     hipLaunchKernelGGL((qk_rope_kernel<DT, V, L, IT>), dim3((unsigned)grid), dim3(kThreads), 0, s, p, (uint32_t)tasks);
   } else {
-    hipLaunchKernelGGL((qk_rope_grad_kernel<DT, V, L, IT>), dim3((unsigned)groups), dim3(kThreads), 0, s, p, (uint32_t)tasks, part);
+    hipLaunchKernelGGL((qk_rope_grad_kernel<DT, V, L, IT>), dim3((unsigned)groups), dim3(kThreads), 0, s, p, part);
   }
   return hipGetLastError();
 }
