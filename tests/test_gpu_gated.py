@@ -213,6 +213,17 @@ def test_strides_and_leading_dimensions(pkg, dev):
     assert torch.equal(leaves[0].grad.reshape(24, 200), ones[1]) and torch.equal(leaves[2].grad, ones[3])
 
 
+def test_lazily_negated_operands(pkg, dev):
+    x, gate, up, gh = _case(dev, 12, 200, 72, F32, F32)
+    want = _run(pkg, -x, -gate, up, -gh, "silu")
+    neg = torch._neg_view
+    leaves = [neg(x).requires_grad_(), neg(gate).requires_grad_(), up.clone().requires_grad_()]
+    h = pkg.gated_bitlinear(*leaves, act="silu")
+    got = torch.autograd.grad(h, leaves, neg(gh))
+    assert torch.equal(h.detach(), want[0])
+    assert all(torch.equal(g.resolve_neg(), w) for g, w in zip(got, want[1:]))
+
+
 def test_another_stream_and_two_at_once(pkg, dev):
     a, b = (_case(dev, 200, 384, 320, BF16, F32, seed=s) for s in (1, 2))
     want = [_run(pkg, *c, "silu") for c in (a, b)]
@@ -263,6 +274,7 @@ def test_module(pkg, dev):
     with torch.no_grad():
         mod.up_proj.weight.mul_(-1.0)
     assert torch.equal(mod(x), -first) and mod.packed() is not pack
+    assert mod.pack() is mod and mod.packed() is not pack and torch.equal(mod(x), -first)
     twin = copy.deepcopy(mod)
     assert torch.equal(twin(x), -first)
     lin = [torch.nn.Linear(200, 96, bias=False, device=dev) for _ in range(2)]

@@ -187,6 +187,15 @@ def test_strides_alignment_and_broadcast(pkg, dev):
                        pkg.qk_norm_rope(one.contiguous(), k, cos, sin, None, wq, wk)[0])
 
 
+def test_lazily_negated_operands(pkg, dev):
+    q, k, wq, wk, gq, gk = _inputs(dev, 1, 5, 4, 2, 64, F32)
+    cos, sin = _tables(dev, 20, 64)
+    neg = torch._neg_view
+    a, ga = _run(pkg, -q, k, cos, sin, None, wq, wk, -gq, gk, "half")
+    b, gb = _run(pkg, neg(q.contiguous()), k, cos, sin, None, wq, wk, neg(gq), gk, "half")
+    assert all(torch.equal(x, y) for x, y in zip((*a, *ga), (*b, *(g.resolve_neg() for g in gb))))
+
+
 def test_offsets_past_32_bits(pkg, dev):
     d = 64
     buf = torch.zeros((1 << 31) + 4096, dtype=BF16, device=dev)

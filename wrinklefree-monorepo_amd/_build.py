@@ -82,7 +82,7 @@ def build_asan(verbose: bool = False) -> Path:
     """Host-code AddressSanitizer build for the CPU tests of the C ABI: the host-only sources (argument
     validation, dispatch, the engine's loader and state) compiled with ASan, linked with the kernel objects
     of the product build (run build() first) into _build/asan/libwfbitnet_asan.so, and the drivers
-    tests/asan/abi_driver.cpp and kv_i8_driver.cpp linked against it.  Returns the first driver's path."""
+    tests/asan/abi_driver.cpp, kv_i8_driver.cpp and train_ops_driver.cpp linked against it.  Returns the first driver's path."""
     hipcc = _hipcc()
     ASAN_DIR.mkdir(parents=True, exist_ok=True)
     host = ["--offload-host-only", "-O1", "-g", "-fPIC", "-std=c++17", "-Wno-unused-command-line-argument"]
@@ -102,7 +102,7 @@ def build_asan(verbose: bool = False) -> Path:
         objs.append(obj)
     lib = ASAN_DIR / "libwfbitnet_asan.so"
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *san, *map(str, objs), "-o", str(lib)])
-    for src in (ASAN_DRIVER_SRC, ASAN_DRIVER_SRC.with_name("kv_i8_driver.cpp")):
+    for src in (ASAN_DRIVER_SRC, *(ASAN_DRIVER_SRC.with_name(n) for n in ("kv_i8_driver.cpp", "train_ops_driver.cpp"))):
         dobj = ASAN_DIR / (src.stem + ".o")
         _run([hipcc, *host, *san, f"-I{PKG_DIR.parent / 'include'}", "-c", str(src), "-o", str(dobj)])
         _run([hipcc, "--offload-host-only", *san, str(dobj), f"-L{ASAN_DIR}", "-lwfbitnet_asan",

@@ -43,6 +43,7 @@ def pack_gated(gate_weight: torch.Tensor, up_weight: torch.Tensor) -> PackedGate
     :func:`pack_ternary_i2s` packs one; in_features is padded to a multiple of 128 with zero weights."""
     name = "pack_gated"
     _check_pair(name, gate_weight, up_weight)
+    gate_weight, up_weight = (w.detach().resolve_neg().contiguous() for w in (gate_weight, up_weight))
     dev = _require_gpu(name, gate_weight, up_weight)
     f, k = gate_weight.shape
     if f == 0 or k == 0:
@@ -90,7 +91,7 @@ class _GatedSTE(torch.autograd.Function):
         need_x, need_gate, need_up = ctx.needs_input_grad[:3]
         f, m, dev = qweight.shape[0] // 2, q.shape[0], q.device
         if gh.stride(-1) != 1 or gh.stride(0) < f or gh.is_neg():
-            gh = gh.contiguous()
+            gh = gh.resolve_neg().contiguous()
         need_w = need_gate or need_up
         gx = torch.empty((m, k), dtype=xdt, device=dev) if need_x else None
         gw = torch.empty((2 * f, k), dtype=wdt, device=dev) if need_w else None
@@ -138,7 +139,7 @@ def gated_bitlinear(
         if gate_weight.device != x.device or up_weight.device != x.device:
             raise RuntimeError(f"{_NAME}: weights must be on {x.device}")
     if packed is None:
-        packed = pack_gated(gate_weight.detach().contiguous(), up_weight.detach().contiguous())
+        packed = pack_gated(gate_weight, up_weight)
     else:
         qw, scales = packed
         _require_gpu(_NAME, qw, scales)
@@ -152,7 +153,7 @@ def gated_bitlinear(
     f = packed.qweight.shape[0] // 2
     x2 = x.reshape(-1, k) if k else x.new_empty((0, 0))
     if not x2.is_contiguous() or x2.is_neg():
-        x2 = x2.contiguous()
+        x2 = x2.resolve_neg().contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, gate_weight, up_weight)):
         if gate_weight is None:
             raise RuntimeError(f"{_NAME}: packed weights alone have no float weights to train")
@@ -192,9 +193,15 @@ class GatedBitLinear(nn.Module):
         """The weights' pack, rebuilt if a weight changed since the last one."""
         stamp = (self.gate_proj._weight_stamp(), self.up_proj._weight_stamp())
         if self._packed is None or self._packed_from != stamp:
-            self._packed = pack_gated(self.gate_proj.weight.detach().contiguous(), self.up_proj.weight.detach().contiguous())
+            self._packed = pack_gated(self.gate_proj.weight, self.up_proj.weight)
             self._packed_from = stamp
         return self._packed
+
+    def pack(self) -> "GatedBitLinear":
+        """Rebuild the pack whether or not the weights show a change (those that a replayed graph steps do not)."""
+        self._packed = None
+        self.packed()
+        return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         _check_lambda("GatedBitLinear")

@@ -83,7 +83,8 @@ def adamw_step(
     params fp32, bf16 or fp16 and their gradients, each of any of these types, contiguous, on one device; ``state`` of
     :func:`adamw_state` for the same list.  Decoupled weight decay; arithmetic in fp32, parameters rounded once.
     For a captured graph ``step`` is an int64 device tensor of one element, which the caller counts up, and ``lr`` may be an
-    fp32 one.  A gradient that is not finite spoils its own element, and in 8 bits the moments of its block of 256."""
+    fp32 one; a replay changes no version counters, so packs that modules keep outside the graph are renewed by their
+    ``pack()``.  No two tensors may share memory.  A gradient that is not finite spoils its own element, and in 8 bits the moments of its block of 256."""
     name = "adamw_step"
     bits, dev = _check_state(name, state)
     if len(params) != len(grads):

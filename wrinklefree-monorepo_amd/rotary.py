@@ -40,6 +40,11 @@ def _rope(cos: torch.Tensor, sin: torch.Tensor, positions: Positions, layout: st
     return RopeStruct(cos.data_ptr(), sin.data_ptr(), n, 2 * half, _LAYOUTS[layout], *where)
 
 
+def _plain(x: torch.Tensor) -> torch.Tensor:
+    """x with contiguous heads in its own memory, as the kernels read it."""
+    return x if x.stride(-1) == 1 and not x.is_neg() else x.resolve_neg().contiguous()
+
+
 def _forward(q, k, cos, sin, positions, wq, wk, eps, layout):
     b, t, _, d = q.shape
     out = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k)]
@@ -79,7 +84,7 @@ class _QkNormRope(torch.autograd.Function):
         rope = _rope(cos, sin, pos if pos is not None else start, layout)
         sides, grads, weights = [], [], []
         for x, w, g, need_x, need_w in ((q, wq, gq, need[0], need[2]), (k, wk, gk, need[1], need[3])):
-            g = g if g.stride(-1) == 1 and not g.is_neg() else g.contiguous()
+            g = _plain(g)
             s = _side(x, w)
             s.g = g.data_ptr()
             s.g_stride_b, s.g_stride_t, s.g_stride_h = g.stride()[:3]
@@ -149,7 +154,7 @@ def qk_norm_rope(
         positions = 0 if positions is None else int(positions)
         if cos.shape[1] and not 0 <= positions <= cos.shape[0] - t:
             raise ValueError(f"{_NAME}: positions {positions}..{positions + t - 1} leave tables of {cos.shape[0]} rows")
-    q, k = (x if x.stride(-1) == 1 and not x.is_neg() else x.contiguous() for x in (q, k))
+    q, k = _plain(q), _plain(k)
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
         out = _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), layout)
     else:
