@@ -548,8 +548,9 @@ int wfb_qk_norm_rope_grad(const wfb_heads* q, const wfb_heads* k, const wfb_rope
  * fp32 operation in this order, parameters rounded once to p_dtype:
  *   m = m b1 + g (1 - b1),  v = v b2 + (g g)(1 - b2),  r = sqrt(v)
  *   p = p (1 - lr wd) - (m (lr / (1 - b1^step))) / (r (1 / sqrt(1 - b2^step)) + eps)
- * The states lie in flat arrays of state_elements (a multiple of WFB_ADAMW_BLOCK); tensor i takes elements first ..
- * first + n - 1 of them, first a multiple of WFB_ADAMW_BLOCK, no two tensors the same block.  bits 32: m, v fp32.
+ * The states lie in flat arrays of state_elements (a multiple of WFB_ADAMW_BLOCK): every tensor takes n elements from a
+ * multiple of WFB_ADAMW_BLOCK on, one behind the other, all of them together; one with a null g is passed over, its
+ * state too.  bits 32: m, v fp32.
  * bits 8: m int8, v uint8 codes with m_scale, v_scale fp32 [state_elements / WFB_ADAMW_BLOCK], see csrc/adamw.hip.
  * step >= 1 on the host, or step_dev int64 [1] on the device (a captured graph's replays count it up there), for which
  * scalars holds WFB_ADAMW_SCALARS floats of device memory; lr_dev fp32 [1] or NULL goes with step_dev only.
@@ -559,7 +560,7 @@ int wfb_qk_norm_rope_grad(const wfb_heads* q, const wfb_heads* k, const wfb_rope
 typedef struct wfb_adamw_tensor {
   void* p;
   const void* g;
-  int64_t n, first;
+  int64_t n;
 } wfb_adamw_tensor;
 int wfb_adamw_step(const wfb_adamw_tensor* tensors, int64_t n_tensors, int p_dtype, int g_dtype, void* m, void* v,
                    float* m_scale, float* v_scale, int64_t state_elements, int bits, double lr, double beta1,

@@ -66,13 +66,13 @@ int main() {
   refused(wfb_rope_tables_scaled(inv, 0, 1.0, 6, cos.data(), sin.data()), "no pairs");
   refused(wfb_rope_tables_scaled(nullptr, 3, 1.0, 6, cos.data(), sin.data()), "null frequencies");
 
-  std::vector<wfb_adamw_tensor> t(200, wfb_adamw_tensor{x, x, 300, 0});
-  for (size_t i = 0; i < t.size(); ++i) t[i].first = 512 * (int64_t)i;
+  std::vector<wfb_adamw_tensor> t(200, wfb_adamw_tensor{x, x, 300});
   auto step = [&](int64_t elements, int bits, int64_t at) {
     return wfb_adamw_step(t.data(), (int64_t)t.size(), WFB_F32, WFB_F32, x, x, bits == 8 ? x : nullptr, bits == 8 ? x : nullptr,
                           elements, bits, 1e-3, 0.9, 0.99, 1e-8, 0.0, at, nullptr, nullptr, nullptr, nullptr);
   };
   refused(step(512 * 199, 32, 1), "the last tensor leaves the state");
+  refused(step(512 * 201, 32, 1), "the state is larger");
   refused(step(512 * 200, 16, 1), "bits");
   refused(step(512 * 200, 8, 0), "step");
   t[150].p = nullptr;

@@ -115,7 +115,7 @@ def test_qk_refusals(pkg):
 
 
 def test_adamw_refusals(pkg):
-    def call(rows=((0x1000, 0x2000, 300, 0),), pdt=0, gdt=1, m=0x3000, v=0x4000, ms=0x100, vs=0x200, n=512, bits=8, lr=1e-3,
+    def call(rows=((0x1000, 0x2000, 300),), pdt=0, gdt=1, m=0x3000, v=0x4000, ms=0x100, vs=0x200, n=512, bits=8, lr=1e-3,
              b1=0.9, b2=0.99, eps=1e-8, wd=0.0, step=1, step_dev=None, lr_dev=None, scalars=None, tensors=True):
         flat = [x for r in rows for x in r]
         table = (ctypes.c_int64 * max(1, len(flat)))(*flat)
@@ -130,14 +130,14 @@ def test_adamw_refusals(pkg):
                       ("betas", dict(b1=1.0)), ("betas", dict(b2=-0.1)), ("betas", dict(b1=math.nan)),
                       ("negative", dict(lr=-1.0)), ("negative", dict(eps=-1.0)), ("negative", dict(wd=math.nan)),
                       ("steps", dict(step=0)), ("device step", dict(lr_dev=0x100)), ("scalars", dict(step_dev=0x100)),
-                      ("leaves the state", dict(rows=((0x1000, 0x2000, 513, 0),))),
-                      ("leaves the state", dict(rows=((0x1000, 0x2000, 300, 256),))),
-                      ("leaves the state", dict(rows=((0x1000, 0x2000, 100, 100),))),
-                      ("leaves the state", dict(rows=((0x1000, 0x2000, -1, 0),))),
-                      ("misaligned", dict(rows=((0x1002, 0x2000, 300, 0),))), ("misaligned", dict(rows=((0x1000, 0x2001, 300, 0),))),
-                      ("null", dict(rows=((0, 0x2000, 300, 0),)))):
+                      ("leaves the state", dict(rows=((0x1000, 0x2000, 513),))),
+                      ("leaves the state", dict(rows=((0x1000, 0x2000, 300), (0x9000, 0x8000, 1)))),
+                      ("leaves the state", dict(rows=((0x1000, 0x2000, -1),))),
+                      ("elements", dict(rows=((0x1000, 0x2000, 100),))),
+                      ("misaligned", dict(rows=((0x1002, 0x2000, 300),))), ("misaligned", dict(rows=((0x1000, 0x2001, 300),))),
+                      ("null", dict(rows=((0, 0x2000, 300),)))):
         _no(pkg, match, call(**kw))
-    assert call(rows=()) == 0 and call(rows=((0, 0, 0, 0),)) == 0
+    assert call(rows=()) == 0 and call(rows=((0, 0, 0), (0, 0, 300), (0x1000, 0, 0))) == 0
 
     def values(m=0x1000, n=512, mo=0x3000):
         return pkg._lib.status("wfb_adamw_values", vp(m), vp(0x2000), vp(0x100), vp(0x200), n, vp(mo), vp(0x4000), None)

@@ -287,15 +287,18 @@ hipError_t launch_adamw(const wfb_adamw_tensor* tensors, int64_t n, int pdt, int
     tb.n = 0;
     return hipGetLastError();
   };
+  int64_t next = 0;
   for (int64_t i = 0; i < n; ++i) {
-    if (tensors[i].n == 0) continue;
+    const int64_t first = next;
+    next += (tensors[i].n + kBlock - 1) / kBlock * kBlock;
+    if (tensors[i].n == 0 || !tensors[i].g) continue;
     const int64_t tiles = (tensors[i].n + kTile - 1) / kTile;
     if (tb.n == kMaxTensors || tb.tile[tb.n] + tiles > kMostTiles)
       if (const hipError_t e = flush(); e != hipSuccess) return e;
     tb.p[tb.n] = tensors[i].p;
     tb.g[tb.n] = tensors[i].g;
     tb.len[tb.n] = tensors[i].n;
-    tb.first[tb.n] = tensors[i].first;
+    tb.first[tb.n] = first;
     tb.tile[tb.n + 1] = tb.tile[tb.n] + (uint32_t)tiles;
     ++tb.n;
   }

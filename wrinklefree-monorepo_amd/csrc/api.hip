@@ -1039,14 +1039,18 @@ int wfb_adamw_step(const wfb_adamw_tensor* tensors, int64_t n_tensors, int p_dty
   if (lr_dev && !step_dev) return fail(WFB_EINVAL, "%s: a device learning rate goes with a device step", name);
   if (step_dev && (!scalars || !aligned(scalars, 4))) return fail(WFB_EINVAL, "%s: null scalars", name);
   const size_t ps = p_dtype == WFB_F32 ? 4 : 2, gs = g_dtype == WFB_F32 ? 4 : 2;
+  int64_t first = 0;
   for (int64_t i = 0; i < n_tensors; ++i) {
     const wfb_adamw_tensor& t = tensors[i];
-    if (t.n < 0 || t.first < 0 || t.first % WFB_ADAMW_BLOCK != 0 || t.n > state_elements - t.first)
+    if (t.n < 0 || t.n > state_elements - first)
       return fail(WFB_EINVAL, "%s: tensor %lld leaves the state (elements %lld from %lld of %lld)", name, (long long)i,
-                  (long long)t.n, (long long)t.first, (long long)state_elements);
-    if (t.n > 0 && (!t.p || !t.g || !aligned(t.p, ps) || !aligned(t.g, gs)))
+                  (long long)t.n, (long long)first, (long long)state_elements);
+    if (t.n > 0 && t.g && (!t.p || !aligned(t.p, ps) || !aligned(t.g, gs)))
       return fail(WFB_EINVAL, "%s: tensor %lld: null or misaligned pointer", name, (long long)i);
+    first += (t.n + WFB_ADAMW_BLOCK - 1) / WFB_ADAMW_BLOCK * WFB_ADAMW_BLOCK;
   }
+  if (n_tensors > 0 && first != state_elements)
+    return fail(WFB_EINVAL, "%s: the tensors take %lld of the state's %lld elements", name, (long long)first, (long long)state_elements);
   const wfb::AdamWState st{m, v, m_scale, v_scale, bits};
   wfb::AdamWScalars c{};
   const wfb::AdamWScalars* dev = nullptr;

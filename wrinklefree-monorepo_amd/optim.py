@@ -9,7 +9,8 @@ change in place and their version counters with them, so that a BitLinear over t
 from __future__ import annotations
 
 from array import array
-from itertools import accumulate
+from itertools import chain
+from operator import attrgetter
 from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -17,6 +18,9 @@ import torch
 from . import _lib
 from ._lib import WFB_ADAMW_BLOCK, WFB_ADAMW_SCALARS
 from .ops import _DT, _on, _stream
+
+
+_dtype_of = attrgetter("dtype")
 
 
 class AdamWState(NamedTuple):
@@ -89,30 +93,41 @@ def adamw_step(
     bits, dev = _check_state(name, state)
     if len(params) != len(grads):
         raise RuntimeError(f"{name}: {len(params)} tensors, {len(grads)} gradients")
-    sizes = [p.numel() for p in params]
-    firsts = list(accumulate(((n + WFB_ADAMW_BLOCK - 1) // WFB_ADAMW_BLOCK * WFB_ADAMW_BLOCK for n in sizes), initial=0))
-    if firsts[-1] != state.m.numel():
-        raise RuntimeError(f"{name}: the state has {state.m.numel()} elements, the tensors take {firsts[-1]}")
-    live = [t for t in zip(params, grads, sizes, firsts) if t[1] is not None and t[2]]
-    # (a few calls a tensor are what a step over small tensors costs: 121 norms 138 us with attributes compared one by one,
-    # ADAMHOSTFIG so)
-    at = dev.index
-    if not all([p.is_same_size(g) and p.get_device() == at and g.get_device() == at for p, g, _, _ in live]):
+    every, have = list(params), list(grads)
+    if any([g is None for g in have]):
+        pairs = [(p, g) for p, g in zip(every, have) if g is not None]
+        live, gs = [p for p, _ in pairs], [g for _, g in pairs]
+    else:
+        live, gs = every, have
+    # (a few calls a tensor are what a step over small tensors costs, so they are made by map over the bound functions: 121
+    # norms 138 us with attributes compared one by one, ADAMHOSTFIG so)
+    tensor, at = torch.Tensor, dev.index
+    if not all(map(tensor.is_same_size, live, gs)) or not {at}.issuperset(map(tensor.get_device, chain(live, gs))):
         raise RuntimeError(f"{name}: a gradient has its tensor's shape, both are on {dev}")
-    if not all([p.is_contiguous() and not p.is_neg() for p, _, _, _ in live]):
+    if not all(map(tensor.is_contiguous, live)) or any(map(tensor.is_neg, live)):
         raise RuntimeError(f"{name}: tensors must be contiguous")
-    if not all([g.is_contiguous() and not g.is_neg() for _, g, _, _ in live]):
-        live = [(p, g.resolve_neg().contiguous(), n, f) for p, g, n, f in live]  # (copies live until the launch)
-    kinds = {(p.dtype, g.dtype) for p, g, _, _ in live}
-    tables = []
+    if not all(map(tensor.is_contiguous, gs)) or any(map(tensor.is_neg, gs)):
+        gs = [g.resolve_neg().contiguous() for g in gs]  # (copies live until the launch)
+    kinds = set(zip(map(_dtype_of, live), map(_dtype_of, gs)))
     for pdt, gdt in kinds:
         if pdt not in _DT or gdt not in _DT:
             raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {pdt} and {gdt}")
-        rows = live if len(kinds) == 1 else [t for t in live if t[0].dtype == pdt and t[1].dtype == gdt]
-        # rows of wfb_adamw_tensor
-        tables.append((_DT[pdt], _DT[gdt], array("q", [x for p, g, n, f in rows for x in (p.data_ptr(), g.data_ptr(), n, f)])))
-    if sum(len(set(t[2][::4])) for t in tables) != len(live):
+    sizes, ptrs, gptrs = (list(map(f, x)) for f, x in ((tensor.numel, every), (tensor.data_ptr, live), (tensor.data_ptr, gs)))
+    if len(set(ptrs)) != len(ptrs) and len({p for p in ptrs if p}) != sum(p != 0 for p in ptrs):
         raise RuntimeError(f"{name}: a tensor is given twice")
+    if len(live) != len(every):  # a null gradient: the tensor is passed over
+        it = iter(zip(ptrs, gptrs))
+        ptrs, gptrs = zip(*[(0, 0) if g is None else next(it) for g in have])
+    tables = []
+    for pdt, gdt in kinds:
+        wanted = gptrs
+        if len(kinds) > 1:
+            wanted = [q if g is not None and p.dtype == pdt and g.dtype == gdt else 0 for p, g, q in zip(every, have, gptrs)]
+        # rows of wfb_adamw_tensor
+        tables.append((_DT[pdt], _DT[gdt], array("q", chain.from_iterable(zip(ptrs, wanted, sizes)))))
+    need = sum([(n + WFB_ADAMW_BLOCK - 1) // WFB_ADAMW_BLOCK for n in sizes]) * WFB_ADAMW_BLOCK
+    if need != state.m.numel():
+        raise RuntimeError(f"{name}: the state has {state.m.numel()} elements, the tensors take {need}")
     step_dev = lr_dev = scalars = None
     if isinstance(step, torch.Tensor):
         if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
@@ -126,12 +141,12 @@ def adamw_step(
     m, v, ms, vs = state
     with _on(dev):
         for pdt, gdt, rows in tables:
-            _lib.call("wfb_adamw_step", rows.buffer_info()[0], len(rows) // 4, pdt, gdt, m.data_ptr(),
+            _lib.call("wfb_adamw_step", rows.buffer_info()[0], len(rows) // 3, pdt, gdt, m.data_ptr(),
                       v.data_ptr(), None if ms is None else ms.data_ptr(), None if vs is None else vs.data_ptr(),
                       m.numel(), bits, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
                       int(step), step_dev, lr_dev, None if scalars is None else scalars.data_ptr(), _stream(dev))
     if live:
-        torch.autograd.graph.increment_version([t[0] for t in live])
+        torch.autograd.graph.increment_version(live)
 
 
 def adamw_state_values(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
