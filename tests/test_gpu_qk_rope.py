@@ -276,7 +276,7 @@ def test_refusals(pkg, dev):
     cos, sin = _tables(dev, 16, 64)
     call = pkg.qk_norm_rope
     for match, err, args, kw in (
-            ("layout", ValueError, (q, k, cos, sin), dict(layout="neox")),
+            ("layout", ValueError, (q, k, cos, sin), dict(layout="quarters")),
             ("must be \\[batch", RuntimeError, (q[0, 0], k[0, 0], cos, sin), {}),
             ("one type", RuntimeError, (q, k.float(), cos, sin), {}),
             ("one type", RuntimeError, (q.double(), k.double(), cos, sin), {}),

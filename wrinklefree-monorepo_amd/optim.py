@@ -100,7 +100,7 @@ def adamw_step(
     else:
         live, gs = every, have
     # (a few calls a tensor are what a step over small tensors costs, so they are made by map over the bound functions: 121
-    # norms 138 us with attributes compared one by one, ADAMHOSTFIG so)
+    # norms 138 us with attributes compared one by one, 89 so)
     tensor, at = torch.Tensor, dev.index
     if not all(map(tensor.is_same_size, live, gs)) or not {at}.issuperset(map(tensor.get_device, chain(live, gs))):
         raise RuntimeError(f"{name}: a gradient has its tensor's shape, both are on {dev}")

@@ -10,13 +10,14 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from array import array
 from typing import Optional, Tuple, Union
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import HeadsStruct, RopeStruct, WFB_QK_MAX_DIM
+from ._lib import HeadsStruct, WFB_QK_MAX_DIM
 from .ops import _DT, _on, _stream
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -25,19 +26,29 @@ _NAME = "qk_norm_rope"
 Positions = Union[None, int, torch.Tensor]
 
 
-def _side(x: torch.Tensor, weight: Optional[torch.Tensor]) -> HeadsStruct:
-    sb, st, sh, _ = x.stride()
-    w, wdt = (None, 0) if weight is None else (weight.data_ptr(), _DT[weight.dtype])
-    return HeadsStruct(x.data_ptr(), sb, st, sh, None, 0, 0, 0, w, wdt, None, None, x.shape[2])
+# The structs of the C interface (wfb_heads, wfb_rope) are made of 8-byte fields: the calls hand them over as one array of
+# integers, which costs a third of three ctypes structures (a single token's call is bound by the host).
 
 
-def _rope(cos: torch.Tensor, sin: torch.Tensor, positions: Positions, layout: str) -> RopeStruct:
+def _heads(x: torch.Tensor, weight: Optional[torch.Tensor], out: int, g: Optional[torch.Tensor] = None, gw: int = 0) -> tuple:
+    """The fields of wfb_heads."""
+    w, wdt = (0, 0) if weight is None else (weight.data_ptr(), _DT[weight.dtype])
+    gs = (0, 0, 0, 0) if g is None else (g.data_ptr(), *g.stride()[:3])
+    return (x.data_ptr(), *x.stride()[:3], *gs, w, wdt, out, gw, x.shape[2])
+
+
+def _rope(cos: torch.Tensor, sin: torch.Tensor, positions: Union[int, torch.Tensor], layout: str) -> tuple:
+    """The fields of wfb_rope."""
     n, half = cos.shape
     if isinstance(positions, torch.Tensor):
-        where = (positions.data_ptr(), positions.element_size(), *positions.stride(), 0)
+        st = positions.stride()
+        where = (positions.data_ptr(), positions.element_size(), st[0] if len(st) == 2 else 0, st[-1], 0)
     else:
-        where = (None, 0, 0, 0, positions)
-    return RopeStruct(cos.data_ptr(), sin.data_ptr(), n, 2 * half, _LAYOUTS[layout], *where)
+        where = (0, 0, 0, 0, positions)
+    return (cos.data_ptr(), sin.data_ptr(), n, 2 * half, _LAYOUTS[layout], *where)
+
+
+_K_AT, _ROPE_AT = ctypes.sizeof(HeadsStruct), 2 * ctypes.sizeof(HeadsStruct)
 
 
 def _plain(x: torch.Tensor) -> torch.Tensor:
@@ -47,13 +58,13 @@ def _plain(x: torch.Tensor) -> torch.Tensor:
 
 def _forward(q, k, cos, sin, positions, wq, wk, eps, layout):
     b, t, _, d = q.shape
-    out = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k)]
-    sq, sk, rope = _side(q, wq), _side(k, wk), _rope(cos, sin, positions, layout)
-    sq.out, sk.out = out[0].data_ptr(), out[1].data_ptr()
-    with _on(q.device):
-        _lib.call("wfb_qk_norm_rope", ctypes.addressof(sq), ctypes.addressof(sk), ctypes.addressof(rope), _DT[q.dtype],
-                  b, t, d, eps, _stream(q.device))
-    return out
+    dev = q.device
+    qo, ko = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
+    args = array("q", (*_heads(q, wq, qo.data_ptr()), *_heads(k, wk, ko.data_ptr()), *_rope(cos, sin, positions, layout)))
+    at = args.buffer_info()[0]
+    with _on(dev):
+        _lib.call("wfb_qk_norm_rope", at, at + _K_AT, at + _ROPE_AT, _DT[q.dtype], b, t, d, eps, _stream(dev))
+    return qo, ko
 
 
 @functools.lru_cache(maxsize=256)
@@ -71,7 +82,7 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, layout):
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions if isinstance(positions, torch.Tensor) else None)
         ctx.meta = (None if isinstance(positions, torch.Tensor) else positions, eps, layout)
-        return tuple(_forward(q, k, cos, sin, positions, wq, wk, eps, layout))
+        return _forward(q, k, cos, sin, positions, wq, wk, eps, layout)
 
     @staticmethod
     @once_differentiable
@@ -79,30 +90,22 @@ class _QkNormRope(torch.autograd.Function):
         q, k, wq, wk, cos, sin, pos = ctx.saved_tensors
         start, eps, layout = ctx.meta
         need = ctx.needs_input_grad
-        b, t, _, d = q.shape
+        b, t, hq, d = q.shape
         dev = q.device
-        rope = _rope(cos, sin, pos if pos is not None else start, layout)
-        sides, grads, weights = [], [], []
-        for x, w, g, need_x, need_w in ((q, wq, gq, need[0], need[2]), (k, wk, gk, need[1], need[3])):
-            g = _plain(g)
-            s = _side(x, w)
-            s.g = g.data_ptr()
-            s.g_stride_b, s.g_stride_t, s.g_stride_h = g.stride()[:3]
-            gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-            gw = torch.empty_like(w) if w is not None and need_w else None
-            s.out = None if gx is None else gx.data_ptr()
-            s.grad_weight = None if gw is None else gw.data_ptr()
-            sides.append((s, g))
-            grads.append(gx)
-            weights.append(gw)
-        work = None
-        if any(w is not None for w in weights):
-            work = torch.empty(_grad_workspace(b, t, q.shape[2], k.shape[2], d), dtype=torch.float32, device=dev)
+        gq, gk = _plain(gq), _plain(gk)
+        gx = [torch.empty_like(x, memory_format=torch.contiguous_format) if n else None for x, n in ((q, need[0]), (k, need[1]))]
+        gw = [torch.empty_like(w) if w is not None and n else None for w, n in ((wq, need[2]), (wk, need[3]))]
+        work = 0
+        if gw[0] is not None or gw[1] is not None:
+            scratch = torch.empty(_grad_workspace(b, t, hq, k.shape[2], d), dtype=torch.float32, device=dev)
+            work = scratch.data_ptr()
+        p = [0 if x is None else x.data_ptr() for x in (*gx, *gw)]
+        args = array("q", (*_heads(q, wq, p[0], gq, p[2]), *_heads(k, wk, p[1], gk, p[3]),
+                           *_rope(cos, sin, start if pos is None else pos, layout)))
+        at = args.buffer_info()[0]
         with _on(dev):
-            _lib.call("wfb_qk_norm_rope_grad", ctypes.addressof(sides[0][0]), ctypes.addressof(sides[1][0]),
-                      ctypes.addressof(rope), _DT[q.dtype], b, t, d, eps, None if work is None else work.data_ptr(),
-                      _stream(dev))
-        return (*grads, *weights, None, None, None, None, None)
+            _lib.call("wfb_qk_norm_rope_grad", at, at + _K_AT, at + _ROPE_AT, _DT[q.dtype], b, t, d, eps, work, _stream(dev))
+        return (*gx, *gw, None, None, None, None, None)
 
 
 def qk_norm_rope(
@@ -122,41 +125,41 @@ def qk_norm_rope(
     (2 i, 2 i + 1).  Statistics and rotation are fp32, a result is rounded once."""
     if layout not in _LAYOUTS:
         raise ValueError(f"{_NAME}: layout must be one of {sorted(_LAYOUTS)}")
-    if q.dim() not in (3, 4) or k.dim() != q.dim():
+    shape, kshape = q.shape, k.shape
+    if len(shape) not in (3, 4) or len(kshape) != len(shape):
         raise RuntimeError(f"{_NAME}: q and k must be [batch, tokens, heads, head_dim] or [tokens, heads, head_dim]")
     if q.dtype not in _DT or k.dtype != q.dtype:
         raise RuntimeError(f"{_NAME}: q and k must be of one type, float32, bfloat16 or float16")
-    dev, d = q.device, q.shape[-1]
-    if dev.type != "cuda":
-        raise RuntimeError(f"{_NAME}: tensors must be on a HIP device (got {dev})")
-    for x in (k, cos, sin, q_weight, k_weight) + ((positions,) if isinstance(positions, torch.Tensor) else ()):
-        if x is not None and x.device != dev:
-            raise RuntimeError(f"{_NAME}: tensors are on different devices ({dev}, {x.device})")
-    if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != d:
-        raise RuntimeError(f"{_NAME}: q {list(q.shape)} and k {list(k.shape)} must agree in all but their heads")
+    if not q.is_cuda:
+        raise RuntimeError(f"{_NAME}: tensors must be on a HIP device (got {q.device})")
+    at, d, by_tensor = q.get_device(), shape[-1], isinstance(positions, torch.Tensor)
+    if k.get_device() != at or cos.get_device() != at or sin.get_device() != at or (by_tensor and positions.get_device() != at):
+        raise RuntimeError(f"{_NAME}: tensors are on different devices")
+    if kshape[-1] != d or kshape[:-2] != shape[:-2]:
+        raise RuntimeError(f"{_NAME}: q {list(shape)} and k {list(kshape)} must agree in all but their heads")
     if d % 2 or not 2 <= d <= WFB_QK_MAX_DIM:
         raise ValueError(f"{_NAME}: head_dim ({d}) must be even and at most {WFB_QK_MAX_DIM}")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape \
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or not cos.is_same_size(sin) \
             or not cos.is_contiguous() or not sin.is_contiguous() or 2 * cos.shape[1] > d:
         raise RuntimeError(f"{_NAME}: cos and sin must be contiguous float32 [positions, at most {d // 2}]")
     for w in (q_weight, k_weight):
-        if w is not None and (w.dtype not in _DT or w.numel() != d or not w.is_contiguous()):
-            raise RuntimeError(f"{_NAME}: norm weights must be contiguous floats of {d} elements")
-    flat = q.dim() == 3
+        if w is not None and (w.dtype not in _DT or w.numel() != d or not w.is_contiguous() or w.get_device() != at):
+            raise RuntimeError(f"{_NAME}: norm weights must be contiguous floats of {d} elements on {q.device}")
+    flat = len(shape) == 3
     if flat:
         q, k = q.unsqueeze(0), k.unsqueeze(0)
-    b, t = q.shape[:2]
-    if isinstance(positions, torch.Tensor):
+    b, t = (1, shape[0]) if flat else shape[:2]
+    if by_tensor:
         if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((t,), (b, t)):
             raise RuntimeError(f"{_NAME}: positions must be int32 or int64 [{t}] or [{b}, {t}]")
-        positions = positions.expand(b, t)
     else:
         positions = 0 if positions is None else int(positions)
         if cos.shape[1] and not 0 <= positions <= cos.shape[0] - t:
             raise ValueError(f"{_NAME}: positions {positions}..{positions + t - 1} leave tables of {cos.shape[0]} rows")
     q, k = _plain(q), _plain(k)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
         out = _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), layout)
     else:
         out = _forward(q, k, cos, sin, positions, q_weight, k_weight, float(eps), layout)
-    return (out[0].squeeze(0), out[1].squeeze(0)) if flat else (out[0], out[1])
+    return (out[0].squeeze(0), out[1].squeeze(0)) if flat else out
