@@ -12,6 +12,8 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
 template <bool F16>
 struct Op16 {
   typedef bf16x8_t v8;
@@ -24,6 +26,9 @@ struct Op16<true> {
   typedef f16x8_t v8;
   static __device__ __forceinline__ f32x16_t mfma(v8 a, v8 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4_t mfma16(v8 a, v8 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
 };
 
@@ -145,7 +150,11 @@ __device__ __forceinline__ void store8(const GradGemm& p, int64_t off, int col, 
 // index advances in stages of BK: the P planes' rows and the B rows of a stage go from global memory straight
 // into one of two LDS buffers (whole 64- or 128-byte row pieces, 16-byte chunks XOR-swizzled by row so that 16
 // rows at one chunk meet 16 distinct bank groups), the next stage's loads in flight while a stage is multiplied.
-// ST = 3, 4: a ring of so many buffers instead, ST - 1 stages in flight; see below.
+// ST = 3, 4: a ring of so many buffers instead, ST - 1 stages in flight (see below), and v_mfma_f32_16x16x32 (lane (i, g),
+// register r: row i of A, row 4 g + r of B).  Its sums are read and written half as often for a product as the 32 x 32
+// form's, and large products are bound by the card's power: with operands out of cache 4096 x 2560 x 13824 302 -> 276 us,
+// 28672 x 4096 x 2048 456 -> 416, 13824 x 2560 x 4096 in two planes 464 -> 427 (1.36 PFLOP/s) with it.  A wave's 64 x 128
+// or 128 x 64 is better than 128 x 128 with half the waves (416 against 493): two waves of a SIMD cover each other's waits.
 template <bool F16, int P, int TI, int TJ, int WI, int WJ, int BK, int WPE, int ST = 2>
 __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void grad_tile_kernel(
     GradGemm p, int tiles_i, int tiles_j) {
@@ -211,65 +220,25 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
     for (int jj = 0; jj < NB; ++jj) lds_load16(bb, lds + ASZ + (NB * w + jj) * 1024, boff[jj] + (uint32_t)ROW * s);
   };
 
-  f32x16_t acc[TJ][TI];
+  constexpr bool kRing = ST > 2;
+  f32x16_t acc[kRing ? 1 : TJ][kRing ? 1 : TI];
+  f32x4_t acc4[kRing ? 2 * TJ : 1][kRing ? 2 * TI : 1];
+  if constexpr (kRing) {
 #pragma unroll
-  for (int tj = 0; tj < TJ; ++tj)
+    for (int tj = 0; tj < 2 * TJ; ++tj)
 #pragma unroll
-    for (int ti = 0; ti < TI; ++ti)
+      for (int ti = 0; ti < 2 * TI; ++ti) acc4[tj][ti] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  } else {
 #pragma unroll
-      for (int q = 0; q < 16; ++q) acc[tj][ti][q] = 0.0f;
+    for (int tj = 0; tj < TJ; ++tj)
+#pragma unroll
+      for (int ti = 0; ti < TI; ++ti)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[tj][ti][q] = 0.0f;
+  }
 
-  const uint32_t afr = (uint32_t)(wi * TI * 32 + i) * ROW, bfr = ASZ + (uint32_t)(wj * TJ * 32 + i) * ROW;
-  // fragments of one 16-element step, two sets: a step's MFMAs run while the next step's are read
   typedef typename Op16<F16>::v8 v8;
-  v8 af[2][P][TI], bf[2][TJ];
-  auto read = [&](const uint8_t* lds, int x) {
-    const uint32_t c = (uint32_t)(((2 * x + g) ^ swz(i)) * 16);
-#pragma unroll
-    for (int tj = 0; tj < TJ; ++tj) bf[x & 1][tj] = *reinterpret_cast<const v8*>(lds + bfr + tj * 32 * ROW + c);
-#pragma unroll
-    for (int q = 0; q < P; ++q)
-#pragma unroll
-      for (int ti = 0; ti < TI; ++ti)
-        af[x & 1][q][ti] = *reinterpret_cast<const v8*>(lds + afr + (q * BI + ti * 32) * ROW + c);
-  };
-  auto multiply = [&](int x, bool reads, int loads = 0) {
-#pragma unroll
-    for (int q = 0; q < P; ++q)
-#pragma unroll
-      for (int ti = 0; ti < TI; ++ti)
-#pragma unroll
-        for (int tj = 0; tj < TJ; ++tj)
-          acc[tj][ti] = Op16<F16>::mfma(bf[x & 1][tj], af[x & 1][q][ti], acc[tj][ti]);
-    // the reads spread over the MFMAs (left alone, the compiler reads each fragment right before its first use
-    // and waits for it)
-#pragma unroll
-    for (int k = 0; k < P * TI * TJ; ++k) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (reads && k < TJ + P * TI) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      if (loads && k * loads / (P * TI * TJ) != (k + 1) * loads / (P * TI * TJ))
-        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  // stage s from cur; its last step's MFMAs run behind the barrier that hands cur over to stage s + 2's loads and
-  // behind the first reads of stage s + 1 from nxt
-  auto stage = [&](int s, uint8_t* cur, uint8_t* nxt) {
-#pragma unroll
-    for (int x = 0; x + 1 < KS; ++x) {
-      read(cur, x + 1);
-      multiply(x, true);
-    }
-    if (s + 1 < s1) {
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of stage s + 1 are in LDS
-      __syncthreads();                      // everyone's, and everyone has read the last of stage s
-      if (s + 2 < s1) issue(s + 2, cur);
-      read(nxt, 0);
-    }
-    multiply(KS - 1, true);
-  };
-  static_assert(KS % 2 == 0, "a stage starts with fragment set 0");
-  if constexpr (ST > 2) {
+  if constexpr (kRing) {
     // Stage s: the loads of stage s + ST - 1 go into the buffer of stage s - 1, which every wave had read before the
     // barrier at that stage's end.  Its own end waits, in every wave, until its reads of cur are done and all but the
     // last ST - 2 stages' loads of this wave have landed, then for the others.  The count is fixed: stages past s1 are
@@ -291,24 +260,60 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
         lds_load16(bb, lds + ASZ + (NB * w + jj) * 1024, on ? boff[jj] + (uint32_t)ROW * s : b_end);
       }
     };
-    constexpr int LP = (AI + NB + KS - 1) / KS;  // loads that go with one step's MFMAs
     auto meet = [&] {
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (orders the LDS accesses for the compiler)
       __builtin_amdgcn_s_waitcnt(kWait);
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
+    // A step is 64 rows of a plane of A by 32 elements: 4 fragments, read during the step before.  B's fragments of 32
+    // elements serve all steps over them, and each is overwritten behind its last use.
+    constexpr int NA = P * TI / 2, KS = BK / 32 * NA, M = 8 * TJ;
+    static_assert(TI % 2 == 0 && KS % 2 == 0, "a stage starts with fragment set 0");
+    constexpr int LP = (AI + NB + KS - 1) / KS;  // loads that go with one step's products
+    const int i4 = l & 15, g4 = l >> 4;
+    const uint32_t afr = (uint32_t)(wi * TI * 32 + i4) * ROW, bfr = ASZ + (uint32_t)(wj * TJ * 32 + i4) * ROW;
+    v8 af[2][4], bf[2 * TJ];
+    auto chunk = [&](int k) { return (uint32_t)(((4 * k + g4) ^ swz(i4)) * 16); };
+    auto read_a = [&](const uint8_t* lds, int x) {
+      const int n = x % NA, q = n / (TI / 2), t = n % (TI / 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        af[x & 1][e] = *reinterpret_cast<const v8*>(lds + afr + (q * BI + 64 * t + 16 * e) * ROW + chunk(x / NA));
+    };
+    auto read_b = [&](const uint8_t* lds, int k, int tj) {
+      bf[tj] = *reinterpret_cast<const v8*>(lds + bfr + 16 * tj * ROW + chunk(k));
+    };
+    // step x of a stage, the reads for the next one from lds and `loads` loads among its products
+    auto step = [&](int x, bool reads, const uint8_t* lds, int loads) __attribute__((always_inline)) {
+      const int nx = (x + 1) % KS, t = x % (TI / 2);
+      const bool turn = (x + 1) % NA == 0;
+      if (reads) read_a(lds, nx);
+#pragma unroll
+      for (int tj = 0; tj < 2 * TJ; ++tj) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc4[tj][4 * t + e] = Op16<F16>::mfma16(bf[tj], af[x & 1][e], acc4[tj][4 * t + e]);
+        if (reads && turn) read_b(lds, nx / NA, tj);
+      }
+#pragma unroll
+      for (int k = 0; k < M; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (reads && k < 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (reads && turn && k % 4 == 3) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (loads && k * loads / M != (k + 1) * loads / M) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
     // stage s from cur, behind the last step of stage s - 1
-    auto ring = [&](int s, uint8_t* cur, uint8_t* last) {
+    auto ring = [&](int s, uint8_t* cur, uint8_t* last) __attribute__((always_inline)) {
       meet();
-      read(cur, 0);
       load(s + ST - 1, last, 0, LP);
-      multiply(KS - 1, true, LP);
+      step(KS - 1, true, cur, LP);
 #pragma unroll
       for (int x = 0; x + 1 < KS; ++x) {
-        read(cur, x + 1);
         load(s + ST - 1, last, LP * (x + 1), LP * (x + 2));
-        multiply(x, true, min(AI + NB - LP * (x + 1), LP));
+        step(x, true, cur, max(min(AI + NB - LP * (x + 1), LP), 0));
       }
     };
     uint8_t* const b2 = ST > 2 ? lds2 : lds0;
@@ -318,14 +323,13 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
       load(s0 + 1, lds1, 0, AI + NB);
       if constexpr (ST > 3) load(s0 + 2, b2, 0, AI + NB);
       meet();
-      read(lds0, 0);
+      read_a(lds0, 0);
+#pragma unroll
+      for (int tj = 0; tj < 2 * TJ; ++tj) read_b(lds0, 0, tj);
       load(s0 + ST - 1, ST > 3 ? b3 : b2, 0, AI + NB);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x + 1 < KS; ++x) {
-        read(lds0, x + 1);
-        multiply(x, true);
-      }
+      for (int x = 0; x + 1 < KS; ++x) step(x, true, lds0, 0);
       // (whole turns of the ring, then what is left: a loop that could end within a turn would have the compiler lose
       // count of the loads in flight and wait for all of them once a turn)
       int s = s0 + 1;
@@ -348,19 +352,70 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
         if (s + 1 < s1) ring(s + 1, b2, lds1);
         if (s + 2 < s1) ring(s + 2, b3, b2);
       }
-      multiply(KS - 1, false);
+      step(KS - 1, false, lds0, 0);
       __builtin_amdgcn_s_waitcnt(0x0F70);  // the last stages' zeros: the buffers are the epilogue's from here on
     }
-  } else if (s0 < s1) {
-    issue(s0, lds0);
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    if (s0 + 1 < s1) issue(s0 + 1, lds1);
-    read(lds0, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    for (int s = s0; s < s1; s += 2) {
-      stage(s, lds0, lds1);
-      if (s + 1 < s1) stage(s + 1, lds1, lds0);
+  } else {
+    const uint32_t afr = (uint32_t)(wi * TI * 32 + i) * ROW, bfr = ASZ + (uint32_t)(wj * TJ * 32 + i) * ROW;
+    // fragments of one 16-element step, two sets: a step's MFMAs run while the next step's are read
+    v8 af[2][P][TI], bf[2][TJ];
+    auto read = [&](const uint8_t* lds, int x) {
+      const uint32_t c = (uint32_t)(((2 * x + g) ^ swz(i)) * 16);
+#pragma unroll
+      for (int tj = 0; tj < TJ; ++tj) bf[x & 1][tj] = *reinterpret_cast<const v8*>(lds + bfr + tj * 32 * ROW + c);
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+#pragma unroll
+        for (int ti = 0; ti < TI; ++ti)
+          af[x & 1][q][ti] = *reinterpret_cast<const v8*>(lds + afr + (q * BI + ti * 32) * ROW + c);
+    };
+    auto multiply = [&](int x, bool reads, int loads = 0) {
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+#pragma unroll
+        for (int ti = 0; ti < TI; ++ti)
+#pragma unroll
+          for (int tj = 0; tj < TJ; ++tj)
+            acc[tj][ti] = Op16<F16>::mfma(bf[x & 1][tj], af[x & 1][q][ti], acc[tj][ti]);
+      // the reads spread over the MFMAs (left alone, the compiler reads each fragment right before its first use
+      // and waits for it)
+#pragma unroll
+      for (int k = 0; k < P * TI * TJ; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (reads && k < TJ + P * TI) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (loads && k * loads / (P * TI * TJ) != (k + 1) * loads / (P * TI * TJ))
+          __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // stage s from cur; its last step's MFMAs run behind the barrier that hands cur over to stage s + 2's loads and
+    // behind the first reads of stage s + 1 from nxt
+    auto stage = [&](int s, uint8_t* cur, uint8_t* nxt) {
+#pragma unroll
+      for (int x = 0; x + 1 < KS; ++x) {
+        read(cur, x + 1);
+        multiply(x, true);
+      }
+      if (s + 1 < s1) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of stage s + 1 are in LDS
+        __syncthreads();                      // everyone's, and everyone has read the last of stage s
+        if (s + 2 < s1) issue(s + 2, cur);
+        read(nxt, 0);
+      }
+      multiply(KS - 1, true);
+    };
+    static_assert(KS % 2 == 0, "a stage starts with fragment set 0");
+    if (s0 < s1) {
+      issue(s0, lds0);
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+      __syncthreads();
+      if (s0 + 1 < s1) issue(s0 + 1, lds1);
+      read(lds0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      for (int s = s0; s < s1; s += 2) {
+        stage(s, lds0, lds1);
+        if (s + 1 < s1) stage(s + 1, lds1, lds0);
+      }
     }
   }
   __syncthreads();  // the operand buffers are free
@@ -383,18 +438,33 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(WP
   };
 #pragma unroll
   for (int ti = 0; ti < TI; ++ti) {
-    if constexpr (F16) alpha = whole ? p.row_scale[min(i0 + wi * 32 * TI + ti * 32 + i, p.I - 1)] : 1.0f;
+    auto scale_of = [&](int r) { return whole ? p.row_scale[min(i0 + wi * 32 * TI + ti * 32 + r, p.I - 1)] : 1.0f; };
+    float alpha4[2];
+    if constexpr (kRing) alpha4[0] = scale_of(l & 15), alpha4[1] = scale_of(16 + (l & 15));
+    else if constexpr (F16) alpha = scale_of(i);
 #pragma unroll
     for (int ts = 0; ts < TJ; ts += TS) {
+      if constexpr (kRing) {
 #pragma unroll
-      for (int tj = 0; tj < TS; ++tj)
+        for (int tj = 0; tj < 2 * TS; ++tj)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x16_t& v = acc[ts + tj][ti];
-          const int c = tj * 8 + 2 * q + g;
-          *reinterpret_cast<float4*>(st + (i * CPR + (c ^ (i & (CPR - 1)))) * 16) =
-              make_float4(v[4 * q] * alpha, v[4 * q + 1] * alpha, v[4 * q + 2] * alpha, v[4 * q + 3] * alpha);
-        }
+          for (int h = 0; h < 2; ++h) {
+            const f32x4_t& v = acc4[2 * ts + tj][2 * ti + h];
+            const int r = 16 * h + (l & 15), c = 4 * tj + (l >> 4);
+            *reinterpret_cast<float4*>(st + (r * CPR + (c ^ (r & (CPR - 1)))) * 16) =
+                make_float4(v[0] * alpha4[h], v[1] * alpha4[h], v[2] * alpha4[h], v[3] * alpha4[h]);
+          }
+      } else {
+#pragma unroll
+        for (int tj = 0; tj < TS; ++tj)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x16_t& v = acc[ts + tj][ti];
+            const int c = tj * 8 + 2 * q + g;
+            *reinterpret_cast<float4*>(st + (i * CPR + (c ^ (i & (CPR - 1)))) * 16) =
+                make_float4(v[4 * q] * alpha, v[4 * q + 1] * alpha, v[4 * q + 2] * alpha, v[4 * q + 3] * alpha);
+          }
+      }
       wave_sync();
       constexpr int kStores = F16 ? 2 : 32 / RP;  // unrolled: whole, the stores' code is several times the products'
 #pragma unroll kStores
