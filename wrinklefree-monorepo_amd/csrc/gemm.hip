@@ -390,6 +390,8 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
   constexpr bool PAIR = GL != 0 && TN == 2;
   static_assert(GL == 0 || PAIR || (TN == 1 && EPI == 0 && BI * (64 / BLPR) == 32), "gated tiles: 128 rows, 32 loaded per wave");
   static_assert(!PAIR || BI * (64 / BLPR) == 64, "pair tiles: a wave loads the rows that it multiplies");
+  constexpr bool S16 = PAIR && TM == 4;  // 16 x 16 x 64 products
+  static_assert(!S16 || (KB == 1 && KSPL == 1), "one block a stage");
   __shared__ __attribute__((aligned(16))) int8_t lds_a0s[KSPL][ASZ];
   __shared__ __attribute__((aligned(16))) int8_t lds_a1s[KSPL][ASZ];
   __shared__ __attribute__((aligned(16))) uint8_t lds_b0s[KSPL][BSZ];
@@ -481,15 +483,74 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
   for (int j = 0; j < SCH; ++j) soffs[j] = srow * AROW + ((l % LPR) * SCH + ((j + srow + (srow >> 2)) % SCH)) * 16;
   int ssum = 0;
 
-  v16i acc[TN][TM];
+  v16i acc[S16 ? 1 : TN][S16 ? 1 : TM];
+  v4i acc4[S16 ? 2 * TN : 1][S16 ? 2 * TM : 1];
+  if constexpr (S16) {
 #pragma unroll
-  for (int tn = 0; tn < TN; ++tn)
+    for (int tn = 0; tn < 2 * TN; ++tn)
 #pragma unroll
-    for (int tm = 0; tm < TM; ++tm)
+      for (int tm = 0; tm < 2 * TM; ++tm) acc4[tn][tm] = v4i{0, 0, 0, 0};
+  } else {
 #pragma unroll
-      for (int q = 0; q < 16; ++q) acc[tn][tm][q] = 0;
+    for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+      for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[tn][tm][q] = 0;
+  }
 
-  auto compute = [&](const int8_t* la, const uint8_t* lb) {
+  // A stage of 16 x 16 x 64 products: step (y, half of the tokens) takes k = 64 y .. + 63, of which lane group g feeds
+  // 16 g .. + 15: field 2 y + g / 2 of half g % 2 of the block.  Four activation fragments a step, read during the one
+  // before; a weight fragment serves both halves, and the next one is unpacked into it behind its last use.
+  const int i16 = l & 15, g16 = l >> 4;
+  auto compute16 = [&](const int8_t* la, const uint8_t* lb) __attribute__((always_inline)) {
+    v4i af[2][4], bw[2 * TN], bf[2 * TN], sv[SCH];
+    auto read_a = [&](int st) {
+      const int8_t* p = la + (64 * (st & 1) + i16) * AROW + (((4 * (st >> 1) + g16) ^ aswz(i16)) * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) af[st & 1][e] = *reinterpret_cast<const v4i*>(p + 16 * e * AROW);
+    };
+    auto unpack = [&](int tj, int y) {
+      const int shift = 6 - 4 * y - 2 * (g16 >> 1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bf[tj][e] = (int)(((uint32_t)bw[tj][e] >> shift) & 0x03030303u);
+    };
+#pragma unroll
+    for (int tj = 0; tj < 2 * TN; ++tj) {
+      const int R = (wn * 2 * TN + tj) * 16 + i16;
+      bw[tj] = *reinterpret_cast<const v4i*>(lb + R * BROW + (((g16 & 1) ^ bswz(R)) * 16));
+    }
+    read_a(0);
+#pragma unroll
+    for (int j = 0; j < SCH; ++j) sv[j] = *reinterpret_cast<const v4i*>(la + soffs[j]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      if (st < 3) read_a(st + 1);
+#pragma unroll
+      for (int tj = 0; tj < 2 * TN; ++tj) {
+        if (st == 0) unpack(tj, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc4[tj][4 * (st & 1) + e] =
+              __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[tj], af[st & 1][e], acc4[tj][4 * (st & 1) + e], 0, 0, 0);
+        if (st == 1) unpack(tj, 1);
+      }
+      if (st < SCH) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ssum = __builtin_amdgcn_sdot4(sv[st][e], 0x01010101, ssum, false);
+      }
+      if (st == 0) __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+#pragma unroll
+      for (int k = 0; k < 8 * TN; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        if (st < 3 && k < 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto compute32 = [&](const int8_t* la, const uint8_t* lb) {
     constexpr int AF = TM >= 4 ? 2 : X;  // A fragments held: all of the stage, or a two-step ring
     v4i af[AF][TM], bw[KB][TN], bf[2][TN], sv[SCH];
     auto read_a = [&](v4i(&dst)[TM], int x) {
@@ -535,6 +596,10 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
     }
   };
 
+  auto compute = [&](const int8_t* la, const uint8_t* lb) {
+    if constexpr (S16) compute16(la, lb);
+    else compute32(la, lb);
+  };
   if constexpr (KSPL == 1) {
     issue(0, lds_a0, lds_b0);
     for (int kb = 0; kb < KS; kb += 2) {
@@ -647,18 +712,35 @@ __global__ __launch_bounds__(256 * KSPL) __attribute__((amdgpu_waves_per_eu(OCC,
     const int64_t up0 = ep.ldgu / 2;
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
-      const int rs = rsum(tm * 32 + i);
-      const float as = epi_ascale(ep, min(m0 + tm * 32 + i, M - 1));
+      if constexpr (S16) {
 #pragma unroll
-      for (int tn = 0; tn < 2; ++tn)
+        for (int h = 0; h < 2; ++h) {
+          const int r = 16 * h + i16, rs = rsum(tm * 32 + r);
+          const float as = epi_ascale(ep, min(m0 + tm * 32 + r, M - 1));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float y[4];
+          for (int tj = 0; tj < 4; ++tj) {
+            float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(__fmul_rn((float)(acc[tn][tm][4 * q + e] - rs), ws[tn]), as);
-          *reinterpret_cast<float4*>(st + tn * 1024 + i * 32 + (((2 * q + g) ^ (i & 7)) * 4)) =
-              make_float4(y[0], y[1], y[2], y[3]);
+            for (int e = 0; e < 4; ++e)
+              y[e] = __fmul_rn(__fmul_rn((float)(acc4[tj][2 * tm + h][e] - rs), ws[tj >> 1]), as);
+            *reinterpret_cast<float4*>(st + (tj >> 1) * 1024 + r * 32 + (((4 * (tj & 1) + g16) ^ (r & 7)) * 4)) =
+                make_float4(y[0], y[1], y[2], y[3]);
+          }
         }
+      } else {
+        const int rs = rsum(tm * 32 + i);
+        const float as = epi_ascale(ep, min(m0 + tm * 32 + i, M - 1));
+#pragma unroll
+        for (int tn = 0; tn < 2; ++tn)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(__fmul_rn((float)(acc[tn][tm][4 * q + e] - rs), ws[tn]), as);
+            *reinterpret_cast<float4*>(st + tn * 1024 + i * 32 + (((2 * q + g) ^ (i & 7)) * 4)) =
+                make_float4(y[0], y[1], y[2], y[3]);
+          }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 8 * j + (l >> 3), c = l & 7;
