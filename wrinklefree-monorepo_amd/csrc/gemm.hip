@@ -1103,14 +1103,19 @@ hipError_t launch_gemm_i2s_glu(const uint8_t* W, int n, int k, const int8_t* A, 
 #undef WFB_GLU
 }
 
-// The gated product of any number of tokens, with or without both products kept: the rules of launch_gemm_i2s for the same
-// 256 weight rows a tile.
+// The gated product of any number of tokens, with or without both products kept.  Tile height by the number of 128-output
+// tiles, every height swept over 1..2048 tokens at 1536 x 640, 6912 x 2560 and 14336 x 4096 outputs x weights (bf16 results,
+// us): 128 tokens from 400 tiles (448 tiles 66.6 against 70.8 of half the height, 336 tiles 65.3 against 58.5), 64 tokens from
+// 400 of theirs (432 tiles 28.3 against 31.5, 324 tiles 26.9 against 24.8), else 32, their K split three ways where that
+// still fits the chip at once and rows are long (112 tiles of 4096 weights 13.8 against 15.7, 336 tiles 29.0 against 23.8;
+// 12 tiles of 640 weights 8.8 against 8.3).  2048 x 14336 x 4096 takes 213 us (2.26 POP/s), 2048 x
+// 6912 x 2560 89 (1.6 POP/s): 864 tiles on 512 places, the second round is two thirds full.
 hipError_t launch_gemm_i2s_pair(const uint8_t* W, int n, int k, const int8_t* A, int m, int64_t lda, int act,
                                 const Epilogue& e, hipStream_t s) {
   const int64_t tn = (n / 2 + 127) / 128, t128 = tn * ((m + 127) / 128), t64 = tn * ((m + 63) / 64), t32 = tn * ((m + 31) / 32);
-  if (t128 >= 320) return launch_tile_pair<4, 1, 2, 1>(W, n, k, A, m, lda, act, e, s);
-  if (t64 >= 160) return launch_tile_pair<2, 2, 2, 1>(W, n, k, A, m, lda, act, e, s);
-  if (t32 <= 256) return launch_tile_pair<1, 2, 3, 3>(W, n, k, A, m, lda, act, e, s);
+  if (t128 >= 400) return launch_tile_pair<4, 1, 2, 1>(W, n, k, A, m, lda, act, e, s);
+  if (t64 >= 400) return launch_tile_pair<2, 2, 2, 1>(W, n, k, A, m, lda, act, e, s);
+  if (t32 <= 256 && k >= 2048) return launch_tile_pair<1, 2, 3, 3>(W, n, k, A, m, lda, act, e, s);
   return launch_tile_pair<1, 2, 3, 1>(W, n, k, A, m, lda, act, e, s);
 }
 
