@@ -146,7 +146,8 @@ __global__ __launch_bounds__(256) void pack_i2s_kernel(const void* __restrict__ 
 
 // Two matrices [n, k] at once (blockIdx.y), rows padded with zero weights from k to kp, each behind its own stage 2: every
 // workgroup repeats that over the 1024 partial sums, 8 KB from L2, instead of a launch between, and packs `chunks` times 256
-// dwords behind it.  VEC: k % 4 == 0 and rows aligned to groups of four weights, one load each.
+// dwords behind it.  VEC: k % 4 == 0 and rows aligned to groups of four weights, one load each.  Two 6912 x 2560 in fp32: 34
+// us for the sums (4.1 TB/s), 26 here (5.8, of what the sums left in the last-level cache).
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void pack_pair_kernel(const void* __restrict__ w0, const void* __restrict__ w1, int64_t n,
                                                         int64_t k, int64_t kp, const double* __restrict__ partial,

@@ -196,7 +196,8 @@ __device__ __forceinline__ void load_angles(const QkRope& p, bool in, int64_t at
 }
 
 // Forward, both sides' tasks in one range, a token's queries before its keys.  655k heads of 128 in bf16 (16384 tokens, 32/8
-// heads): QKFWDFIG, against 70 us for a copy of the same bytes.
+// heads) 66 us, 5.1 TB/s; a copy of the same bytes takes 70.  While loads were
+// converted as they came: 94.
 template <int DT, int V, int L, int IT>
 __global__ __launch_bounds__(kThreads) void qk_rope_kernel(QkRope p, uint32_t tasks) {
   const int lane = threadIdx.x % L;
@@ -272,7 +273,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(QkRope p, uint32_t ta
 }
 
 // Backward: the workgroups walk the queries' tasks, then the keys', and leave each side's part of the weight's gradient.
-// 205k heads of 128 in bf16 (8192 tokens, 20/5 heads): QKBWDFIG.
+// 205k heads of 128 in bf16 (8192 tokens, 20/5 heads): 38 us for 157 MB (4.1 TB/s), and 4 for the sum over the groups.
+// With the forward pass 64 us; 94 while a thread held both sides' sums and converted its loads as they came.
 template <int DT, int V, int L, int IT>
 __global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, float* __restrict__ part) {
   __shared__ float red[kThreads / L][2 * V * IT * L];
@@ -389,6 +391,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, float*
   }
 }
 
+// Workgroups of the backward pass, three per CU: each leaves a row of partial sums for each weight, which the second launch
+// adds up.
 constexpr int kGradGroups = 768;
 
 // The widest chunk that the sizes, strides and addresses allow: whole pairs on either side of the rotated part's end,

@@ -1,9 +1,9 @@
 """AdamW over many tensors in one launch, with states in fp32 or in 8 bits.
 
-The reference trains its float weights with torch's and 8-bit AdamW; here one kernel walks every tensor of a group, and
-the states of a group lie in one flat array each, so that a state in 8 bits (codes and one scale for 256 elements, about
-a quarter of the bytes) needs no bookkeeping per tensor.  The arithmetic is in csrc/adamw.hip's first lines.  Weights
-change in place and their version counters with them, so that a BitLinear over them repacks.
+One kernel walks every tensor of a group, and the states of a group lie in one flat array each, so that a state in 8 bits
+(codes and one scale for 256 elements, about a quarter of the bytes) needs no bookkeeping per tensor.  The arithmetic is in
+csrc/adamw.hip's first lines.  Weights change in place and their version counters with them, so that a BitLinear over them
+repacks.
 """
 
 from __future__ import annotations
