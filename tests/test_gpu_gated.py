@@ -325,3 +325,29 @@ def test_refusals(pkg, dev):
     (gx,) = torch.autograd.grad(call(leaf, gate, up), [leaf], g2, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         gx.sum().backward()
+
+def _negated_view(t):
+    """t's values as a lazily negated, strided view (what .imag of a conjugate is)."""
+    return torch.complex(torch.zeros_like(t), -t).conj().imag
+
+
+def _otherwise(form):
+    """An unpack hook that gives float32 tensors back as negated views, or matrices with their last dimensions in other
+    memory order."""
+    if form == "negated":
+        return lambda t: _negated_view(t) if t.dtype == torch.float32 else t
+    return lambda t: t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() >= 2 else t
+
+
+@pytest.mark.parametrize("m", [1, 7])
+@pytest.mark.parametrize("form", ["negated", "columns"])
+def test_saved_tensor_hooks_may_change_the_form(pkg, dev, form, m):
+    """The same values in other memory, so the same bits (a single token's scale counts as contiguous in any view)."""
+    x = torch.randn(m, 200, device=dev, requires_grad=True)
+    g, u = (torch.randn(96, 200, device=dev, requires_grad=True) for _ in range(2))
+    gh = torch.randn(m, 96, device=dev)
+    want = torch.autograd.grad(pkg.gated_bitlinear(x, g, u), (x, g, u), gh)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _otherwise(form)):
+        h = pkg.gated_bitlinear(x, g, u)
+    for a, b in zip(torch.autograd.grad(h, (x, g, u), gh), want):
+        assert torch.equal(a, b)

@@ -295,3 +295,33 @@ def test_refusals(pkg, dev):
             ("leave tables", ValueError, (q, k, cos, sin, -1), {})):
         with pytest.raises(err, match=match):
             call(*args, **kw)
+
+def _negated_view(t):
+    """t's values as a lazily negated, strided view (what .imag of a conjugate is)."""
+    return torch.complex(torch.zeros_like(t), -t).conj().imag
+
+
+def _otherwise(form):
+    """An unpack hook that gives float32 tensors back as negated views, or matrices with their last dimensions in other
+    memory order."""
+    if form == "negated":
+        return lambda t: _negated_view(t) if t.dtype == torch.float32 else t
+    return lambda t: t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() >= 2 else t
+
+
+@pytest.mark.parametrize("form", ["negated", "columns"])
+def test_saved_tensor_hooks_may_change_the_form(pkg, dev, form):
+    """The same values in other memory, so the same bits."""
+    q, k, wq, wk, gq, gk = _inputs(dev, 2, 5, 3, 1, 64, F32)
+    (cos, sin), pos = _tables(dev, 64, 32), torch.arange(3, 8, device=dev)
+    ins = [x.detach().requires_grad_(True) for x in (q, k, wq, wk)]
+
+    def grads():
+        out = pkg.qk_norm_rope(ins[0], ins[1], cos, sin, pos, ins[2], ins[3])
+        return lambda: torch.autograd.grad(out, ins, (gq, gk))
+
+    want = grads()()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _otherwise(form)):
+        got = grads()
+    for x, y in zip(got(), want):
+        assert torch.equal(x, y)

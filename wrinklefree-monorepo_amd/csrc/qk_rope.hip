@@ -401,12 +401,13 @@ int chunk_of(const QkRope& p, int dtype, bool grad) {
   const int esz = dtype == WFB_F32 ? 4 : 2;
   auto fits = [&](int v) {
     if (p.rotary % (2 * v) || (p.head_dim - p.rotary) % (2 * v)) return false;
-    auto whole = [&](const void* q, int64_t a, int64_t b, int64_t c) {
-      return (uintptr_t)q % (v * esz) == 0 && a % v == 0 && b % v == 0 && c % v == 0;
+    auto whole = [&](const void* q, int64_t a, int64_t b, int64_t c, int heads) {  // (a stride along one element never counts)
+      return (uintptr_t)q % (v * esz) == 0 && (a % v == 0 || p.batch <= 1) && (b % v == 0 || p.t <= 1) &&
+             (c % v == 0 || heads <= 1);
     };
     for (const HeadRows& s : p.side) {
-      if (!whole(s.x, s.xb, s.xt, s.xh) || !whole(s.out, 0, 0, 0)) return false;
-      if (grad && !whole(s.g, s.gb, s.gt, s.gh)) return false;
+      if (!whole(s.x, s.xb, s.xt, s.xh, s.heads) || !whole(s.out, 0, 0, 0, s.heads)) return false;
+      if (grad && !whole(s.g, s.gb, s.gt, s.gh, s.heads)) return false;
       const int wv = v * (s.wdt == WFB_F32 ? 4 : 2);
       if (s.w && (uintptr_t)s.w % (wv < 16 ? wv : 16) != 0) return false;
     }

@@ -85,8 +85,8 @@ class _GatedSTE(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gh):
-        # (contiguous: a saved-tensor hook may give them back otherwise; no products of no tokens)
-        gate_up, q, a_scale, qweight, scales = (t if t is None else t.contiguous() for t in ctx.saved_tensors)
+        # (a saved-tensor hook may give them back as other views; no products of no tokens)
+        gate_up, q, a_scale, qweight, scales = (t if t is None else t.resolve_neg().contiguous() for t in ctx.saved_tensors)
         act, xdt, wdt, k = ctx.meta
         need_x, need_gate, need_up = ctx.needs_input_grad[:3]
         f, m, dev = qweight.shape[0] // 2, q.shape[0], q.device

@@ -87,7 +87,10 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk, cos, sin, pos = ctx.saved_tensors
+        # (a saved-tensor hook may give them back as other views)
+        q, k, wq, wk, cos, sin, pos = (t if t is None else t.resolve_neg() for t in ctx.saved_tensors)
+        q, k = _plain(q), _plain(k)
+        wq, wk, cos, sin = (t if t is None else t.contiguous() for t in (wq, wk, cos, sin))
         start, eps, layout = ctx.meta
         need = ctx.needs_input_grad
         b, t, hq, d = q.shape
