@@ -9,6 +9,7 @@ integer sums.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -18,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._lib import WFB_ABSMEAN_WS_DOUBLES
 from .bitlinear import BitLinear, _check_lambda
-from .ops import _ACTS, _DT, QK_I2_S, _on, _p, _require_gpu, _stream, quantize_activations_i8_per_token
+from .ops import _ACTS, _DT, QK_I2_S, _on, _p, _require_gpu, _stream
 
 _NAME = "gated_bitlinear"
 
@@ -37,7 +38,6 @@ def _check_pair(name: str, gate: torch.Tensor, up: torch.Tensor) -> None:
         raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {gate.dtype}")
 
 
-@torch.no_grad()
 def pack_gated(gate_weight: torch.Tensor, up_weight: torch.Tensor) -> PackedGated:
     """Both matrices [hidden, in_features] ternarised and packed, each with its own absmean scale, as
     :func:`pack_ternary_i2s` packs one; in_features is padded to a multiple of 128 with zero weights."""
@@ -61,14 +61,25 @@ def pack_gated(gate_weight: torch.Tensor, up_weight: torch.Tensor) -> PackedGate
 def _forward(x2: torch.Tensor, packed: PackedGated, act: str, keep: bool):
     """(h, gate|up or None, codes, a_scale) of the rows x2."""
     n, kb = packed.qweight.shape
-    f, kp, m, dev = n // 2, 4 * kb, x2.shape[0], x2.device
-    q, a_scale = quantize_activations_i8_per_token(x2, k_pad=kp)
+    (m, k), dev, dt = x2.shape, x2.device, _DT[x2.dtype]
+    f, kp = n // 2, 4 * kb
+    q = torch.empty((m, kp), dtype=torch.int8, device=dev)
+    a_scale = torch.empty(m, dtype=torch.float32, device=dev)
     h = torch.empty((m, f), dtype=x2.dtype, device=dev)
     gate_up = torch.empty(2 * m * ((f + 63) // 64 * 64), dtype=torch.float32, device=dev) if keep and m else None
+    stream, qp, ap = _stream(dev), q.data_ptr(), a_scale.data_ptr()
     with _on(dev):
-        _lib.call("wfb_gated_i2s", _p(packed.qweight), f, kp, _p(q), m, kp, _p(a_scale), _p(packed.scales), _ACTS[act],
-                  _p(h), _DT[h.dtype], _p(gate_up), _stream(dev))
+        _lib.call("wfb_quantize_act_i8", x2.data_ptr(), dt, m, k, k, qp, kp, kp, ap, stream)
+        _lib.call("wfb_gated_i2s", packed.qweight.data_ptr(), f, kp, qp, m, kp, ap, packed.scales.data_ptr(), _ACTS[act],
+                  h.data_ptr(), dt, _p(gate_up), stream)
     return h, gate_up, q, a_scale
+
+
+@functools.lru_cache(maxsize=256)
+def _grad_workspace(m: int, f: int, k: int, xdt: int, need_x: bool, wdt: int, need_w: bool) -> int:
+    size = ctypes.c_int64(0)
+    _lib.call("wfb_gated_grad_workspace", m, f, k, xdt, int(need_x), wdt, int(need_w), ctypes.addressof(size))
+    return size.value
 
 
 class _GatedSTE(torch.autograd.Function):
@@ -97,10 +108,7 @@ class _GatedSTE(torch.autograd.Function):
         gw = torch.empty((2 * f, k), dtype=wdt, device=dev) if need_w else None
         if m == 0:
             return gx, *([gw[:f].zero_(), gw[f:].zero_()] if need_w else [None, None]), None, None, None
-        size = ctypes.c_int64(0)
-        _lib.call("wfb_gated_grad_workspace", m, f, k, _DT[xdt], int(need_x), _DT[wdt], int(need_w),
-                  ctypes.addressof(size))
-        work = torch.empty(size.value, dtype=torch.uint8, device=dev)
+        work = torch.empty(_grad_workspace(m, f, k, _DT[xdt], need_x, _DT[wdt], need_w), dtype=torch.uint8, device=dev)
         kp = 4 * qweight.shape[1]
         with _on(dev):
             _lib.call("wfb_gated_grad", _p(gate_up), _p(gh), _DT[gh.dtype], gh.stride(0) if m > 1 else f, m, f, _ACTS[act],
@@ -129,38 +137,39 @@ def gated_bitlinear(
         raise RuntimeError(f"{_NAME}: weights or their pack are needed")
     if x.dtype not in _DT or x.dim() < 1:
         raise RuntimeError(f"{_NAME}: x must be float32, bfloat16 or float16 with a feature dimension")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise RuntimeError(f"{_NAME}: tensors must be on a HIP device (got {x.device})")
     k = x.shape[-1]
     if gate_weight is not None:
         _check_pair(_NAME, gate_weight, up_weight)
         if gate_weight.shape[1] != k:
             raise RuntimeError(f"{_NAME}: x has {k} features, the weights {gate_weight.shape[1]}")
-        if gate_weight.device != x.device or up_weight.device != x.device:
+        if gate_weight.get_device() != x.get_device() or up_weight.get_device() != x.get_device():
             raise RuntimeError(f"{_NAME}: weights must be on {x.device}")
     if packed is None:
         packed = pack_gated(gate_weight, up_weight)
     else:
         qw, scales = packed
         _require_gpu(_NAME, qw, scales)
-        if qw.dtype != torch.uint8 or qw.dim() != 2 or qw.shape[0] % 2 or qw.shape[0] == 0 or qw.device != x.device \
-                or scales.dtype != torch.float32 or scales.numel() != 2 or scales.device != x.device:
+        if qw.dtype != torch.uint8 or qw.dim() != 2 or qw.shape[0] % 2 or qw.shape[0] == 0 \
+                or scales.dtype != torch.float32 or scales.numel() != 2 or qw.get_device() != x.get_device():
             raise RuntimeError(f"{_NAME}: packed must be uint8 [2 * hidden, k_pad / 4] and fp32 [2] on {x.device}")
         if 4 * qw.shape[1] != (k + QK_I2_S - 1) // QK_I2_S * QK_I2_S:
             raise RuntimeError(f"{_NAME}: x has {k} features, packed rows hold {4 * qw.shape[1]}")
         if gate_weight is not None and gate_weight.shape[0] != qw.shape[0] // 2:
             raise RuntimeError(f"{_NAME}: packed has {qw.shape[0] // 2} hidden features, the weights {gate_weight.shape[0]}")
     f = packed.qweight.shape[0] // 2
-    x2 = x.reshape(-1, k) if k else x.new_empty((0, 0))
+    x2 = x if x.dim() == 2 else x.reshape(-1, k) if k else x.new_empty((0, 0))
     if not x2.is_contiguous() or x2.is_neg():
         x2 = x2.resolve_neg().contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, gate_weight, up_weight)):
+    if torch.is_grad_enabled() and (
+            x2.requires_grad or (gate_weight is not None and (gate_weight.requires_grad or up_weight.requires_grad))):
         if gate_weight is None:
             raise RuntimeError(f"{_NAME}: packed weights alone have no float weights to train")
         h = _GatedSTE.apply(x2, gate_weight, up_weight, packed.qweight, packed.scales, act)
     else:
         h = _forward(x2, packed, act, False)[0]
-    return h.view(*x.shape[:-1], f)
+    return h if x.dim() == 2 else h.view(*x.shape[:-1], f)
 
 
 class GatedBitLinear(nn.Module):
