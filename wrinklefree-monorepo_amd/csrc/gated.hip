@@ -92,33 +92,33 @@ __device__ __forceinline__ void load_d(const GradSrc& p, int row, int c, float (
 __device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // The largest magnitude (as bits: a NaN is the largest) of every row of [d_gate w_gate | d_up w_up] and of every
-// column of d a, over tiles of 64 columns and kTopRows rows: row_part[f tile][m], col_part[row tile][2 f].
-constexpr int kTopRows = 256;
-
+// column of d a, over tiles of 64 columns and `rows` rows: row_part[f tile][m], col_part[row tile][2 f].
 template <int ACT, int GDT>
-__device__ __forceinline__ void gated_top(const GradSrc& p, int bx, int by, uint32_t* __restrict__ row_part,
+__device__ __forceinline__ void gated_top(const GradSrc& p, int bx, int by, int rows, uint32_t* __restrict__ row_part,
                                           uint32_t* __restrict__ col_part, uint32_t (&red)[2][16][64]) {
-  const int cq = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = bx * 64 + 4 * cq, m0 = by * kTopRows;
+  const int cq = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = bx * 64 + 4 * cq, m0 = by * rows;
   const float w0 = p.scales[0], w1 = p.scales[1];
   uint32_t cg[4] = {0, 0, 0, 0}, cu[4] = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int j = 0; j < kTopRows / 16; ++j) {
-    const int row = m0 + r0 + 16 * j, rc = min(row, p.m - 1);
-    float dg[4], du[4];
-    load_d<ACT, GDT>(p, rc, c, dg, du);
-    const float a = p.a_scale[rc];
-    uint32_t top = 0;
+  for (int j0 = 0; j0 < rows; j0 += 64) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      top = max(top, max(mag(dg[e] * w0), mag(du[e] * w1)));
-      cg[e] = max(cg[e], mag(dg[e] * a));
-      cu[e] = max(cu[e], mag(du[e] * a));
+    for (int j = 0; j < 4; ++j) {
+      const int row = m0 + j0 + r0 + 16 * j, rc = min(row, p.m - 1);
+      float dg[4], du[4];
+      load_d<ACT, GDT>(p, rc, c, dg, du);
+      const float a = p.a_scale[rc];
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        top = max(top, max(mag(dg[e] * w0), mag(du[e] * w1)));
+        cg[e] = max(cg[e], mag(dg[e] * a));
+        cu[e] = max(cu[e], mag(du[e] * a));
+      }
+      top = max(top, (uint32_t)xor_lanes<1>((int)top));
+      top = max(top, (uint32_t)xor_lanes<2>((int)top));
+      top = max(top, (uint32_t)xor_lanes<4>((int)top));
+      top = max(top, (uint32_t)xor_lanes<8>((int)top));
+      if (cq == 0 && row < p.m) row_part[(int64_t)bx * p.m + row] = top;
     }
-    top = max(top, (uint32_t)xor_lanes<1>((int)top));
-    top = max(top, (uint32_t)xor_lanes<2>((int)top));
-    top = max(top, (uint32_t)xor_lanes<4>((int)top));
-    top = max(top, (uint32_t)xor_lanes<8>((int)top));
-    if (cq == 0 && row < p.m) row_part[(int64_t)bx * p.m + row] = top;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) red[0][r0][4 * cq + e] = cg[e], red[1][r0][4 * cq + e] = cu[e];
@@ -173,7 +173,7 @@ struct Operands {
   bool vec;  // codes' rows 16-byte aligned
   int K, mp;
   uint16_t *wt, *ct;  // null: not wanted
-  int tops, top_tiles, weights, weight_tiles, code_tiles;  // workgroups of each part, tiles of its first dimension
+  int top_rows, tops, top_tiles, weights, weight_tiles, code_tiles;  // workgroups of each part, tiles of its first dimension
 };
 
 template <int ACT, int GDT>
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) void gated_top_kernel(GradSrc p, Operands o, u
     __attribute__((aligned(4))) int8_t c[64][68];
   } lds;
   int b = blockIdx.x;
-  if (b < o.tops) return gated_top<ACT, GDT>(p, b % o.top_tiles, b / o.top_tiles, row_part, col_part, lds.red);
+  if (b < o.tops) return gated_top<ACT, GDT>(p, b % o.top_tiles, b / o.top_tiles, o.top_rows, row_part, col_part, lds.red);
   b -= o.tops;
   if (b < o.weights)
     return gated_weights_t(o.qw, o.row_bytes, p.f, p.fp, o.K, b % o.weight_tiles, b / o.weight_tiles, o.wt, lds.w);
@@ -212,8 +212,10 @@ __global__ __launch_bounds__(256) void gated_scale_kernel(const uint32_t* __rest
   const uint32_t* src = i < m ? row_part + i : col_part + (i - m);
   const int tiles = i < m ? row_tiles : col_tiles, ld = i < m ? m : n;
   uint32_t v = 0;
-#pragma unroll 8
-  for (int t = 0; t < tiles; ++t) v = max(v, src[(int64_t)t * ld]);
+  for (int t = 0; t < tiles; t += 32) {  // (the last one again past the end: 32 loads in flight, of one thread's chain)
+#pragma unroll
+    for (int u = 0; u < 32; ++u) v = max(v, src[(int64_t)min(t + u, tiles - 1) * ld]);
+  }
   const float s = plane_scale(v);
   scale[i] = s;
   inverse[i] = 1.0f / s;  // (a power of two)
@@ -330,7 +332,7 @@ hipError_t run_gemm16(GradGemm p, const Plan& pl, int64_t C, float* parts, hipSt
 // The backward pass's buffers, one behind the other in its workspace.
 struct GradLayout {
   int px, pw;  // planes, 0: result not wanted
-  int64_t fp, mp, row_tiles, col_tiles;
+  int64_t fp, mp, top_rows, row_tiles, col_tiles;
   int64_t row_part, col_part, scale, inverse, ax, bx, aw, bw, parts_x, parts_w, bytes;
   Plan plan_x, plan_w;
 };
@@ -342,7 +344,11 @@ GradLayout grad_layout(const GatedGrad& p) {
   l.fp = gated_pad(p.f);
   l.mp = pad_to(p.m, kPad);
   l.row_tiles = l.fp / 64;
-  l.col_tiles = (p.m + kTopRows - 1) / kTopRows;
+  // Rows of a tile that gated_top takes: 256, or 64 where that makes fewer than three workgroups a CU (509 x 1536 6.2 against
+  // 13.9 us, 1024 x 6912 27 against 35, 700 x 14336 62 against 74; 2048 x 6912 44 both, 2000 x 14336 102 against 99).  Many
+  // rows leave enough of them, and more parts would only lengthen the columns' maxima.
+  l.top_rows = p.m <= 4096 && l.row_tiles * ((p.m + 255) / 256) < 768 ? 64 : 256;
+  l.col_tiles = (p.m + l.top_rows - 1) / l.top_rows;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -441,7 +447,7 @@ hipError_t launch_gated_grad(const GatedGrad& p, void* work, hipStream_t s) {
   ops.codes = p.codes, ops.lda = p.lda, ops.vec = (uintptr_t)p.codes % 16 == 0 && p.lda % 16 == 0;
   ops.K = (int)p.k, ops.mp = (int)l.mp;
   ops.wt = l.px ? bx : nullptr, ops.ct = l.pw ? bw : nullptr;
-  ops.top_tiles = (int)l.row_tiles, ops.tops = (int)(l.row_tiles * l.col_tiles);
+  ops.top_rows = (int)l.top_rows, ops.top_tiles = (int)l.row_tiles, ops.tops = (int)(l.row_tiles * l.col_tiles);
   ops.weight_tiles = (int)(2 * l.fp / 64), ops.weights = l.px ? ops.weight_tiles * (int)((p.k + 127) / 128) : 0;
   ops.code_tiles = (int)(l.mp / 64);
   hipError_t e;
