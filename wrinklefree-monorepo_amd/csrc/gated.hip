@@ -18,8 +18,8 @@
 // Three passes: the largest of every row and column of d (gated_top_kernel, gated_scale_kernel), the planes in the order in
 // which the products read them (gated_planes_kernel; ternary weights and codes likewise), the two products (grad_tile.h).
 // The largest values have to be known before the first plane is written, so d is formed twice, and both passes are bound by
-// memory: 4096 tokens of 2560 -> 6912 with fp32 weights 74 us (393 MB with the transposed operands), 11 for the factors and
-// 120 us (622 MB, 5.2 TB/s).  The products take 450 (two planes) and 259 us there, 1.29 and 1.12 PFLOP/s.
+// memory: 4096 tokens of 2560 -> 6912 with fp32 weights 73 us (393 MB with the transposed operands), 6 for the factors and
+// 120 us (622 MB, 5.2 TB/s).  The products take 440 (two planes) and 259 us there, 1.32 and 1.12 PFLOP/s.
 #include <algorithm>
 
 #include "grad_tile.h"
