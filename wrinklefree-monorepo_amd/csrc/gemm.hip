@@ -356,6 +356,8 @@ hipError_t launch_skinny(const uint8_t* W, int n, int C, const int8_t* A, int m,
 //  * GL with TN = 2 (pair tiles): a wave's two weight tiles are 32 gate rows and their 32 up rows, so a lane holds both
 //    products of an output.  They pass through the wave's LDS to lie in rows (as for EPI = 2); act(gate) * up is computed
 //    and stored in the output's type and, for a backward pass, both products are stored fp32 as well.
+//    Of 128 tokens (TM = 4) they multiply by v_mfma_i32_16x16x64_i8, whose sums pass through the registers half as often for a
+//    product: 2048 x 2560 x 6912 96 -> 91 us with the quantiser.
 constexpr int kGroupM = 8;
 
 typedef __attribute__((address_space(3))) void lds_void;
