@@ -356,8 +356,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, float*
 #pragma unroll
             for (int e = 0; e < 2 * V; ++e) {
               const float n = (e < V ? xa[it][h].get(e) : xb[it][h].get(e - V)) * r;
-              // (a row past the last one has g = x = 0; one without a position adds its NaN)
-              acc[it][e] = __builtin_fmaf(on ? g[it][e] : 0.0f, n, acc[it][e]);
+              // (a row past the last one has x = 0, and with eps = 0 its n is NaN; one without a position adds its NaN)
+              acc[it][e] = on ? __builtin_fmaf(g[it][e], n, acc[it][e]) : acc[it][e];
               y[e] = r * __builtin_fmaf(g[it][e], w[it][e], -(n * m));
             }
           } else {
