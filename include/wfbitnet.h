@@ -532,7 +532,7 @@ typedef struct wfb_rope {
 
 /* out = rotate(x * rsqrt(mean(x^2) + eps) * weight) of every query and key head, fp32 arithmetic, rounded once to dtype
  * (that of x, g and out).  head_dim even, 2..WFB_QK_MAX_DIM; rotary_dim even, 0..head_dim.  The rotation: WF/models/
- * attention.py:14-64 (interleaved), the stage-1 model's (halves). */
+ * attention.py:14-64 (interleaved), the stage-1 model's (halves).  eps >= 0. */
 #define WFB_QK_MAX_DIM 256
 int wfb_qk_norm_rope(const wfb_heads* q, const wfb_heads* k, const wfb_rope* rope, int dtype, int64_t batch, int64_t t,
                      int64_t head_dim, float eps, void* stream);

@@ -947,6 +947,7 @@ static int qk_rope_args(const char* name, const wfb_heads* q, const wfb_heads* k
   if (!valid_dtype(dtype)) return fail(WFB_EINVAL, "%s: bad dtype %d", name, dtype);
   if (head_dim < 2 || head_dim > WFB_QK_MAX_DIM || head_dim % 2 != 0)
     return fail(WFB_EINVAL, "%s: head_dim (%lld) must be even and in 2..%d", name, (long long)head_dim, WFB_QK_MAX_DIM);
+  if (!(eps >= 0.0f)) return fail(WFB_EINVAL, "%s: eps must be >= 0", name);
   if (rope->rotary_dim < 0 || rope->rotary_dim > head_dim || rope->rotary_dim % 2 != 0)
     return fail(WFB_EINVAL, "%s: rotary_dim (%lld) must be even and in 0..head_dim", name, (long long)rope->rotary_dim);
   if (batch < 0 || t < 0 || batch > INT32_MAX || t > INT32_MAX || q->heads < 0 || k->heads < 0 || q->heads > 65535 || k->heads > 65535)

@@ -124,7 +124,7 @@ def qk_norm_rope(
     fp32, bf16 or fp16 with contiguous heads (slices of one q|k|v projection go as they are); the results are contiguous.
     cos / sin fp32 [positions, rotary_dim / 2].  ``positions``: int32 or int64 [batch, tokens] or [tokens] on the
     device, or the first token's as a number (None: 0).  One of the device's that the tables do not hold gives a row of
-    NaN.  layout "half" turns pairs (i, i + rotary_dim / 2) of a head's first rotary_dim elements, "interleaved" pairs
+    NaN.  eps >= 0; layout "half" turns pairs (i, i + rotary_dim / 2) of a head's first rotary_dim elements, "interleaved" pairs
     (2 i, 2 i + 1).  Statistics and rotation are fp32, a result is rounded once."""
     if layout not in _LAYOUTS:
         raise ValueError(f"{_NAME}: layout must be one of {sorted(_LAYOUTS)}")
