@@ -11,7 +11,8 @@
 // so an element's step never grows because its r went below the grid.  z in [0, 1) runs through a Weyl sequence over
 // steps and elements: a moment that moves by less than a code's distance in a step still moves on average, which with
 // rounding to the nearest it would not (b2 = 0.999 moves r by 0.05% a step, neighbouring codes lie 0.8% apart at best).
-// Blocks whose largest is below 2^-100 are held as zeros; one with an infinity or a NaN has scale NaN.
+// Blocks whose largest is below 2^-100 are held as zeros; one with an infinity or a NaN has scale NaN.  A finite gradient
+// from 2^64 on has an infinite v: its element then only decays, in 32 bits for good; in 8 bits r is held as 2^63.
 #include <cmath>
 
 #include "train_ops.h"
@@ -23,6 +24,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBlock = WFB_ADAMW_BLOCK;          // elements of a block: a wave's 64 x 4
 constexpr int kTileBlocks = 16;                  // blocks of one workgroup
+constexpr float kLargestRoot = 0x1p63f;          // of a v past fp32's range, in 8 bits
 constexpr int kMaxTensors = 64;                  // of one launch: the table travels with the kernel's arguments
 
 struct Table {
@@ -122,9 +124,13 @@ __device__ __forceinline__ float root_of(float v) {
   return plain ? r : 0.0f;
 }
 
-// n / d, off by a rounding at most (equal to the rounded quotient in 10^8 random pairs): the reciprocal corrected once, the
-// quotient once.
+// n / d, correctly rounded: the reciprocal corrected once, the quotient once (every pair of significands tried on MI355X, 2^46)
+// where no step leaves the normal numbers; the few others, an infinite or a zero divisor among them, by the compiler's
+// division, about twice as long.
 __device__ __forceinline__ float quotient(float n, float d) {
+  const float a = fabsf(n);
+  const bool plain = d >= 0x1p-40f && d <= 0x1p20f && a <= 0x1p80f && (a >= 0x1p-100f || a == 0.0f);
+  if (__builtin_expect(!plain, 0)) return __fdiv_rn(n, d);
   float y = __builtin_amdgcn_rcpf(d);
   y = __builtin_fmaf(__builtin_fmaf(-d, y, 1.0f), y, y);
   const float q = __fmul_rn(n, y);
@@ -195,7 +201,14 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(Table tb, AdamWState st
         return __uint_as_float(max(max(__float_as_uint(fabsf(a)), __float_as_uint(fabsf(b))),
                                    max(__float_as_uint(fabsf(c)), __float_as_uint(fabsf(d)))));
       };
-      const float a = scale_of(wave_top(top4(m[0], m[1], m[2], m[3]))), t = scale_of(wave_top(top4(r[0], r[1], r[2], r[3])));
+      const float a = scale_of(wave_top(top4(m[0], m[1], m[2], m[3])));
+      float t = wave_top(top4(r[0], r[1], r[2], r[3]));
+      if (__builtin_expect(t == __builtin_inff() && a == a, 0)) {  // (the wave agrees) a square past fp32, of a finite gradient
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = fminf(r[e], kLargestRoot);
+        t = kLargestRoot;
+      }
+      t = scale_of(t);
       const float ka = a > 0.0f ? __fdiv_rn(16129.0f, a) : 0.0f, kt = t > 0.0f ? __fdiv_rn(65025.0f, t) : 0.0f;
       const uint32_t turn = (uint32_t)s * 0x9E3779B1u + c.turn;
       uint32_t q[4], u[4];

@@ -88,7 +88,9 @@ def adamw_step(
     :func:`adamw_state` for the same list.  Decoupled weight decay; arithmetic in fp32, parameters rounded once.
     For a captured graph ``step`` is an int64 device tensor of one element, which the caller counts up, and ``lr`` may be an
     fp32 one; a replay changes no version counters, so packs that modules keep outside the graph are renewed by their
-    ``pack()``.  No two tensors may share memory.  A gradient that is not finite spoils its own element, and in 8 bits the moments of its block of 256."""
+    ``pack()``.  No two tensors may share memory.  A gradient that is not finite spoils its own element, and in 8 bits the
+    moments of its block of 256.  One whose square fp32 does not hold (from 1.8e19) has v = infinity: its element only decays
+    from then on; in 8 bits sqrt(v) is held as 2^63, and its block takes small steps until that has decayed."""
     name = "adamw_step"
     bits, dev = _check_state(name, state)
     if len(params) != len(grads):
