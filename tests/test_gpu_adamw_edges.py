@@ -91,3 +91,36 @@ def test_a_square_that_is_subnormal(pkg, dev):
     eight = pkg.adamw_state(own, 8)
     pkg.adamw_step([torch.ones(512, device=dev)], [g.to(dev)], eight, 1, **hyper)
     assert bool((eight.v == 255).all()) and float(eight.v_scale[0]) == float(v.sqrt()[0])
+
+
+def test_the_root_of_every_significand(pkg, dev):
+    """All 2^24 significands under both parities of the exponent: with m = r, the rounded root of v, the step is r / sqrt(v),
+    which is 1 only where the kernel's root is r: one that is an ulp off, a relative 2^-24 at least, gives another quotient
+    (an ulp below r a relative step above 2^-24 past 1, an ulp above r a step of 2^-25 at least below it)."""
+    v = torch.arange(1 << 24, dtype=torch.int32, device=dev).add_(127 << 23).view(F32)  # [1, 4)
+    r = v.double().sqrt().float()  # (53 bits round to 24 as the root itself does)
+    p = [torch.zeros(1 << 24, device=dev)]
+    # b = 1/2 halves m and v exactly; after 200 steps both corrections are 1
+    state = pkg.AdamWState(2.0 * r, 2.0 * v)
+    pkg.adamw_step(p, [torch.zeros(1 << 24, device=dev)], state, 200, lr=1.0, betas=(0.5, 0.5), eps=0.0, weight_decay=0.0)
+    assert torch.equal(state.v, v) and torch.equal(state.m, r)
+    assert bool((p[0] == -1.0).all())
+
+
+@pytest.mark.parametrize("exponent", [-60, -1, 0, 40])
+def test_the_quotient_of_every_divisor(pkg, dev, exponent):
+    """Every significand of the divisor under significands of the numerator next to it, at its ends and at random; 64 bits
+    round to 24 as the quotient itself does."""
+    d = torch.arange(1 << 23, dtype=torch.int32, device=dev).add_(127 << 23).view(F32)  # [1, 2)
+    v = d * d
+    d = v.double().sqrt().float()
+    ulp = 2.0 ** -23
+    gen = torch.Generator(device=dev).manual_seed(11)
+    tops = [torch.ones_like(d), torch.full_like(d, 2.0 - ulp), (d - ulp).clamp(min=1.0), (d + ulp).clamp(max=2.0 - ulp),
+            *(1.0 + torch.randint(1 << 23, d.shape, generator=gen, device=dev).float() * ulp for _ in range(4))]
+    for n in tops:
+        n = n * 2.0 ** exponent
+        p = [torch.zeros_like(d)]
+        state = pkg.AdamWState(2.0 * n, 2.0 * v)
+        pkg.adamw_step(p, [torch.zeros_like(d)], state, 200, lr=1.0, betas=(0.5, 0.5), eps=0.0, weight_decay=0.0)
+        assert torch.equal(p[0], -(n.double() / d.double()).float())

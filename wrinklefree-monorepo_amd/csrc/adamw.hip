@@ -109,7 +109,7 @@ __device__ __forceinline__ float scale_of(float v) {
 
 // The correctly rounded square root of x in [2^-100, 2^127]: x times the reciprocal root and one correction by the
 // residual, whose fused rounding is the last.  Equal to the rounded double root for every significand under both
-// parities of the exponent (all 2^25 inputs tried on MI355X); five operations, where the compiler's sqrtf, which also
+// parities of the exponent (all 2^24 tried on MI355X); five operations, where the compiler's sqrtf, which also
 // takes subnormal numbers, needs about sixteen.
 __device__ __forceinline__ float root_rn(float x) {
   const float y = __builtin_amdgcn_rsqf(x), s = __fmul_rn(x, y), h = 0.5f * y;
