@@ -1,0 +1,94 @@
+"""The gated product and its gradients in the forms that only large calls take, with remainders in every dimension, against
+float64.
+
+Bounds: forward, the sums are exact; gate and up take two fp32 roundings each, relu squared three more: 8 of 2^-24, silu
+4 |g| + 16, and half a step of the result's type.  Gradients: a term is off by 2^-12 (bf16 results: one fp16 plane) or 2^-23 (two planes) and
+by the few roundings of d, their sum by at most sqrt(C / 8) of 2^-24, and half a step of the result's type: relative to the
+root of the sum's squared terms, over the whole and three times that over every row and column."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+GRAD_BOUND = {F32: 2e-6, BF16: 2.0 ** -12 + 2.0 ** -9, F16: 2e-6 + 2.0 ** -11}
+
+
+def _case(dev, m, k, f, dtype, wdtype):
+    g = torch.Generator(device=dev).manual_seed(31 * m + 7 * k + f)
+    rand = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    x = (rand(m, k) * (1 + rand(m, 1).abs())).to(dtype)
+    return x, (rand(f, k) * 0.05).to(wdtype), (rand(f, k) * 0.03).to(wdtype), rand(m, f).to(dtype)
+
+
+def _exact(pkg, x, gate, up, act, gh):
+    """(h, gate, (grad_x, root), (grad_gate, root), (grad_up, root)) in float64 from the packs' and the quantiser's own codes."""
+    k = x.shape[1]
+    mats = []
+    for w in (gate, up):
+        qw, s = pkg.pack_ternary_i2s(w, k_pad=(k + 127) // 128 * 128)
+        mats.append((pkg.unpack_i2s(qw)[:, :k].double(), float(s)))
+    q, a = pkg.quantize_activations_i8_per_token(x)
+    held = q.double() * a.double()[:, None]
+    yg, yu = (held @ t.t() * s for t, s in mats)
+    if act == "silu":
+        sig = torch.sigmoid(yg)
+        z, slope = yg * sig, sig * (1 + yg * (1 - sig))
+    else:
+        z, slope = yg.clamp(min=0) ** 2, 2 * yg.clamp(min=0)
+    d = [gh.double() * yu * slope, gh.double() * z]
+    gx = sum((di * s) @ t for di, (t, s) in zip(d, mats))
+    rx = sum((di * s).square() @ t.square() for di, (t, s) in zip(d, mats)).sqrt()
+    out = [z * yu, yg, (gx, rx)]
+    for di in d:
+        dt = di.t().contiguous()
+        out.append((dt @ held, (dt.square() @ held.square()).sqrt()))
+    return out
+
+
+def _near(got, ref, bound, what):
+    value, root = ref
+    d = got.double() - value
+    assert torch.isfinite(got).all(), what
+    size = value.abs().maximum(root)
+    assert float(d.norm()) <= bound * float(size.norm()), (what, float(d.norm() / size.norm()))
+    for dim in (0, 1):
+        off, s = d.norm(dim=dim), size.norm(dim=dim)
+        # below its normal numbers a type's half step is constant, tiny * eps / 2: sqrt(n) of them in a norm
+        least = torch.finfo(got.dtype).tiny * torch.finfo(got.dtype).eps / 2 * value.shape[dim] ** 0.5
+        assert bool((off <= 3 * bound * s + least).all()), (what, dim, float((off / s).max()))
+
+
+def _run(pkg, x, gate, up, gh, act):
+    leaves = [t.detach().clone().requires_grad_() for t in (x, gate, up)]
+    h = pkg.gated_bitlinear(*leaves, act=act)
+    return (h.detach(), *torch.autograd.grad(h, leaves, gh))
+
+
+# The forward takes its tiles of 128 tokens in each (from 400 of them): one token and two columns past whole tiles, so that no
+# row of the output starts aligned; four columns past them; and the gradients' products take their tiles of 128 x 128 in one
+# plane (grad_x of the fourth, the weights' of the second), 128 x 256 in two (grad_x of the third) and the ring of 256 x 256 in two
+# planes with a part of a tile's columns (the weights' of the second and the third)
+@pytest.mark.parametrize("m,k,f", [(2433, 200, 2690), (2500, 640, 2564), (1099, 194, 19764), (4100, 300, 2180)])
+@pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("act", ["silu", "relu2"])
+def test_forms_of_large_calls(pkg, dev, m, k, f, dtype, wdtype, act):
+    x, gate, up, gh = _case(dev, m, k, f, dtype, wdtype)
+    if dtype == F16:
+        gh = gh * 2.0 ** -10  # (weight gradients within fp16's range)
+    h, gx, gg, gu = _run(pkg, x, gate, up, gh, act)
+    rh, yg, rx, rg, ru = _exact(pkg, x, gate, up, act, gh)
+    roundings = 4 * yg.abs() + 16 if act == "silu" else 8
+    assert bool(((h.double() - rh).abs() <= rh.abs() * (roundings * 2.0 ** -24 + torch.finfo(dtype).eps / 2) * 1.001
+                 + torch.finfo(dtype).tiny).all())
+    _near(gx, rx, GRAD_BOUND[dtype], "grad_x")
+    _near(gg, rg, GRAD_BOUND[wdtype], "grad_gate")
+    _near(gu, ru, GRAD_BOUND[wdtype], "grad_up")
+    with torch.no_grad():
+        packed = pkg.pack_gated(gate, up)
+        assert torch.equal(pkg.gated_bitlinear(x, act=act, packed=packed), h)
+        # the same operations on the same integers in every form: the few-token forms' bits
+        for first in (0, 1000, m - 40):
+            assert torch.equal(pkg.gated_bitlinear(x[first:first + 40], act=act, packed=packed), h[first:first + 40])
+        assert torch.equal(pkg.gated_bitlinear(x[-5:], act=act, packed=packed), h[-5:])
