@@ -58,6 +58,14 @@ def pack_gated(gate_weight: torch.Tensor, up_weight: torch.Tensor) -> PackedGate
     return PackedGated(qweight, scales)
 
 
+def _capturing(dev: torch.device) -> bool:
+    """Whether the device's current stream is being captured into a graph."""
+    if dev.type != "cuda":
+        return False
+    with _on(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _forward(x2: torch.Tensor, packed: PackedGated, act: str, keep: bool):
     """(h, gate|up or None, codes, a_scale) of the rows x2."""
     n, kb = packed.qweight.shape
@@ -176,7 +184,9 @@ class GatedBitLinear(nn.Module):
     """act(gate_proj(x)) * up_proj(x) of two bias-free ternary projections, on one set of activation codes; in front of a
     :class:`SubLNBitLinear` it is the feed-forward block of the converted models
     (packages/training/src/wrinklefree/training/stage1.py:93-166).  ``gate_proj`` and ``up_proj`` hold the float weights under
-    the names of the linears that they replace; the pack of both is rebuilt when either has changed."""
+    the names of the linears that they replace; the pack of both is rebuilt when either has changed, and made anew by every
+    replay of a captured call (a graph that serves fixed weights saves that with ``gated_bitlinear(x, packed=mod.packed())``,
+    the pack kept as long as the graph)."""
 
     def __init__(self, in_features: int, hidden_features: int, act: str = "silu", device=None, dtype=None):
         super().__init__()
@@ -187,6 +197,7 @@ class GatedBitLinear(nn.Module):
         self.up_proj = BitLinear(in_features, hidden_features, device=device, dtype=dtype)
         self._packed: Optional[PackedGated] = None
         self._packed_from = None
+        self._packed_on = None
 
     @classmethod
     def from_linears(cls, gate_proj: nn.Linear, up_proj: nn.Linear, act: str = "silu") -> "GatedBitLinear":
@@ -199,17 +210,31 @@ class GatedBitLinear(nn.Module):
         return mod
 
     def packed(self) -> PackedGated:
-        """The weights' pack, rebuilt if a weight changed since the last one."""
+        """The weights' pack, rebuilt if a weight changed since the last one, and ready for the current stream.  While that
+        stream is captured, a new pack that belongs to the graph, whose replays make it of what the weights hold then."""
+        gate, up = self.gate_proj.weight, self.up_proj.weight
+        if _capturing(gate.device):
+            return pack_gated(gate, up)
         stamp = (self.gate_proj._weight_stamp(), self.up_proj._weight_stamp())
         if self._packed is None or self._packed_from != stamp:
-            self._packed = pack_gated(self.gate_proj.weight, self.up_proj.weight)
+            self._packed = pack_gated(gate, up)
             self._packed_from = stamp
+            stream = torch.cuda.current_stream(gate.device)
+            self._packed_on = (stream.cuda_stream, stream.record_event())
+        elif self._packed_on[0] != _stream(gate.device):
+            # made on another stream: wait for it there, and keep its memory until this stream has read it
+            stream = torch.cuda.current_stream(gate.device)
+            stream.wait_event(self._packed_on[1])
+            for t in self._packed:
+                t.record_stream(stream)
         return self._packed
 
     def pack(self) -> "GatedBitLinear":
-        """Rebuild the pack whether or not the weights show a change (those that a replayed graph steps do not)."""
-        self._packed = None
-        self.packed()
+        """Rebuild the pack whether or not the weights show a change (those that a replayed graph steps do not).  Within a
+        capture there is nothing to rebuild: its calls pack for themselves."""
+        if not _capturing(self.gate_proj.weight.device):
+            self._packed = None
+            self.packed()
         return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -217,7 +242,7 @@ class GatedBitLinear(nn.Module):
         return gated_bitlinear(x, self.gate_proj.weight, self.up_proj.weight, self.act, self.packed())
 
     def __getstate__(self):
-        return {**self.__dict__, "_packed": None, "_packed_from": None}
+        return {**self.__dict__, "_packed": None, "_packed_from": None, "_packed_on": None}
 
     def extra_repr(self) -> str:
         return f"act={self.act}"
