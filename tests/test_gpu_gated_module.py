@@ -106,3 +106,19 @@ def test_a_training_step_without_a_pack_in_it(pkg, dev):
         assert all(torch.equal(a, b) for a, b in zip(*weights))
     assert not torch.equal(_fresh(pkg, mod, x), _fresh(pkg, _module(pkg, dev)[0], x))  # (the packs did change)
     assert torch.equal(mod.pack()(x).detach(), _fresh(pkg, mod, x))
+
+
+def test_weights_replaced_by_apply(pkg, dev):
+    """What a module's casts and moves go through may leave other values at the same address and version: so may a cast to
+    bf16 and back, whose last memory is the first one's, and here a function that writes through .data."""
+    mod, x = _module(pkg, dev)
+    with torch.no_grad():
+        first = mod(x)
+        stamps = [(w.data_ptr(), w._version) for w in mod.parameters()]
+        mod.apply(lambda m: None)
+        assert torch.equal(mod(x), first)
+        mod._apply(lambda t: t.data.mul_(torch.where(torch.arange(t.shape[1], device=dev) % 3 == 0, -1.0, 1.0)))
+        assert [(w.data_ptr(), w._version) for w in mod.parameters()] == stamps
+        assert torch.equal(mod(x), _fresh(pkg, mod, x)) and not torch.equal(mod(x), first)
+        mod.bfloat16().float()
+        assert torch.equal(mod(x), _fresh(pkg, mod, x))

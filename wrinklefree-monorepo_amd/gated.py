@@ -241,6 +241,11 @@ class GatedBitLinear(nn.Module):
         _check_lambda("GatedBitLinear")
         return gated_bitlinear(x, self.gate_proj.weight, self.up_proj.weight, self.act, self.packed())
 
+    def _apply(self, fn, recurse=True):
+        # (a weight that is cast and cast back may lie where it lay, its version counter unmoved)
+        self._packed = None
+        return super()._apply(fn, recurse)
+
     def __getstate__(self):
         return {**self.__dict__, "_packed": None, "_packed_from": None, "_packed_on": None}
 
