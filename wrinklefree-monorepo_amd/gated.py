@@ -14,12 +14,13 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import WFB_ABSMEAN_WS_DOUBLES
 from .bitlinear import BitLinear, _check_lambda
-from .ops import _ACTS, _DT, QK_I2_S, _on, _p, _require_gpu, _stream
+from .ops import _ACTS, _DT, QK_I2_S, _no_tangents, _on, _p, _require_gpu, _stream
 
 _NAME = "gated_bitlinear"
 
@@ -134,8 +135,8 @@ def gated_bitlinear(
     :func:`bitnet_linear_glu` with ``mid_dtype=float32``, rounded once.
 
     ``packed`` (of :func:`pack_gated`) saves packing the float weights; without them the call serves only.  With autograd on
-    and x or a weight requiring a gradient, the result is differentiable once, straight through both quantisers, and the
-    products are kept for it (8 bytes per token and hidden feature); x, gate_weight and up_weight get gradients in their
+    and x or a weight requiring a gradient, the result is differentiable once, straight through both quantisers (in reverse mode;
+    tangents of forward mode are refused), and the products are kept for it (8 bytes per token and hidden feature); x, gate_weight and up_weight get gradients in their
     types.  ``packed`` must then be the weights' own pack."""
     if act not in _ACTS:
         raise ValueError(f"{_NAME}: act must be one of {sorted(_ACTS)}")
@@ -170,6 +171,8 @@ def gated_bitlinear(
     x2 = x if x.dim() == 2 else x.reshape(-1, k) if k else x.new_empty((0, 0))
     if not x2.is_contiguous() or x2.is_neg():
         x2 = x2.resolve_neg().contiguous()
+    if forward_ad._current_level >= 0:
+        _no_tangents(_NAME, x2, gate_weight, up_weight)
     if torch.is_grad_enabled() and (
             x2.requires_grad or (gate_weight is not None and (gate_weight.requires_grad or up_weight.requires_grad))):
         if gate_weight is None:

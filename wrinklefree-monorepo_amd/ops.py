@@ -22,6 +22,7 @@ import weakref
 from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import (WFB_ABSMEAN_WS_DOUBLES, WFB_ACT_RELU2, WFB_ACT_SILU, WFB_BF16, WFB_F16, WFB_F32,
@@ -77,6 +78,13 @@ def _require_gpu(name: str, *ts: Optional[torch.Tensor]) -> torch.device:
             raise RuntimeError(f"{name}: tensors are on different devices ({first.device}, {t.device})")
     assert first is not None
     return first.device
+
+
+def _no_tangents(name: str, *ts: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors: the kernels give values without tangents.  (Called where a forward-mode level is entered.)"""
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name}: forward-mode derivatives are not supported")
 
 
 def _float_dtype(name: str, t: torch.Tensor) -> int:

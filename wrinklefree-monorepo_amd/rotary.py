@@ -14,11 +14,12 @@ from array import array
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import HeadsStruct, WFB_QK_MAX_DIM
-from .ops import _DT, _on, _stream
+from .ops import _DT, _no_tangents, _on, _stream
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _NAME = "qk_norm_rope"
@@ -118,7 +119,7 @@ def qk_norm_rope(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Queries and keys with their heads normed (x / sqrt(mean(x^2) + eps) * weight over the head's elements; a side
     without a weight is not normed) and turned by their positions' angles, in one pass; differentiable once, by q, k and
-    the weights.
+    the weights (in reverse mode; tangents of forward mode are refused).
 
     q [batch, tokens, heads, head_dim] and k [batch, tokens, kv_heads, head_dim], or both without the batch dimension,
     fp32, bf16 or fp16 with contiguous heads (slices of one q|k|v projection go as they are); the results are contiguous.
@@ -159,6 +160,8 @@ def qk_norm_rope(
         positions = 0 if positions is None else int(positions)
         if cos.shape[1] and not 0 <= positions <= cos.shape[0] - t:
             raise ValueError(f"{_NAME}: positions {positions}..{positions + t - 1} leave tables of {cos.shape[0]} rows")
+    if forward_ad._current_level >= 0:
+        _no_tangents(_NAME, q, k, q_weight, k_weight, cos, sin)
     q, k = _plain(q), _plain(k)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
