@@ -23,3 +23,26 @@ def test_epsilon_of_the_head_norm(pkg, eps, grad):
     at = [ctypes.addressof(s) for s in (heads, heads, rope)]
     name = "wfb_qk_norm_rope_grad" if grad else "wfb_qk_norm_rope"
     _no(pkg, "eps", pkg._lib.status(name, *at, 1, 2, 8, 64, eps, *([vp(0x100)] if grad else []), None))
+
+
+YARN = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096)
+
+
+@pytest.mark.parametrize("scaling", [
+    dict(YARN, mscale=1.0), dict(YARN, mscale_all_dim=0.7), dict(YARN, truncate=False), dict(YARN, low_freq_factor=1.0),
+    dict(type="linear", factor=2.0, beta_fast=32.0), dict(type="linear", factor=2.0, atention_factor=1.0),
+    dict(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192, short_factor=[1.0])])
+def test_scalings_with_unknown_keys(pkg, scaling):
+    with pytest.raises(ValueError, match="does not know"):
+        pkg.rope_tables(10000.0, 64, 16, scaling=scaling)
+
+
+def test_scalings_with_keys_that_are_not_set(pkg):
+    plain = pkg.rope_tables(10000.0, 64, 16, scaling=YARN)
+    same = pkg.rope_tables(10000.0, 64, 16, scaling=dict(YARN, type="yarn", attention_factor=None, mscale=None, beta_fast=32))
+    assert all(torch.equal(a, b) for a, b in zip(plain, same))
+    a = pkg.rope_tables(10000.0, 64, 16, scaling=dict(type="linear", factor=2.0))
+    b = pkg.rope_tables(10000.0, 64, 16, scaling=dict(type="linear", factor=2.0, original_max_position_embeddings=2048))
+    assert torch.equal(a[0], b[0])
+    with pytest.raises(ValueError, match="theta"):
+        pkg.rope_tables(1.0, 64, 16, scaling=YARN)

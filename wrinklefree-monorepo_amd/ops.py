@@ -864,10 +864,24 @@ def _rows2d(name: str, t: torch.Tensor, b: int, width: int) -> Tuple[torch.Tenso
     return t2, (t2.stride(0) if b > 1 else width)
 
 
+# What each type of scaling is made of.  (linear's original length has no part in it, but configurations carry it)
+_SCALING_KEYS = {
+    "linear": {"original_max_position_embeddings"},
+    "llama3": {"original_max_position_embeddings", "low_freq_factor", "high_freq_factor"},
+    "yarn": {"original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor"},
+}
+
+
 def _scaled_frequencies(theta: float, head_dim: int, scaling: dict) -> Tuple[List[float], float]:
     """(inverse frequencies, factor of the tables) of a rotary embedding scaled for longer contexts, in double precision."""
     name = "rope_tables"
     kind = scaling.get("rope_type", scaling.get("type"))
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"{name}: scaling type must be linear, llama3 or yarn, not {kind!r}")
+    unknown = {k for k, v in scaling.items() if v is not None} - _SCALING_KEYS[kind] - {"rope_type", "type", "factor"}
+    if unknown:  # (tables without their part would be other tables than the model's)
+        raise ValueError(f"{name}: {kind} scaling does not know {sorted(unknown)}")
+    scaling = {k: v for k, v in scaling.items() if v is not None}
     factor = float(scaling.get("factor", 1.0))
     if not factor >= 1.0:
         raise ValueError(f"{name}: scaling factor must be at least 1, not {factor}")
@@ -885,20 +899,20 @@ def _scaled_frequencies(theta: float, head_dim: int, scaling: dict) -> Tuple[Lis
             raise ValueError(f"{name}: low_freq_factor must be positive and below high_freq_factor")
         keep = [min(1.0, max(0.0, (length * f / (2 * math.pi) - low) / (high - low))) for f in inv]
         return [f * w + f / factor * (1.0 - w) for f, w in zip(inv, keep)], 1.0
-    if kind == "yarn":
-        # the same by the pair's index, between the pairs that turn beta_fast and beta_slow times; the tables grow with
-        # the factor's logarithm
-        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
-        if not 0 < slow < fast:
-            raise ValueError(f"{name}: beta_slow must be positive and below beta_fast")
-        index = [head_dim * math.log(length / (b * 2 * math.pi)) / (2 * math.log(theta)) for b in (fast, slow)]
-        first, last = max(math.floor(index[0]), 0), min(math.ceil(index[1]), head_dim - 1)
-        span = max(last - first, 1e-3)
-        keep = [1.0 - min(1.0, max(0.0, (i - first) / span)) for i in range(head_dim // 2)]
-        mscale = scaling.get("attention_factor")
-        mscale = 0.1 * math.log(factor) + 1.0 if mscale is None else float(mscale)
-        return [f * w + f / factor * (1.0 - w) for f, w in zip(inv, keep)], mscale
-    raise ValueError(f"{name}: scaling type must be linear, llama3 or yarn, not {kind!r}")
+    # yarn: the same by the pair's index, between the pairs that turn beta_fast and beta_slow times; the tables grow with
+    # the factor's logarithm
+    fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+    if not 0 < slow < fast:
+        raise ValueError(f"{name}: beta_slow must be positive and below beta_fast")
+    if not theta > 1:
+        raise ValueError(f"{name}: yarn scaling needs theta above 1, not {theta}")
+    index = [head_dim * math.log(length / (b * 2 * math.pi)) / (2 * math.log(theta)) for b in (fast, slow)]
+    first, last = max(math.floor(index[0]), 0), min(math.ceil(index[1]), head_dim - 1)
+    span = max(last - first, 1e-3)
+    keep = [1.0 - min(1.0, max(0.0, (i - first) / span)) for i in range(head_dim // 2)]
+    mscale = scaling.get("attention_factor")
+    mscale = 0.1 * math.log(factor) + 1.0 if mscale is None else float(mscale)
+    return [f * w + f / factor * (1.0 - w) for f, w in zip(inv, keep)], mscale
 
 
 def rope_tables(theta: float, head_dim: int, max_len: int,
@@ -907,7 +921,8 @@ def rope_tables(theta: float, head_dim: int, max_len: int,
     0..max_len-1 (angle p * theta^(-2i/head_dim) in double precision, rounded once to float): the tables
     the decode / prefill attention kernels take, the same values the native engine computes.  ``head_dim`` is the number of
     elements turned where that is only a part of a head (qk_norm_rope).  ``scaling`` is a model configuration's
-    ``rope_scaling`` of type linear, llama3 or yarn."""
+    ``rope_scaling`` of type linear, llama3 or yarn; one with a key that these do not know (yarn's ``mscale``, ``truncate``) is
+    refused."""
     name = "rope_tables"
     if head_dim < 2 or head_dim % 2 != 0 or max_len < 1 or not theta > 0:
         raise ValueError(f"{name}: bad theta / head_dim / max_len")
