@@ -158,6 +158,8 @@ def gated_bitlinear(
     if packed is None:
         packed = pack_gated(gate_weight, up_weight)
     else:
+        if packed.scales.is_neg():
+            packed = packed._replace(scales=packed.scales.resolve_neg())
         qw, scales = packed
         _require_gpu(_NAME, qw, scales)
         if qw.dtype != torch.uint8 or qw.dim() != 2 or qw.shape[0] % 2 or qw.shape[0] == 0 \

@@ -889,7 +889,7 @@ def _scaled_frequencies(theta: float, head_dim: int, scaling: dict) -> Tuple[Lis
     if kind == "linear":  # positions divided by the factor
         return [f / factor for f in inv], 1.0
     length = float(scaling.get("original_max_position_embeddings", 0))
-    if kind in ("llama3", "yarn") and not length > 0:
+    if not length > 0:
         raise ValueError(f"{name}: {kind} scaling needs original_max_position_embeddings")
     if kind == "llama3":
         # by the turns that a pair makes over the original length: few are slowed by the factor, many are left, and the

@@ -71,7 +71,7 @@ def _check_state(name: str, state: AdamWState) -> Tuple[int, torch.device]:
     if v.numel() != n or n % WFB_ADAMW_BLOCK:
         raise RuntimeError(f"{name}: m and v must have as many elements, a multiple of {WFB_ADAMW_BLOCK}")
     for t in (m, *rest):
-        if not t.is_contiguous() or t.device != m.device:
+        if not t.is_contiguous() or t.is_neg() or t.device != m.device:
             raise RuntimeError(f"{name}: the state must be contiguous and on one device")
     return bits, m.device
 
@@ -133,19 +133,21 @@ def adamw_step(
     if isinstance(step, torch.Tensor):
         if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
             raise RuntimeError(f"{name}: a step tensor must be one int64 element on {dev}")
-        step_dev, step = step.data_ptr(), 0
+        step = step.resolve_neg()
+        step_dev = step.data_ptr()
         scalars = torch.empty(WFB_ADAMW_SCALARS, dtype=torch.float32, device=dev)
     if isinstance(lr, torch.Tensor):
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev or step_dev is None:
             raise RuntimeError(f"{name}: a lr tensor must be one fp32 element on {dev} and goes with a step tensor")
-        lr_dev, lr = lr.data_ptr(), 0.0
+        lr = lr.resolve_neg()
+        lr_dev = lr.data_ptr()
     m, v, ms, vs = state
     with _on(dev):
         for pdt, gdt, rows in tables:
             _lib.call("wfb_adamw_step", rows.buffer_info()[0], len(rows) // 3, pdt, gdt, m.data_ptr(),
                       v.data_ptr(), None if ms is None else ms.data_ptr(), None if vs is None else vs.data_ptr(),
-                      m.numel(), bits, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
-                      int(step), step_dev, lr_dev, None if scalars is None else scalars.data_ptr(), _stream(dev))
+                      m.numel(), bits, 0.0 if lr_dev else float(lr), float(betas[0]), float(betas[1]), float(eps),
+                      float(weight_decay), 0 if step_dev else int(step), step_dev, lr_dev, None if scalars is None else scalars.data_ptr(), _stream(dev))
     if live:
         torch.autograd.graph.increment_version(live)
 
