@@ -1,0 +1,79 @@
+"""The optimizer class: steps counted for each tensor as torch counts them, refusals that leave no trace, state dicts that are
+checked before they are taken."""
+
+import copy
+import pickle
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = ((64, 33), (5,), (1000,), (300,))
+
+
+def _models(dev, n=2):
+    torch.manual_seed(0)
+    first = [torch.randn(s, device=dev) for s in SHAPES]
+    return [[torch.nn.Parameter(t.clone()) for t in first] for _ in range(n)]
+
+
+def _fill(models, have, seed):
+    g = torch.Generator(device=models[0][0].device).manual_seed(seed)
+    for i, ps in enumerate(zip(*models)):
+        grad = torch.randn(ps[0].shape, generator=g, device=ps[0].device)
+        for p in ps:
+            p.grad = grad.clone() if i in have else None
+
+
+# tensors that come late, that pause, that never come, and all from the start
+PATTERNS = [[{0, 1}] * 4 + [{0, 1, 2}] * 3 + [{0, 2}, {0, 1, 2}, {1}], [set(range(4))] * 5 + [{1, 3}] * 3 + [set(range(4))] * 2]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("pattern", PATTERNS)
+def test_each_tensor_counts_its_own_steps(pkg, dev, pattern, capturable):
+    """Against torch.optim.AdamW, whose operations are ordered otherwise: 10 steps of at most 4 lr (a moment that paused keeps
+    its size while its count stands) by 10 * 8 * 4 * 2^-24 lr, and 10 roundings of the parameter."""
+    a, b = _models(dev)
+    ours, theirs = pkg.AdamW(a, lr=1e-2, capturable=capturable), torch.optim.AdamW(b, lr=1e-2)
+    for t, have in enumerate(pattern):
+        _fill((a, b), have, t)
+        ours.step()
+        theirs.step()
+        if t == 5:  # a copy and a state dict on the way carry the counts
+            saved = pickle.loads(pickle.dumps(ours.state_dict()))
+            a, ours = copy.deepcopy((a, ours))
+            ours.load_state_dict(saved)
+    for p, q in zip(a, b):
+        bound = 10 * (8 * 4 * 1e-2 + float(q.detach().abs().max())) * 2.0 ** -24
+        assert float((p - q).detach().abs().max()) <= bound
+
+
+
+
+def test_captured_steps_of_some_tensors(pkg, dev):
+    a, b = _models(dev)
+    oa, ob = pkg.AdamW(a, lr=1e-2, capturable=True), pkg.AdamW(b, lr=1e-2)
+    for have, seed in ((set(range(4)), 0), ({0, 2}, 1)):
+        _fill((a, b), have, seed)
+        oa.step()
+        ob.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        oa.step()
+    for t in range(4):
+        grads = [p.grad for p in a]
+        _fill((b,), {0, 2}, 10 + t)
+        for g, q in zip(grads, b):
+            if g is not None:
+                g.copy_(q.grad)
+        graph.replay()
+        torch.cuda.synchronize()
+        ob.step()
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    _fill((a, b), set(range(4)), 20)  # and on, outside the graph
+    oa.step()
+    ob.step()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))

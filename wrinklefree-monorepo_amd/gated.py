@@ -20,7 +20,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._lib import WFB_ABSMEAN_WS_DOUBLES
 from .bitlinear import BitLinear, _check_lambda
-from .ops import _ACTS, _DT, QK_I2_S, _no_tangents, _on, _p, _require_gpu, _stream
+from .ops import _ACTS, _DT, QK_I2_S, _capturing, _no_tangents, _on, _p, _require_gpu, _stream
 
 _NAME = "gated_bitlinear"
 
@@ -57,14 +57,6 @@ def pack_gated(gate_weight: torch.Tensor, up_weight: torch.Tensor) -> PackedGate
     with _on(dev):
         _lib.call("wfb_pack_gated", _p(gate_weight), _p(up_weight), dt, f, k, _p(scales), _p(qweight), _p(ws), _stream(dev))
     return PackedGated(qweight, scales)
-
-
-def _capturing(dev: torch.device) -> bool:
-    """Whether the device's current stream is being captured into a graph."""
-    if dev.type != "cuda":
-        return False
-    with _on(dev):
-        return torch.cuda.is_current_stream_capturing()
 
 
 def _forward(x2: torch.Tensor, packed: PackedGated, act: str, keep: bool):

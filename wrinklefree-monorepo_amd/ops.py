@@ -63,6 +63,14 @@ def _on(dev: torch.device):
     return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
+def _capturing(dev: torch.device) -> bool:
+    """Whether the device's current stream is being captured into a graph."""
+    if dev.type != "cuda":
+        return False
+    with _on(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _require_gpu(name: str, *ts: Optional[torch.Tensor]) -> torch.device:
     first = None
     for t in ts:

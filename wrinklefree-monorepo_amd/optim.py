@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import WFB_ADAMW_BLOCK, WFB_ADAMW_SCALARS
-from .ops import _DT, _on, _stream
+from .ops import _DT, _capturing, _on, _stream
 
 
 _dtype_of = attrgetter("dtype")
@@ -53,16 +53,14 @@ def adamw_state(params: Iterable[torch.Tensor], bits: int = 32) -> AdamWState:
                       *(torch.zeros(blocks, dtype=torch.float32, device=dev) for _ in range(2)))
 
 
-def _check_state(name: str, state: AdamWState) -> Tuple[int, torch.device]:
-    """(bits, device) of a state."""
+def _bits_of(name: str, state: AdamWState) -> int:
+    """32 or 8, by types and sizes."""
     m, v, ms, vs = state
-    if m.device.type != "cuda":
-        raise RuntimeError(f"{name}: the state must be on a HIP device (got {m.device})")
     n = m.numel()
     if m.dtype == v.dtype == torch.float32 and ms is None and vs is None:
-        bits, rest = 32, (v,)
+        bits = 32
     elif m.dtype == torch.int8 and v.dtype == torch.uint8 and ms is not None and vs is not None:
-        bits, rest = 8, (v, ms, vs)
+        bits = 8
         if ms.dtype != torch.float32 or vs.dtype != torch.float32 or ms.numel() * WFB_ADAMW_BLOCK != n \
                 or vs.numel() * WFB_ADAMW_BLOCK != n:
             raise RuntimeError(f"{name}: scales must be fp32, one for each {WFB_ADAMW_BLOCK} elements")
@@ -70,7 +68,16 @@ def _check_state(name: str, state: AdamWState) -> Tuple[int, torch.device]:
         raise RuntimeError(f"{name}: a state is fp32 m and v, or int8 m and uint8 v with their scales")
     if v.numel() != n or n % WFB_ADAMW_BLOCK:
         raise RuntimeError(f"{name}: m and v must have as many elements, a multiple of {WFB_ADAMW_BLOCK}")
-    for t in (m, *rest):
+    return bits
+
+
+def _check_state(name: str, state: AdamWState) -> Tuple[int, torch.device]:
+    """(bits, device) of a state."""
+    m = state.m
+    if m.device.type != "cuda":
+        raise RuntimeError(f"{name}: the state must be on a HIP device (got {m.device})")
+    bits = _bits_of(name, state)
+    for t in state if bits == 8 else state[:2]:
         if not t.is_contiguous() or t.is_neg() or t.device != m.device:
             raise RuntimeError(f"{name}: the state must be contiguous and on one device")
     return bits, m.device
@@ -166,11 +173,14 @@ def adamw_state_values(state: AdamWState) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW``'s arguments and step over :func:`adamw_step`, ``state_bits`` 32 or 8.
+    """The step of ``torch.optim.AdamW`` over :func:`adamw_step`, with its ``lr``, ``betas``, ``eps`` and ``weight_decay`` (no
+    ``amsgrad``, ``maximize`` or ``foreach``) and states of ``state_bits`` 32 or 8.
 
-    A group has one state and one count of steps; its tensors are of one device.  With ``capturable`` the count lies on the
-    device and :meth:`step` can be captured into a graph (``lr`` may then be an fp32 device tensor); the first step, which makes
-    the state, comes before the capture.  The state dict holds the states as they are."""
+    A group has one flat state (:meth:`group_state`; ``state``, torch's dictionary of each parameter's, stays empty); its tensors
+    are of one device.  A tensor's steps are counted from its first gradient on and only where it has one, as torch counts
+    them; tensors of one count step in one call.  With ``capturable`` the counts lie on the device and :meth:`step` can be
+    captured into a graph (``lr`` may then be an fp32 device tensor), behind a step that made the state with gradients for
+    the same tensors.  The state dict holds the states as they are."""
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32, capturable: bool = False):
@@ -206,29 +216,61 @@ class AdamW(torch.optim.Optimizer):
         for i, group in enumerate(self.param_groups):
             params = group["params"]
             grads = [p.grad for p in params]
-            if all(g is None for g in grads):
+            have = [g is not None for g in grads]
+            if not any(have):
                 continue
-            if any(g is not None and g.is_sparse for g in grads):
+            if any([g is not None and g.is_sparse for g in grads]):
                 raise RuntimeError("AdamW: sparse gradients are not supported")
             flat = self._flat[i]
             if flat is None:
                 count = torch.zeros(1, dtype=torch.int64, device=params[0].device) if group["capturable"] else 0
-                flat = self._flat[i] = {"state": adamw_state(params, group["state_bits"]), "step": count}
-            flat["step"] += 1
-            adamw_step(params, grads, flat["state"], flat["step"], group["lr"], group["betas"], group["eps"],
-                       group["weight_decay"])
+                flat = self._flat[i] = {"state": adamw_state(params, group["state_bits"]), "steps": [(count, list(range(len(params))))]}
+            if len(flat["steps"]) > 1 or not all(have):
+                flat["steps"] = self._cohorts(flat["steps"], have)
+            for k, (count, of) in enumerate(flat["steps"]):
+                if not have[of[0]]:
+                    continue
+                if len(of) < len(params):
+                    mine = set(of)
+                    wanted = [g if j in mine else None for j, g in enumerate(grads)]
+                else:
+                    wanted = grads
+                args = (group["lr"], group["betas"], group["eps"], group["weight_decay"])
+                if group["capturable"]:
+                    count += 1
+                    adamw_step(params, wanted, flat["state"], count, *args)
+                else:
+                    flat["steps"][k] = (count + 1, of)
+                    adamw_step(params, wanted, flat["state"], count + 1, *args)
         return loss
+
+    @staticmethod
+    def _cohorts(steps, have: List[bool]) -> List[tuple]:
+        """(count, tensors) such that the tensors of one count all step now or all do not; equal counts on the host as one."""
+        out = []
+        for count, of in steps:
+            parts = [part for part in ([j for j in of if have[j]], [j for j in of if not have[j]]) if part]
+            if len(parts) == 2 and isinstance(count, torch.Tensor) and _capturing(count.device):
+                raise RuntimeError("AdamW: a captured step needs gradients for the tensors that stepped together before")
+            for n, part in enumerate(parts):
+                out.append((count.clone() if n and isinstance(count, torch.Tensor) else count, part))
+        if out and not isinstance(out[0][0], torch.Tensor):
+            joined: dict = {}
+            for count, part in out:
+                joined.setdefault((count, have[part[0]]), []).extend(part)
+            out = [(count, sorted(part)) for (count, _), part in joined.items()]
+        return out
 
     def state_dict(self) -> dict:
         d = super().state_dict()
-        d["flat"] = [None if f is None else {"state": tuple(f["state"]), "step": f["step"]} for f in self._flat]
+        d["flat"] = [None if f is None else {"state": tuple(f["state"]), "steps": [(c, list(of)) for c, of in f["steps"]]}
+                     for f in self._flat]
         return d
 
     def load_state_dict(self, state_dict: dict) -> None:
-        flat = state_dict["flat"]
         super().load_state_dict({k: v for k, v in state_dict.items() if k != "flat"})
         self._flat = []
-        for group, f in zip(self.param_groups, flat):
+        for group, f in zip(self.param_groups, state_dict["flat"]):
             if f is None:
                 self._flat.append(None)
                 continue
@@ -237,7 +279,7 @@ class AdamW(torch.optim.Optimizer):
             need = sum(_blocks(p.numel()) for p in group["params"]) * WFB_ADAMW_BLOCK
             if state.m.numel() != need:
                 raise ValueError(f"AdamW: the state has {state.m.numel()} elements, the group's tensors take {need}")
-            step = f["step"]
-            if group["capturable"]:
-                step = torch.as_tensor(step, dtype=torch.int64).reshape(1).to(dev, copy=True)
-            self._flat.append({"state": state, "step": step if group["capturable"] else int(step)})
+            steps = f["steps"] if "steps" in f else [(f["step"], range(len(group["params"])))]
+            counts = [torch.as_tensor(c, dtype=torch.int64).reshape(1).to(dev, copy=True) if group["capturable"] else int(c)
+                      for c, _ in steps]
+            self._flat.append({"state": state, "steps": [(c, list(of)) for c, (_, of) in zip(counts, steps)]})
