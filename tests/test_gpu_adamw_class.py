@@ -50,6 +50,24 @@ def test_each_tensor_counts_its_own_steps(pkg, dev, pattern, capturable):
         assert float((p - q).detach().abs().max()) <= bound
 
 
+def test_a_refused_step_is_not_counted(pkg, dev):
+    for capturable in (False, True):
+        a, b = _models(dev)
+        oa, ob = (pkg.AdamW(m, lr=1e-2, capturable=capturable) for m in (a, b))
+        for t in range(3):
+            _fill((a, b), set(range(4)), t)
+            if t == 1:
+                good = a[2].data
+                a[2].grad, a[2].data = None, torch.randn(1000, 2, device=dev).t()[:1].reshape(1000).as_strided((1000,), (0,))
+                a[2].grad = torch.zeros(1000, device=dev)
+                with pytest.raises(RuntimeError, match="contiguous"):
+                    oa.step()
+                a[2].grad, a[2].data = None, good
+                a[2].grad = b[2].grad.clone()
+            oa.step()
+            ob.step()
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
 
 
 def test_captured_steps_of_some_tensors(pkg, dev):

@@ -224,7 +224,7 @@ class AdamW(torch.optim.Optimizer):
             flat = self._flat[i]
             if flat is None:
                 count = torch.zeros(1, dtype=torch.int64, device=params[0].device) if group["capturable"] else 0
-                flat = self._flat[i] = {"state": adamw_state(params, group["state_bits"]), "steps": [(count, list(range(len(params))))]}
+                flat = {"state": adamw_state(params, group["state_bits"]), "steps": [(count, list(range(len(params))))]}
             if len(flat["steps"]) > 1 or not all(have):
                 flat["steps"] = self._cohorts(flat["steps"], have)
             for k, (count, of) in enumerate(flat["steps"]):
@@ -238,10 +238,15 @@ class AdamW(torch.optim.Optimizer):
                 args = (group["lr"], group["betas"], group["eps"], group["weight_decay"])
                 if group["capturable"]:
                     count += 1
-                    adamw_step(params, wanted, flat["state"], count, *args)
+                    try:
+                        adamw_step(params, wanted, flat["state"], count, *args)
+                    except Exception:
+                        count -= 1  # (refused, not stepped)
+                        raise
                 else:
-                    flat["steps"][k] = (count + 1, of)
                     adamw_step(params, wanted, flat["state"], count + 1, *args)
+                    flat["steps"][k] = (count + 1, of)
+            self._flat[i] = flat
         return loss
 
     @staticmethod
