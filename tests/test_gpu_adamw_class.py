@@ -69,6 +69,25 @@ def test_a_refused_step_is_not_counted(pkg, dev):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_captures_that_would_not_count(pkg, dev, monkeypatch):
+    (a,) = _models(dev, 1)
+    _fill((a,), {0, 1}, 0)
+    plain, fresh, warm = pkg.AdamW(a), pkg.AdamW(a, capturable=True), pkg.AdamW(a, capturable=True)
+    plain.step()
+    warm.step()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capturable"):
+        plain.step()
+    with pytest.raises(RuntimeError, match="first step"):
+        fresh.step()
+    assert fresh.group_state() is None
+    _fill((a,), {0}, 1)
+    with pytest.raises(RuntimeError, match="together"):
+        warm.step()
+    _fill((a,), {0, 1}, 1)
+    warm.step()
+    assert [int(c) for c, _ in warm.state_dict()["flat"][0]["steps"]] == [2, 0]
+
 
 def test_captured_steps_of_some_tensors(pkg, dev):
     a, b = _models(dev)

@@ -222,6 +222,11 @@ class AdamW(torch.optim.Optimizer):
             if any([g is not None and g.is_sparse for g in grads]):
                 raise RuntimeError("AdamW: sparse gradients are not supported")
             flat = self._flat[i]
+            if _capturing(params[0].device):
+                if not group["capturable"]:
+                    raise RuntimeError("AdamW: a step that is captured needs capturable=True")
+                if flat is None:
+                    raise RuntimeError("AdamW: the first step, which makes the state, comes before the capture")
             if flat is None:
                 count = torch.zeros(1, dtype=torch.int64, device=params[0].device) if group["capturable"] else 0
                 flat = {"state": adamw_state(params, group["state_bits"]), "steps": [(count, list(range(len(params))))]}
