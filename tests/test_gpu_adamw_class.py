@@ -114,3 +114,31 @@ def test_captured_steps_of_some_tensors(pkg, dev):
     oa.step()
     ob.step()
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_state_dicts_are_checked_first(pkg, dev):
+    (a, b) = _models(dev)
+    opt, other = pkg.AdamW(a, lr=1e-2, state_bits=8), pkg.AdamW(b, lr=2e-2, state_bits=8)
+    _fill((a, b), {0, 1, 3}, 0)
+    opt.step()
+    other.step()
+    good = opt.state_dict()
+    before = [t.clone() for t in other.group_state()]
+
+    def refused(match, d):
+        with pytest.raises(ValueError, match=match):
+            other.load_state_dict(d)
+        assert other.param_groups[0]["lr"] == 2e-2
+        assert all(torch.equal(x, y) for x, y in zip(other.group_state(), before))
+
+    flat = good["flat"][0]
+    refused("not this optimizer's", torch.optim.AdamW(a).state_dict())
+    refused("not this optimizer's", {**good, "flat": []})
+    refused("elements", {**good, "flat": [{**flat, "state": pkg.adamw_state(a[:2], 8)}]})
+    refused("bits", {**good, "flat": [{**flat, "state": pkg.adamw_state(a)}]})
+    refused("counts", {**good, "flat": [{**flat, "steps": flat["steps"][:1]}]})
+    other.load_state_dict(good)
+    assert other.param_groups[0]["lr"] == 1e-2
+    assert all(torch.equal(x, y) for x, y in zip(other.group_state(), opt.group_state()))
+    other.load_state_dict({**good, "flat": [{"state": flat["state"], "step": 1}]})  # one count for a whole group
+    assert other.state_dict()["flat"][0]["steps"] == [(1, [0, 1, 2, 3])]

@@ -278,18 +278,27 @@ class AdamW(torch.optim.Optimizer):
         return d
 
     def load_state_dict(self, state_dict: dict) -> None:
-        super().load_state_dict({k: v for k, v in state_dict.items() if k != "flat"})
-        self._flat = []
-        for group, f in zip(self.param_groups, state_dict["flat"]):
+        flat, groups = state_dict.get("flat"), self.param_groups
+        if flat is None or len(flat) != len(groups) or len(state_dict["param_groups"]) != len(groups):
+            raise ValueError("AdamW: the state dict is not this optimizer's, with one state for each group")
+        made = []
+        for group, saved, f in zip(groups, state_dict["param_groups"], flat):  # all of it, before anything changes
             if f is None:
-                self._flat.append(None)
+                made.append(None)
                 continue
-            dev = group["params"][0].device
-            state = AdamWState(*(None if t is None else t.detach().to(dev, copy=True) for t in f["state"]))
+            state, n = AdamWState(*f["state"]), len(group["params"])
             need = sum(_blocks(p.numel()) for p in group["params"]) * WFB_ADAMW_BLOCK
             if state.m.numel() != need:
                 raise ValueError(f"AdamW: the state has {state.m.numel()} elements, the group's tensors take {need}")
-            steps = f["steps"] if "steps" in f else [(f["step"], range(len(group["params"])))]
-            counts = [torch.as_tensor(c, dtype=torch.int64).reshape(1).to(dev, copy=True) if group["capturable"] else int(c)
+            if _bits_of("AdamW", state) != saved["state_bits"]:
+                raise ValueError(f"AdamW: the state is not one of {saved['state_bits']} bits")
+            steps = f["steps"] if "steps" in f else [(f["step"], range(n))]
+            if sorted(j for _, of in steps for j in of) != list(range(n)):
+                raise ValueError(f"AdamW: the counts of steps are not of {n} tensors")
+            dev = group["params"][0].device
+            state = AdamWState(*(None if t is None else t.detach().to(dev, copy=True) for t in state))
+            counts = [torch.as_tensor(c, dtype=torch.int64).reshape(1).to(dev, copy=True) if saved["capturable"] else int(c)
                       for c, _ in steps]
-            self._flat.append({"state": state, "steps": [(c, list(of)) for c, (_, of) in zip(counts, steps)]})
+            made.append({"state": state, "steps": [(c, list(of)) for c, (_, of) in zip(counts, steps)]})
+        super().load_state_dict({k: v for k, v in state_dict.items() if k != "flat"})
+        self._flat = made
