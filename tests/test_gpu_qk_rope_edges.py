@@ -63,3 +63,19 @@ def test_no_epsilon(pkg, dev, b, t, hq, hk, d, r, dtype):
         # a sum over N rows: sqrt(N) / 8 + 24 roundings at the most, and half a step
         off = float((grads[2 + i].double() - rw).norm() / rw.norm())
         assert off <= (24 + (b * t * x.shape[2]) ** 0.5) * U + torch.finfo(dtype).eps / 2, off
+
+
+@pytest.mark.parametrize("exponent", [0, -62, -66])
+def test_the_inverse_root_is_rounded(pkg, dev, exponent):
+    """Heads of two equal elements of 11 bits, no epsilon: the mean of squares and its root are exact, r is off by half a step,
+    a r by 2^-24 of 1, and 1 + 2^-24 rounds to 1.  At 2^-62 the squares lie at the least normal numbers, at 2^-66 they are
+    subnormal and hold the squares of 8 bits exactly."""
+    bits = 11 if exponent > -66 else 8
+    a = torch.arange(1, 1 << bits, device=dev).float() * 2.0 ** exponent
+    q = torch.stack([a, -a], -1)[None, :, None]  # [1, tokens, 1, 2]
+    one = torch.ones(2, device=dev)
+    cos, sin = torch.ones(1, 1, device=dev), torch.zeros(1, 1, device=dev)
+    pos = torch.zeros(a.numel(), dtype=torch.int64, device=dev)
+    out, _ = pkg.qk_norm_rope(q, q, cos, sin, pos, one, one, eps=0.0)
+    off = (out.double() - torch.tensor([1.0, -1.0], device=dev, dtype=torch.float64)).abs()
+    assert float(off.max()) <= 2.0 ** -24

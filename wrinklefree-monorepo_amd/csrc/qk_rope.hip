@@ -124,6 +124,10 @@ __device__ __forceinline__ float row_sum(float v) {
   }
 }
 
+// v^(-1/2), root and quotient each correctly rounded, subnormal v too.  (The one-instruction form is off by an ulp and takes
+// subnormal numbers for 0; either way the passes wait for memory: TIMES)
+__device__ __forceinline__ float inverse_root(float v) { return __fdiv_rn(1.0f, sqrtf(v)); }
+
 // Where item j lies: its two chunks' first elements and its first pair, -1 behind the rotated part.
 template <int V>
 __device__ __forceinline__ void item_place(const QkRope& p, int j, int& ea, int& eb, int& pair) {
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(QkRope p, uint32_t ta
           ss = __builtin_fmaf(xa[it][h].get(e), xa[it][h].get(e), ss);
           ss = __builtin_fmaf(xb[it][h].get(e), xb[it][h].get(e), ss);
         }
-      r = __builtin_amdgcn_rsqf(row_sum<L>(ss) / (float)D + p.eps);
+      r = inverse_root(row_sum<L>(ss) / (float)D + p.eps);
     }
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
@@ -345,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, float*
         }
         float r = 1.0f, m = 0.0f;
         if (sd.w) {
-          r = __builtin_amdgcn_rsqf(row_sum<L>(ss) / (float)D + p.eps);
+          r = inverse_root(row_sum<L>(ss) / (float)D + p.eps);
           m = r * (row_sum<L>(sg) / (float)D);
         }
 #pragma unroll
