@@ -92,3 +92,38 @@ def test_forms_of_large_calls(pkg, dev, m, k, f, dtype, wdtype, act):
         for first in (0, 1000, m - 40):
             assert torch.equal(pkg.gated_bitlinear(x[first:first + 40], act=act, packed=packed), h[first:first + 40])
         assert torch.equal(pkg.gated_bitlinear(x[-5:], act=act, packed=packed), h[-5:])
+
+
+def test_slopes_of_large_gates(pkg, dev):
+    """One token, gates from -40 to 40: a weight's gradient is one product d code a, so d itself shows.
+
+    Roundings of 2^-24: exp(-g) 4 (the exponential's ulp counts 2), 1 + exp one, the reciprocal's ulp 2: s has 7, a = g s 8,
+    exp(-g) s 12, slope = s + a (exp(-g) s): 7 s + 21 |a exp(-g) s|, and one of the sum.  gh up, its product with the slope, the
+    scale of the token, two planes (2), a code's product and the result's rounding: 7 more.  The products kept by the forward have 2
+    each (gate's move the slope by 2 |g| |slope'|, up's count as 2)."""
+    n = torch.arange(-128, 128, device=dev)
+    cols = torch.arange(128, device=dev)
+    gate = ((cols[None] < n[:, None].abs()).float() * n[:, None].sign())
+    up = torch.ones(256, 128, device=dev)
+    w = gate.abs().mean()
+    x = torch.full((1, 128), 40.0 / 128.0, device=dev) / w
+    gh = torch.randn(1, 256, device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    _, gx, gg, gu = _run(pkg, x, gate, up, gh, "silu")
+    q, a = pkg.quantize_activations_i8_per_token(x)
+    held = float(q[0, 0]) * float(a)
+    g = (n.double() * held * float(pkg.pack_gated(gate, up).scales[0]))
+    u = 128.0 * held * float(pkg.pack_gated(gate, up).scales[1])
+    s = torch.sigmoid(g)
+    # (1 - s written so that it keeps its digits)
+    rest = torch.sigmoid(-g)
+    slope, bend = s * (1 + g * rest), (s * rest * (2 + g * (rest - s))).abs()
+    dg, du = gh[0].double() * u * slope, gh[0].double() * g * s
+    size = gh[0].double().abs() * u * held
+    lim = 2.0 ** -24 * size * (7 * s + 21 * (g * s * rest).abs() + (1 + 7 + 2) * slope.abs() + 2 * g.abs() * bend)
+    off = (gg.double() - (dg * held)[:, None]).abs()
+    assert float(n.abs().max()) * held * float(pkg.pack_gated(gate, up).scales[0]) > 39.0
+    assert bool((off <= 1.001 * lim[:, None]).all()), float((off / lim[:, None]).max())
+    # d_up = gh (g s): 8 and the same 6 behind it, 2 of the gate through (g s)'
+    lim = 2.0 ** -24 * gh[0].double().abs() * held * ((8 + 6) * (g * s).abs() + 2 * g.abs() * slope.abs())
+    off = (gu.double() - (du * held)[:, None]).abs()
+    assert bool((off <= 1.001 * lim[:, None]).all()), float((off / lim[:, None].clamp(min=1e-300)).max())

@@ -43,12 +43,18 @@ struct GradSrc {
   const float* a_scale;  // [m]
 };
 
-// (d_gate, d_up): the exponential and the division by the hardware's instructions, both within an ulp.
+// (d_gate, d_up).  exp(-gate) by the hardware's base-2 exponential of the rounded product and a correction for what the
+// product's rounding left (|gate| 2^-24 of the result): four roundings whatever the gate.  1 - s as exp(-gate) s, which keeps its
+// digits where s is next to 1.  Seven operations more an element than without, which the passes over memory hide (2000 x 14336:
+// the whole step 1344 us both).
 template <int ACT>
 __device__ __forceinline__ void gated_slopes(float gate, float up, float g, float& dg, float& du) {
   if constexpr (ACT == WFB_ACT_SILU) {
-    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gate * -1.4426950408889634f)), a = gate * s;
-    dg = g * up * (s + a * (1.0f - s));
+    constexpr float kHi = -1.4426950408889634f, kLo = (float)(-1.4426950408889634 - (double)kHi);  // -1 / ln 2
+    const float p = gate * kHi, rest = __builtin_fmaf(gate, kLo, __builtin_fmaf(gate, kHi, -p));
+    const float t = __builtin_amdgcn_exp2f(fminf(p, 127.9f)), x = __builtin_fmaf(t, rest * 0.6931471805599453f, t);
+    const float s = __builtin_amdgcn_rcpf(1.0f + x), a = gate * s;
+    dg = g * up * __builtin_fmaf(a, x * s, s);
     du = g * a;
   } else {
     const float r = fmaxf(gate, 0.0f);
