@@ -127,3 +127,28 @@ def test_slopes_of_large_gates(pkg, dev):
     lim = 2.0 ** -24 * gh[0].double().abs() * held * ((8 + 6) * (g * s).abs() + 2 * g.abs() * slope.abs())
     off = (gu.double() - (du * held)[:, None]).abs()
     assert bool((off <= 1.001 * lim[:, None]).all()), float((off / lim[:, None].clamp(min=1e-300)).max())
+
+
+@pytest.mark.parametrize("scale", [90.0, 130.0, 1e4, 3e7, 1e12, 1e18])
+def test_gates_of_any_size(pkg, dev, scale):
+    """Gates of +- scale: silu's slope is 1 and its value the gate, or both are next to nothing (88 e^-88 of up, below 1e-36)."""
+    gate = torch.ones(64, 128, device=dev)
+    gate[::2] = -1.0
+    up = torch.ones(64, 128, device=dev)
+    x = torch.full((2, 128), scale / 128.0, device=dev)
+    x[1] = -x[1]
+    gh = torch.randn(2, 64, device=dev, generator=torch.Generator(device=dev).manual_seed(2)) * 1e-3
+    _, gx, gg, gu = _run(pkg, x, gate, up, gh, "silu")
+    q, a = pkg.quantize_activations_i8_per_token(x)
+    held = q.double() * a.double()[:, None]
+    y = held @ gate.double().t(), held @ up.double().t()
+    on = (y[0] > 0).double()
+    d = gh.double() * y[1] * on, gh.double() * y[0] * on
+    # kept products 2 roundings each, d 8 (slope and value within 8 of 1 and the gate), planes and scales 4, the sum of two tokens
+    # or 128 features and the result 3
+    for got, ref, size in ((gg, d[0].t() @ held, d[0].abs().t() @ held.abs()), (gu, d[1].t() @ held, d[1].abs().t() @ held.abs()),
+                           (gx, d[0] @ gate.double() + d[1] @ up.double(), (d[0].abs() + d[1].abs()) @ up.double())):
+        assert torch.isfinite(got).all()
+        # (a plane pair holds what is 2^-18 of its row's largest and more to 22 bits, the rest to 2^-40 of it)
+        lim = 19 * 2.0 ** -24 * size + 2.0 ** -40 * size.amax(1, keepdim=True) + 1e-36 * scale * scale
+        assert bool(((got.double() - ref).abs() <= lim).all())

@@ -45,15 +45,18 @@ struct GradSrc {
 
 // (d_gate, d_up).  exp(-gate) by the hardware's base-2 exponential of the rounded product and a correction for what the
 // product's rounding left (|gate| 2^-24 of the result): four roundings whatever the gate.  1 - s as exp(-gate) s, which keeps its
-// digits where s is next to 1.  Seven operations more an element than without, which the passes over memory hide (2000 x 14336:
+// digits where s is next to 1.  Nine operations more an element than without, which the passes over memory hide (2000 x 14336:
 // the whole step 1344 us both).
 template <int ACT>
 __device__ __forceinline__ void gated_slopes(float gate, float up, float g, float& dg, float& du) {
   if constexpr (ACT == WFB_ACT_SILU) {
     constexpr float kHi = -1.4426950408889634f, kLo = (float)(-1.4426950408889634 - (double)kHi);  // -1 / ln 2
-    const float p = gate * kHi, rest = __builtin_fmaf(gate, kLo, __builtin_fmaf(gate, kHi, -p));
-    const float t = __builtin_amdgcn_exp2f(fminf(p, 127.9f)), x = __builtin_fmaf(t, rest * 0.6931471805599453f, t);
-    const float s = __builtin_amdgcn_rcpf(1.0f + x), a = gate * s;
+    // (within [-88, 120] exp(-gate) is finite and the correction small; below, s and what it multiplies are next to nothing,
+    // above, s is 1; a NaN stays one in a)
+    const float low = gate < -88.0f ? -88.0f : gate, e = fminf(low, 120.0f);
+    const float p = e * kHi, rest = __builtin_fmaf(e, kLo, __builtin_fmaf(e, kHi, -p));
+    const float t = __builtin_amdgcn_exp2f(p), x = __builtin_fmaf(t, rest * 0.6931471805599453f, t);
+    const float s = __builtin_amdgcn_rcpf(1.0f + x), a = low * s;
     dg = g * up * __builtin_fmaf(a, x * s, s);
     du = g * a;
   } else {
