@@ -152,3 +152,21 @@ def test_gates_of_any_size(pkg, dev, scale):
         # (a plane pair holds what is 2^-18 of its row's largest and more to 22 bits, the rest to 2^-40 of it)
         lim = 19 * 2.0 ** -24 * size + 2.0 ** -40 * size.amax(1, keepdim=True) + 1e-36 * scale * scale
         assert bool(((got.double() - ref).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("m,k,f", [(33, 320, 96), (700, 640, 1536), (2500, 640, 2564)])
+@pytest.mark.parametrize("wdtype", [BF16, F32])
+def test_wide_gradients(pkg, dev, m, k, f, wdtype):
+    """bf16 gradients of operands in 22 bits are the fp32 ones, rounded: the same planes, sums and order."""
+    x, gate, up, gh = _case(dev, m, k, f, BF16, wdtype)
+    leaves = [t.detach().requires_grad_() for t in (x, gate, up)]
+    got = torch.autograd.grad(pkg.gated_bitlinear(*leaves, wide_grads=True), leaves, gh)
+    full = _run(pkg, x.float(), gate.float(), up.float(), gh.float(), "silu")[1:]
+    for a, b, t in zip(got, full, leaves):
+        assert a.dtype == t.dtype and torch.equal(a, b.to(t.dtype))
+    mod = pkg.GatedBitLinear.from_linears(*(torch.nn.Linear(k, f, bias=False, device=dev, dtype=wdtype) for _ in range(2)),
+                                          wide_grads=True)
+    with torch.no_grad():
+        mod.gate_proj.weight.copy_(gate)
+        mod.up_proj.weight.copy_(up)
+    assert torch.equal(torch.autograd.grad(mod(leaves[0]), [leaves[0]], gh)[0], got[0])

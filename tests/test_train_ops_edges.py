@@ -46,3 +46,16 @@ def test_scalings_with_keys_that_are_not_set(pkg):
     assert torch.equal(a[0], b[0])
     with pytest.raises(ValueError, match="theta"):
         pkg.rope_tables(1.0, 64, 16, scaling=YARN)
+
+
+def test_workspace_of_wide_gradients(pkg):
+    n, wide = ctypes.c_int64(-1), pkg._lib.WFB_GRAD_WIDE
+    bf16, f32 = pkg._lib.WFB_BF16, pkg._lib.WFB_F32
+
+    def size(gx, gw):
+        assert pkg._lib.status("wfb_gated_grad_workspace", 100, 65, 200, gx, 1, gw, 1, ctypes.addressof(n)) == 0
+        return n.value
+
+    assert size(bf16, bf16) < size(bf16 | wide, bf16) < size(bf16 | wide, bf16 | wide) == size(f32, f32) == size(f32 | wide, f32)
+    _no(pkg, "dtype", pkg._lib.status("wfb_gated_grad_workspace", 100, 65, 200, 2 * wide, 1, f32, 1, ctypes.addressof(n)))
+    _no(pkg, "dtype", pkg._lib.status("wfb_gated_grad_workspace", 100, 65, 200, -1, 1, f32, 1, ctypes.addressof(n)))

@@ -25,6 +25,7 @@ WFB_MAX_SEGMENTS = 8
 WFB_SCALE_REFERENCE = 0
 WFB_SCALE_CHECKPOINT = 1
 WFB_KV_I8_BLOCK = 64
+WFB_GRAD_WIDE = 0x100
 WFB_QK_MAX_DIM = 256
 WFB_ADAMW_BLOCK = 256
 WFB_ADAMW_SCALARS = 16

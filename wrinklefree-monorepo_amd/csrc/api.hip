@@ -876,6 +876,13 @@ static int check_gated(const char* name, int64_t m, int64_t f, int64_t k) {
   return WFB_OK;
 }
 
+// Takes WFB_GRAD_WIDE out of a result's type.
+static bool take_wide(int& dtype) {
+  const bool wide = dtype >= 0 && (dtype & WFB_GRAD_WIDE);
+  if (wide) dtype &= ~WFB_GRAD_WIDE;
+  return wide;
+}
+
 int wfb_pack_gated(const void* gate, const void* up, int w_dtype, int64_t f, int64_t k, float* scales_dev, uint8_t* qweight,
                    double* workspace, void* stream) {
   const char* name = "wfb_pack_gated";
@@ -910,10 +917,11 @@ int wfb_gated_grad_workspace(int64_t m, int64_t f, int64_t k, int gx_dtype, int 
                              int64_t* bytes) {
   const char* name = "wfb_gated_grad_workspace";
   if (const int st = check_gated(name, m, f, k)) return st;
+  const bool wide_x = take_wide(gx_dtype), wide_w = take_wide(gw_dtype);
   if (!valid_dtype(gx_dtype) || !valid_dtype(gw_dtype)) return fail(WFB_EINVAL, "%s: bad dtype", name);
   if (!bytes) return fail(WFB_EINVAL, "%s: null pointer", name);
   wfb::GatedGrad p{};
-  p.m = m, p.f = f, p.k = k, p.gx_dtype = gx_dtype, p.gw_dtype = gw_dtype;
+  p.m = m, p.f = f, p.k = k, p.gx_dtype = gx_dtype, p.gw_dtype = gw_dtype, p.wide_x = wide_x, p.wide_w = wide_w;
   p.gx = want_x ? bytes : nullptr;  // (only whether they are null counts)
   p.gw = want_w ? bytes : nullptr;
   *bytes = m == 0 ? 0 : wfb::gated_grad_workspace(p);
@@ -928,6 +936,7 @@ int wfb_gated_grad(const float* gate_up, const void* grad_h, int gh_dtype, int64
   if (const int st = check_gated(name, m, f, k)) return st;
   if (m == 0) return fail(WFB_EINVAL, "%s: no rows", name);
   if (act != WFB_ACT_SILU && act != WFB_ACT_RELU2) return fail(WFB_EINVAL, "%s: bad activation %d", name, act);
+  const bool wide_x = take_wide(gx_dtype), wide_w = take_wide(gw_dtype);
   if (!valid_dtype(gh_dtype) || !valid_dtype(gx_dtype) || !valid_dtype(gw_dtype)) return fail(WFB_EINVAL, "%s: bad dtype", name);
   if (!gate_up || !grad_h || !qweight || !scales_dev || !codes || !a_scale || !work || (!grad_x && !grad_w))
     return fail(WFB_EINVAL, "%s: null pointer", name);
@@ -936,7 +945,7 @@ int wfb_gated_grad(const float* gate_up, const void* grad_h, int gh_dtype, int64
   if (ldg < f || lda < k) return fail(WFB_EINVAL, "%s: row strides below the rows' length", name);
   if (!aligned(gate_up, 16) || !aligned(work, 256)) return fail(WFB_EINVAL, "%s: gate_up must be 16-byte, work 256-byte aligned", name);
   wfb::GatedGrad p{gate_up, grad_h, gh_dtype, ldg, m, f, act, qweight, k, k_pad, scales_dev, codes, lda, a_scale,
-                   grad_x, gx_dtype, grad_w, gw_dtype};
+                   grad_x, gx_dtype, grad_w, gw_dtype, wide_x, wide_w};
   return hip_status(wfb::launch_gated_grad(p, work, as_stream(stream)), name);
 }
 

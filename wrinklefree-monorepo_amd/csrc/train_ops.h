@@ -94,6 +94,7 @@ struct GatedGrad {
   int gx_dtype;
   void* gw;  // [2f, k] or null
   int gw_dtype;
+  bool wide_x, wide_w;  // operands in two planes for a bf16 result too
 };
 int64_t gated_grad_workspace(const GatedGrad& p);
 hipError_t launch_gated_grad(const GatedGrad& p, void* work, hipStream_t s);

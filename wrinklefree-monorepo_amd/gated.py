@@ -18,7 +18,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import WFB_ABSMEAN_WS_DOUBLES
+from ._lib import WFB_ABSMEAN_WS_DOUBLES, WFB_GRAD_WIDE
 from .bitlinear import BitLinear, _check_lambda
 from .ops import _ACTS, _DT, QK_I2_S, _capturing, _no_tangents, _on, _p, _require_gpu, _stream
 
@@ -88,10 +88,10 @@ class _GatedSTE(torch.autograd.Function):
     act(x~ gate~^T) * (x~ up~^T) at the quantised operands, from the two products that the forward kept."""
 
     @staticmethod
-    def forward(ctx, x2, gate_weight, up_weight, qweight, scales, act):
+    def forward(ctx, x2, gate_weight, up_weight, qweight, scales, act, wide):
         h, gate_up, q, a_scale = _forward(x2, PackedGated(qweight, scales), act, True)
         ctx.save_for_backward(gate_up, q, a_scale, qweight, scales)
-        ctx.meta = (act, x2.dtype, gate_weight.dtype, x2.shape[1])
+        ctx.meta = (act, x2.dtype, gate_weight.dtype, x2.shape[1], WFB_GRAD_WIDE if wide else 0)
         return h
 
     @staticmethod
@@ -99,7 +99,7 @@ class _GatedSTE(torch.autograd.Function):
     def backward(ctx, gh):
         # (a saved-tensor hook may give them back as other views; no products of no tokens)
         gate_up, q, a_scale, qweight, scales = (t if t is None else t.resolve_neg().contiguous() for t in ctx.saved_tensors)
-        act, xdt, wdt, k = ctx.meta
+        act, xdt, wdt, k, wide = ctx.meta
         need_x, need_gate, need_up = ctx.needs_input_grad[:3]
         f, m, dev = qweight.shape[0] // 2, q.shape[0], q.device
         if gh.stride(-1) != 1 or gh.stride(0) < f or gh.is_neg():
@@ -108,19 +108,20 @@ class _GatedSTE(torch.autograd.Function):
         gx = torch.empty((m, k), dtype=xdt, device=dev) if need_x else None
         gw = torch.empty((2 * f, k), dtype=wdt, device=dev) if need_w else None
         if m == 0:
-            return gx, *([gw[:f].zero_(), gw[f:].zero_()] if need_w else [None, None]), None, None, None
-        work = torch.empty(_grad_workspace(m, f, k, _DT[xdt], need_x, _DT[wdt], need_w), dtype=torch.uint8, device=dev)
+            return gx, *([gw[:f].zero_(), gw[f:].zero_()] if need_w else [None, None]), None, None, None, None
+        gxdt, gwdt = _DT[xdt] | wide, _DT[wdt] | wide
+        work = torch.empty(_grad_workspace(m, f, k, gxdt, need_x, gwdt, need_w), dtype=torch.uint8, device=dev)
         kp = 4 * qweight.shape[1]
         with _on(dev):
             _lib.call("wfb_gated_grad", _p(gate_up), _p(gh), _DT[gh.dtype], gh.stride(0) if m > 1 else f, m, f, _ACTS[act],
-                      _p(qweight), k, kp, _p(scales), _p(q), kp, _p(a_scale), _p(gx), _DT[xdt], _p(gw), _DT[wdt], _p(work),
+                      _p(qweight), k, kp, _p(scales), _p(q), kp, _p(a_scale), _p(gx), gxdt, _p(gw), gwdt, _p(work),
                       _stream(dev))
-        return gx, gw[:f] if need_gate else None, gw[f:] if need_up else None, None, None, None
+        return gx, gw[:f] if need_gate else None, gw[f:] if need_up else None, None, None, None, None
 
 
 def gated_bitlinear(
     x: torch.Tensor, gate_weight: Optional[torch.Tensor] = None, up_weight: Optional[torch.Tensor] = None,
-    act: str = "silu", packed: Optional[PackedGated] = None,
+    act: str = "silu", packed: Optional[PackedGated] = None, wide_grads: bool = False,
 ) -> torch.Tensor:
     """act(gate) * up, [..., hidden] in x's type, of x [..., in_features] (fp32, bf16 or fp16) through two ternary
     projections; ``act`` is "silu" or "relu2" (relu squared).  Products and activation are those of
@@ -129,7 +130,9 @@ def gated_bitlinear(
     ``packed`` (of :func:`pack_gated`) saves packing the float weights; without them the call serves only.  With autograd on
     and x or a weight requiring a gradient, the result is differentiable once, straight through both quantisers (in reverse mode;
     tangents of forward mode are refused), and the products are kept for it (8 bytes per token and hidden feature); x, gate_weight and up_weight get gradients in their
-    types.  ``packed`` must then be the weights' own pack."""
+    types.  ``packed`` must then be the weights' own pack.  What the activation's backward pass hands to the products is held in
+    22 bits of each row's scale for fp32 and fp16 gradients and in 11 for bf16 ones, an eighth of their own rounding;
+    ``wide_grads`` holds it in 22 for those too, at twice their products."""
     if act not in _ACTS:
         raise ValueError(f"{_NAME}: act must be one of {sorted(_ACTS)}")
     if (gate_weight is None) != (up_weight is None):
@@ -171,7 +174,7 @@ def gated_bitlinear(
             x2.requires_grad or (gate_weight is not None and (gate_weight.requires_grad or up_weight.requires_grad))):
         if gate_weight is None:
             raise RuntimeError(f"{_NAME}: packed weights alone have no float weights to train")
-        h = _GatedSTE.apply(x2, gate_weight, up_weight, packed.qweight, packed.scales, act)
+        h = _GatedSTE.apply(x2, gate_weight, up_weight, packed.qweight, packed.scales, act, wide_grads)
     else:
         h = _forward(x2, packed, act, False)[0]
     return h if x.dim() == 2 else h.view(*x.shape[:-1], f)
@@ -185,11 +188,13 @@ class GatedBitLinear(nn.Module):
     replay of a captured call (a graph that serves fixed weights saves that with ``gated_bitlinear(x, packed=mod.packed())``,
     the pack kept as long as the graph)."""
 
-    def __init__(self, in_features: int, hidden_features: int, act: str = "silu", device=None, dtype=None):
+    def __init__(self, in_features: int, hidden_features: int, act: str = "silu", device=None, dtype=None,
+                 wide_grads: bool = False):
         super().__init__()
         if act not in _ACTS:
             raise ValueError(f"GatedBitLinear: act must be one of {sorted(_ACTS)}")
         self.act = act
+        self.wide_grads = wide_grads
         self.gate_proj = BitLinear(in_features, hidden_features, device=device, dtype=dtype)
         self.up_proj = BitLinear(in_features, hidden_features, device=device, dtype=dtype)
         self._packed: Optional[PackedGated] = None
@@ -197,12 +202,14 @@ class GatedBitLinear(nn.Module):
         self._packed_on = None
 
     @classmethod
-    def from_linears(cls, gate_proj: nn.Linear, up_proj: nn.Linear, act: str = "silu") -> "GatedBitLinear":
+    def from_linears(cls, gate_proj: nn.Linear, up_proj: nn.Linear, act: str = "silu",
+                     wide_grads: bool = False) -> "GatedBitLinear":
         """A module that shares the weights of two linears."""
         if gate_proj.bias is not None or up_proj.bias is not None:
             raise RuntimeError("GatedBitLinear: projections with a bias are not gated in one product")
         _check_pair("GatedBitLinear", gate_proj.weight, up_proj.weight)
-        mod = cls(gate_proj.in_features, gate_proj.out_features, act, device="meta", dtype=gate_proj.weight.dtype)
+        mod = cls(gate_proj.in_features, gate_proj.out_features, act, device="meta", dtype=gate_proj.weight.dtype,
+                  wide_grads=wide_grads)
         mod.gate_proj.weight, mod.up_proj.weight = gate_proj.weight, up_proj.weight
         return mod
 
@@ -236,7 +243,7 @@ class GatedBitLinear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         _check_lambda("GatedBitLinear")
-        return gated_bitlinear(x, self.gate_proj.weight, self.up_proj.weight, self.act, self.packed())
+        return gated_bitlinear(x, self.gate_proj.weight, self.up_proj.weight, self.act, self.packed(), self.wide_grads)
 
     def _apply(self, fn, recurse=True):
         # (a weight that is cast and cast back may lie where it lay, its version counter unmoved)
