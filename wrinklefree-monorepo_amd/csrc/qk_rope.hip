@@ -384,8 +384,10 @@ __global__ __launch_bounds__(kThreads) void qk_rope_grad_kernel(QkRope p, float*
       for (int e = 0; e < 2 * V; ++e) red[grp][(it * 2 * V + e) * L + lane] = acc[it][e];
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * V * IT * L; i += kThreads) {
-      float v = 0.0f;
-      for (int q = 0; q < G; ++q) v += red[q][i];
+      float u[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (short chains: the sum's error grows with their length)
+#pragma unroll
+      for (int q = 0; q < G; ++q) u[q % 4] += red[q][i];
+      const float v = (u[0] + u[1]) + (u[2] + u[3]);
       const int ln = i % L, e = i / L % (2 * V), it = i / L / (2 * V), j = ln + L * it;
       if (j >= items) continue;
       int a, b, pr;
@@ -477,7 +479,8 @@ __global__ __launch_bounds__(256) void qk_weight_sum_kernel(const float* __restr
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)min(i + 16 * u, rows - 1) * 2 * D + cc];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) acc += i + 16 * u < rows ? v[u] : 0.0f;
+    for (int u = 0; u < 8; ++u) v[u] = i + 16 * u < rows ? v[u] : 0.0f;
+    acc += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
   }
   red[r][c] = acc;
   __syncthreads();
