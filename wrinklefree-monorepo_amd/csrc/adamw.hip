@@ -11,6 +11,9 @@
 // so an element's step never grows because its r went below the grid.  z in [0, 1) runs through a Weyl sequence over
 // steps and elements: a moment that moves by less than a code's distance in a step still moves on average, which with
 // rounding to the nearest it would not (b2 = 0.999 moves r by 0.05% a step, neighbouring codes lie 0.8% apart at best).
+// The average is right in the code, not in its square: with a root of n + f the value held is y + f (1 - f) on average, never
+// too small, so a moment rises faster and falls slower by 1 / (2 n) of its way.  One that stays is held within 0.4% at n = 8
+// and 0.03% from 18 on (simulated, b2 = 0.95 and 0.999).
 // Blocks whose largest is below 2^-100 are held as zeros; one with an infinity or a NaN has scale NaN.  A finite gradient
 // from 2^64 on has an infinite v: its element then only decays, in 32 bits for good; in 8 bits r is held as 2^63.
 #include <cmath>
@@ -143,8 +146,8 @@ __device__ __forceinline__ int code_of(float x, float k, int top, float z) {
 }
 
 // A wave takes a block: its largest is a reduction over the lanes, and nothing is read twice.  fp32 states move 28 bytes an
-// element (134M elements in six launches of up to 64 tensors 680-740 us, 5.1-5.5 TB/s), 8-bit states with bf16 gradients 14
-// (139M elements 478 us, 4.1 TB/s: bound by an element's three square roots and division; 561 us with the compiler's sqrtf).
+// element (134M elements in six launches of up to 64 tensors 745-765 us, 4.9-5.05 TB/s), 8-bit states with bf16 gradients 14
+// (139M elements 413 us, 4.7 TB/s; 476 with the compiler's sqrtf for an element's three roots; steps one behind the other).
 template <int PDT, int GDT, int BITS>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(Table tb, AdamWState st, AdamWScalars host,
                                                          const AdamWScalars* __restrict__ dev) {
@@ -249,7 +252,8 @@ __global__ void adamw_scalars_kernel(double lr, const float* __restrict__ lr_dev
   *out = c;
 }
 
-// What the codes stand for, 4 elements a thread: 139M elements, 2 bytes read and 8 written each, 228 us (6.1 TB/s).
+// What the codes stand for, 4 elements a thread: 139M elements, 2 bytes read and 8 written each, 238 us (5.8 TB/s),
+// 226 behind a step.
 __global__ __launch_bounds__(kThreads) void adamw_values_kernel(AdamWState st, int64_t quads, float* __restrict__ m,
                                                                 float* __restrict__ v) {
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < quads; i += (int64_t)gridDim.x * kThreads) {
