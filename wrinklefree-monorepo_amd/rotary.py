@@ -156,12 +156,14 @@ def qk_norm_rope(
     if by_tensor:
         if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((t,), (b, t)):
             raise RuntimeError(f"{_NAME}: positions must be int32 or int64 [{t}] or [{b}, {t}]")
-        positions = positions.resolve_neg()
+        if positions.is_neg():
+            positions = positions.resolve_neg()
     else:
         positions = 0 if positions is None else int(positions)
         if cos.shape[1] and not 0 <= positions <= cos.shape[0] - t:
             raise ValueError(f"{_NAME}: positions {positions}..{positions + t - 1} leave tables of {cos.shape[0]} rows")
-    cos, sin, q_weight, k_weight = (t.resolve_neg() if t is not None and t.is_neg() else t for t in (cos, sin, q_weight, k_weight))
+    if cos.is_neg() or sin.is_neg() or (q_weight is not None and q_weight.is_neg()) or (k_weight is not None and k_weight.is_neg()):
+        cos, sin, q_weight, k_weight = (t if t is None else t.resolve_neg() for t in (cos, sin, q_weight, k_weight))
     if forward_ad._current_level >= 0:
         _no_tangents(_NAME, q, k, q_weight, k_weight, cos, sin)
     q, k = _plain(q), _plain(k)
