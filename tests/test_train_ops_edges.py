@@ -59,3 +59,10 @@ def test_workspace_of_wide_gradients(pkg):
     assert size(bf16, bf16) < size(bf16 | wide, bf16) < size(bf16 | wide, bf16 | wide) == size(f32, f32) == size(f32 | wide, f32)
     _no(pkg, "dtype", pkg._lib.status("wfb_gated_grad_workspace", 100, 65, 200, 2 * wide, 1, f32, 1, ctypes.addressof(n)))
     _no(pkg, "dtype", pkg._lib.status("wfb_gated_grad_workspace", 100, 65, 200, -1, 1, f32, 1, ctypes.addressof(n)))
+
+
+def test_a_gated_pair_of_packed_projections(pkg):
+    packed = pkg.BitLinear.from_packed(torch.zeros(8, 32, dtype=torch.uint8), torch.ones(1), 128)
+    for pair in ((packed, packed), (pkg.BitLinear(128, 8), packed)):
+        with pytest.raises(RuntimeError, match="no float weight"):
+            pkg.GatedBitLinear.from_linears(*pair)

@@ -207,6 +207,8 @@ class GatedBitLinear(nn.Module):
         """A module that shares the weights of two linears."""
         if gate_proj.bias is not None or up_proj.bias is not None:
             raise RuntimeError("GatedBitLinear: projections with a bias are not gated in one product")
+        if gate_proj.weight is None or up_proj.weight is None:
+            raise RuntimeError("GatedBitLinear: a projection built from packed weights has no float weight")
         _check_pair("GatedBitLinear", gate_proj.weight, up_proj.weight)
         mod = cls(gate_proj.in_features, gate_proj.out_features, act, device="meta", dtype=gate_proj.weight.dtype,
                   wide_grads=wide_grads)
