@@ -3,6 +3,7 @@
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.utils._pytree import tree_map
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +71,43 @@ def test_lazily_negated_tables_weights_and_states(pkg, dev):
         pkg.adamw_step(p, rows, state._replace(m=neg(state.m)), 1)
     with pytest.raises(RuntimeError, match="state must be contiguous"):
         pkg.adamw_state_values(state._replace(v=neg(state.v)))
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor class whose objects have no memory but that of the tensor they wrap (as distributed tensors are)."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+    def __init__(self, t):
+        self.inner = t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        return func(*tree_map(lambda x: x.inner if isinstance(x, cls) else x, args), **(kwargs or {}))
+
+
+def test_tensors_without_memory_are_refused(pkg, dev):
+    """Their pointer is null, which for a gradient, a norm's weight or positions would mean that there is none."""
+    p, g = [torch.randn(300, device=dev), torch.randn(20, device=dev)], [torch.randn(300, device=dev), torch.randn(20, device=dev)]
+    before = [t.clone() for t in p]
+    for params, grads in ((p, [_Wrapped(g[0]), g[1]]), ([_Wrapped(p[0]), p[1]], g), ([_Wrapped(t) for t in p], [_Wrapped(t) for t in g])):
+        with pytest.raises(RuntimeError):
+            pkg.adamw_step(params, grads, pkg.adamw_state(p), 1)
+    assert all(torch.equal(a, b) for a, b in zip(p, before))
+    empty = [torch.randn(300, device=dev), torch.empty(0, device=dev)]  # (no elements, no memory: fine)
+    pkg.adamw_step(empty, [g[0], torch.empty(0, device=dev)], pkg.adamw_state(empty), 1)
+    q, k, w = torch.randn(1, 3, 2, 64, device=dev), torch.randn(1, 3, 1, 64, device=dev), torch.ones(64, device=dev)
+    cos, sin = (t.to(dev) for t in pkg.rope_tables(1e4, 64, 8))
+    pos = torch.arange(3, device=dev)
+    for args in ((q, k, cos, sin, _Wrapped(pos), w, w), (q, k, cos, sin, pos, _Wrapped(w), w), (q, k, cos, sin, pos, w, _Wrapped(w)),
+                 (_Wrapped(q), k, cos, sin, pos, w, w), (q, k, _Wrapped(cos), sin, pos, w, w)):
+        with pytest.raises(RuntimeError):
+            pkg.qk_norm_rope(*args)
+    x, gate, up = torch.randn(5, 128, device=dev), torch.randn(64, 128, device=dev), torch.randn(64, 128, device=dev)
+    want = pkg.gated_bitlinear(x, gate, up)
+    with pytest.raises(RuntimeError):
+        pkg.gated_bitlinear(_Wrapped(x), gate, up)
+    for args in ((x, _Wrapped(gate), up), (x, gate, _Wrapped(up))):  # (this class unwraps where its weights are detached)
+        assert torch.equal(pkg.gated_bitlinear(*args), want)

@@ -123,6 +123,8 @@ def adamw_step(
         if pdt not in _DT or gdt not in _DT:
             raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {pdt} and {gdt}")
     sizes, ptrs, gptrs = (list(map(f, x)) for f, x in ((tensor.numel, every), (tensor.data_ptr, live), (tensor.data_ptr, gs)))
+    if not (all(ptrs) and all(gptrs)) and any(t.numel() and not t.data_ptr() for t in chain(live, gs)):
+        raise RuntimeError(f"{name}: a tensor without memory of its own (of a wrapping class): step what it wraps")
     if len(set(ptrs)) != len(ptrs) and len({p for p in ptrs if p}) != sum(p != 0 for p in ptrs):
         raise RuntimeError(f"{name}: a tensor is given twice")
     if len(live) != len(every):  # a null gradient: the tensor is passed over

@@ -31,9 +31,17 @@ Positions = Union[None, int, torch.Tensor]
 # integers, which costs a third of three ctypes structures (a single token's call is bound by the host).
 
 
+def _memory(t: torch.Tensor) -> int:
+    """Where t lies, for the operands whose null pointer means that there is none."""
+    at = t.data_ptr()
+    if not at and t.numel():
+        raise RuntimeError(f"{_NAME}: a tensor without memory of its own (of a wrapping class)")
+    return at
+
+
 def _heads(x: torch.Tensor, weight: Optional[torch.Tensor], out: int, g: Optional[torch.Tensor] = None, gw: int = 0) -> tuple:
     """The fields of wfb_heads."""
-    w, wdt = (0, 0) if weight is None else (weight.data_ptr(), _DT[weight.dtype])
+    w, wdt = (0, 0) if weight is None else (_memory(weight), _DT[weight.dtype])
     gs = (0, 0, 0, 0) if g is None else (g.data_ptr(), *g.stride()[:3])
     return (x.data_ptr(), *x.stride()[:3], *gs, w, wdt, out, gw, x.shape[2])
 
@@ -43,7 +51,7 @@ def _rope(cos: torch.Tensor, sin: torch.Tensor, positions: Union[int, torch.Tens
     n, half = cos.shape
     if isinstance(positions, torch.Tensor):
         st = positions.stride()
-        where = (positions.data_ptr(), positions.element_size(), st[0] if len(st) == 2 else 0, st[-1], 0)
+        where = (_memory(positions), positions.element_size(), st[0] if len(st) == 2 else 0, st[-1], 0)
     else:
         where = (0, 0, 0, 0, positions)
     return (cos.data_ptr(), sin.data_ptr(), n, 2 * half, _LAYOUTS[layout], *where)
