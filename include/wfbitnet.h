@@ -491,8 +491,8 @@ int wfb_gated_i2s(const uint8_t* qweight, int64_t f, int64_t k, const int8_t* ac
  * t the ternary weights, in fp32 arithmetic, each result rounded once to its type.  gate_up as wfb_gated_i2s left it;
  * grad_h [M, ldg]; qweight [2F, k_pad/4] 8-byte aligned; codes [M, lda].  grad_x or grad_w may be NULL.
  * d times its scale enters the products in 22 bits (11 where the result is bf16) down to 2^-18 (2^-28) of the largest of its
- * row, see csrc/gated.hip; gx_dtype / gw_dtype | WFB_GRAD_WIDE: in 22 bits for a bf16 result too (the workspace likewise).  work: wfb_gated_grad_workspace bytes (host only; the
- * same sizes, types and wanted results), 256-byte aligned. */
+ * row, see csrc/gated.hip; gx_dtype / gw_dtype | WFB_GRAD_WIDE: in 22 bits for a bf16 result too (the workspace likewise).
+ * work: wfb_gated_grad_workspace bytes (host only; the same sizes, types and wanted results), 256-byte aligned. */
 #define WFB_GRAD_WIDE 0x100
 int wfb_gated_grad_workspace(int64_t m, int64_t f, int64_t k, int gx_dtype, int want_x, int gw_dtype, int want_w,
                              int64_t* bytes);
